@@ -143,6 +143,12 @@ _SIGNATURES = {
                                        c_void_p, c_int, c_void_p],
     ("gemm_tc5_pair", "vl_gemm_bf16_tc5_pair"): [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                                  c_void_p, c_int, c_void_p],
+    ("rows_8bit", "vl_add_rmsnorm_8bit"): [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                                           c_float, c_void_p],
+    ("rows_8bit", "vl_rows_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
+    ("rows_8bit", "vl_pack_8bit"): [c_void_p, c_void_p, c_int, c_int, c_void_p],
+    ("gemm_8bit", "vl_gemm_8bit"): [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                    c_int, c_void_p, c_void_p],
     ("memprobe", "vl_read_only"): [c_void_p, c_longlong, c_void_p, c_void_p],
     ("sampling", "vl_apply_penalties"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_void_p],
@@ -1530,6 +1536,107 @@ def gemm_bf16_tc5_pair(a, w, out, err=None, swiglu=False):
     _check(_fn("gemm_tc5_pair", "vl_gemm_bf16_tc5_pair")(_ptr(a), _ptr(w), _ptr(out), dtype_code(out.dtype), M, N, K,
                                                          K, K, width, _ptr(err), int(swiglu), _stream()),
            "vl_gemm_bf16_tc5_pair")
+    return out
+
+
+# ---------------------------------------------------------------- linear layers in 8 bits
+E4M3 = torch.float8_e4m3fn
+E4M3_MAX = 448.0
+
+
+def eight_bit_columns(K) -> int:
+    """Columns of a row of K values in 8 bits: zeros follow the values up to a multiple of 128."""
+    return -(-int(K) // 128) * 128
+
+
+def _need_8bit_rows(out, scale, R, cols, name):
+    _need(out, E4M3, "out", 2); _need(scale, torch.float32, "scale", 1)
+    if cols < 1 or out.shape != (R, eight_bit_columns(cols)) or scale.shape[0] != R:
+        raise KernelError(f"{name}: {R} rows of {cols} values go to out [{R}, {eight_bit_columns(cols)}] and scale [{R}], got out "
+                          f"{tuple(out.shape)}, scale {tuple(scale.shape)}")
+
+
+def add_rmsnorm_8bit(x, delta, weight, eps, out, scale, rows=None, into=None):
+    """The RMS norm of the stream's rows in 8 bits: x float32 [T, H] (+= delta when given and rows is None), h = rmsnorm(x[row r] (+ delta)) *
+    weight, scale[r] = max |h| / 448, out[r] = e4m3(h / scale[r]), so that h is out * scale; out e4m3 [R, eight_bit_columns(H)] with
+    zeros behind the H values, scale float32 [R].  delta float32 or bfloat16; weight float32 [H].  `into` (float32 [T, H]): where x + delta
+    goes instead of x.  A row of zeros has scale 0, a row with a NaN or an infinity a scale that is none either.  Returns out."""
+    _need(x, torch.float32, "x", 2); _need(weight, torch.float32, "weight", 1)
+    T, H = x.shape
+    R = T if rows is None else rows.shape[0]
+    if weight.shape[0] != H:
+        raise KernelError(f"add_rmsnorm_8bit: weight has {weight.shape[0]} entries for rows of {H}")
+    _need_8bit_rows(out, scale, R, H, "add_rmsnorm_8bit")
+    if delta is not None:
+        _need(delta, None, "delta", 2)
+        if delta.shape != x.shape:
+            raise KernelError(f"delta {tuple(delta.shape)} must match x {tuple(x.shape)}")
+    if rows is not None:
+        _need(rows, torch.int32, "rows", 1)
+    if into is not None:
+        _need(into, torch.float32, "into", 2)
+        if into.shape != x.shape:
+            raise KernelError(f"into {tuple(into.shape)} must match x {tuple(x.shape)}")
+    _check(_fn("rows_8bit", "vl_add_rmsnorm_8bit")(_ptr(x), _ptr(delta), F32 if delta is None else dtype_code(delta.dtype), _ptr(rows),
+                                                   _ptr(weight), _ptr(x if into is None else into), _ptr(out), _ptr(scale), R, H, out.shape[1],
+                                                   float(eps), _stream()), "vl_add_rmsnorm_8bit")
+    return out
+
+
+def rows_8bit(x, out, scale):
+    """Rows to 8 bits: scale[r] = max |x[r]| / 448, out[r] = e4m3(x[r] / scale[r]); x float32 or bfloat16 [R, K], out and scale as in
+    `add_rmsnorm_8bit`.  Returns out."""
+    _need(x, None, "x", 2)
+    R, K = x.shape
+    _need_8bit_rows(out, scale, R, K, "rows_8bit")
+    _check(_fn("rows_8bit", "vl_rows_8bit")(_ptr(x), dtype_code(x.dtype), _ptr(out), _ptr(scale), R, K, out.shape[1], _stream()), "vl_rows_8bit")
+    return out
+
+
+def pack_8bit(w):
+    """Weights w e4m3 [N, width] (rows as `rows_8bit` leaves them) in the layout that `gemm_8bit` reads: e4m3 [strips, blocks, 16, 128], a strip
+    being 16 rows, a block 128 columns of K (zeros fill both up), the eight 16-byte pieces of a block's row exchanged by xor with the row's
+    last three bits, as the tensor cores' 128-byte swizzle has it.  Done once, when a model is loaded."""
+    _need(w, E4M3, "w", 2)
+    N, columns = w.shape
+    if N < 1 or columns < 1 or columns % 128:
+        raise KernelError(f"pack_8bit: rows of a multiple of 128 columns, got {tuple(w.shape)}")
+    out = torch.empty((-(-N // 16), columns // 128, 16, 128), dtype=E4M3, device=w.device)
+    _check(_fn("rows_8bit", "vl_pack_8bit")(_ptr(w), _ptr(out), N, columns, _stream()), "vl_pack_8bit")
+    return out
+
+
+GEMM_8BIT_ACTIVATIONS = ("silu", "relu")                          # f(gate) * up
+GEMM_8BIT_UNARY = ("silu", "relu", "relu2", "tanh", "gelu")       # f(y)
+
+
+def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, residual=None, err=None):
+    """y = f(a_scale[m] w_scale[n] (a @ w^T)[m, n] + bias[n]) + residual[m, n] for rows in 8 bits (a e4m3 [M, width], a_scale float32 [M]:
+    `rows_8bit`, `add_rmsnorm_8bit`) and packed weights (w: `pack_8bit`, w_scale float32 [N]); float32 sums, scales, bias (float32 [N]) and
+    activation, rounded once to out (bfloat16 or float32 [M, N]).  act: one of GEMM_8BIT_UNARY or None.  gated: w's rows are blocks of
+    SWIGLU_GROUP gates and their ups, act one of GEMM_8BIT_ACTIVATIONS, out = f(gate) * up [M, N / 2].  residual: out's shape and type, may
+    be out itself."""
+    _need(a, E4M3, "a", 2); _need(a_scale, torch.float32, "a_scale", 1); _need(w, E4M3, "w", 4); _need(w_scale, torch.float32, "w_scale", 1)
+    _need(out, None, "out", 2)
+    M, columns = a.shape
+    N = w_scale.shape[0]
+    width = N // 2 if gated else N
+    if (w.shape != (-(-N // 16), columns // 128, 16, 128) or columns % 128 or a_scale.shape[0] != M or out.shape != (M, width)
+            or (gated and N % (2 * SWIGLU_GROUP))):
+        raise KernelError(f"gemm_8bit: shapes disagree a{tuple(a.shape)} a_scale{tuple(a_scale.shape)} w{tuple(w.shape)} "
+                          f"w_scale{tuple(w_scale.shape)} out{tuple(out.shape)}" + (" (gated)" if gated else ""))
+    if act not in GEMM_8BIT_ACTIVATIONS if gated else act is not None and act not in GEMM_8BIT_UNARY:
+        raise KernelError(f"gemm_8bit: unknown activation {act!r}; known: {', '.join(GEMM_8BIT_ACTIVATIONS if gated else GEMM_8BIT_UNARY)}")
+    if bias is not None:
+        _need(bias, torch.float32, "bias", 1)
+        if bias.shape[0] != N:
+            raise KernelError(f"gemm_8bit: the bias has {bias.shape[0]} entries for {N} rows of w")
+    if residual is not None:
+        _need(residual, out.dtype, "residual", 2)
+        if residual.shape != out.shape:
+            raise KernelError(f"gemm_8bit: residual {tuple(residual.shape)} must match out {tuple(out.shape)}")
+    _check(_fn("gemm_8bit", "vl_gemm_8bit")(_ptr(a), _ptr(a_scale), _ptr(w), _ptr(w_scale), _ptr(out), dtype_code(out.dtype), _ptr(bias),
+                                            _ptr(residual), _act_code(act), int(gated), M, N, columns, _ptr(err), _stream()), "vl_gemm_8bit")
     return out
 
 
