@@ -305,6 +305,30 @@ def test_another_stream(m):
 
 
 @gpu
+@pytest.mark.parametrize("m", [4, 50, 600])
+def test_another_thread(m):
+    """A thread whose first call this is."""
+    import threading
+    a, sa, w, sw = operands(65, m, 256, 512)
+    p, got = ops.pack_8bit(w), []
+    want, out = torch.empty(m, 256, device=DEV), torch.empty(m, 256, device=DEV)
+    ops.gemm_8bit(a, sa, p, sw, want)
+    torch.cuda.synchronize()
+
+    def work():
+        try:
+            got.append(ops.gemm_8bit(a, sa, p, sw, out))
+        except Exception as e:
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert got[0] is out and torch.equal(out, want)
+
+
+@gpu
 def test_products_in_a_graph():
     a, sa, w, sw = operands(70, 8, 256, 512)
     p = ops.pack_8bit(w)

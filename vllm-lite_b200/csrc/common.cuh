@@ -31,7 +31,8 @@
 #define VL_DEV_IN_GEMM_EXPERTS 0x8000u
 #define VL_DEV_IN_GEMM_GROUPED 0x100000u
 #define VL_DEV_IN_GEMM_FEW 0x200000u
-// ... and, in the three tcgen05 products, which waits gave up in the block (shifted left by 16):
+#define VL_DEV_IN_GEMM_8BIT 0x400000u
+// ... and, in the tcgen05 products, which waits gave up in the block (shifted left by 16):
 // 1 a free stage (copying thread), 2 a free accumulator, 4 a filled stage (both: issuing thread),
 // 8 a complete accumulator (epilogue)
 #define VL_DEV_ROLE_SHIFT 16
