@@ -5,11 +5,12 @@
 // (gated) f(gate) * up with w's rows in blocks of 8 gates and their 8 ups: out then has N / 2 columns.
 #include "tc5.cuh"
 #include <cuda_fp8.h>
+#include <math.h>
 
 using namespace tc5;
 
 namespace {
-enum { ACT_NONE = -1, ACT_SILU = 0, ACT_RELU = 1, ACT_RELU2 = 16, ACT_TANH = 17, ACT_GELU = 18 };
+enum { ACT_NONE = -1, ACT_SILU = 0, ACT_RELU = 1, ACT_RELU2 = 16, ACT_TANH = 17, ACT_GELU = 18 };   // codes of csrc/ops.py
 
 struct Epilogue {
     const float* a_scale;                    // [M]
@@ -23,119 +24,162 @@ struct Epilogue {
 // v / (1 + exp(-v)).  The quick quotient (2 units in the last place): the exact one leaves the straight path where exp(-v) overflows, and a tile's
 // epilogue then takes longer than its products
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
-__device__ __forceinline__ float activate_gate(float v, int act) { return act == ACT_SILU ? silu(v) : v < 0.f ? 0.f : v; }
+__device__ __forceinline__ float relu(float v) { return v < 0.f ? 0.f : v; }
+// v times the normal distribution function, max(v, 0) - |v| / 2 erfc(|v| / sqrt(2)).  erfc(x) = t exp(-x^2) P(t), t = 1 / (1 + 0.4 x), P the
+// polynomial of degree 8 nearest to erfc(x) exp(x^2) / t in relative error for x up to 10 (least squares at Chebyshev nodes: 7e-8; in float32 4e-7),
+// which holds far below zero, where 1 + erf cancels.  17 operations: with erfcf, 2,048 x 4,096 -> 8,192 took 66.5 us for 60.7 (52 without activation).
+__device__ __forceinline__ float gelu(float v) {
+    const float x = fabsf(v), t = __fdividef(1.0f, fmaf(0.282842712f, x, 1.0f));
+    float p = 0.0419418029f;
+    p = fmaf(p, t, -0.143589124f);
+    p = fmaf(p, t, 0.0905594453f);
+    p = fmaf(p, t, 0.0806835741f);
+    p = fmaf(p, t, 0.0846026987f);
+    p = fmaf(p, t, 0.191415131f);
+    p = fmaf(p, t, 0.202369645f);
+    p = fmaf(p, t, 0.226379126f);
+    p = fmaf(p, t, 0.225637764f);
+    return relu(v) - 0.5f * fminf(x, 20.0f) * (t * p * __expf(-0.5f * x * x));
+}
+// called, not repeated for each of a chunk's values
+__device__ __noinline__ float tanh_of(float v) { return tanhf(v); }
+template <int ACT> __device__ __forceinline__ float activate(float v) {
+    if (ACT == ACT_SILU) return silu(v);
+    if (ACT == ACT_RELU) return relu(v);
+    if (ACT == ACT_RELU2) return v < 0.f ? 0.f : v * v;
+    if (ACT == ACT_TANH) return tanh_of(v);
+    if (ACT == ACT_GELU) return gelu(v);
+    return v;
+}
 __device__ __forceinline__ float activate(float v, int act) {
     switch (act) {
         case ACT_SILU: return silu(v);
-        case ACT_RELU: return v < 0.f ? 0.f : v;
+        case ACT_RELU: return relu(v);
         case ACT_RELU2: return v < 0.f ? 0.f : v * v;
-        case ACT_TANH: return tanhf(v);
-        case ACT_GELU: return 0.5f * v * erfcf(v * -0.70710678118654752f);      // erfc: exact far below zero, where 1 + erf cancels
+        case ACT_TANH: return tanh_of(v);
+        case ACT_GELU: return gelu(v);
         default: return v;
     }
 }
 
 // ---- from an accumulator in TMEM to out ------------------------------------------------------------
-// W's rows lie along the accumulator's lanes and the rows of a along its columns: a thread holds CH values of its row n of W, for the
-// rows t0 .. t0 + CH - 1 of a.  MODE 0: no activation, 1: of one argument, 2: gated.
-// A warp's 32 lanes are 32 neighbouring columns of out, 2 or 4 bytes each.  Two lanes that are neighbours exchange halves, so that each
-// stores two neighbouring columns of every second row (`pairs`: out has an even number of columns and begins on 8 bytes); gated, lanes
-// 8 apart hold a gate and its up and take turns likewise.
-template <typename TO> struct Two;
-template <> struct Two<float> {
-    static __device__ __forceinline__ void load(const float* p, float& a, float& b) { const float2 v = *reinterpret_cast<const float2*>(p); a = v.x; b = v.y; }
-    static __device__ __forceinline__ void store(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
-};
-template <> struct Two<bf16> {
-    static __device__ __forceinline__ void load(const bf16* p, float& a, float& b) {
-        const unsigned v = *reinterpret_cast<const unsigned*>(p);
-        a = __uint_as_float(v << 16);
-        b = __uint_as_float(v & 0xffff0000u);
+// W's rows lie along the accumulator's lanes and the rows of a along its columns: a thread holds CHUNK values of its row n of W, for the
+// rows t0 .. t0 + CHUNK - 1 of a, whose scales lie in shared memory; `end` is the row of a behind the tile's last.  A warp's 32 lanes are 32 neighbouring columns of out, 64 or 128 bytes of a row a store; gated, lanes 8 apart hold a gate and
+// its up and take every second row each.  The instructions of a value are what a tile's epilogue costs: stores of two neighbouring columns, which
+// lanes have to exchange values for, took three times as many as these (256 rows x 1,024 -> 1,024 on pairs of SMs: 11.5 us and 9.1).
+constexpr int CHUNK = 16;
+
+__device__ __forceinline__ void load_tmem(unsigned taddr, float (&v)[CHUNK]) {
+    unsigned r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr));
+    tc5_wait_ld();
+#pragma unroll
+    for (int i = 0; i < CHUNK; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// What a thread adds to its values of such a chunk and where they go.
+template <typename TO, bool GATED>
+struct Place {
+    static constexpr int STEP = GATED ? 2 : 1, COUNT = CHUNK / STEP;
+    size_t at, step;
+    int rows;
+    __device__ __forceinline__ Place(const Epilogue& e, int n, int t0, int end) {
+        const int up = GATED ? (threadIdx.x >> 3) & 1 : 0, ld = GATED ? e.N >> 1 : e.N;
+        at = (size_t)(t0 + up) * ld + (GATED ? ((n >> 4) << 3) + (n & 7) : n);
+        step = (size_t)STEP * ld;
+        rows = n < e.N ? min(end, e.M) - t0 - up : 0;
     }
-    static __device__ __forceinline__ void store(bf16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
+    __device__ __forceinline__ void load(const Epilogue& e, TO (&x)[COUNT]) const {
+        const TO* r = reinterpret_cast<const TO*>(e.residual) + at;
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c, r += step) x[c] = c * STEP < rows ? *r : from_f32<TO>(0.f);
+    }
 };
 
-template <typename TO, int MODE, int CH>
-__device__ __forceinline__ void finish(float (&v)[CH], const Epilogue& e, int n, float sw, float b, int t0, bool pairs) {
-    const int lane = threadIdx.x & 31;
-    const float mine = t0 + (lane & (CH - 1)) < e.M ? e.a_scale[t0 + (lane & (CH - 1))] : 0.f;
-    TO* out = reinterpret_cast<TO*>(e.out);
-    const TO* res = reinterpret_cast<const TO*>(e.residual);
+template <typename TO, int ACT, bool GATED>
+__device__ __forceinline__ void finish(float (&v)[CHUNK], TO (&x)[CHUNK / (GATED ? 2 : 1)], int n, int t0, int end, int next, const Epilogue& e,
+                                       const float* scales, float sw, float b) {
+    const Place<TO, GATED> p(e, n, t0, end);
+    const float4* s4 = reinterpret_cast<const float4*>(scales);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) v[c] = v[c] * (__shfl_sync(0xffffffffu, mine, c) * sw) + b;
-    if (MODE == 2) {
-        const int ld = e.N >> 1, up = (lane >> 3) & 1, col = ((n >> 4) << 3) + (n & 7);
-        float r[CH / 2];
+    for (int c = 0; c < CHUNK; c += 4) {
+        const float4 s = s4[c / 4];
+        v[c] = v[c] * s.x * sw + b;
+        v[c + 1] = v[c + 1] * s.y * sw + b;
+        v[c + 2] = v[c + 2] * s.z * sw + b;
+        v[c + 3] = v[c + 3] * s.w * sw + b;
+    }
+    constexpr int STEP = Place<TO, GATED>::STEP, COUNT = Place<TO, GATED>::COUNT;
+    if (GATED) {
+        const int up = (threadIdx.x >> 3) & 1;
 #pragma unroll
-        for (int c = 0; c < CH; c += 2) {
-            const int t = t0 + c + up;
-            r[c / 2] = res && n < e.N && t < e.M ? to_f32(res[(size_t)t * ld + col]) : 0.f;
-        }
-#pragma unroll
-        for (int c = 0; c < CH; c += 2) {
+        for (int c = 0; c < CHUNK; c += 2) {
             const float got = __shfl_xor_sync(0xffffffffu, up ? v[c] : v[c + 1], 8);
-            const int t = t0 + c + up;
-            const float y = activate_gate(up ? got : v[c], e.act) * (up ? v[c + 1] : got) + r[c / 2];
-            if (n < e.N && t < e.M) out[(size_t)t * ld + col] = from_f32<TO>(y);
+            v[c / 2] = activate<ACT>(up ? got : v[c]) * (up ? v[c + 1] : got);
         }
-        return;
+    } else {
+#pragma unroll
+        for (int c = 0; c < CHUNK; ++c) v[c] = activate<ACT>(v[c]);
     }
-    if (MODE == 1) {
+    if (e.residual) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) v[c] = activate(v[c], e.act);
+        for (int c = 0; c < COUNT; ++c) v[c] += to_f32(x[c]);
+        if (next < end) Place<TO, GATED>(e, n, next, end).load(e, x);
     }
-    const int ld = e.N;
-    if (pairs) {
-        const int odd = lane & 1, col = n & ~1;
-        float r[CH];
+    TO* o = reinterpret_cast<TO*>(e.out) + p.at;
 #pragma unroll
-        for (int c = 0; c < CH; c += 2) {
-            r[c] = r[c + 1] = 0.f;
-            if (res && col < e.N && t0 + c + odd < e.M) Two<TO>::load(res + (size_t)(t0 + c + odd) * ld + col, r[c], r[c + 1]);
-        }
-#pragma unroll
-        for (int c = 0; c < CH; c += 2) {
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[c] : v[c + 1], 1);
-            const float lo = odd ? got : v[c], hi = odd ? v[c + 1] : got;
-            if (col < e.N && t0 + c + odd < e.M) Two<TO>::store(out + (size_t)(t0 + c + odd) * ld + col, lo + r[c], hi + r[c + 1]);
-        }
-        return;
+    for (int c = 0; c < COUNT; ++c, o += p.step)
+        if (c * STEP < p.rows) *o = from_f32<TO>(v[c]);
+}
+
+// The chunks of a warp, every second of a tile's (rows t0 + c0 .. of a, c0 < cols): what they are added to is asked for ahead, the first
+// before `ready` waits for the sums (-> whether they came), the others before the stores of the one in front; `sums(c0, v)` brings the sums.
+// Residual and out may be the same memory: a thread reads what it writes, and before.
+template <typename TO, int ACT, bool GATED, typename Ready, typename Sums>
+__device__ __forceinline__ bool finish_chunks(const Epilogue& e, int n, const float* scales, float sw, float b, int t0, int end, int half, int cols, Ready ready,
+                                              Sums sums) {
+    TO x[Place<TO, GATED>::COUNT];
+    end = min(end, t0 + cols);
+    int c0 = half * CHUNK;
+    if (c0 < cols && e.residual) Place<TO, GATED>(e, n, t0 + c0, end).load(e, x);
+    if (!ready()) return false;
+#pragma unroll 1
+    for (; c0 < cols; c0 += 2 * CHUNK) {
+        float v[CHUNK];
+        sums(c0, v);
+        finish<TO, ACT, GATED>(v, x, n, t0 + c0, end, t0 + c0 + 2 * CHUNK, e, scales + c0, sw, b);
     }
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-        if (n < e.N && t0 + c < e.M) {
-            const size_t at = (size_t)(t0 + c) * ld + n;
-            out[at] = from_f32<TO>(res ? v[c] + to_f32(res[at]) : v[c]);
-        }
+    return true;
 }
 
 constexpr int STRIP = 16, KB = 128;          // a strip of W, a block of K: 128 bytes
 constexpr int ROWS = 128;                    // W's rows of a block
 constexpr unsigned W_BYTES = ROWS * KB;
-
-__device__ __forceinline__ bool stores_pairs(const Epilogue& e) { return (e.N & 1) == 0 && (((uintptr_t)e.out | (uintptr_t)e.residual) & 7) == 0; }
 }  // namespace
 
 // ---- many rows: two SMs on a tile of 256 rows of W by 256 rows of a ---------------------------------
 namespace pair8 {
-constexpr int BT = 256, STAGES = 6, NUM_THREADS = 64 + 256;
-constexpr unsigned A_BYTES = BT / 2 * KB, STAGE_BYTES = W_BYTES + A_BYTES, TMEM_COLS = 512;
+constexpr int MOST = 256, STAGES = 6, NUM_THREADS = 64 + 256;
+constexpr unsigned STAGE_BYTES = W_BYTES + MOST / 2 * KB, TMEM_COLS = 512;
 
-__device__ __forceinline__ void tile_corner(int tile, int tiles_t, int tiles_n, int& t0, int& n0) {
+__device__ __forceinline__ void tile_corner(int tile, int tiles_t, int tiles_n, int bt, int& t0, int& n0) {
     constexpr int BAND = 8;                                  // pairs that run together share W's tiles in L2
     const int band = tile / (BAND * tiles_n), in_band = tile - band * BAND * tiles_n;
     const int band_rows = min(BAND, tiles_t - band * BAND);
-    t0 = (band * BAND + in_band % band_rows) * BT;
+    t0 = (band * BAND + in_band % band_rows) * bt;
     n0 = (in_band / band_rows) * 2 * ROWS;
 }
 
-template <typename TO, int MODE>
+template <typename TO, int ACT, bool GATED>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, Epilogue e, int k_blocks, int tiles_t,
-                      int tiles_n, unsigned* err) {
+gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, Epilogue e, int k_blocks, int bt,
+                      int tiles_t, int tiles_n, unsigned* err) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[2], acc_empty_bar[2];
+    __shared__ __align__(16) float scales[2][MOST];          // of a tile's rows of a, by accumulator
     __shared__ unsigned tmem_base_slot;
     __shared__ int failed;
     const int warp = warp_number();
@@ -162,8 +206,8 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         bool ok = true;
         for (int tile = pair; tile < total_tiles && ok; tile += num_pairs) {
             int t0, n0;
-            tile_corner(tile, tiles_t, tiles_n, t0, n0);
-            const int strip = n0 / STRIP + (int)rank * (ROWS / STRIP), row = t0 + (int)rank * (BT / 2);
+            tile_corner(tile, tiles_t, tiles_n, bt, t0, n0);
+            const int strip = n0 / STRIP + (int)rank * (ROWS / STRIP), row = t0 + (int)rank * (bt / 2);
             for (int kb = 0; kb < k_blocks; ++kb) {
                 if (!warp_wait(&empty_bar[s], phase)) {
                     if (lead) atomicOr(&failed, 1);
@@ -171,7 +215,7 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                     break;
                 }
                 if (lead) {
-                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * STAGE_BYTES);       // the bytes of both blocks
+                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * W_BYTES + (unsigned)(bt * KB));       // the bytes of both blocks
                     const unsigned bar = map_to_rank(smem_u32(&full_bar[s]), 0);
                     unsigned char* st = smem + (size_t)s * STAGE_BYTES;
                     tma_load_3d_pair(st, &map_w, 0, kb * STRIP, strip, bar);
@@ -183,7 +227,7 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     } else if (warp == 1) {
         if (rank == 0) {                                     // ---- the pair's products ----
             const bool lead = elect_one();
-            constexpr unsigned idesc = make_idesc_8bit(2 * ROWS, BT);
+            const unsigned idesc = make_idesc_8bit(2 * ROWS, bt);
             int s = 0, local = 0;
             unsigned phase = 0;
             bool ok = true;
@@ -194,7 +238,7 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                     break;
                 }
                 tc5_fence_after();
-                const unsigned tmem_c = tmem_base + (unsigned)(acc * BT);
+                const unsigned tmem_c = tmem_base + (unsigned)(acc * MOST);
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     if (!warp_wait(&full_bar[s], phase)) {
                         if (lead) atomicOr(&failed, 4);
@@ -217,28 +261,28 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         }
     } else {                                                 // ---- epilogue: warps 2..9 ----
         const int quarter = warp & 3, half = (warp - 2) >> 2, lane = threadIdx.x & 31;
-        const bool pairs = stores_pairs(e);
         const unsigned freed = map_to_rank(smem_u32(&acc_empty_bar[0]), 0);
         int local = 0;
         for (int tile = pair; tile < total_tiles; tile += num_pairs, ++local) {
             const int acc = local & 1;
             int t0, n0;
-            tile_corner(tile, tiles_t, tiles_n, t0, n0);
+            tile_corner(tile, tiles_t, tiles_n, bt, t0, n0);
             const int n = n0 + (int)rank * ROWS + quarter * 32 + lane;
             const float sw = n < e.N ? e.w_scale[n] : 0.f, b = e.bias && n < e.N ? e.bias[n] : 0.f;
-            if (!warp_wait(&acc_full_bar[acc], (unsigned)((local / 2) & 1))) {
+            const int i = threadIdx.x - 64;                  // (who read this place last has passed the barrier of the tile between)
+            scales[acc][i] = t0 + i < e.M ? e.a_scale[t0 + i] : 0.f;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const unsigned tmem = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * MOST);
+            if (!finish_chunks<TO, ACT, GATED>(
+                    e, n, scales[acc], sw, b, t0, t0 + bt, half, min(bt, e.M - t0),
+                    [&] {
+                        const bool there = warp_wait(&acc_full_bar[acc], (unsigned)((local / 2) & 1));
+                        tc5_fence_after();
+                        return there;
+                    },
+                    [&](int c0, float (&v)[CHUNK]) { load_tmem(tmem + (unsigned)c0, v); })) {
                 atomicOr(&failed, 8);
                 break;
-            }
-            tc5_fence_after();
-            const unsigned tmem = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * BT);
-            for (int c0 = half * 32; c0 < BT && t0 + c0 < e.M; c0 += 64) {
-                unsigned raw[32];
-                float v[32];
-                tc5_ld32(tmem + (unsigned)c0, raw);
-#pragma unroll
-                for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(raw[c]);
-                finish<TO, MODE, 32>(v, e, n, sw, b, t0 + c0, pairs);
             }
             tc5_fence_before();
             mbar_arrive_remote(freed + (unsigned)(acc * sizeof(unsigned long long)));
@@ -253,6 +297,350 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 }
 }  // namespace pair8
 
+// ---- in between: one SM on a tile of 128 rows of W by BT rows of a, the blocks of a cluster sharing its K -----------------
+// A block multiplies a run of the blocks of K (W as the 128-row operand) and hands the sums of the columns that another block finishes to that
+// block, through the cluster's shared memory: every block finishes an even share of the tile's rows of a, adding the parts in the order of K.
+namespace split8 {
+constexpr int NUM_THREADS = 64 + 256;
+
+// bt: a multiple of 16 up to 256.  The parts that blocks hand each other take the ring's place.
+template <typename TO, int ACT, bool GATED, int PER_SM>
+__global__ void __launch_bounds__(NUM_THREADS, PER_SM)
+gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, Epilogue e, int k_blocks, int bt,
+                       int tiles_t, int splits, int stages, unsigned* err) {
+    const unsigned stage_bytes = W_BYTES + (unsigned)(bt * KB);
+    extern __shared__ __align__(1024) unsigned char smem[];   // (nothing else is shared: it begins on a kilobyte)
+    unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(smem + stages * stage_bytes);
+    unsigned long long *empty_bar = full_bar + stages, *acc_bar = empty_bar + stages;
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(acc_bar + 1);
+    int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+    float* scales = reinterpret_cast<float*>(((uintptr_t)(failed + 1) + 15) & ~(uintptr_t)15);     // of the tile's rows of a
+    const int warp = warp_number(), lane = threadIdx.x & 31;
+    const int rank = (int)(blockIdx.x % splits), tile = (int)(blockIdx.x / splits);          // a cluster's blocks are neighbours
+    const int t0 = (tile % tiles_t) * bt, n0 = (tile / tiles_t) * ROWS;
+    const int kb0 = (int)((long long)k_blocks * rank / splits), kb1 = (int)((long long)k_blocks * (rank + 1) / splits);
+    const unsigned tmem_cols = bt <= 32 ? 32 : bt <= 64 ? 64 : bt <= 128 ? 128 : 256;
+    auto copy = [&](int s, int kb) {
+        unsigned char* st = smem + s * stage_bytes;
+        mbar_arrive_expect_tx(&full_bar[s], stage_bytes);
+        tma_load_3d(st, &map_w, 0, kb * STRIP, n0 / STRIP, &full_bar[s]);
+        tma_load_2d(st + W_BYTES, &map_a, kb * KB, t0, &full_bar[s]);
+    };
+    const int early = min(stages, kb1 - kb0);
+
+    if (warp == 0) {
+        if (elect_one()) {                                   // the first copies go out before anything else is set up
+            for (int i = 0; i < stages; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], 1); }
+            mbar_init(acc_bar, 1);
+            mbar_fence_init();
+            *failed = 0;
+            for (int i = 0; i < early; ++i) copy(i, kb0 + i);
+        }
+        __syncwarp();
+    }
+    if (warp == 1) tc5_alloc(tmem_slot, tmem_cols);
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int row = quarter * 32 + lane, n = n0 + row;
+    float sw = 0.f, b = 0.f;
+    if (warp >= 2) {
+        const int i = threadIdx.x - 64;
+        if (i < bt) scales[i] = t0 + i < e.M ? e.a_scale[t0 + i] : 0.f;
+        if (n < e.N) {
+            sw = e.w_scale[n];
+            if (e.bias) b = e.bias[n];
+        }
+    }
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    const unsigned tmem_base = *tmem_slot;
+
+    if (warp == 0) {                                         // ---- copies ----
+        const bool lead = elect_one();
+        int s = 0;
+        unsigned phase = 0;
+        for (int kb = kb0 + early; kb < kb1; ++kb) {
+            if (!warp_wait(&empty_bar[s], phase)) {
+                if (lead) atomicOr(failed, 1);
+                break;
+            }
+            if (lead) copy(s, kb);
+            if (++s == stages) { s = 0; phase ^= 1u; }
+        }
+    } else if (warp == 1) {                                  // ---- products ----
+        const bool lead = elect_one();
+        const unsigned idesc = make_idesc_8bit(ROWS, bt);
+        int s = 0;
+        unsigned phase = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (!warp_wait(&full_bar[s], phase)) {
+                if (lead) atomicOr(failed, 4);
+                break;
+            }
+            tc5_fence_after();
+            const unsigned char* st = smem + s * stage_bytes;
+            const unsigned long long wdesc = make_smem_desc(st), adesc = make_smem_desc(st + W_BYTES);
+            if (lead) {
+#pragma unroll
+                for (int k = 0; k < KB / 32; ++k)
+                    tc5_mma_8bit(tmem_base, wdesc + (unsigned long long)(k * 2), adesc + (unsigned long long)(k * 2), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                tc5_commit(&empty_bar[s]);
+                if (kb + 1 == kb1) tc5_commit(acc_bar);
+            }
+            if (++s == stages) { s = 0; phase ^= 1u; }
+        }
+    }
+    const unsigned tmem = tmem_base + ((unsigned)(quarter * 32) << 16);
+    const int cols = min(bt, (e.M - t0 + CHUNK - 1) / CHUNK * CHUNK);          // columns that hold rows of a (bt is a multiple of 16)
+    auto wait_sums = [&] {
+        const bool there = warp_wait(acc_bar, 0);
+        if (!there) atomicOr(failed, 8);
+        tc5_fence_after();
+        return there;
+    };
+    if (splits == 1) {
+        if (warp >= 2)
+            finish_chunks<TO, ACT, GATED>(e, n, scales, sw, b, t0, t0 + bt, half, cols, wait_sums,
+                                    [&](int c0, float (&v)[CHUNK]) { load_tmem(tmem + (unsigned)c0, v); });
+    } else {
+        // Parts as the block that finishes them reads them: by block of K, by four columns, by row, four columns of 4 bytes.
+        const int share = (cols / CHUNK + splits - 1) / splits * CHUNK;        // columns a block finishes
+        if (warp >= 2) wait_sums();
+        __syncthreads();
+        cluster_sync();                                      // nobody multiplies from its ring any more
+        if (warp >= 2) {
+            const unsigned base = smem_u32(smem);
+#pragma unroll 1
+            for (int c0 = half * CHUNK; c0 < cols; c0 += 2 * CHUNK) {
+                float v[CHUNK];
+                load_tmem(tmem + (unsigned)c0, v);
+                const int owner = c0 / share;
+                const unsigned to = map_to_rank(base, (unsigned)owner) + (unsigned)(((rank * share + c0 - owner * share) * ROWS + 4 * row) * 4);
+#pragma unroll
+                for (int c = 0; c < CHUNK; c += 4)
+                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};"
+                                 ::"r"(to + (unsigned)(c * ROWS * 4)), "f"(v[c]), "f"(v[c + 1]), "f"(v[c + 2]), "f"(v[c + 3]) : "memory");
+            }
+        }
+        tc5_fence_before();
+        __syncwarp();
+        const int first = rank * share, mine = min(cols - first, share);
+        const float* part = reinterpret_cast<const float*>(smem) + 4 * row;
+        if (warp < 2) {
+            cluster_sync();
+        } else {
+            finish_chunks<TO, ACT, GATED>(
+                e, n, scales + first, sw, b, t0 + first, t0 + bt, half, mine,
+                [&] {
+                    cluster_sync();
+                    return true;
+                },
+                [&](int c0, float (&v)[CHUNK]) {
+#pragma unroll
+                    for (int c = 0; c < CHUNK; ++c) v[c] = 0.f;
+#pragma unroll 1
+                    for (int r = 0; r < splits; ++r)
+#pragma unroll
+                        for (int c = 0; c < CHUNK; c += 4) {
+                            const float4 q = *reinterpret_cast<const float4*>(part + (r * share + c0 + c) * ROWS);
+                            v[c] += q.x; v[c + 1] += q.y; v[c + 2] += q.z; v[c + 3] += q.w;
+                        }
+                });
+        }
+    }
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    if (warp == 1) tc5_dealloc(tmem_base, tmem_cols);
+    if (threadIdx.x == 0 && *failed && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_GEMM_8BIT | ((unsigned)*failed << VL_DEV_ROLE_SHIFT));
+}
+}  // namespace split8
+
+// ---- few rows (a decode step): W's stream is all that counts ------------------------------------------
+// A block walks tiles of NS strips of 16 rows of W.  A warp brings them in, with the rows of a they meet, through a ring of stages that
+// goes on across tiles: 8 / NS blocks of K of every strip (they lie one behind the other: a bulk copy a strip; W is a constant, so its first copies
+// begin before the kernel in front has ended).  Eight warps multiply, each a block of K of a strip.  mma.sync m16n8k32 pairs operand
+// elements by their index along K and mixes no rows, so the bytes a lane holds may stand for any columns as long as both operands
+// agree: pieces t and t + 4 of W's row against pieces t and t + 4 of the row of a, 16 bytes at a time.  Row (column) g of the instruction
+// is W's (a's) row (g >> 1) + 4 (g & 1): eight neighbouring lanes then read all 32 banks (rows 0 and 4 have their pieces exchanged by 4).
+// The sums of a strip's warps are added in their order; a thread asks for its outputs' scales, bias and residual when the tile begins.
+namespace few8 {
+constexpr int WARPS = 8;
+constexpr unsigned BLOCK_BYTES = STRIP * KB;
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_16832(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Who gives up notes that for the block and goes on as if the stage were there; from then on nobody waits long, and no lane leaves a loop by itself.
+__device__ __forceinline__ void wait_or_note(unsigned long long* bar, unsigned parity, volatile int* gave_up) {
+    if (mbar_try_wait(bar, parity)) return;
+    const long long t0 = clock64();
+    for (int i = 0; i < VL_WAIT_POLL_LIMIT; ++i) {
+        if (mbar_try_wait(bar, parity)) return;
+        if ((i & 31) == 31 && (*gave_up || vl_wait_gave_up(i, t0))) break;
+    }
+    *gave_up = 1;
+}
+
+// MT: rows of a in eights, NS: strips of a tile
+template <int MT, int NS> struct Shape {
+    static constexpr int DEEP = WARPS / NS;                   // blocks of K of a stage
+    static constexpr unsigned W_STRIP = DEEP * BLOCK_BYTES, A_OFF = NS * W_STRIP, A_BYTES = DEEP * MT * 8 * KB, STAGE_BYTES = A_OFF + A_BYTES;
+    static constexpr int OUTS = MT * NS > 2 ? MT * NS / 2 : 1;       // outputs of a thread
+    // the sums of a tile's warps: twice, so that a tile's are added while the next tile's arrive, where two blocks of an SM leave the room
+    static constexpr int BUFS = MT <= 2 ? 2 : 1;
+    typedef float Sums[DEEP][MT * 8][NS * STRIP + 1];
+    static constexpr unsigned smem(int stages) { return stages * STAGE_BYTES + BUFS * (unsigned)sizeof(Sums) + 16 * stages + 16; }
+};
+
+template <typename TO, int MT, int NS, int STAGES, int PER_SM>
+__global__ void __launch_bounds__(32 * WARPS + 32, PER_SM)
+gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned char* __restrict__ W, Epilogue e, int k_blocks, int strips, unsigned* err) {
+    using S = Shape<MT, NS>;
+    constexpr int DEEP = S::DEEP, OUTS = S::OUTS;
+    extern __shared__ __align__(1024) unsigned char ring[];   // (nothing else is shared: it begins on a kilobyte)
+    typename S::Sums* red = reinterpret_cast<typename S::Sums*>(ring + STAGES * S::STAGE_BYTES);
+    unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(red + S::BUFS);
+    unsigned long long* empty_bar = full_bar + STAGES;
+    volatile int& gave_up = *reinterpret_cast<volatile int*>(empty_bar + STAGES);
+    const int warp = warp_number(), lane = threadIdx.x & 31;
+    const int per_tile = (k_blocks + DEEP - 1) / DEEP;
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        gave_up = 0;
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], WARPS); }
+        mbar_fence_init();
+    }
+    __syncthreads();
+    if (warp == WARPS) {                                      // ---- copies ----
+        if (elect_one()) {
+            auto copy_w = [&](int s, int strip, int it) {
+                const unsigned bytes = (unsigned)min(DEEP, k_blocks - it * DEEP) * BLOCK_BYTES;
+                mbar_arrive_expect_tx(&full_bar[s], bytes * (unsigned)min(NS, strips - strip) + S::A_BYTES);
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+                    if (strip + i < strips)
+                        bulk_copy(ring + (size_t)s * S::STAGE_BYTES + i * S::W_STRIP, W + ((size_t)(strip + i) * k_blocks + it * DEEP) * BLOCK_BYTES, bytes,
+                                  &full_bar[s]);
+            };
+            auto copy_a = [&](int s, int it) { tma_load_3d(ring + (size_t)s * S::STAGE_BYTES + S::A_OFF, &map_a, 0, 0, it * DEEP, &full_bar[s]); };
+            const int mine = (strips - (int)blockIdx.x * NS + (int)gridDim.x * NS - 1) / ((int)gridDim.x * NS), total = mine * per_tile;
+            const int early = min(STAGES, total);
+            int strip = blockIdx.x * NS, it = 0;
+            auto step = [&]() { if (++it == per_tile) { it = 0; strip += gridDim.x * NS; } };
+            for (int s = 0; s < early; ++s, step()) copy_w(s, strip, it);
+            pdl_wait();                                       // a comes from the kernel before
+            for (int s = 0; s < early; ++s) copy_a(s, s % per_tile);
+            int s = 0;
+            unsigned phase = 0;
+            for (int i = early; i < total; ++i, step()) {
+                if (!mbar_wait_bounded(&empty_bar[s], phase)) {
+                    gave_up = 1;
+                    break;
+                }
+                copy_w(s, strip, it);
+                copy_a(s, it);
+                if (++s == STAGES) { s = 0; phase ^= 1u; }
+            }
+        }
+        return;
+    }
+    pdl_wait();
+    const int deep = warp % DEEP, mine = warp / DEEP;         // this warp's block of a stage's K, and its strip
+    const int g = lane >> 2, t = lane & 3, row = (g >> 1) | ((g & 1) << 2);
+    const int at = row * 128 + ((t ^ row) << 4);              // piece t of the row in a block of K; piece t + 4 is this xor 64
+    const int each = NS * (e.gated ? STRIP / 2 : STRIP), ld = e.gated ? e.N >> 1 : e.N;
+    TO* out = reinterpret_cast<TO*>(e.out);
+    const TO* res = reinterpret_cast<const TO*>(e.residual);
+    int s = 0, buf = 0;
+    unsigned phase = 0;
+    for (int strip = blockIdx.x * NS; strip < strips; strip += gridDim.x * NS, buf = (buf + 1) % S::BUFS) {
+        // only asked for here: a use would wait for memory
+        float am[OUTS], ws[OUTS], wb[OUTS], us[OUTS], ub[OUTS];
+        TO yr[OUTS];
+#pragma unroll
+        for (int o = 0; o < OUTS; ++o) {
+            const int i = threadIdx.x + o * 32 * WARPS, m = i / each, c = i % each, col = strip * (each / NS) + c;
+            const int n = strip * STRIP + (e.gated ? 2 * c - (c & 7) : c);      // gated: eight gates, their eight ups, ...
+            am[o] = ws[o] = wb[o] = us[o] = ub[o] = 0.f;
+            yr[o] = from_f32<TO>(0.f);
+            if (m < e.M && col < ld) {
+                am[o] = e.a_scale[m];
+                ws[o] = e.w_scale[n];
+                if (e.bias) wb[o] = e.bias[n];
+                if (e.gated) {
+                    us[o] = e.w_scale[n + 8];
+                    if (e.bias) ub[o] = e.bias[n + 8];
+                }
+                if (res) yr[o] = res[(size_t)m * ld + col];
+            }
+        }
+        float acc[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT * 4; ++i) (&acc[0][0])[i] = 0.f;
+        for (int it = 0; it < per_tile; ++it) {
+            wait_or_note(&full_bar[s], phase, &gave_up);
+            if (it * DEEP + deep < k_blocks) {                // (a strip that is not there left the stage as it was: nothing of it is stored)
+                const unsigned char* w = ring + (size_t)s * S::STAGE_BYTES + mine * S::W_STRIP + deep * BLOCK_BYTES;
+                const unsigned char* a = ring + (size_t)s * S::STAGE_BYTES + S::A_OFF + deep * (MT * 8 * KB);
+                const uint4 l0 = *reinterpret_cast<const uint4*>(w + at), h0 = *reinterpret_cast<const uint4*>(w + at + 1024);
+                const uint4 l1 = *reinterpret_cast<const uint4*>(w + (at ^ 64)), h1 = *reinterpret_cast<const uint4*>(w + (at ^ 64) + 1024);
+                uint4 x0[MT], x1[MT];
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    x0[j] = *reinterpret_cast<const uint4*>(a + j * 1024 + at);
+                    x1[j] = *reinterpret_cast<const uint4*>(a + j * 1024 + (at ^ 64));
+                }
+#pragma unroll
+                for (int j = 0; j < MT; ++j) mma_16832(acc[j], l0.x, h0.x, l0.y, h0.y, x0[j].x, x0[j].y);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) mma_16832(acc[j], l0.z, h0.z, l0.w, h0.w, x0[j].z, x0[j].w);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) mma_16832(acc[j], l1.x, h1.x, l1.y, h1.y, x1[j].x, x1[j].y);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) mma_16832(acc[j], l1.z, h1.z, l1.w, h1.w, x1[j].z, x1[j].w);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty_bar[s]);
+            if (++s == STAGES) { s = 0; phase ^= 1u; }
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {                        // acc: (row g, columns 2t and 2t + 1), (row g + 8, the same): rows t and t + 4 of a
+            red[buf][deep][8 * j + t][mine * STRIP + row] = acc[j][0];
+            red[buf][deep][8 * j + t + 4][mine * STRIP + row] = acc[j][1];
+            red[buf][deep][8 * j + t][mine * STRIP + row + 8] = acc[j][2];
+            red[buf][deep][8 * j + t + 4][mine * STRIP + row + 8] = acc[j][3];
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+#pragma unroll
+        for (int o = 0; o < OUTS; ++o) {
+            const int i = threadIdx.x + o * 32 * WARPS, m = i / each, c = i % each, col = strip * (each / NS) + c;
+            if (m >= e.M || col >= ld) continue;
+            const int place = e.gated ? 2 * c - (c & 7) : c;
+            float y = 0.f, u = 0.f;
+#pragma unroll
+            for (int v = 0; v < DEEP; ++v) y += red[buf][v][m][place];
+            y = y * (am[o] * ws[o]) + wb[o];
+            if (e.gated) {
+#pragma unroll
+                for (int v = 0; v < DEEP; ++v) u += red[buf][v][m][place + 8];
+                y = activate(y, e.act) * (u * (am[o] * us[o]) + ub[o]);
+            } else {
+                y = activate(y, e.act);
+            }
+            out[(size_t)m * ld + col] = from_f32<TO>(y + to_f32(yr[o]));
+        }
+        if (S::BUFS == 1) asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+    }
+    if (threadIdx.x == 0 && gave_up && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_GEMM_8BIT);
+}
+}  // namespace few8
+
 // ---- host side --------------------------------------------------------------------------------------
 // rows [M, width] in boxes of `box` rows x 128 bytes with the 128-byte swizzle
 static int map_rows(CUtensorMap* map, const void* a, int M, int width, int box_rows) {
@@ -262,6 +650,16 @@ static int map_rows(CUtensorMap* map, const void* a, int M, int width, int box_r
     cuuint64_t strides[1] = {(cuuint64_t)width};
     cuuint32_t box[2] = {(cuuint32_t)KB, (cuuint32_t)box_rows}, estr[2] = {1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(a), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : VL_ERR_ARGUMENT;
+}
+// the same rows as (128 columns, rows, blocks of 128 columns): a box brings `deep` blocks of `box_rows` rows, block after block
+static int map_row_blocks(CUtensorMap* map, const void* a, int M, int width, int box_rows, int deep) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return VL_ERR_UNSUPPORTED;
+    cuuint64_t dims[3] = {(cuuint64_t)KB, (cuuint64_t)M, (cuuint64_t)(width / KB)};
+    cuuint64_t strides[2] = {(cuuint64_t)width, (cuuint64_t)KB};
+    cuuint32_t box[3] = {(cuuint32_t)KB, (cuuint32_t)box_rows, (cuuint32_t)deep}, estr[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(a), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : VL_ERR_ARGUMENT;
 }
 // packed strips in boxes of 8 strips x 16 rows x 128 bytes: 128 rows of one block of K, already in the swizzle's order
@@ -285,18 +683,18 @@ static int sm_count() {
     return num_sms;
 }
 
-template <typename TO, int MODE>
-static int launch_pair(const void* a, const void* w, const Epilogue& e, int width, unsigned* err, cudaStream_t s) {
+template <typename TO, int ACT, bool GATED>
+static int launch_pair(const void* a, const void* w, const Epilogue& e, int width, int bt, unsigned* err, cudaStream_t s) {
     const size_t smem = (size_t)pair8::STAGES * pair8::STAGE_BYTES + 1024;
-    auto kern = pair8::gemm_8bit_pair_kernel<TO, MODE>;
+    auto kern = pair8::gemm_8bit_pair_kernel<TO, ACT, GATED>;
     // first of all: a thread that has made no call yet has no context, and a tensor map wants one
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (ce != cudaSuccess) return (int)ce;
     CUtensorMap map_a, map_w;
-    int rc = map_rows(&map_a, a, e.M, width, pair8::BT / 2);
+    int rc = map_rows(&map_a, a, e.M, width, bt / 2);
     if (!rc) rc = map_strips(&map_w, w, e.N, width / KB);
     if (rc) return rc;
-    const int tiles_t = (e.M + pair8::BT - 1) / pair8::BT, tiles_n = (e.N + 2 * ROWS - 1) / (2 * ROWS);
+    const int tiles_t = (e.M + bt - 1) / bt, tiles_n = (e.N + 2 * ROWS - 1) / (2 * ROWS);
     const int total = tiles_t * tiles_n, pairs = sm_count() / 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (total < pairs ? total : pairs));
@@ -309,14 +707,137 @@ static int launch_pair(const void* a, const void* w, const Epilogue& e, int widt
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_w, e, width / KB, tiles_t, tiles_n, err);
+    return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_w, e, width / KB, bt, tiles_t, tiles_n, err);
+}
+
+constexpr unsigned SPLIT_ROOM = 232448;      // the most shared memory of a block
+template <typename TO, int ACT, bool GATED, int PER_SM>
+static int launch_split(const void* a, const void* w, const Epilogue& e, int width, int bt, int splits, unsigned* err, cudaStream_t s) {
+    // what an SM's 228 KB leave a block, less 1 KB that the system keeps of it, in stages; behind them barriers, a few words and the scales
+    const unsigned stage = W_BYTES + (unsigned)(bt * KB), beside = 2048, room = (PER_SM == 2 ? 115712u : SPLIT_ROOM) - beside;
+    const int stages = (int)(room / stage) < 12 ? (int)(room / stage) : 12;
+    const size_t smem = stages * stage + beside;
+    while (splits > 1 && (size_t)stages * stage < (size_t)(bt / CHUNK + splits - 1) * CHUNK * ROWS * 4) --splits;       // the parts' room
+    auto kern = split8::gemm_8bit_split_kernel<TO, ACT, GATED, PER_SM>;
+    cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (ce != cudaSuccess) return (int)ce;
+    CUtensorMap map_a, map_w;
+    int rc = map_rows(&map_a, a, e.M, width, bt);
+    if (!rc) rc = map_strips(&map_w, w, e.N, width / KB);
+    if (rc) return rc;
+    const int tiles_t = (e.M + bt - 1) / bt, tiles_n = (e.N + ROWS - 1) / ROWS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles_t * tiles_n * splits);
+    cfg.blockDim = dim3(split8::NUM_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    // as the paired product, never as a programmatic dependent
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_w, e, width / KB, bt, tiles_t, splits, stages, err);
+}
+template <typename TO, int MT, int NS, int STAGES, int PER_SM>
+static int launch_few(const void* a, const void* w, const Epilogue& e, int width, unsigned* err, cudaStream_t s) {
+    const size_t smem = few8::Shape<MT, NS>::smem(STAGES);
+    auto kern = few8::gemm_8bit_few_kernel<TO, MT, NS, STAGES, PER_SM>;
+    cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (ce != cudaSuccess) return (int)ce;
+    CUtensorMap map_a;
+    if (int rc = map_row_blocks(&map_a, a, e.M, width, MT * 8, few8::Shape<MT, NS>::DEEP)) return rc;
+    const int strips = (e.N + STRIP - 1) / STRIP, tiles = (strips + NS - 1) / NS, places = PER_SM * sm_count();
+    return vl_launch(kern, dim3(tiles < places ? tiles : places), dim3(32 * few8::WARPS + 32), smem, s, map_a, (const unsigned char*)w, e, width / KB,
+                     strips, err);
+}
+// Blocks of clusters of `splits` that run at the same time, one an SM: a cluster lies within a group of SMs, and clusters of 3 leave some idle.
+static int cluster_places(int splits) {
+    static int known[9] = {};
+    if (splits <= 1) return sm_count();
+    if (!known[splits]) {
+        auto kern = split8::gemm_8bit_split_kernel<bf16, ACT_NONE, false, 1>;
+        const size_t smem = SPLIT_ROOM;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(splits);
+        cfg.blockDim = dim3(split8::NUM_THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess || clusters <= 0)
+            clusters = sm_count() / (2 * splits);
+        known[splits] = clusters * splits;
+    }
+    return known[splits];
+}
+
+// Which kernel and tile for more than 16 rows: what it would take, in cycles of an SM.  An SM takes 64 bytes a cycle in, and that, not the tensor cores,
+// paces a block of K (128 rows of W and its rows of a: 256 + 2 bt cycles, half of a for each block of a pair, 384 at least); tiles run in rounds of the SMs, W
+// comes at the memory's pace, and the two together take the root of the sum of their squares (x 12,288 -> 4,096, 24 rows on 32, 64, 96, 128 SMs: 17.5, 11.5,
+// 9.0 and 8.2 us beside the start, 18.0, 11.3, 9.5 and 8.8 by this).  Beside it a start (6,300, pairs 9,500,
+// and 2,500 for each further round of pairs or of blocks two an SM), 23 a column of the epilogue that no products
+// hide, and where K is cut a barrier (1,500) and 50 for each column that goes to another block.
+struct Plan {
+    int pair, bt, splits, per_sm;
+};
+static Plan plan_of(int M, int N, int k_blocks) {
+    const int sms = sm_count();
+    const double stream = (double)N * k_blocks * KB / 3370;
+    Plan best{1, 256, 1, 1};
+    double least = -1;
+    for (int tall : {256, 224, 192, 160, 128, 96, 64, 32}) {
+        const int tiles_t = (M + tall - 1) / tall, each = (M + tiles_t - 1) / tiles_t;
+        if (tall >= 128) {
+            const int bt = (each + 31) / 32 * 32;
+            const long long rounds = ((long long)tiles_t * ((N + 2 * ROWS - 1) / (2 * ROWS)) + sms / 2 - 1) / (sms / 2);
+            const double paced = (double)rounds * k_blocks * (bt > 128 ? 256 + bt : 384), cost = 9500 + 2500 * (double)(rounds - 1) + sqrt(paced * paced + stream * stream) + 23 * bt;
+            if (least < 0 || cost < least) { least = cost; best = {1, bt, 1, 1}; }
+        }
+        const int bt = (each + 15) / 16 * 16;
+        const long long tiles = (long long)tiles_t * ((N + ROWS - 1) / ROWS);
+        if (tiles > 4 * sms) continue;
+        for (int splits = 1; splits <= 8 && 2 * splits <= k_blocks + 1; ++splits) {
+            const int places = cluster_places(splits), share = (bt / CHUNK + splits - 1) / splits * CHUNK;
+            const long long rounds = (tiles * splits + places - 1) / places;
+            const double paced = (double)rounds * ((k_blocks + splits - 1) / splits) * (256 + 2 * bt);
+            const double cost = 6300 + 2500 * (double)((rounds + 1) / 2 - 1) + sqrt(paced * paced + stream * stream) + 23 * share + (splits > 1 ? 1500 + 50 * (bt - share) : 0);
+            // two blocks an SM where there are more blocks than SMs, or little of a in a stage (24 rows: 13.7 us and 14.5; 64 rows 14.8 and 14.5)
+            if (cost < least) { least = cost; best = {0, bt, splits, bt <= 160 && (rounds > 1 || bt <= 32) ? 2 : 1}; }
+        }
+    }
+    return best;
+}
+
+template <typename TO, int ACT, bool GATED>
+static int launch_many(const void* a, const void* w, const Epilogue& e, int width, unsigned* err, cudaStream_t s) {
+    const Plan p = plan_of(e.M, e.N, width / KB);
+    if (p.pair) return launch_pair<TO, ACT, GATED>(a, w, e, width, p.bt, err, s);
+    return p.per_sm == 2 ? launch_split<TO, ACT, GATED, 2>(a, w, e, width, p.bt, p.splits, err, s) : launch_split<TO, ACT, GATED, 1>(a, w, e, width, p.bt, p.splits, err, s);
 }
 
 template <typename TO>
 static int launch(const void* a, const void* w, const Epilogue& e, int width, unsigned* err, cudaStream_t s) {
-    if (e.gated) return launch_pair<TO, 2>(a, w, e, width, err, s);
-    if (e.act != ACT_NONE) return launch_pair<TO, 1>(a, w, e, width, err, s);
-    return launch_pair<TO, 0>(a, w, e, width, err, s);
+    // Up to 8 rows: strips one by one, four stages of 16 + 8 KB and two blocks an SM.  Up to 16: in twos where that leaves more tiles than SMs (each
+    // strip's copy of a is half the bytes then: x 4,096 -> 24,576 19.3 us and 24.8, -> 6,144 6.9 and 9.1), else one by one with two stages and
+    // three blocks an SM (x 12,288 -> 4,096 12.2 and 14.6).
+    if (e.M <= 8) return launch_few<TO, 1, 1, 4, 2>(a, w, e, width, err, s);
+    if (e.M <= 16)
+        return (e.N + 2 * STRIP - 1) / (2 * STRIP) > sm_count() ? launch_few<TO, 2, 2, 4, 2>(a, w, e, width, err, s) : launch_few<TO, 2, 1, 2, 3>(a, w, e, width, err, s);
+    if (e.gated) return e.act == ACT_SILU ? launch_many<TO, ACT_SILU, true>(a, w, e, width, err, s) : launch_many<TO, ACT_RELU, true>(a, w, e, width, err, s);
+    switch (e.act) {
+        case ACT_NONE: return launch_many<TO, ACT_NONE, false>(a, w, e, width, err, s);
+        case ACT_SILU: return launch_many<TO, ACT_SILU, false>(a, w, e, width, err, s);
+        case ACT_RELU: return launch_many<TO, ACT_RELU, false>(a, w, e, width, err, s);
+        case ACT_RELU2: return launch_many<TO, ACT_RELU2, false>(a, w, e, width, err, s);
+        case ACT_TANH: return launch_many<TO, ACT_TANH, false>(a, w, e, width, err, s);
+        case ACT_GELU: return launch_many<TO, ACT_GELU, false>(a, w, e, width, err, s);
+        default: return VL_ERR_UNSUPPORTED;
+    }
 }
 
 extern "C" int vl_gemm_8bit(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out, int out_dtype, const float* bias,
@@ -324,6 +845,8 @@ extern "C" int vl_gemm_8bit(const void* a, const float* a_scale, const void* w, 
     if (M <= 0 || N <= 0) return VL_OK;
     if (width <= 0 || width % KB || (gated && N % 16)) return VL_ERR_ARGUMENT;
     if (((uintptr_t)a | (uintptr_t)w) & 15) return VL_ERR_UNSUPPORTED;
+    if (gated ? act != ACT_SILU && act != ACT_RELU : act != ACT_NONE && act != ACT_SILU && act != ACT_RELU && act != ACT_RELU2 && act != ACT_TANH && act != ACT_GELU)
+        return VL_ERR_UNSUPPORTED;
     const Epilogue e{a_scale, w_scale, bias, residual, out, M, N, act, gated};
     if (out_dtype == VL_BF16) return launch<bf16>(a, w, e, width, err, (cudaStream_t)stream);
     if (out_dtype == VL_F32) return launch<float>(a, w, e, width, err, (cudaStream_t)stream);
