@@ -87,12 +87,15 @@ class ClockSampler:
         return {"sm_mhz": mhz[len(mhz) // 2], "sm_max_mhz": int(rows[0][1]), "reasons": reasons, "samples": len(rows)}
 
 
-def model_bytes_and_flops(cfg, layers):
+def model_bytes_and_flops(cfg, layers, eight_bit=False):
+    """eight_bit: the layers' matrices are one byte an element and a float32 scale a row."""
     H, I, V = cfg["hidden_size"], cfg["intermediate_size"], cfg["vocab_size"]
     nq, nkv, hd = cfg["num_attention_heads"], cfg["num_key_value_heads"], cfg["head_dim"]
     per_layer = (nq + 2 * nkv) * hd * H + H * nq * hd + 3 * H * I          # matrix elements of one layer
     norms = layers * (2 * H + 2 * hd) + H
     weight_bytes = 2 * (layers * per_layer + V * H) + 4 * norms            # bf16 matrices, every one read once
+    if eight_bit:
+        weight_bytes -= layers * (per_layer - 4 * ((nq + 2 * nkv) * hd + 2 * H + 2 * I))
     kv_bytes_per_token = layers * 2 * nkv * hd * 2
     T = PREFILL_TOKENS
     prefill_flops = 2 * T * layers * per_layer + layers * 4 * nq * hd * (T * (T + 1) // 2) + 2 * V * H
@@ -1343,6 +1346,7 @@ def main(argv=None):
     ap.add_argument("--context", type=int, default=4096)
     ap.add_argument("--size", default="8b", choices=sorted(SIZES), help="layer sizes of Qwen3-8B (default), 14B or 32B")
     ap.add_argument("--layers", type=int, default=None, help="fewer layers than the size has (both numbers are reported)")
+    ap.add_argument("--eight-bit", action="store_true", help="the layers' linear products in 8 bits (weights and activations)")
     ap.add_argument("--block-size", type=int, default=64, help="positions per page of the cache")
     ap.add_argument("--no-points", action="store_true", help="skip the batch 1 / 64 points and the prefill")
     ap.add_argument("--only-prefill", action="store_true", help="time the 2,048-token prefill alone (for profiling)")
@@ -1413,19 +1417,20 @@ def main(argv=None):
     if args.read_ceiling:
         return read_ceiling(cfg, args.batch, args.context)
     _, plan, weights = random_model(cfg, seed=0, dtype="bfloat16", device="cuda:0")
+    dtype = "bf16, layers' products in e4m3" if args.eight_bit else "bf16"
     if args.continuous:
         R, out_len, prompt_range = args.continuous, 512, (256, args.context // 2)
         pages = R * (-(-(prompt_range[1] + out_len) // args.block_size) + 1) + 64
         engine = LLMEngine(plan=plan, weights=weights, dtype="bfloat16", kv_blocks=pages, block_size=args.block_size, max_batch_size=R,
-                           max_num_batched_tokens=4096, prefill_chunk_size=512, max_model_len=args.context)
+                           max_num_batched_tokens=4096, prefill_chunk_size=512, max_model_len=args.context, eight_bit=args.eight_bit)
         del weights
         continuous_run(engine, min(R, 4), vocab, (256, 512), 16)          # warm-up: builds, graphs of the small buckets
         clocks = ClockSampler().start()
         w0 = time.time()
         out = continuous_run(engine, R, vocab, prompt_range, out_len)
         clocks.stop()
-        out = {"metric": f"continuous batching, generated tok/s (Qwen3-{args.size.upper()}, bf16)", **out, "n_gpus": 1,
-               "dtype": "bf16", "data": "synthetic (random weights N(0,0.02), uniform token ids)",
+        out = {"metric": f"continuous batching, generated tok/s (Qwen3-{args.size.upper()}, {dtype})", **out, "n_gpus": 1,
+               "dtype": dtype, "data": "synthetic (random weights N(0,0.02), uniform token ids)",
                "config": {"model": f"Qwen3-{args.size.upper()} layer sizes", "layers": args.layers, "layers_full": full_layers,
                           "context": args.context, "prompt_lengths": f"uniform in [{prompt_range[0]}, {prompt_range[1]}]",
                           "generated_each": out_len, "block_size": args.block_size, "max_num_batched_tokens": 4096,
@@ -1444,12 +1449,12 @@ def main(argv=None):
         pages = int(args.kv_blocks)
     engine = LLMEngine(plan=plan, weights=weights, dtype="bfloat16", kv_blocks=pages, block_size=args.block_size, max_batch_size=big,
                        max_num_batched_tokens=PREFILL_TOKENS, prefill_chunk_size=PREFILL_TOKENS,
-                       max_model_len=args.context + slack)
+                       max_model_len=args.context + slack, eight_bit=args.eight_bit)
     del weights
     runner, sampler = engine.runner, engine.sampler
     for t in runner.storage.paged:                        # pages that no prompt wrote hold random numbers
         t.normal_()
-    weight_bytes, kv_per_token, prefill_flops = model_bytes_and_flops(cfg, args.layers)
+    weight_bytes, kv_per_token, prefill_flops = model_bytes_and_flops(cfg, args.layers, args.eight_bit)
     pk = peaks()
 
     if args.only_prefill:
@@ -1468,9 +1473,9 @@ def main(argv=None):
     step_bytes = weight_bytes + args.batch * mean_ctx * kv_per_token
     achieved = step_bytes / (ms * 1e-3) / 1e9
     out = {
-        "metric": METRIC.replace("8B", args.size.upper()).replace("batch 8", f"batch {args.batch}"), "value": round(value, 1), "unit": "tokens/s", "n_gpus": 1, "steps": args.steps,
+        "metric": METRIC.replace("8B", args.size.upper()).replace("batch 8", f"batch {args.batch}").replace("bf16", dtype), "value": round(value, 1), "unit": "tokens/s", "n_gpus": 1, "steps": args.steps,
         "warmup": warmup, "ms_per_step": round(ms, 4), "higher_is_better": True, "scaling": "weak",
-        "vs_baseline": None, "dtype": "bf16", "data": "synthetic (random weights N(0,0.02), uniform token ids)",
+        "vs_baseline": None, "dtype": dtype, "data": "synthetic (random weights N(0,0.02), uniform token ids)",
         "config": {"model": f"Qwen3-{args.size.upper()} layer sizes", "layers": args.layers, "layers_full": full_layers,
                    "hidden": cfg["hidden_size"], "heads": cfg["num_attention_heads"], "kv_heads": cfg["num_key_value_heads"],
                    "head_dim": cfg["head_dim"], "intermediate": cfg["intermediate_size"], "vocab": vocab,

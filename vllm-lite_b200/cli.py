@@ -62,6 +62,7 @@ def build_parser() -> argparse.ArgumentParser:
                     default=_env("VLLM_KV_QUANTIZATION", "false").lower() in ("1", "true"))
     ap.add_argument("--log-level", default=_env("VLLM_LOG_LEVEL", "info"))
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    ap.add_argument("--eight-bit", action="store_true", help="run the layers' linear products in 8 bits (weights and activations)")
     ap.add_argument("--block-size", type=_bounded(1, 256, "--block-size"), default=64,
                     help="positions per page of the cache (the reference's constant is 16; 64 suits the TMA copies)")
     ap.add_argument("--max-num-batched-tokens", type=int, default=4096)
@@ -116,7 +117,7 @@ def main(argv=None) -> int:
     engine = LLMEngine(args.model, dtype=args.dtype, kv_blocks=args.kv_blocks, block_size=args.block_size,
                        max_batch_size=args.max_batch_size, max_num_batched_tokens=args.max_num_batched_tokens,
                        prefill_chunk_size=args.prefill_chunk_size, max_model_len=args.max_model_len,
-                       gpu_memory_fraction=args.gpu_memory_fraction)
+                       gpu_memory_fraction=args.gpu_memory_fraction, eight_bit=args.eight_bit)
     if verbose:
         print(f"[vllm-lite_b200] model loaded in {time.time() - t0:.1f} s", file=sys.stderr)
     params = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,

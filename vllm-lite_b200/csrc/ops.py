@@ -1606,6 +1606,14 @@ def pack_8bit(w):
     return out
 
 
+GEMM_8BIT_FEW = 16                                                # most rows of the kernel that streams w alone
+
+
+def gemm_8bit_clusters(M) -> bool:
+    """Whether `gemm_8bit` of M rows may run as clusters of blocks, which are never launched as programmatic dependents."""
+    return M > GEMM_8BIT_FEW
+
+
 GEMM_8BIT_ACTIVATIONS = ("silu", "relu")                          # f(gate) * up
 GEMM_8BIT_UNARY = ("silu", "relu", "relu2", "tanh", "gelu")       # f(y)
 

@@ -170,7 +170,7 @@ class ModelRunner:
             logits = self._forward_graph(batch)[:sum(len(e.want) for e in entries)]
         else:
             from ..csrc import ops
-            ops.set_pdl(launches_dependent(batch.num_tokens, False, self.model.may_pair))
+            ops.set_pdl(self._launches_dependent(batch.num_tokens, False))
             logits = self.model.forward(batch, self.storage.call_caches)
         self.finish(batch)
         return logits
@@ -255,6 +255,12 @@ class ModelRunner:
         self.graph_replays += 1
         return entry[1][:B]
 
+    def _launches_dependent(self, tokens: int, recorded: bool) -> bool:
+        """`launches_dependent`, and no kernel of clusters among them: those are launched the plain way and stay among plain launches, as the
+        paired products do."""
+        clusters = getattr(self.model, "clusters", None)
+        return launches_dependent(tokens, recorded, self.model.may_pair) and not (clusters and clusters(tokens))
+
     def _forward_graph(self, batch: StepBatch) -> torch.Tensor:
         """Rows of padded requests come after the real ones, so the caller slices them off."""
         key = (batch.graph_bucket, batch.groups[0].max_context if batch.groups else 0)
@@ -262,7 +268,7 @@ class ModelRunner:
         if entry is None:
             # first sight of this bucket: run it as it is (also sizes the workspace), then record
             from ..csrc import ops
-            ops.set_pdl(launches_dependent(batch.num_tokens, True, self.model.may_pair))
+            ops.set_pdl(self._launches_dependent(batch.num_tokens, True))
             logits = self.model.forward(batch, self.storage.call_caches)
             torch.cuda.current_stream().synchronize()
             before = ops.launch_count

@@ -7,3 +7,5 @@ from .model import CausalLM, cache_needs, cache_sources, declare_model  # noqa: 
 from .registry import BLOCKS, EMBEDDINGS, FEED_FORWARDS, HEADS, MIXERS, NORMS, POSITIONS  # noqa: F401
 from . import recurrent, parallel, conv_attention, token_shift    # noqa: F401  (registration)
 from . import differential_attention, linear_recurrent            # noqa: F401  (registration)
+from . import eight_bit                                            # noqa: F401  (registration)
+from .eight_bit import in_8_bits                                   # noqa: F401

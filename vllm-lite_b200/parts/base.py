@@ -37,6 +37,8 @@ class BuildContext:
     dtype: torch.dtype            # activation / model dtype: torch.bfloat16 or torch.float32
     # what the parts add that may launch a product of paired blocks: tokens of a step -> whether it can be among its kernels
     paired: list = field(default_factory=list, compare=False)
+    # the same for kernels whose blocks work in clusters and that serve steps of few tokens too
+    clustered: list = field(default_factory=list, compare=False)
 
 
 class Workspace:

@@ -72,6 +72,10 @@ class CausalLM:
         from ..csrc import ops
         return tokens >= ops.TC5_MIN_M_FULL or any(asks(tokens) for asks in self.ctx.paired)
 
+    def clusters(self, tokens: int) -> bool:
+        """Whether a step of so many tokens can hold a kernel of `BuildContext.clustered` (csrc/gemm_8bit.cu)."""
+        return any(asks(tokens) for asks in self.ctx.clustered)
+
     def forward(self, step, caches, watch=None) -> torch.Tensor:
         """Logits float32 [len(step.logit_rows), vocab].  `watch(i, x)`, when given, is called after every entry of
         the running order with the stream brought up to date (a reader for tests and comparisons)."""
