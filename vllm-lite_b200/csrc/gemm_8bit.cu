@@ -134,24 +134,30 @@ __device__ __forceinline__ void finish(float (&v)[CHUNK], TO (&x)[CHUNK / (GATED
         if (c * STEP < p.rows) *o = from_f32<TO>(v[c]);
 }
 
-// The chunks of a warp, every second of a tile's (rows t0 + c0 .. of a, c0 < cols): what they are added to is asked for ahead, the first
+// The chunks of a warp, one of PARTS of a tile's (rows t0 + c0 .. of a, c0 < cols): what they are added to is asked for ahead, the first
 // before `ready` waits for the sums (-> whether they came), the others before the stores of the one in front; `sums(c0, v)` brings the sums.
 // Residual and out may be the same memory: a thread reads what it writes, and before.
-template <typename TO, int ACT, bool GATED, typename Ready, typename Sums>
-__device__ __forceinline__ bool finish_chunks(const Epilogue& e, int n, const float* scales, float sw, float b, int t0, int end, int half, int cols, Ready ready,
+template <typename TO, int ACT, bool GATED, int PARTS, typename Ready, typename Sums>
+__device__ __forceinline__ bool finish_chunks(const Epilogue& e, int n, const float* scales, float sw, float b, int t0, int end, int first, int cols, Ready ready,
                                               Sums sums) {
     TO x[Place<TO, GATED>::COUNT];
     end = min(end, t0 + cols);
-    int c0 = half * CHUNK;
+    int c0 = first * CHUNK;
     if (c0 < cols && e.residual) Place<TO, GATED>(e, n, t0 + c0, end).load(e, x);
     if (!ready()) return false;
 #pragma unroll 1
-    for (; c0 < cols; c0 += 2 * CHUNK) {
+    for (; c0 < cols; c0 += PARTS * CHUNK) {
         float v[CHUNK];
         sums(c0, v);
-        finish<TO, ACT, GATED>(v, x, n, t0 + c0, end, t0 + c0 + 2 * CHUNK, e, scales + c0, sw, b);
+        finish<TO, ACT, GATED>(v, x, n, t0 + c0, end, t0 + c0 + PARTS * CHUNK, e, scales + c0, sw, b);
     }
     return true;
+}
+
+// The last copies that a block issued, of `issued` through a ring of `stages`, have arrived (or each had its time): no block leaves with copies on
+// their way into its shared memory, whatever happened to those who wait for them.  One thread; a fill nobody has waited for yet is no hurry.
+__device__ __forceinline__ void see_copies_in(unsigned long long* full_bar, int issued, int stages) {
+    for (int j = max(0, issued - stages); j < issued; ++j) mbar_wait_bounded(&full_bar[j % stages], (unsigned)((j / stages) & 1));
 }
 
 constexpr int STRIP = 16, KB = 128;          // a strip of W, a block of K: 128 bytes
@@ -161,7 +167,7 @@ constexpr unsigned W_BYTES = ROWS * KB;
 
 // ---- many rows: two SMs on a tile of 256 rows of W by 256 rows of a ---------------------------------
 namespace pair8 {
-constexpr int MOST = 256, STAGES = 6, NUM_THREADS = 64 + 256;
+constexpr int MOST = 256, STAGES = 6, PARTS = 4, EPILOGUE = PARTS * 128, NUM_THREADS = 64 + EPILOGUE;
 constexpr unsigned STAGE_BYTES = W_BYTES + MOST / 2 * KB, TMEM_COLS = 512;
 
 __device__ __forceinline__ void tile_corner(int tile, int tiles_t, int tiles_n, int bt, int& t0, int& n0) {
@@ -188,20 +194,24 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full_bar[i], 1); mbar_init(&acc_empty_bar[i], 2 * 256); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full_bar[i], 1); mbar_init(&acc_empty_bar[i], 2 * EPILOGUE); }
         mbar_fence_init();
         failed = 0;
     }
-    if (warp == 1) alloc_pair(&tmem_base_slot, TMEM_COLS);
-    tc5_fence_before();
     __syncthreads();
     cluster_sync();                                          // the other block's mbarriers exist before anything arrives there
-    tc5_fence_after();
-    const unsigned tmem_base = tmem_base_slot;
+    unsigned tmem_base = 0;
+    if (warp > 0) {                                          // tensor memory comes while the first copies are under way
+        if (warp == 1) alloc_pair(&tmem_base_slot, TMEM_COLS);
+        tc5_fence_before();
+        asm volatile("bar.sync 2, %0;" ::"n"(NUM_THREADS - 32) : "memory");
+        tc5_fence_after();
+        tmem_base = tmem_base_slot;
+    }
 
     if (warp == 0) {                                         // ---- copies ----
         const bool lead = elect_one();
-        int s = 0;
+        int s = 0, issued = 0;
         unsigned phase = 1;
         bool ok = true;
         for (int tile = pair; tile < total_tiles && ok; tile += num_pairs) {
@@ -221,9 +231,12 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                     tma_load_3d_pair(st, &map_w, 0, kb * STRIP, strip, bar);
                     tma_load_2d_pair(st + W_BYTES, &map_a, kb * KB, row, bar);
                 }
+                ++issued;
                 if (++s == STAGES) { s = 0; phase ^= 1u; }
             }
         }
+        if (lead && rank == 0) see_copies_in(full_bar, issued, STAGES);          // both blocks' (the other waits at the last barrier)
+        __syncwarp();
     } else if (warp == 1) {
         if (rank == 0) {                                     // ---- the pair's products ----
             const bool lead = elect_one();
@@ -259,8 +272,8 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 }
             }
         }
-    } else {                                                 // ---- epilogue: warps 2..9 ----
-        const int quarter = warp & 3, half = (warp - 2) >> 2, lane = threadIdx.x & 31;
+    } else {                                                 // ---- epilogue: warps 2..17 ----
+        const int quarter = warp & 3, part = (warp - 2) >> 2, lane = threadIdx.x & 31;
         const unsigned freed = map_to_rank(smem_u32(&acc_empty_bar[0]), 0);
         int local = 0;
         for (int tile = pair; tile < total_tiles; tile += num_pairs, ++local) {
@@ -270,20 +283,19 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             const int n = n0 + (int)rank * ROWS + quarter * 32 + lane;
             const float sw = n < e.N ? e.w_scale[n] : 0.f, b = e.bias && n < e.N ? e.bias[n] : 0.f;
             const int i = threadIdx.x - 64;                  // (who read this place last has passed the barrier of the tile between)
-            scales[acc][i] = t0 + i < e.M ? e.a_scale[t0 + i] : 0.f;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (i < MOST) scales[acc][i] = t0 + i < e.M ? e.a_scale[t0 + i] : 0.f;
+            asm volatile("bar.sync 1, %0;" ::"n"(EPILOGUE) : "memory");
             const unsigned tmem = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * MOST);
-            if (!finish_chunks<TO, ACT, GATED>(
-                    e, n, scales[acc], sw, b, t0, t0 + bt, half, min(bt, e.M - t0),
+            // no warp leaves the tiles before the others: they meet at the barrier above.  Where a wait ran out, nobody waits any more.
+            if (!finish_chunks<TO, ACT, GATED, PARTS>(
+                    e, n, scales[acc], sw, b, t0, t0 + bt, part, min(bt, e.M - t0),
                     [&] {
-                        const bool there = warp_wait(&acc_full_bar[acc], (unsigned)((local / 2) & 1));
+                        const bool there = __all_sync(0xffffffffu, *(volatile int*)&failed == 0) && warp_wait(&acc_full_bar[acc], (unsigned)((local / 2) & 1));
                         tc5_fence_after();
                         return there;
                     },
-                    [&](int c0, float (&v)[CHUNK]) { load_tmem(tmem + (unsigned)c0, v); })) {
+                    [&](int c0, float (&v)[CHUNK]) { load_tmem(tmem + (unsigned)c0, v); }))
                 atomicOr(&failed, 8);
-                break;
-            }
             tc5_fence_before();
             mbar_arrive_remote(freed + (unsigned)(acc * sizeof(unsigned long long)));
         }
@@ -301,7 +313,7 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 // A block multiplies a run of the blocks of K (W as the 128-row operand) and hands the sums of the columns that another block finishes to that
 // block, through the cluster's shared memory: every block finishes an even share of the tile's rows of a, adding the parts in the order of K.
 namespace split8 {
-constexpr int NUM_THREADS = 64 + 256;
+constexpr int PARTS = 2, NUM_THREADS = 64 + PARTS * 128;      // (sixteen warps of epilogue, as pairs have, start later: x 12,288 -> 4,096 at 64 rows 14.4 us and 15.1)
 
 // bt: a multiple of 16 up to 256.  The parts that blocks hand each other take the ring's place.
 template <typename TO, int ACT, bool GATED, int PER_SM>
@@ -339,7 +351,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         __syncwarp();
     }
     if (warp == 1) tc5_alloc(tmem_slot, tmem_cols);
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
     const int row = quarter * 32 + lane, n = n0 + row;
     float sw = 0.f, b = 0.f;
     if (warp >= 2) {
@@ -357,7 +369,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 
     if (warp == 0) {                                         // ---- copies ----
         const bool lead = elect_one();
-        int s = 0;
+        int s = 0, issued = early;
         unsigned phase = 0;
         for (int kb = kb0 + early; kb < kb1; ++kb) {
             if (!warp_wait(&empty_bar[s], phase)) {
@@ -365,8 +377,11 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
                 break;
             }
             if (lead) copy(s, kb);
+            ++issued;
             if (++s == stages) { s = 0; phase ^= 1u; }
         }
+        if (lead) see_copies_in(full_bar, issued, stages);
+        __syncwarp();
     } else if (warp == 1) {                                  // ---- products ----
         const bool lead = elect_one();
         const unsigned idesc = make_idesc_8bit(ROWS, bt);
@@ -400,7 +415,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     };
     if (splits == 1) {
         if (warp >= 2)
-            finish_chunks<TO, ACT, GATED>(e, n, scales, sw, b, t0, t0 + bt, half, cols, wait_sums,
+            finish_chunks<TO, ACT, GATED, PARTS>(e, n, scales, sw, b, t0, t0 + bt, part, cols, wait_sums,
                                     [&](int c0, float (&v)[CHUNK]) { load_tmem(tmem + (unsigned)c0, v); });
     } else {
         // Parts as the block that finishes them reads them: by block of K, by four columns, by row, four columns of 4 bytes.
@@ -411,7 +426,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         if (warp >= 2) {
             const unsigned base = smem_u32(smem);
 #pragma unroll 1
-            for (int c0 = half * CHUNK; c0 < cols; c0 += 2 * CHUNK) {
+            for (int c0 = part * CHUNK; c0 < cols; c0 += PARTS * CHUNK) {
                 float v[CHUNK];
                 load_tmem(tmem + (unsigned)c0, v);
                 const int owner = c0 / share;
@@ -425,12 +440,12 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         tc5_fence_before();
         __syncwarp();
         const int first = rank * share, mine = min(cols - first, share);
-        const float* part = reinterpret_cast<const float*>(smem) + 4 * row;
+        const float* parts = reinterpret_cast<const float*>(smem) + 4 * row;
         if (warp < 2) {
             cluster_sync();
         } else {
-            finish_chunks<TO, ACT, GATED>(
-                e, n, scales + first, sw, b, t0 + first, t0 + bt, half, mine,
+            finish_chunks<TO, ACT, GATED, PARTS>(
+                e, n, scales + first, sw, b, t0 + first, t0 + bt, part, mine,
                 [&] {
                     cluster_sync();
                     return true;
@@ -442,7 +457,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
                     for (int r = 0; r < splits; ++r)
 #pragma unroll
                         for (int c = 0; c < CHUNK; c += 4) {
-                            const float4 q = *reinterpret_cast<const float4*>(part + (r * share + c0 + c) * ROWS);
+                            const float4 q = *reinterpret_cast<const float4*>(parts + (r * share + c0 + c) * ROWS);
                             v[c] += q.x; v[c + 1] += q.y; v[c + 2] += q.z; v[c + 3] += q.w;
                         }
                 });
@@ -538,7 +553,8 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
             for (int s = 0; s < early; ++s) copy_a(s, s % per_tile);
             int s = 0;
             unsigned phase = 0;
-            for (int i = early; i < total; ++i, step()) {
+            int i = early;
+            for (; i < total; ++i, step()) {
                 if (!mbar_wait_bounded(&empty_bar[s], phase)) {
                     gave_up = 1;
                     break;
@@ -547,6 +563,7 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
                 copy_a(s, it);
                 if (++s == STAGES) { s = 0; phase ^= 1u; }
             }
+            see_copies_in(full_bar, i, STAGES);
         }
         return;
     }
