@@ -549,6 +549,23 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
             int strip = blockIdx.x * NS, it = 0;
             auto step = [&]() { if (++it == per_tile) { it = 0; strip += gridDim.x * NS; } };
             for (int s = 0; s < early; ++s, step()) copy_w(s, strip, it);
+            // What lies AHEAD stages behind the ring is asked for into L2: where half of a stage is a's, the ring alone does not keep memory busy (16
+            // rows x 12,288 -> 4,096 12.3 us without, 10.3 two stages ahead, 11.2 four; up to 8 rows 9.2 either way).
+            constexpr int AHEAD = MT > 1 ? 2 : 0;
+            int next_strip = strip, next_it = it, asked = early;
+            auto ask = [&]() {
+                if (asked >= total) return;
+                const unsigned bytes = (unsigned)min(DEEP, k_blocks - next_it * DEEP) * BLOCK_BYTES;
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+                    if (next_strip + i < strips)
+                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
+                                     ::"l"(W + ((size_t)(next_strip + i) * k_blocks + next_it * DEEP) * BLOCK_BYTES), "r"(bytes) : "memory");
+                ++asked;
+                if (++next_it == per_tile) { next_it = 0; next_strip += gridDim.x * NS; }
+            };
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) ask();
             pdl_wait();                                       // a comes from the kernel before
             for (int s = 0; s < early; ++s) copy_a(s, s % per_tile);
             int s = 0;
@@ -561,6 +578,7 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
                 }
                 copy_w(s, strip, it);
                 copy_a(s, it);
+                if (AHEAD) ask();
                 if (++s == STAGES) { s = 0; phase ^= 1u; }
             }
             see_copies_in(full_bar, i, STAGES);
