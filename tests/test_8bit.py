@@ -234,6 +234,22 @@ EPILOGUE_SIZES = [(1, 32, 256), (7, 1008, 300), (16, 176, 512), (40, 1008, 512),
 
 
 @gpu
+@pytest.mark.parametrize("m,n,k", [(2100, 2600, 256), (1000, 10000, 128), (700, 14000, 300), (3000, 5000, 128), (4500, 4100, 384), (257, 40000, 128)])
+def test_products_of_several_rounds(m, n, k):
+    """More tiles than pairs of SMs: both accumulators in turn, whole tiles and halves of tiles in the last round."""
+    a, sa, w, sw = operands(25, m, n, k)
+    p, bias = ops.pack_8bit(w), normal(26, n).to(DEV)
+    res = normal(27, m, n).to(DEV)
+    out = torch.full((m, n), float("nan"), device=DEV)
+    ops.gemm_8bit(a, sa, p, sw, out, bias=bias, residual=res)
+    check_product(out, a, sa, w, sw, bias, residual=res)
+    if n % 16 == 0:
+        half = torch.full((m, n // 2), float("nan"), device=DEV, dtype=torch.bfloat16)
+        ops.gemm_8bit(a, sa, p, sw, half, act="silu", gated=True)
+        check_product(half, a, sa, w, sw, act="silu", gated=True)
+
+
+@gpu
 @pytest.mark.parametrize("how", EPILOGUES, ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
 @pytest.mark.parametrize("m,n,k", EPILOGUE_SIZES)
 def test_epilogues(m, n, k, how):

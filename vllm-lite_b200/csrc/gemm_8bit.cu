@@ -170,18 +170,24 @@ namespace pair8 {
 constexpr int MOST = 256, STAGES = 6, PARTS = 4, EPILOGUE = PARTS * 128, NUM_THREADS = 64 + EPILOGUE;
 constexpr unsigned STAGE_BYTES = W_BYTES + MOST / 2 * KB, TMEM_COLS = 512;
 
-__device__ __forceinline__ void tile_corner(int tile, int tiles_t, int tiles_n, int bt, int& t0, int& n0) {
+// Tile `place` of the pairs' order: its corner and its rows of a.  From `whole` on places are halves of tiles: where the last round of the pairs
+// has at most half of them a tile, its tiles are cut in two (4,096 x 12,288 -> 4,096, 256 tiles for 74 pairs: 150.0 us in whole tiles, 144.6 so).
+__device__ __forceinline__ int tile_corner(int place, int whole, int tiles_t, int tiles_n, int bt, int& t0, int& n0) {
+    const int beyond = place - whole, tile = beyond < 0 ? place : whole + (beyond >> 1);
     constexpr int BAND = 8;                                  // pairs that run together share W's tiles in L2
     const int band = tile / (BAND * tiles_n), in_band = tile - band * BAND * tiles_n;
     const int band_rows = min(BAND, tiles_t - band * BAND);
     t0 = (band * BAND + in_band % band_rows) * bt;
     n0 = (in_band / band_rows) * 2 * ROWS;
+    if (beyond < 0) return bt;
+    t0 += (beyond & 1) * (bt >> 1);
+    return bt >> 1;
 }
 
 template <typename TO, int ACT, bool GATED>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, Epilogue e, int k_blocks, int bt,
-                      int tiles_t, int tiles_n, unsigned* err) {
+gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_half, const __grid_constant__ CUtensorMap map_w,
+                      Epilogue e, int k_blocks, int bt, int whole, int places, int tiles_t, int tiles_n, unsigned* err) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full_bar[2], acc_empty_bar[2];
@@ -190,7 +196,7 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     __shared__ int failed;
     const int warp = warp_number();
     const unsigned rank = cluster_rank();
-    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1, total_tiles = tiles_t * tiles_n;
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], 1); }
@@ -214,10 +220,11 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         int s = 0, issued = 0;
         unsigned phase = 1;
         bool ok = true;
-        for (int tile = pair; tile < total_tiles && ok; tile += num_pairs) {
+        for (int place = pair; place < places && ok; place += num_pairs) {
             int t0, n0;
-            tile_corner(tile, tiles_t, tiles_n, bt, t0, n0);
-            const int strip = n0 / STRIP + (int)rank * (ROWS / STRIP), row = t0 + (int)rank * (bt / 2);
+            const int rows = tile_corner(place, whole, tiles_t, tiles_n, bt, t0, n0);
+            const int strip = n0 / STRIP + (int)rank * (ROWS / STRIP), row = t0 + (int)rank * (rows / 2);
+            const CUtensorMap* map = rows == bt ? &map_a : &map_half;
             for (int kb = 0; kb < k_blocks; ++kb) {
                 if (!warp_wait(&empty_bar[s], phase)) {
                     if (lead) atomicOr(&failed, 1);
@@ -225,11 +232,11 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                     break;
                 }
                 if (lead) {
-                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * W_BYTES + (unsigned)(bt * KB));       // the bytes of both blocks
+                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * W_BYTES + (unsigned)(rows * KB));     // the bytes of both blocks
                     const unsigned bar = map_to_rank(smem_u32(&full_bar[s]), 0);
                     unsigned char* st = smem + (size_t)s * STAGE_BYTES;
                     tma_load_3d_pair(st, &map_w, 0, kb * STRIP, strip, bar);
-                    tma_load_2d_pair(st + W_BYTES, &map_a, kb * KB, row, bar);
+                    tma_load_2d_pair(st + W_BYTES, map, kb * KB, row, bar);
                 }
                 ++issued;
                 if (++s == STAGES) { s = 0; phase ^= 1u; }
@@ -240,11 +247,11 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     } else if (warp == 1) {
         if (rank == 0) {                                     // ---- the pair's products ----
             const bool lead = elect_one();
-            const unsigned idesc = make_idesc_8bit(2 * ROWS, bt);
             int s = 0, local = 0;
             unsigned phase = 0;
             bool ok = true;
-            for (int tile = pair; tile < total_tiles && ok; tile += num_pairs, ++local) {
+            for (int place = pair; place < places && ok; place += num_pairs, ++local) {
+                const unsigned idesc = make_idesc_8bit(2 * ROWS, place < whole ? bt : bt >> 1);
                 const int acc = local & 1;
                 if (local >= 2 && !warp_wait(&acc_empty_bar[acc], (unsigned)((local / 2 - 1) & 1))) {
                     if (lead) atomicOr(&failed, 2);
@@ -276,10 +283,10 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         const int quarter = warp & 3, part = (warp - 2) >> 2, lane = threadIdx.x & 31;
         const unsigned freed = map_to_rank(smem_u32(&acc_empty_bar[0]), 0);
         int local = 0;
-        for (int tile = pair; tile < total_tiles; tile += num_pairs, ++local) {
+        for (int place = pair; place < places; place += num_pairs, ++local) {
             const int acc = local & 1;
             int t0, n0;
-            tile_corner(tile, tiles_t, tiles_n, bt, t0, n0);
+            const int rows = tile_corner(place, whole, tiles_t, tiles_n, bt, t0, n0);
             const int n = n0 + (int)rank * ROWS + quarter * 32 + lane;
             const float sw = n < e.N ? e.w_scale[n] : 0.f, b = e.bias && n < e.N ? e.bias[n] : 0.f;
             const int i = threadIdx.x - 64;                  // (who read this place last has passed the barrier of the tile between)
@@ -288,7 +295,7 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             const unsigned tmem = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * MOST);
             // no warp leaves the tiles before the others: they meet at the barrier above.  Where a wait ran out, nobody waits any more.
             if (!finish_chunks<TO, ACT, GATED, PARTS>(
-                    e, n, scales[acc], sw, b, t0, t0 + bt, part, min(bt, e.M - t0),
+                    e, n, scales[acc], sw, b, t0, t0 + rows, part, min(rows, e.M - t0),
                     [&] {
                         const bool there = __all_sync(0xffffffffu, *(volatile int*)&failed == 0) && warp_wait(&acc_full_bar[acc], (unsigned)((local / 2) & 1));
                         tc5_fence_after();
@@ -718,6 +725,12 @@ static int sm_count() {
     return num_sms;
 }
 
+// Whether the tiles of the pairs' last round are cut in two (halves of at least 64 rows, a multiple of 32).
+static bool halves(int tiles, int bt) {
+    const int pairs = sm_count() / 2, last = tiles % pairs;
+    return tiles > pairs && last > 0 && 2 * last <= pairs && bt >= 128 && bt % 64 == 0;
+}
+
 template <typename TO, int ACT, bool GATED>
 static int launch_pair(const void* a, const void* w, const Epilogue& e, int width, int bt, unsigned* err, cudaStream_t s) {
     const size_t smem = (size_t)pair8::STAGES * pair8::STAGE_BYTES + 1024;
@@ -725,12 +738,13 @@ static int launch_pair(const void* a, const void* w, const Epilogue& e, int widt
     // first of all: a thread that has made no call yet has no context, and a tensor map wants one
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (ce != cudaSuccess) return (int)ce;
-    CUtensorMap map_a, map_w;
+    const int tiles_t = (e.M + bt - 1) / bt, tiles_n = (e.N + 2 * ROWS - 1) / (2 * ROWS);
+    const int total = tiles_t * tiles_n, pairs = sm_count() / 2, whole = halves(total, bt) ? total - total % pairs : total, places = 2 * total - whole;
+    CUtensorMap map_a, map_half, map_w;
     int rc = map_rows(&map_a, a, e.M, width, bt / 2);
+    if (!rc) rc = map_rows(&map_half, a, e.M, width, whole < total ? bt / 4 : bt / 2);
     if (!rc) rc = map_strips(&map_w, w, e.N, width / KB);
     if (rc) return rc;
-    const int tiles_t = (e.M + bt - 1) / bt, tiles_n = (e.N + 2 * ROWS - 1) / (2 * ROWS);
-    const int total = tiles_t * tiles_n, pairs = sm_count() / 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (total < pairs ? total : pairs));
     cfg.blockDim = dim3(pair8::NUM_THREADS);
@@ -742,7 +756,7 @@ static int launch_pair(const void* a, const void* w, const Epilogue& e, int widt
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_w, e, width / KB, bt, tiles_t, tiles_n, err);
+    return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_half, map_w, e, width / KB, bt, whole, places, tiles_t, tiles_n, err);
 }
 
 constexpr unsigned SPLIT_ROOM = 232448;      // the most shared memory of a block
@@ -812,7 +826,7 @@ static int cluster_places(int splits) {
 }
 
 // Which kernel and tile for more than 16 rows: what it would take, in cycles of an SM.  An SM takes 64 bytes a cycle in, and that, not the tensor cores,
-// paces a block of K (128 rows of W and its rows of a: 256 + 2 bt cycles, half of a for each block of a pair, 384 at least); tiles run in rounds of the SMs, W
+// paces a block of K (128 rows of W and its rows of a: 256 + 2 bt cycles, half of a for each block of a pair, 384 at least, which halves of tiles take too); tiles run in rounds of the SMs, W
 // comes at the memory's pace, and the two together take the root of the sum of their squares (x 12,288 -> 4,096, 24 rows on 32, 64, 96, 128 SMs: 17.5, 11.5,
 // 9.0 and 8.2 us beside the start, 18.0, 11.3, 9.5 and 8.8 by this).  Beside it a start (6,300, pairs 9,500,
 // and 2,500 for each further round of pairs or of blocks two an SM), 23 a column of the epilogue that no products
@@ -829,8 +843,9 @@ static Plan plan_of(int M, int N, int k_blocks) {
         const int tiles_t = (M + tall - 1) / tall, each = (M + tiles_t - 1) / tiles_t;
         if (tall >= 128) {
             const int bt = (each + 31) / 32 * 32;
-            const long long rounds = ((long long)tiles_t * ((N + 2 * ROWS - 1) / (2 * ROWS)) + sms / 2 - 1) / (sms / 2);
-            const double paced = (double)rounds * k_blocks * (bt > 128 ? 256 + bt : 384), cost = 9500 + 2500 * (double)(rounds - 1) + sqrt(paced * paced + stream * stream) + 23 * bt;
+            const long long tiles = (long long)tiles_t * ((N + 2 * ROWS - 1) / (2 * ROWS)), rounds = (tiles + sms / 2 - 1) / (sms / 2);
+            const int step = bt > 128 ? 256 + bt : 384, last = tiles < (1 << 30) && halves((int)tiles, bt) ? 384 : step;
+            const double paced = ((double)(rounds - 1) * step + last) * k_blocks, cost = 9500 + 2500 * (double)(rounds - 1) + sqrt(paced * paced + stream * stream) + 23 * bt;
             if (least < 0 || cost < least) { least = cost; best = {1, bt, 1, 1}; }
         }
         const int bt = (each + 15) / 16 * 16;
