@@ -148,9 +148,12 @@ static inline bool vl_pdl_enabled() { return g_vl_pdl == 1; }
 extern "C" void vl_set_pdl(int on) { g_vl_pdl = (on && !vl_pdl_forbidden()) ? 1 : 0; }
 extern "C" int vl_get_pdl() { return g_vl_pdl; }
 
+// A kernel that touches no global memory at all before its pdl_wait(), and that works in no clusters, may carry the attribute whatever the
+// switch says: it then only saves the gap between two launches (`vl_launch_waiting`; a call outside a recorded step starts 1 to 4 us
+// sooner: launched the plain way, kernels behind one another begin on ticks of 2.05 us).
 template <typename... KArgs, typename... Args>
-static inline int vl_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                            Args... args) {
+static inline int vl_launch_as(bool dependent, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                               Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -160,8 +163,18 @@ static inline int vl_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, siz
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = vl_pdl_enabled() ? 1 : 0;
+    cfg.numAttrs = dependent ? 1 : 0;
     return (int)cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+template <typename... KArgs, typename... Args>
+static inline int vl_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                            Args... args) {
+    return vl_launch_as(vl_pdl_enabled(), kernel, grid, block, smem, stream, args...);
+}
+template <typename... KArgs, typename... Args>
+static inline int vl_launch_waiting(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                    Args... args) {
+    return vl_launch_as(!vl_pdl_forbidden(), kernel, grid, block, smem, stream, args...);
 }
 
 // Four neighbouring values of a row as float32: one 16-byte (float32) or 8-byte (bfloat16) access.

@@ -347,6 +347,10 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     };
     const int early = min(stages, kb1 - kb0);
 
+    if (splits == 1) {                                       // no cluster: it may have been launched as a dependent
+        pdl_launch_dependents();
+        pdl_wait();
+    }
     if (warp == 0) {
         if (elect_one()) {                                   // the first copies go out before anything else is set up
             for (int i = 0; i < stages; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], 1); }
@@ -480,8 +484,8 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 
 // ---- few rows (a decode step): W's stream is all that counts ------------------------------------------
 // A block walks tiles of NS strips of 16 rows of W.  A warp brings them in, with the rows of a they meet, through a ring of stages that
-// goes on across tiles: 8 / NS blocks of K of every strip (they lie one behind the other: a bulk copy a strip; W is a constant, so its first copies
-// begin before the kernel in front has ended).  Eight warps multiply, each a block of K of a strip.  mma.sync m16n8k32 pairs operand
+// goes on across tiles: 8 / NS blocks of K of every strip (they lie one behind the other: a bulk copy a strip; where W is known to be a constant, `ahead`,
+// its first copies begin before the kernel in front has ended).  Eight warps multiply, each a block of K of a strip.  mma.sync m16n8k32 pairs operand
 // elements by their index along K and mixes no rows, so the bytes a lane holds may stand for any columns as long as both operands
 // agree: pieces t and t + 4 of W's row against pieces t and t + 4 of the row of a, 16 bytes at a time.  Row (column) g of the instruction
 // is W's (a's) row (g >> 1) + 4 (g & 1): eight neighbouring lanes then read all 32 banks (rows 0 and 4 have their pieces exchanged by 4).
@@ -522,7 +526,7 @@ template <int MT, int NS> struct Shape {
 
 template <typename TO, int MT, int NS, int STAGES, int PER_SM>
 __global__ void __launch_bounds__(32 * WARPS + 32, PER_SM)
-gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned char* __restrict__ W, Epilogue e, int k_blocks, int strips, unsigned* err) {
+gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned char* __restrict__ W, Epilogue e, int k_blocks, int strips, int ahead, unsigned* err) {
     using S = Shape<MT, NS>;
     constexpr int DEEP = S::DEEP, OUTS = S::OUTS;
     extern __shared__ __align__(1024) unsigned char ring[];   // (nothing else is shared: it begins on a kilobyte)
@@ -555,6 +559,7 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
             const int early = min(STAGES, total);
             int strip = blockIdx.x * NS, it = 0;
             auto step = [&]() { if (++it == per_tile) { it = 0; strip += gridDim.x * NS; } };
+            if (!ahead) pdl_wait();                            // W may be as young as a
             for (int s = 0; s < early; ++s, step()) copy_w(s, strip, it);
             // What lies AHEAD stages behind the ring is asked for into L2: where half of a stage is a's, the ring alone does not keep memory busy (16
             // rows x 12,288 -> 4,096 12.3 us without, 10.3 two stages ahead, 11.2 four; up to 8 rows 9.2 either way).
@@ -775,6 +780,8 @@ static int launch_split(const void* a, const void* w, const Epilogue& e, int wid
     if (!rc) rc = map_strips(&map_w, w, e.N, width / KB);
     if (rc) return rc;
     const int tiles_t = (e.M + bt - 1) / bt, tiles_n = (e.N + ROWS - 1) / ROWS;
+    if (splits == 1)
+        return vl_launch_waiting(kern, dim3(tiles_t * tiles_n), dim3(split8::NUM_THREADS), smem, s, map_a, map_w, e, width / KB, bt, tiles_t, 1, stages, err);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles_t * tiles_n * splits);
     cfg.blockDim = dim3(split8::NUM_THREADS);
@@ -797,8 +804,9 @@ static int launch_few(const void* a, const void* w, const Epilogue& e, int width
     CUtensorMap map_a;
     if (int rc = map_row_blocks(&map_a, a, e.M, width, MT * 8, few8::Shape<MT, NS>::DEEP)) return rc;
     const int strips = (e.N + STRIP - 1) / STRIP, tiles = (strips + NS - 1) / NS, places = PER_SM * sm_count();
-    return vl_launch(kern, dim3(tiles < places ? tiles : places), dim3(32 * few8::WARPS + 32), smem, s, map_a, (const unsigned char*)w, e, width / KB,
-                     strips, err);
+    // W is a constant to the steps of the engine, which turns the switch on; to anybody else it may be what the kernel in front writes
+    return vl_launch_waiting(kern, dim3(tiles < places ? tiles : places), dim3(32 * few8::WARPS + 32), smem, s, map_a, (const unsigned char*)w, e,
+                             width / KB, strips, vl_pdl_enabled() ? 1 : 0, err);
 }
 // Blocks of clusters of `splits` that run at the same time, one an SM: a cluster lies within a group of SMs, and clusters of 3 leave some idle.
 static int cluster_places(int splits) {

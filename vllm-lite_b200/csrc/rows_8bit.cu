@@ -263,7 +263,7 @@ static int launch_rows(const void* x, const void* delta, const int* rows, const 
     if (!NORM && sizeof(TX) == 2 && aligned && pieces <= 8192) {
         const int each = pieces <= 256 ? 1 : pieces <= 1024 ? 2 : pieces <= 2048 ? 4 : 8;
         const dim3 threads(((pieces + each - 1) / each + 31) / 32 * 32);
-#define ROWS(n) vl_launch(bf16_rows_8bit_kernel<n>, dim3(R), threads, 0, s, (const bf16*)x, (unsigned char*)out, scale, cols, width)
+#define ROWS(n) vl_launch_waiting(bf16_rows_8bit_kernel<n>, dim3(R), threads, 0, s, (const bf16*)x, (unsigned char*)out, scale, cols, width)
         switch (each) {
             case 1: return ROWS(1);
             case 2: return ROWS(2);
@@ -275,7 +275,7 @@ static int launch_rows(const void* x, const void* delta, const int* rows, const 
     const int each = aligned ? (pieces <= (NORM ? 512 : 256) ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 0)
                              : (pieces <= 256 ? 1 : pieces <= 1024 ? 2 : pieces <= 2048 ? 4 : 0);
     const dim3 threads(each ? ((pieces + each - 1) / each + 31) / 32 * 32 : 1024);
-#define ROWS(kernel) vl_launch(kernel, dim3(R), threads, 0, s, (const TX*)x, (const TD*)delta, rows, w, (TX*)into, (unsigned char*)out, scale, cols, width, eps)
+#define ROWS(kernel) vl_launch_waiting(kernel, dim3(R), threads, 0, s, (const TX*)x, (const TD*)delta, rows, w, (TX*)into, (unsigned char*)out, scale, cols, width, eps)
     switch (each) {
         case 1: return aligned ? ROWS((rows_8bit_kernel<TX, TD, 1, NORM, true>)) : ROWS((rows_8bit_kernel<TX, TD, 1, NORM, false>));
         case 2: return aligned ? ROWS((rows_8bit_kernel<TX, TD, 2, NORM, true>)) : ROWS((rows_8bit_kernel<TX, TD, 2, NORM, false>));
