@@ -397,6 +397,34 @@ def test_refusals():
         ops.gemm_8bit(a, sa, ops.pack_8bit(torch.zeros(40, 128, **d).to(F8)), torch.zeros(40, **d), torch.zeros(4, 20, **d), act="silu", gated=True)
 
 
+def test_what_a_product_wants():
+    """Scratch memory holds every part of a shared K; few rows want neither scratch nor clusters, many rows clusters."""
+    for n, columns in ((16, 128), (4096, 12288), (24576, 4096), (1003, 1024)):
+        for m in (1, 8, 16):
+            assert ops.gemm_8bit_plan(m, n, columns) == (0, False)
+        for m in (17, 24, 64, 128, 300, 512):
+            floats, clusters = ops.gemm_8bit_plan(m, n, columns)
+            parts, rest = divmod(floats, m * -(-n // 128) * 128)
+            assert rest == 0 and parts in (0, 2, 3, 4, 5, 6, 7, 8) and not (parts and clusters) and parts <= max(1, columns // 128)
+    assert ops.gemm_8bit_plan(64, 4096, 12288)[0] and ops.gemm_8bit_plan(4096, 4096, 12288) == (0, True)
+    with pytest.raises(ops.KernelError):
+        ops.gemm_8bit_plan(64, 4096, 100)
+
+
+@gpu
+def test_scratch_of_the_callers():
+    a, sa, w, sw = operands(90, 64, 4096, 12288)
+    p, floats = ops.pack_8bit(w), ops.gemm_8bit_plan(64, 4096, 12288)[0]
+    assert floats
+    want, out = torch.empty(64, 4096, device=DEV), torch.empty(64, 4096, device=DEV)
+    ops.gemm_8bit(a, sa, p, sw, want)
+    ops.gemm_8bit(a, sa, p, sw, out, scratch=torch.full((floats + 5,), float("nan"), device=DEV))
+    assert torch.equal(out, want)
+    for bad in (torch.empty(floats - 1, device=DEV), torch.empty(floats, device=DEV, dtype=torch.float64), torch.empty(floats)):
+        with pytest.raises(ops.KernelError):
+            ops.gemm_8bit(a, sa, p, sw, out, scratch=bad)
+
+
 def test_columns_of_a_row():
     assert [ops.eight_bit_columns(k) for k in (1, 128, 129, 4096, 4097)] == [128, 128, 256, 4096, 4224]
 

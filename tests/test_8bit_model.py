@@ -104,7 +104,7 @@ def test_prompts_and_single_tokens(which):
 
 @pytest.mark.gpu
 def test_many_requests_side_by_side():
-    """Twenty requests decoding: a recorded step whose products run as clusters."""
+    """Twenty requests decoding: a recorded step beyond the kernel of few rows."""
     runner = make_runner("B")
     requests = {i: H.tokens_for("B", 6 + i % 5, 30 + i) for i in range(20)}
     steps = [([(i, t[:-3], [len(t) - 4]) for i, t in requests.items()], [])]
@@ -151,12 +151,10 @@ def test_refusals():
 
 def test_steps_of_clusters_are_launched_the_plain_way(monkeypatch):
     from types import SimpleNamespace
-    from vllm_lite_b200.csrc import ops
     from vllm_lite_b200.engine.runner import ModelRunner
-    assert not ops.gemm_8bit_clusters(ops.GEMM_8BIT_FEW) and ops.gemm_8bit_clusters(ops.GEMM_8BIT_FEW + 1)
-    model = SimpleNamespace(may_pair=lambda tokens: False, clusters=ops.gemm_8bit_clusters)
+    model = SimpleNamespace(may_pair=lambda tokens: False, clusters=lambda tokens: tokens > 40)
     runner = SimpleNamespace(model=model)
-    asked = [ModelRunner._launches_dependent(runner, t, recorded) for t in (1, 16, 17, 64, 100) for recorded in (False, True)]
+    asked = [ModelRunner._launches_dependent(runner, t, recorded) for t in (1, 40, 41, 64, 100) for recorded in (False, True)]
     assert asked == [True, True, True, True, False, False, False, False, False, False]
     del model.clusters
     assert ModelRunner._launches_dependent(runner, 64, False) and ModelRunner._launches_dependent(runner, 100, True)

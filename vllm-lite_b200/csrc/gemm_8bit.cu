@@ -316,17 +316,19 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 }
 }  // namespace pair8
 
-// ---- in between: one SM on a tile of 128 rows of W by BT rows of a, the blocks of a cluster sharing its K -----------------
-// A block multiplies a run of the blocks of K (W as the 128-row operand) and hands the sums of the columns that another block finishes to that
-// block, through the cluster's shared memory: every block finishes an even share of the tile's rows of a, adding the parts in the order of K.
+// ---- in between: one SM on a tile of 128 rows of W by bt rows of a, several blocks sharing its K ------------------------
+// A block multiplies a run of the blocks of K (W as the 128-row operand).  Where a tile's K is shared out, the blocks leave their sums in scratch memory,
+// [blocks of a tile, rows of a, W's rows rounded up to whole tiles], and a second launch adds them in the order of K and finishes them; it starts behind the
+// first without a gap.  (Joined through the shared memory of a cluster, x 12,288 -> 4,096 took 14.5 us in a graph at 64 rows and 16.4 in calls
+// behind one another, 13.8 and 14.8 so; kernels of clusters are launched the plain way, and a step that holds one has no programmatic launches.)
 namespace split8 {
 constexpr int PARTS = 2, NUM_THREADS = 64 + PARTS * 128;      // (sixteen warps of epilogue, as pairs have, start later: x 12,288 -> 4,096 at 64 rows 14.4 us and 15.1)
 
-// bt: a multiple of 16 up to 256.  The parts that blocks hand each other take the ring's place.
+// bt: a multiple of 16 up to 256; ahead: W is a constant, its first copies begin before the kernel in front has ended.
 template <typename TO, int ACT, bool GATED, int PER_SM>
 __global__ void __launch_bounds__(NUM_THREADS, PER_SM)
 gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, Epilogue e, int k_blocks, int bt,
-                       int tiles_t, int splits, int stages, unsigned* err) {
+                       int tiles_t, int splits, float* scratch, int stages, int ahead, unsigned* err) {
     const unsigned stage_bytes = W_BYTES + (unsigned)(bt * KB);
     extern __shared__ __align__(1024) unsigned char smem[];   // (nothing else is shared: it begins on a kilobyte)
     unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(smem + stages * stage_bytes);
@@ -335,30 +337,33 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     int* failed = reinterpret_cast<int*>(tmem_slot + 1);
     float* scales = reinterpret_cast<float*>(((uintptr_t)(failed + 1) + 15) & ~(uintptr_t)15);     // of the tile's rows of a
     const int warp = warp_number(), lane = threadIdx.x & 31;
-    const int rank = (int)(blockIdx.x % splits), tile = (int)(blockIdx.x / splits);          // a cluster's blocks are neighbours
+    const int rank = (int)(blockIdx.x % splits), tile = (int)(blockIdx.x / splits);
     const int t0 = (tile % tiles_t) * bt, n0 = (tile / tiles_t) * ROWS;
     const int kb0 = (int)((long long)k_blocks * rank / splits), kb1 = (int)((long long)k_blocks * (rank + 1) / splits);
     const unsigned tmem_cols = bt <= 32 ? 32 : bt <= 64 ? 64 : bt <= 128 ? 128 : 256;
-    auto copy = [&](int s, int kb) {
-        unsigned char* st = smem + s * stage_bytes;
+    auto copy_w = [&](int s, int kb) {
         mbar_arrive_expect_tx(&full_bar[s], stage_bytes);
-        tma_load_3d(st, &map_w, 0, kb * STRIP, n0 / STRIP, &full_bar[s]);
-        tma_load_2d(st + W_BYTES, &map_a, kb * KB, t0, &full_bar[s]);
+        tma_load_3d(smem + s * stage_bytes, &map_w, 0, kb * STRIP, n0 / STRIP, &full_bar[s]);
     };
+    auto copy_a = [&](int s, int kb) { tma_load_2d(smem + s * stage_bytes + W_BYTES, &map_a, kb * KB, t0, &full_bar[s]); };
     const int early = min(stages, kb1 - kb0);
 
-    if (splits == 1) {                                       // no cluster: it may have been launched as a dependent
-        pdl_launch_dependents();
-        pdl_wait();
-    }
+    pdl_launch_dependents();
+    if (!ahead) pdl_wait();                                  // W may be as young as a
     if (warp == 0) {
         if (elect_one()) {                                   // the first copies go out before anything else is set up
             for (int i = 0; i < stages; ++i) { mbar_init(&full_bar[i], 1); mbar_init(&empty_bar[i], 1); }
             mbar_init(acc_bar, 1);
             mbar_fence_init();
             *failed = 0;
-            for (int i = 0; i < early; ++i) copy(i, kb0 + i);
+            for (int i = 0; i < early; ++i) copy_w(i, kb0 + i);
         }
+        __syncwarp();
+    }
+    if (ahead) pdl_wait();
+    if (warp == 0) {
+        if (elect_one())
+            for (int i = 0; i < early; ++i) copy_a(i, kb0 + i);
         __syncwarp();
     }
     if (warp == 1) tc5_alloc(tmem_slot, tmem_cols);
@@ -387,7 +392,10 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
                 if (lead) atomicOr(failed, 1);
                 break;
             }
-            if (lead) copy(s, kb);
+            if (lead) {
+                copy_w(s, kb);
+                copy_a(s, kb);
+            }
             ++issued;
             if (++s == stages) { s = 0; phase ^= 1u; }
         }
@@ -424,54 +432,22 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         tc5_fence_after();
         return there;
     };
-    if (splits == 1) {
-        if (warp >= 2)
+    if (warp >= 2) {
+        if (splits == 1) {
             finish_chunks<TO, ACT, GATED, PARTS>(e, n, scales, sw, b, t0, t0 + bt, part, cols, wait_sums,
-                                    [&](int c0, float (&v)[CHUNK]) { load_tmem(tmem + (unsigned)c0, v); });
-    } else {
-        // Parts as the block that finishes them reads them: by block of K, by four columns, by row, four columns of 4 bytes.
-        const int share = (cols / CHUNK + splits - 1) / splits * CHUNK;        // columns a block finishes
-        if (warp >= 2) wait_sums();
-        __syncthreads();
-        cluster_sync();                                      // nobody multiplies from its ring any more
-        if (warp >= 2) {
-            const unsigned base = smem_u32(smem);
+                                                 [&](int c0, float (&v)[CHUNK]) { load_tmem(tmem + (unsigned)c0, v); });
+        } else if (wait_sums()) {
+            const size_t ld = (size_t)((e.N + ROWS - 1) / ROWS) * ROWS;
 #pragma unroll 1
             for (int c0 = part * CHUNK; c0 < cols; c0 += PARTS * CHUNK) {
                 float v[CHUNK];
                 load_tmem(tmem + (unsigned)c0, v);
-                const int owner = c0 / share;
-                const unsigned to = map_to_rank(base, (unsigned)owner) + (unsigned)(((rank * share + c0 - owner * share) * ROWS + 4 * row) * 4);
+                float* p = scratch + ((size_t)rank * e.M + t0 + c0) * ld + n;
+                const int rows = min(t0 + bt, e.M) - t0 - c0;
 #pragma unroll
-                for (int c = 0; c < CHUNK; c += 4)
-                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};"
-                                 ::"r"(to + (unsigned)(c * ROWS * 4)), "f"(v[c]), "f"(v[c + 1]), "f"(v[c + 2]), "f"(v[c + 3]) : "memory");
+                for (int c = 0; c < CHUNK; ++c, p += ld)
+                    if (c < rows) *p = v[c];
             }
-        }
-        tc5_fence_before();
-        __syncwarp();
-        const int first = rank * share, mine = min(cols - first, share);
-        const float* parts = reinterpret_cast<const float*>(smem) + 4 * row;
-        if (warp < 2) {
-            cluster_sync();
-        } else {
-            finish_chunks<TO, ACT, GATED, PARTS>(
-                e, n, scales + first, sw, b, t0 + first, t0 + bt, part, mine,
-                [&] {
-                    cluster_sync();
-                    return true;
-                },
-                [&](int c0, float (&v)[CHUNK]) {
-#pragma unroll
-                    for (int c = 0; c < CHUNK; ++c) v[c] = 0.f;
-#pragma unroll 1
-                    for (int r = 0; r < splits; ++r)
-#pragma unroll
-                        for (int c = 0; c < CHUNK; c += 4) {
-                            const float4 q = *reinterpret_cast<const float4*>(parts + (r * share + c0 + c) * ROWS);
-                            v[c] += q.x; v[c + 1] += q.y; v[c + 2] += q.z; v[c + 3] += q.w;
-                        }
-                });
         }
     }
     tc5_fence_before();
@@ -479,6 +455,51 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     tc5_fence_after();
     if (warp == 1) tc5_dealloc(tmem_base, tmem_cols);
     if (threadIdx.x == 0 && *failed && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_GEMM_8BIT | ((unsigned)*failed << VL_DEV_ROLE_SHIFT));
+}
+
+// Four neighbouring outputs a thread, a row of a by blockIdx.y.  WIDE: rows of out hold a multiple of four and everything begins on 16 bytes.
+template <bool WIDE, typename T>
+__device__ __forceinline__ float4 load4(const T* p, int left) {
+    if (WIDE) return Quad<T>::load(p);
+    return make_float4(to_f32(p[0]), left > 1 ? to_f32(p[1]) : 0.f, left > 2 ? to_f32(p[2]) : 0.f, left > 3 ? to_f32(p[3]) : 0.f);
+}
+template <typename TO, int ACT, bool GATED, bool WIDE>
+__global__ void __launch_bounds__(256)
+gemm_8bit_join_kernel(const float* __restrict__ scratch, Epilogue e, int splits) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int width = GATED ? e.N >> 1 : e.N, m = blockIdx.y, col = 4 * (blockIdx.x * 256 + threadIdx.x);
+    if (col >= width) return;
+    const int n = GATED ? 2 * col - (col & 7) : col, left = width - col;
+    const size_t ld = (size_t)((e.N + ROWS - 1) / ROWS) * ROWS;
+    const float* p = scratch + (size_t)m * ld + n;
+    TO* out = reinterpret_cast<TO*>(e.out) + (size_t)m * width + col;
+    const float s = e.a_scale[m];
+    auto scaled = [&](int at) {                              // the sums of columns n + at .. with scales and bias
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < splits; ++r) {
+            const float4 q = *reinterpret_cast<const float4*>(p + at + (size_t)r * e.M * ld);
+            v = make_float4(v.x + q.x, v.y + q.y, v.z + q.z, v.w + q.w);
+        }
+        const float4 w = load4<WIDE>(e.w_scale + n + at, left), b = e.bias ? load4<WIDE>(e.bias + n + at, left) : make_float4(0.f, 0.f, 0.f, 0.f);
+        return make_float4(v.x * s * w.x + b.x, v.y * s * w.y + b.y, v.z * s * w.z + b.z, v.w * s * w.w + b.w);
+    };
+    float4 y = scaled(0), r = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (e.residual) r = load4<WIDE>(reinterpret_cast<const TO*>(e.residual) + (size_t)m * width + col, left);
+    y = make_float4(activate<ACT>(y.x), activate<ACT>(y.y), activate<ACT>(y.z), activate<ACT>(y.w));
+    if (GATED) {
+        const float4 u = scaled(8);
+        y = make_float4(y.x * u.x, y.y * u.y, y.z * u.z, y.w * u.w);
+    }
+    y = make_float4(y.x + r.x, y.y + r.y, y.z + r.z, y.w + r.w);
+    if (WIDE) {
+        Quad<TO>::store(out, y);
+        return;
+    }
+    out[0] = from_f32<TO>(y.x);
+    if (left > 1) out[1] = from_f32<TO>(y.y);
+    if (left > 2) out[2] = from_f32<TO>(y.z);
+    if (left > 3) out[3] = from_f32<TO>(y.w);
 }
 }  // namespace split8
 
@@ -764,14 +785,12 @@ static int launch_pair(const void* a, const void* w, const Epilogue& e, int widt
     return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_half, map_w, e, width / KB, bt, whole, places, tiles_t, tiles_n, err);
 }
 
-constexpr unsigned SPLIT_ROOM = 232448;      // the most shared memory of a block
 template <typename TO, int ACT, bool GATED, int PER_SM>
-static int launch_split(const void* a, const void* w, const Epilogue& e, int width, int bt, int splits, unsigned* err, cudaStream_t s) {
+static int launch_split(const void* a, const void* w, const Epilogue& e, int width, int bt, int splits, float* scratch, unsigned* err, cudaStream_t s) {
     // what an SM's 228 KB leave a block, less 1 KB that the system keeps of it, in stages; behind them barriers, a few words and the scales
-    const unsigned stage = W_BYTES + (unsigned)(bt * KB), beside = 2048, room = (PER_SM == 2 ? 115712u : SPLIT_ROOM) - beside;
+    const unsigned stage = W_BYTES + (unsigned)(bt * KB), beside = 2048, room = (PER_SM == 2 ? 115712u : 232448u) - beside;
     const int stages = (int)(room / stage) < 12 ? (int)(room / stage) : 12;
     const size_t smem = stages * stage + beside;
-    while (splits > 1 && (size_t)stages * stage < (size_t)(bt / CHUNK + splits - 1) * CHUNK * ROWS * 4) --splits;       // the parts' room
     auto kern = split8::gemm_8bit_split_kernel<TO, ACT, GATED, PER_SM>;
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (ce != cudaSuccess) return (int)ce;
@@ -780,20 +799,14 @@ static int launch_split(const void* a, const void* w, const Epilogue& e, int wid
     if (!rc) rc = map_strips(&map_w, w, e.N, width / KB);
     if (rc) return rc;
     const int tiles_t = (e.M + bt - 1) / bt, tiles_n = (e.N + ROWS - 1) / ROWS;
-    if (splits == 1)
-        return vl_launch_waiting(kern, dim3(tiles_t * tiles_n), dim3(split8::NUM_THREADS), smem, s, map_a, map_w, e, width / KB, bt, tiles_t, 1, stages, err);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles_t * tiles_n * splits);
-    cfg.blockDim = dim3(split8::NUM_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    // as the paired product, never as a programmatic dependent
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_w, e, width / KB, bt, tiles_t, splits, stages, err);
+    rc = vl_launch_waiting(kern, dim3(tiles_t * tiles_n * splits), dim3(split8::NUM_THREADS), smem, s, map_a, map_w, e, width / KB, bt, tiles_t, splits,
+                           scratch, stages, vl_pdl_enabled() ? 1 : 0, err);
+    if (rc || splits == 1) return rc;
+    const int cols = GATED ? e.N >> 1 : e.N;
+    const bool wide = cols % 4 == 0 && (((uintptr_t)e.out | (uintptr_t)e.residual | (uintptr_t)e.w_scale | (uintptr_t)e.bias) & 15) == 0;
+    const dim3 grid((cols + 1023) / 1024, e.M);
+    return wide ? vl_launch_waiting(split8::gemm_8bit_join_kernel<TO, ACT, GATED, true>, grid, dim3(256), 0, s, (const float*)scratch, e, splits)
+                : vl_launch_waiting(split8::gemm_8bit_join_kernel<TO, ACT, GATED, false>, grid, dim3(256), 0, s, (const float*)scratch, e, splits);
 }
 template <typename TO, int MT, int NS, int STAGES, int PER_SM>
 static int launch_few(const void* a, const void* w, const Epilogue& e, int width, unsigned* err, cudaStream_t s) {
@@ -808,39 +821,16 @@ static int launch_few(const void* a, const void* w, const Epilogue& e, int width
     return vl_launch_waiting(kern, dim3(tiles < places ? tiles : places), dim3(32 * few8::WARPS + 32), smem, s, map_a, (const unsigned char*)w, e,
                              width / KB, strips, vl_pdl_enabled() ? 1 : 0, err);
 }
-// Blocks of clusters of `splits` that run at the same time, one an SM: a cluster lies within a group of SMs, and clusters of 3 leave some idle.
-static int cluster_places(int splits) {
-    static int known[9] = {};
-    if (splits <= 1) return sm_count();
-    if (!known[splits]) {
-        auto kern = split8::gemm_8bit_split_kernel<bf16, ACT_NONE, false, 1>;
-        const size_t smem = SPLIT_ROOM;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(splits);
-        cfg.blockDim = dim3(split8::NUM_THREADS);
-        cfg.dynamicSmemBytes = smem;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        int clusters = 0;
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-            cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess || clusters <= 0)
-            clusters = sm_count() / (2 * splits);
-        known[splits] = clusters * splits;
-    }
-    return known[splits];
-}
-
 // Which kernel and tile for more than 16 rows: what it would take, in cycles of an SM.  An SM takes 64 bytes a cycle in, and that, not the tensor cores,
 // paces a block of K (128 rows of W and its rows of a: 256 + 2 bt cycles, half of a for each block of a pair, 384 at least, which halves of tiles take too); tiles run in rounds of the SMs, W
 // comes at the memory's pace, and the two together take the root of the sum of their squares (x 12,288 -> 4,096, 24 rows on 32, 64, 96, 128 SMs: 17.5, 11.5,
-// 9.0 and 8.2 us beside the start, 18.0, 11.3, 9.5 and 8.8 by this).  Beside it a start (6,300, pairs 9,500,
+// 9.0 and 8.2 us beside the start, 18.0, 11.3, 9.5 and 8.8 by this).  Of 50 sizes (24 to 512 rows, five weights) the choice is within 4 % of the fastest
+// way that was measured but for two (48 x 4,096 -> 6,144 7 %, 200 x 4,096 -> 24,576 9 %).  Beside it a start (6,300, pairs 9,500,
 // and 2,500 for each further round of pairs or of blocks two an SM), 23 a column of the epilogue that no products
-// hide, and where K is cut a barrier (1,500) and 50 for each column that goes to another block.
+// hide, and where K is cut a second launch (2,500) and a cycle for each 10,000 bytes that it reads behind the first.
 struct Plan {
     int pair, bt, splits, per_sm;
+    long long scratch(int M, int N) const { return splits > 1 ? (long long)splits * M * ((N + ROWS - 1) / ROWS * ROWS) : 0; }
 };
 static Plan plan_of(int M, int N, int k_blocks) {
     const int sms = sm_count();
@@ -860,10 +850,9 @@ static Plan plan_of(int M, int N, int k_blocks) {
         const long long tiles = (long long)tiles_t * ((N + ROWS - 1) / ROWS);
         if (tiles > 4 * sms) continue;
         for (int splits = 1; splits <= 8 && 2 * splits <= k_blocks + 1; ++splits) {
-            const int places = cluster_places(splits), share = (bt / CHUNK + splits - 1) / splits * CHUNK;
-            const long long rounds = (tiles * splits + places - 1) / places;
+            const long long rounds = (tiles * splits + sms - 1) / sms;
             const double paced = (double)rounds * ((k_blocks + splits - 1) / splits) * (256 + 2 * bt);
-            const double cost = 6300 + 2500 * (double)((rounds + 1) / 2 - 1) + sqrt(paced * paced + stream * stream) + 23 * share + (splits > 1 ? 1500 + 50 * (bt - share) : 0);
+            const double cost = 6300 + 2500 * (double)((rounds + 1) / 2 - 1) + sqrt(paced * paced + stream * stream) + 23 * bt + (splits > 1 ? 2500 + 8.0 * splits * M * N / 10000 : 0);
             // two blocks an SM where there are more blocks than SMs, or little of a in a stage (24 rows: 13.7 us and 14.5; 64 rows 14.8 and 14.5)
             if (cost < least) { least = cost; best = {0, bt, splits, bt <= 160 && (rounds > 1 || bt <= 32) ? 2 : 1}; }
         }
@@ -872,41 +861,55 @@ static Plan plan_of(int M, int N, int k_blocks) {
 }
 
 template <typename TO, int ACT, bool GATED>
-static int launch_many(const void* a, const void* w, const Epilogue& e, int width, unsigned* err, cudaStream_t s) {
+static int launch_many(const void* a, const void* w, const Epilogue& e, int width, float* scratch, long long floats, unsigned* err, cudaStream_t s) {
     const Plan p = plan_of(e.M, e.N, width / KB);
     if (p.pair) return launch_pair<TO, ACT, GATED>(a, w, e, width, p.bt, err, s);
-    return p.per_sm == 2 ? launch_split<TO, ACT, GATED, 2>(a, w, e, width, p.bt, p.splits, err, s) : launch_split<TO, ACT, GATED, 1>(a, w, e, width, p.bt, p.splits, err, s);
+    if (p.scratch(e.M, e.N) > (scratch ? floats : 0)) return VL_ERR_ARGUMENT;
+    return p.per_sm == 2 ? launch_split<TO, ACT, GATED, 2>(a, w, e, width, p.bt, p.splits, scratch, err, s)
+                         : launch_split<TO, ACT, GATED, 1>(a, w, e, width, p.bt, p.splits, scratch, err, s);
 }
 
 template <typename TO>
-static int launch(const void* a, const void* w, const Epilogue& e, int width, unsigned* err, cudaStream_t s) {
+static int launch(const void* a, const void* w, const Epilogue& e, int width, float* scratch, long long floats, unsigned* err, cudaStream_t s) {
     // Up to 8 rows: strips one by one, four stages of 16 + 8 KB and two blocks an SM.  Up to 16: in twos where that leaves more tiles than SMs (each
     // strip's copy of a is half the bytes then: x 4,096 -> 24,576 19.3 us and 24.8, -> 6,144 6.9 and 9.1), else one by one with two stages and
     // three blocks an SM (x 12,288 -> 4,096 12.2 and 14.6).
     if (e.M <= 8) return launch_few<TO, 1, 1, 4, 2>(a, w, e, width, err, s);
     if (e.M <= 16)
         return (e.N + 2 * STRIP - 1) / (2 * STRIP) > sm_count() ? launch_few<TO, 2, 2, 4, 2>(a, w, e, width, err, s) : launch_few<TO, 2, 1, 2, 3>(a, w, e, width, err, s);
-    if (e.gated) return e.act == ACT_SILU ? launch_many<TO, ACT_SILU, true>(a, w, e, width, err, s) : launch_many<TO, ACT_RELU, true>(a, w, e, width, err, s);
+    if (e.gated) return e.act == ACT_SILU ? launch_many<TO, ACT_SILU, true>(a, w, e, width, scratch, floats, err, s) : launch_many<TO, ACT_RELU, true>(a, w, e, width, scratch, floats, err, s);
     switch (e.act) {
-        case ACT_NONE: return launch_many<TO, ACT_NONE, false>(a, w, e, width, err, s);
-        case ACT_SILU: return launch_many<TO, ACT_SILU, false>(a, w, e, width, err, s);
-        case ACT_RELU: return launch_many<TO, ACT_RELU, false>(a, w, e, width, err, s);
-        case ACT_RELU2: return launch_many<TO, ACT_RELU2, false>(a, w, e, width, err, s);
-        case ACT_TANH: return launch_many<TO, ACT_TANH, false>(a, w, e, width, err, s);
-        case ACT_GELU: return launch_many<TO, ACT_GELU, false>(a, w, e, width, err, s);
+        case ACT_NONE: return launch_many<TO, ACT_NONE, false>(a, w, e, width, scratch, floats, err, s);
+        case ACT_SILU: return launch_many<TO, ACT_SILU, false>(a, w, e, width, scratch, floats, err, s);
+        case ACT_RELU: return launch_many<TO, ACT_RELU, false>(a, w, e, width, scratch, floats, err, s);
+        case ACT_RELU2: return launch_many<TO, ACT_RELU2, false>(a, w, e, width, scratch, floats, err, s);
+        case ACT_TANH: return launch_many<TO, ACT_TANH, false>(a, w, e, width, scratch, floats, err, s);
+        case ACT_GELU: return launch_many<TO, ACT_GELU, false>(a, w, e, width, scratch, floats, err, s);
         default: return VL_ERR_UNSUPPORTED;
     }
 }
 
+// What a product of these sizes wants: plan[0] floats of scratch memory; plan[1]: whether it runs as clusters of blocks.
+extern "C" int vl_gemm_8bit_plan(int M, int N, int width, long long* plan) {
+    if (!plan || width <= 0 || width % KB) return VL_ERR_ARGUMENT;
+    plan[0] = plan[1] = 0;
+    if (M <= 16 || N <= 0) return VL_OK;
+    const Plan p = plan_of(M, N, width / KB);
+    plan[0] = p.scratch(M, N);
+    plan[1] = p.pair;
+    return VL_OK;
+}
+
 extern "C" int vl_gemm_8bit(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out, int out_dtype, const float* bias,
-                            const void* residual, int act, int gated, int M, int N, int width, unsigned* err, void* stream) {
+                            const void* residual, int act, int gated, int M, int N, int width, float* scratch, long long floats, unsigned* err,
+                            void* stream) {
     if (M <= 0 || N <= 0) return VL_OK;
     if (width <= 0 || width % KB || (gated && N % 16)) return VL_ERR_ARGUMENT;
     if (((uintptr_t)a | (uintptr_t)w) & 15) return VL_ERR_UNSUPPORTED;
     if (gated ? act != ACT_SILU && act != ACT_RELU : act != ACT_NONE && act != ACT_SILU && act != ACT_RELU && act != ACT_RELU2 && act != ACT_TANH && act != ACT_GELU)
         return VL_ERR_UNSUPPORTED;
     const Epilogue e{a_scale, w_scale, bias, residual, out, M, N, act, gated};
-    if (out_dtype == VL_BF16) return launch<bf16>(a, w, e, width, err, (cudaStream_t)stream);
-    if (out_dtype == VL_F32) return launch<float>(a, w, e, width, err, (cudaStream_t)stream);
+    if (out_dtype == VL_BF16) return launch<bf16>(a, w, e, width, scratch, floats, err, (cudaStream_t)stream);
+    if (out_dtype == VL_F32) return launch<float>(a, w, e, width, scratch, floats, err, (cudaStream_t)stream);
     return VL_ERR_UNSUPPORTED;
 }

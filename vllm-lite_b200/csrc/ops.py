@@ -8,6 +8,7 @@ A non-zero return code of an entry point raises `KernelError`.
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -148,7 +149,8 @@ _SIGNATURES = {
     ("rows_8bit", "vl_rows_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     ("rows_8bit", "vl_pack_8bit"): [c_void_p, c_void_p, c_int, c_int, c_void_p],
     ("gemm_8bit", "vl_gemm_8bit"): [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                                    c_int, c_void_p, c_void_p],
+                                    c_int, c_void_p, c_longlong, c_void_p, c_void_p],
+    ("gemm_8bit", "vl_gemm_8bit_plan"): [c_int, c_int, c_int, c_void_p],
     ("memprobe", "vl_read_only"): [c_void_p, c_longlong, c_void_p, c_void_p],
     ("sampling", "vl_apply_penalties"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_void_p],
@@ -1609,21 +1611,30 @@ def pack_8bit(w):
 GEMM_8BIT_FEW = 16                                                # most rows of the kernel that streams w alone
 
 
-def gemm_8bit_clusters(M) -> bool:
-    """Whether `gemm_8bit` of M rows may run as clusters of blocks, which are never launched as programmatic dependents."""
-    return M > GEMM_8BIT_FEW
+@functools.lru_cache(maxsize=8192)
+def gemm_8bit_plan(M, N, columns):
+    """(floats of scratch memory that `gemm_8bit` of M rows and N weights of `columns` columns wants, whether it runs as clusters of blocks, which
+    are never launched as programmatic dependents)."""
+    if M <= GEMM_8BIT_FEW:
+        return 0, False
+    plan = (ctypes.c_longlong * 2)()
+    code = _fn("gemm_8bit", "vl_gemm_8bit_plan")(M, N, columns, ctypes.addressof(plan))
+    if code:
+        raise KernelError(f"vl_gemm_8bit_plan refused {M} rows, {N} weights of {columns} columns: {_ERRORS.get(code, code)}")
+    return int(plan[0]), bool(plan[1])
 
 
 GEMM_8BIT_ACTIVATIONS = ("silu", "relu")                          # f(gate) * up
 GEMM_8BIT_UNARY = ("silu", "relu", "relu2", "tanh", "gelu")       # f(y)
 
 
-def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, residual=None, err=None):
+def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, residual=None, err=None, scratch=None):
     """y = f(a_scale[m] w_scale[n] (a @ w^T)[m, n] + bias[n]) + residual[m, n] for rows in 8 bits (a e4m3 [M, width], a_scale float32 [M]:
     `rows_8bit`, `add_rmsnorm_8bit`) and packed weights (w: `pack_8bit`, w_scale float32 [N]); float32 sums, scales, bias (float32 [N]) and
     activation, rounded once to out (bfloat16 or float32 [M, N]).  act: one of GEMM_8BIT_UNARY or None.  gated: w's rows are blocks of
     SWIGLU_GROUP gates and their ups, act one of GEMM_8BIT_ACTIVATIONS, out = f(gate) * up [M, N / 2].  residual: out's shape and type, may
-    be out itself."""
+    be out itself.  scratch: float32, at least `gemm_8bit_plan(M, N, width)[0]` numbers that nobody else on the stream needs; without it the call
+    takes its own."""
     _need(a, E4M3, "a", 2); _need(a_scale, torch.float32, "a_scale", 1); _need(w, E4M3, "w", 4); _need(w_scale, torch.float32, "w_scale", 1)
     _need(out, None, "out", 2)
     M, columns = a.shape
@@ -1643,8 +1654,19 @@ def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, res
         _need(residual, out.dtype, "residual", 2)
         if residual.shape != out.shape:
             raise KernelError(f"gemm_8bit: residual {tuple(residual.shape)} must match out {tuple(out.shape)}")
+    floats = gemm_8bit_plan(M, N, columns)[0] if M > GEMM_8BIT_FEW else 0
+    if floats:
+        if scratch is None:
+            scratch = torch.empty(floats, dtype=torch.float32, device=a.device)
+        _need(scratch, torch.float32, "scratch", 1)
+        if scratch.shape[0] < floats:
+            raise KernelError(f"gemm_8bit: {floats} floats of scratch memory are wanted, got {scratch.shape[0]}")
     _check(_fn("gemm_8bit", "vl_gemm_8bit")(_ptr(a), _ptr(a_scale), _ptr(w), _ptr(w_scale), _ptr(out), dtype_code(out.dtype), _ptr(bias),
-                                            _ptr(residual), _act_code(act), int(gated), M, N, columns, _ptr(err), _stream()), "vl_gemm_8bit")
+                                            _ptr(residual), _act_code(act), int(gated), M, N, columns, _ptr(scratch) if floats else None, floats, _ptr(err), _stream()),
+           "vl_gemm_8bit")
+    if floats:
+        global launch_count
+        launch_count += 1                                         # the second kernel, which adds the parts
     return out
 
 

@@ -54,7 +54,20 @@ class Linear8:
         ops.rows_8bit(weight, values, self.scale)
         self.weight = ops.pack_8bit(values)
         self.bias = linear.bias
-        ctx.clustered.append(ops.gemm_8bit_clusters)
+        ctx.clustered.append(self.clusters)
+
+    def _plan(self, M):
+        return ops.gemm_8bit_plan(M, self.out_features, self.weight.shape[1] * 128)
+
+    def clusters(self, M) -> bool:
+        """Whether the product of M rows runs as clusters of blocks."""
+        return self._plan(M)[1]
+
+    def _product(self, rows, out, step, **how):
+        M = rows.values.shape[0]
+        floats = self._plan(M)[0]
+        scratch = step.workspace.get(step.tag + "gemm_8bit.scratch", (floats,), torch.float32) if floats else None
+        return ops.gemm_8bit(rows.values, rows.scale, self.weight, self.scale, out, bias=self.bias, err=step.err, scratch=scratch, **how)
 
     def _rows(self, a, step, tag) -> Rows8:
         return a if isinstance(a, Rows8) else to_rows8(a, step, tag + ".in")
@@ -62,18 +75,18 @@ class Linear8:
     def __call__(self, a, step, tag, out_dtype=None):
         rows = self._rows(a, step, tag)
         out = step.workspace.get(step.tag + tag, (rows.values.shape[0], self.out_features), out_dtype or torch.bfloat16)
-        return ops.gemm_8bit(rows.values, rows.scale, self.weight, self.scale, out, bias=self.bias, err=step.err)
+        return self._product(rows, out, step)
 
     def swiglu(self, a, step, tag):
         """silu(gate) * up, the weight holding blocks of SWIGLU_GROUP gate rows and their up rows."""
         rows = self._rows(a, step, tag)
         out = step.workspace.get(step.tag + tag + ".act", (rows.values.shape[0], self.out_features // 2), torch.bfloat16)
-        return ops.gemm_8bit(rows.values, rows.scale, self.weight, self.scale, out, bias=self.bias, act="silu", gated=True, err=step.err)
+        return self._product(rows, out, step, act="silu", gated=True)
 
     def into_stream(self, a, stream, step, tag):
         """stream (float32 [M, out]) += y."""
         rows = self._rows(a, step, tag)
-        ops.gemm_8bit(rows.values, rows.scale, self.weight, self.scale, stream, bias=self.bias, residual=stream, err=step.err)
+        self._product(rows, stream, step, residual=stream)
 
     def can_factor_norms(self, M) -> bool:
         return False
