@@ -1552,10 +1552,13 @@ def eight_bit_columns(K) -> int:
 
 
 def _need_8bit_rows(out, scale, R, cols, name):
+    """Checks where R rows of `cols` values go; their columns."""
     _need(out, E4M3, "out", 2); _need(scale, torch.float32, "scale", 1)
-    if cols < 1 or out.shape != (R, eight_bit_columns(cols)) or scale.shape[0] != R:
-        raise KernelError(f"{name}: {R} rows of {cols} values go to out [{R}, {eight_bit_columns(cols)}] and scale [{R}], got out "
+    width = -(-cols // 128) * 128
+    if cols < 1 or out.shape != (R, width) or scale.numel() != R:
+        raise KernelError(f"{name}: {R} rows of {cols} values go to out [{R}, {width}] and scale [{R}], got out "
                           f"{tuple(out.shape)}, scale {tuple(scale.shape)}")
+    return width
 
 
 def add_rmsnorm_8bit(x, delta, weight, eps, out, scale, rows=None, into=None):
@@ -1564,24 +1567,24 @@ def add_rmsnorm_8bit(x, delta, weight, eps, out, scale, rows=None, into=None):
     zeros behind the H values, scale float32 [R].  delta float32 or bfloat16; weight float32 [H].  `into` (float32 [T, H]): where x + delta
     goes instead of x.  A row of zeros has scale 0, a row with a NaN or an infinity a scale that is none either.  Returns out."""
     _need(x, torch.float32, "x", 2); _need(weight, torch.float32, "weight", 1)
-    T, H = x.shape
-    R = T if rows is None else rows.shape[0]
-    if weight.shape[0] != H:
-        raise KernelError(f"add_rmsnorm_8bit: weight has {weight.shape[0]} entries for rows of {H}")
-    _need_8bit_rows(out, scale, R, H, "add_rmsnorm_8bit")
+    R, H = x.shape
+    if rows is not None:
+        _need(rows, torch.int32, "rows", 1)
+        R = rows.numel()
+    if weight.numel() != H:
+        raise KernelError(f"add_rmsnorm_8bit: weight has {weight.numel()} entries for rows of {H}")
+    width = _need_8bit_rows(out, scale, R, H, "add_rmsnorm_8bit")
     if delta is not None:
         _need(delta, None, "delta", 2)
         if delta.shape != x.shape:
             raise KernelError(f"delta {tuple(delta.shape)} must match x {tuple(x.shape)}")
-    if rows is not None:
-        _need(rows, torch.int32, "rows", 1)
     if into is not None:
         _need(into, torch.float32, "into", 2)
         if into.shape != x.shape:
             raise KernelError(f"into {tuple(into.shape)} must match x {tuple(x.shape)}")
-    _check(_fn("rows_8bit", "vl_add_rmsnorm_8bit")(_ptr(x), _ptr(delta), F32 if delta is None else dtype_code(delta.dtype), _ptr(rows),
-                                                   _ptr(weight), _ptr(x if into is None else into), _ptr(out), _ptr(scale), R, H, out.shape[1],
-                                                   float(eps), _stream()), "vl_add_rmsnorm_8bit")
+    _check(_fn("rows_8bit", "vl_add_rmsnorm_8bit")(x, delta, F32 if delta is None else dtype_code(delta.dtype), rows, weight,
+                                                   x if into is None else into, out, scale, R, H, width, float(eps), _stream()),
+           "vl_add_rmsnorm_8bit")
     return out
 
 
@@ -1590,8 +1593,8 @@ def rows_8bit(x, out, scale):
     `add_rmsnorm_8bit`.  Returns out."""
     _need(x, None, "x", 2)
     R, K = x.shape
-    _need_8bit_rows(out, scale, R, K, "rows_8bit")
-    _check(_fn("rows_8bit", "vl_rows_8bit")(_ptr(x), dtype_code(x.dtype), _ptr(out), _ptr(scale), R, K, out.shape[1], _stream()), "vl_rows_8bit")
+    width = _need_8bit_rows(out, scale, R, K, "rows_8bit")
+    _check(_fn("rows_8bit", "vl_rows_8bit")(x, dtype_code(x.dtype), out, scale, R, K, width, _stream()), "vl_rows_8bit")
     return out
 
 
@@ -1638,9 +1641,9 @@ def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, res
     _need(a, E4M3, "a", 2); _need(a_scale, torch.float32, "a_scale", 1); _need(w, E4M3, "w", 4); _need(w_scale, torch.float32, "w_scale", 1)
     _need(out, None, "out", 2)
     M, columns = a.shape
-    N = w_scale.shape[0]
+    N = w_scale.numel()
     width = N // 2 if gated else N
-    if (w.shape != (-(-N // 16), columns // 128, 16, 128) or columns % 128 or a_scale.shape[0] != M or out.shape != (M, width)
+    if (w.shape != (-(-N // 16), columns // 128, 16, 128) or columns % 128 or a_scale.numel() != M or out.shape != (M, width)
             or (gated and N % (2 * SWIGLU_GROUP))):
         raise KernelError(f"gemm_8bit: shapes disagree a{tuple(a.shape)} a_scale{tuple(a_scale.shape)} w{tuple(w.shape)} "
                           f"w_scale{tuple(w_scale.shape)} out{tuple(out.shape)}" + (" (gated)" if gated else ""))
@@ -1648,8 +1651,8 @@ def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, res
         raise KernelError(f"gemm_8bit: unknown activation {act!r}; known: {', '.join(GEMM_8BIT_ACTIVATIONS if gated else GEMM_8BIT_UNARY)}")
     if bias is not None:
         _need(bias, torch.float32, "bias", 1)
-        if bias.shape[0] != N:
-            raise KernelError(f"gemm_8bit: the bias has {bias.shape[0]} entries for {N} rows of w")
+        if bias.numel() != N:
+            raise KernelError(f"gemm_8bit: the bias has {bias.numel()} entries for {N} rows of w")
     if residual is not None:
         _need(residual, out.dtype, "residual", 2)
         if residual.shape != out.shape:
@@ -1661,9 +1664,8 @@ def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, res
         _need(scratch, torch.float32, "scratch", 1)
         if scratch.shape[0] < floats:
             raise KernelError(f"gemm_8bit: {floats} floats of scratch memory are wanted, got {scratch.shape[0]}")
-    _check(_fn("gemm_8bit", "vl_gemm_8bit")(_ptr(a), _ptr(a_scale), _ptr(w), _ptr(w_scale), _ptr(out), dtype_code(out.dtype), _ptr(bias),
-                                            _ptr(residual), _act_code(act), int(gated), M, N, columns, _ptr(scratch) if floats else None, floats, _ptr(err), _stream()),
-           "vl_gemm_8bit")
+    _check(_fn("gemm_8bit", "vl_gemm_8bit")(a, a_scale, w, w_scale, out, dtype_code(out.dtype), bias, residual, _act_code(act), int(gated), M, N,
+                                            columns, scratch if floats else None, floats, err, _stream()), "vl_gemm_8bit")
     if floats:
         global launch_count
         launch_count += 1                                         # the second kernel, which adds the parts
