@@ -320,7 +320,7 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 // A block multiplies a run of the blocks of K (W as the 128-row operand).  Where a tile's K is shared out, the blocks leave their sums in scratch memory,
 // [blocks of a tile, rows of a, W's rows rounded up to whole tiles], and a second launch adds them in the order of K and finishes them; it starts behind the
 // first without a gap.  (Joined through the shared memory of a cluster, x 12,288 -> 4,096 took 14.5 us in a graph at 64 rows and 16.4 in calls
-// behind one another, 13.8 and 14.8 so; kernels of clusters are launched the plain way, and a step that holds one has no programmatic launches.)
+// behind one another, 13.8 and 15.0 so; kernels of clusters are launched the plain way, and a step that holds one has no programmatic launches.)
 namespace split8 {
 constexpr int PARTS = 2, NUM_THREADS = 64 + PARTS * 128;      // (sixteen warps of epilogue, as pairs have, start later: x 12,288 -> 4,096 at 64 rows 14.4 us and 15.1)
 
@@ -457,7 +457,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     if (threadIdx.x == 0 && *failed && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_GEMM_8BIT | ((unsigned)*failed << VL_DEV_ROLE_SHIFT));
 }
 
-// Four neighbouring outputs a thread, a row of a by blockIdx.y.  WIDE: rows of out hold a multiple of four and everything begins on 16 bytes.
+// Four neighbouring outputs a thread, a row of a by blockIdx.x (which has no limit of 65,535).  WIDE: rows of out hold a multiple of four and everything begins on 16 bytes.
 template <bool WIDE, typename T>
 __device__ __forceinline__ float4 load4(const T* p, int left) {
     if (WIDE) return Quad<T>::load(p);
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(256)
 gemm_8bit_join_kernel(const float* __restrict__ scratch, Epilogue e, int splits) {
     pdl_launch_dependents();
     pdl_wait();
-    const int width = GATED ? e.N >> 1 : e.N, m = blockIdx.y, col = 4 * (blockIdx.x * 256 + threadIdx.x);
+    const int width = GATED ? e.N >> 1 : e.N, m = blockIdx.x, col = 4 * (blockIdx.y * 256 + threadIdx.x);
     if (col >= width) return;
     const int n = GATED ? 2 * col - (col & 7) : col, left = width - col;
     const size_t ld = (size_t)((e.N + ROWS - 1) / ROWS) * ROWS;
@@ -785,12 +785,61 @@ static int launch_pair(const void* a, const void* w, const Epilogue& e, int widt
     return (int)cudaLaunchKernelEx(&cfg, kern, map_a, map_half, map_w, e, width / KB, bt, whole, places, tiles_t, tiles_n, err);
 }
 
+// Which kernel and tile for more than 16 rows: what it would take, in cycles of an SM at 1.85 GHz.  A block of K costs by the rows of a that meet it (an SM takes
+// some 64 bytes a cycle in: that paces small tiles, the tensor cores large ones), 1,230 cycles of a copy's way where few stages are in flight; tiles
+// run in rounds of the SMs, W comes at the memory's pace, and the two together take the root of the sum of their squares.  Beside it a start (longer for
+// a block that leaves no room for the next launch's on its SM), what a further round costs, the epilogue's columns that no products hide, and where K is cut
+// a second launch and its bytes.  The numbers were fitted to 311 sizes (17 to 4,096 rows, weights of 16 KB to 178 MB) in every way that this
+// function weighs, calls behind one another and in graphs: the choice is on average 0.9 % slower than the fastest way measured, at worst 16 % (3,200 rows
+// x 320 -> 768: 6.8 us for 5.8).  512 x 4,096 -> 6,144: one SM a tile of 176 rows 14.0 us, pairs with 192 rows 16.4 (14.9 in a graph).
+struct Plan {
+    int pair, bt, splits, per_sm;
+    long long scratch(int M, int N) const { return splits > 1 ? (long long)splits * M * ((N + ROWS - 1) / ROWS * ROWS) : 0; }
+};
+// A block's stages: what an SM's 228 KB leave it, less 1 KB that the system keeps of it; behind them barriers, a few words and the scales (SPLIT_BESIDE).
+constexpr unsigned SPLIT_BESIDE = 2048;
+static int split_stages(int bt, int per_sm) {
+    const int fit = (int)(((per_sm == 2 ? 115712u : 232448u) - SPLIT_BESIDE) / (W_BYTES + (unsigned)(bt * KB)));
+    return fit < 12 ? fit : 12;
+}
+static Plan plan_of(int M, int N, int k_blocks) {
+    const int sms = sm_count();
+    const double stream = (double)N * k_blocks * KB / 3370;
+    const auto longer = [](double a, double b) { return a > b ? a : b; };
+    Plan best{1, 256, 1, 1};
+    double least = -1;
+    for (int tall : {256, 224, 192, 160, 128, 96, 64, 32}) {
+        const int tiles_t = (M + tall - 1) / tall, each = (M + tiles_t - 1) / tiles_t;
+        if (tall >= 128) {
+            const int bt = each <= 128 ? 128 : (each + 31) / 32 * 32;
+            const long long tiles = (long long)tiles_t * ((N + 2 * ROWS - 1) / (2 * ROWS)), rounds = (tiles + sms / 2 - 1) / (sms / 2);
+            const int last = tiles < (1 << 30) && halves((int)tiles, bt) ? bt / 2 : bt;
+            const auto step = [&](int rows) { return longer(85 + 2.41 * rows, 417); };
+            const double paced = ((double)(rounds - 1) * step(bt) + step(last)) * k_blocks;
+            const double cost = 6950 + 4860 * (double)(rounds - 1) + sqrt(paced * paced + stream * stream) + 12.4 * last;
+            if (least < 0 || cost < least) { least = cost; best = {1, bt, 1, 1}; }
+        }
+        const int bt = (each + 15) / 16 * 16;
+        const long long tiles = (long long)tiles_t * ((N + ROWS - 1) / ROWS);
+        for (int splits = 1; splits <= 8 && (splits == 1 || 2 * splits <= k_blocks + 1) && tiles * splits <= 3 * sms; ++splits) {
+            const int rounds = (int)((tiles * splits + sms - 1) / sms);
+            // two blocks an SM where there are more blocks than SMs, or little of a in a stage
+            for (int per_sm = 1; per_sm <= (bt <= 160 && (rounds > 1 || bt <= 64) ? 2 : 1); ++per_sm) {
+                const int turns = (rounds + per_sm - 1) / per_sm, in_flight = split_stages(bt, per_sm) * (rounds > 1 ? per_sm : 1);
+                const double paced = (double)rounds * ((k_blocks + splits - 1) / splits) * longer(longer(146 + 2.17 * bt, 266), 1230.0 / in_flight);
+                const double cost = 6480 + (per_sm == 1 ? 466 : 0) + sqrt(paced * paced + stream * stream) + 7.91 * bt * turns + 8430 * (turns - 1) +
+                                    (splits > 1 ? 3970 + 3.48 * splits * M * N / 10000 : 0);
+                if (cost < least) { least = cost; best = {0, bt, splits, per_sm}; }
+            }
+        }
+    }
+    return best;
+}
+
 template <typename TO, int ACT, bool GATED, int PER_SM>
 static int launch_split(const void* a, const void* w, const Epilogue& e, int width, int bt, int splits, float* scratch, unsigned* err, cudaStream_t s) {
-    // what an SM's 228 KB leave a block, less 1 KB that the system keeps of it, in stages; behind them barriers, a few words and the scales
-    const unsigned stage = W_BYTES + (unsigned)(bt * KB), beside = 2048, room = (PER_SM == 2 ? 115712u : 232448u) - beside;
-    const int stages = (int)(room / stage) < 12 ? (int)(room / stage) : 12;
-    const size_t smem = stages * stage + beside;
+    const int stages = split_stages(bt, PER_SM);
+    const size_t smem = (size_t)stages * (W_BYTES + (unsigned)(bt * KB)) + SPLIT_BESIDE;
     auto kern = split8::gemm_8bit_split_kernel<TO, ACT, GATED, PER_SM>;
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (ce != cudaSuccess) return (int)ce;
@@ -804,7 +853,7 @@ static int launch_split(const void* a, const void* w, const Epilogue& e, int wid
     if (rc || splits == 1) return rc;
     const int cols = GATED ? e.N >> 1 : e.N;
     const bool wide = cols % 4 == 0 && (((uintptr_t)e.out | (uintptr_t)e.residual | (uintptr_t)e.w_scale | (uintptr_t)e.bias) & 15) == 0;
-    const dim3 grid((cols + 1023) / 1024, e.M);
+    const dim3 grid(e.M, (cols + 1023) / 1024);
     return wide ? vl_launch_waiting(split8::gemm_8bit_join_kernel<TO, ACT, GATED, true>, grid, dim3(256), 0, s, (const float*)scratch, e, splits)
                 : vl_launch_waiting(split8::gemm_8bit_join_kernel<TO, ACT, GATED, false>, grid, dim3(256), 0, s, (const float*)scratch, e, splits);
 }
@@ -821,45 +870,6 @@ static int launch_few(const void* a, const void* w, const Epilogue& e, int width
     return vl_launch_waiting(kern, dim3(tiles < places ? tiles : places), dim3(32 * few8::WARPS + 32), smem, s, map_a, (const unsigned char*)w, e,
                              width / KB, strips, vl_pdl_enabled() ? 1 : 0, err);
 }
-// Which kernel and tile for more than 16 rows: what it would take, in cycles of an SM.  An SM takes 64 bytes a cycle in, and that, not the tensor cores,
-// paces a block of K (128 rows of W and its rows of a: 256 + 2 bt cycles, half of a for each block of a pair, 384 at least, which halves of tiles take too); tiles run in rounds of the SMs, W
-// comes at the memory's pace, and the two together take the root of the sum of their squares (x 12,288 -> 4,096, 24 rows on 32, 64, 96, 128 SMs: 17.5, 11.5,
-// 9.0 and 8.2 us beside the start, 18.0, 11.3, 9.5 and 8.8 by this).  Of 50 sizes (24 to 512 rows, five weights) the choice is within 4 % of the fastest
-// way that was measured but for two (48 x 4,096 -> 6,144 7 %, 200 x 4,096 -> 24,576 9 %).  Beside it a start (6,300, pairs 9,500,
-// and 2,500 for each further round of pairs or of blocks two an SM), 23 a column of the epilogue that no products
-// hide, and where K is cut a second launch (2,500) and a cycle for each 10,000 bytes that it reads behind the first.
-struct Plan {
-    int pair, bt, splits, per_sm;
-    long long scratch(int M, int N) const { return splits > 1 ? (long long)splits * M * ((N + ROWS - 1) / ROWS * ROWS) : 0; }
-};
-static Plan plan_of(int M, int N, int k_blocks) {
-    const int sms = sm_count();
-    const double stream = (double)N * k_blocks * KB / 3370;
-    Plan best{1, 256, 1, 1};
-    double least = -1;
-    for (int tall : {256, 224, 192, 160, 128, 96, 64, 32}) {
-        const int tiles_t = (M + tall - 1) / tall, each = (M + tiles_t - 1) / tiles_t;
-        if (tall >= 128) {
-            const int bt = (each + 31) / 32 * 32;
-            const long long tiles = (long long)tiles_t * ((N + 2 * ROWS - 1) / (2 * ROWS)), rounds = (tiles + sms / 2 - 1) / (sms / 2);
-            const int step = bt > 128 ? 256 + bt : 384, last = tiles < (1 << 30) && halves((int)tiles, bt) ? 384 : step;
-            const double paced = ((double)(rounds - 1) * step + last) * k_blocks, cost = 9500 + 2500 * (double)(rounds - 1) + sqrt(paced * paced + stream * stream) + 23 * bt;
-            if (least < 0 || cost < least) { least = cost; best = {1, bt, 1, 1}; }
-        }
-        const int bt = (each + 15) / 16 * 16;
-        const long long tiles = (long long)tiles_t * ((N + ROWS - 1) / ROWS);
-        if (tiles > 4 * sms) continue;
-        for (int splits = 1; splits <= 8 && 2 * splits <= k_blocks + 1; ++splits) {
-            const long long rounds = (tiles * splits + sms - 1) / sms;
-            const double paced = (double)rounds * ((k_blocks + splits - 1) / splits) * (256 + 2 * bt);
-            const double cost = 6300 + 2500 * (double)((rounds + 1) / 2 - 1) + sqrt(paced * paced + stream * stream) + 23 * bt + (splits > 1 ? 2500 + 8.0 * splits * M * N / 10000 : 0);
-            // two blocks an SM where there are more blocks than SMs, or little of a in a stage (24 rows: 13.7 us and 14.5; 64 rows 14.8 and 14.5)
-            if (cost < least) { least = cost; best = {0, bt, splits, bt <= 160 && (rounds > 1 || bt <= 32) ? 2 : 1}; }
-        }
-    }
-    return best;
-}
-
 template <typename TO, int ACT, bool GATED>
 static int launch_many(const void* a, const void* w, const Epilogue& e, int width, float* scratch, long long floats, unsigned* err, cudaStream_t s) {
     const Plan p = plan_of(e.M, e.N, width / KB);
