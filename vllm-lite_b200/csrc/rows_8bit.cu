@@ -243,6 +243,7 @@ long_rows_8bit_kernel(const TX* x, const TD* __restrict__ delta, const int* __re
 // the eight 16-byte pieces of a block's row exchanged by xor with the row's last three bits.  Rows of zeros fill N up to 16.
 __global__ void __launch_bounds__(128)
 pack_8bit_kernel(const uint4* __restrict__ w, uint4* __restrict__ out, int N, int k_blocks) {
+    pdl_wait();
     const int kb = blockIdx.x, row = threadIdx.x >> 3, piece = threadIdx.x & 7;
     for (int strip = blockIdx.y; strip < (N + 15) / 16; strip += gridDim.y) {
         const int n = strip * 16 + row;
