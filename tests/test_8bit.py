@@ -269,6 +269,73 @@ def test_epilogues(m, n, k, how):
             assert torch.equal(same, out)
 
 
+# sizes that the plan gives to pairs of SMs, and such whose K is shared out among blocks and joined by a second launch
+PAIRED, JOINED = [(1030, 8208, 384), (999, 12001, 200)], [(130, 144, 6000), (50, 99, 5100)]
+
+
+@pytest.fixture(params=[False, True], ids=["", "dependent"])
+def dependent(request):
+    ops.set_pdl(request.param)
+    yield request.param
+    ops.set_pdl(False)
+
+
+def run_product(m, n, k, how, dtype=torch.float32):
+    a, sa, w, sw = operands(35, m, n, k, std_w=0.2)
+    gated = how.get("gated", False)
+    width = n // 2 if gated else n
+    bias = normal(36, n).to(DEV) if how.get("bias") else None
+    res = normal(37, m, width).to(DEV, dtype) if how.get("residual") else None
+    out = torch.full((m, width), float("nan"), device=DEV, dtype=dtype)
+    p = ops.pack_8bit(w)
+    torch.cuda.synchronize()                                  # with dependent launches W counts as a constant
+    ops.gemm_8bit(a, sa, p, sw, out, bias=bias, act=how.get("act"), gated=gated, residual=res)
+    check_product(out, a, sa, w, sw, bias, how.get("act"), gated, res)
+
+
+@gpu
+@pytest.mark.parametrize("how", EPILOGUES, ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
+@pytest.mark.parametrize("m,n,k", [PAIRED[0], JOINED[0]])
+def test_epilogues_of_pairs_and_of_the_join(m, n, k, how, dependent):
+    run_product(m, n, k, how)
+    run_product(m, n, k, how, torch.bfloat16)
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [PAIRED[1], JOINED[1], (24, 2048, 2048), (64, 4096, 1024)])
+def test_odd_sizes_of_pairs_and_of_the_join(m, n, k, dependent):
+    run_product(m, n, k, dict(bias=True, act="silu", residual=True))
+    run_product(m, n, k, dict(bias=True), torch.bfloat16)
+
+
+def test_the_sizes_above_reach_those_kernels():
+    for m, n, k in PAIRED + JOINED:
+        for overlapped in (False, True):
+            floats, clusters = ops.gemm_8bit_plan(m, n, ops.eight_bit_columns(k), overlapped)
+            assert clusters == ((m, n, k) in PAIRED) and (floats > 0) == ((m, n, k) in JOINED)
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", PAIRED + JOINED)
+def test_pairs_and_the_join_repeat_to_the_bit_and_rows_stay_apart(m, n, k):
+    a, sa, w, sw = operands(41, m, n, k)
+    p = ops.pack_8bit(w)
+    first, second = torch.empty(m, n, device=DEV), torch.empty(m, n, device=DEV)
+    ops.gemm_8bit(a, sa, p, sw, first)
+    ops.gemm_8bit(a, sa, p, sw, second)
+    assert torch.equal(first, second)
+    changed, sb = a.clone(), sa.clone()
+    changed.view(torch.uint8)[m // 2].fill_(0x7F)            # NaN
+    sb[m // 2] = float("nan")
+    sb[3] = 0
+    changed.view(torch.uint8)[3] = 0
+    bias = normal(42, n).to(DEV)
+    ops.gemm_8bit(a, sa, p, sw, first, bias=bias)
+    ops.gemm_8bit(changed, sb, p, sw, second, bias=bias)
+    keep = [i for i in range(m) if i not in (3, m // 2)]
+    assert torch.isnan(second[m // 2]).all() and torch.equal(second[3], bias) and torch.equal(second[keep], first[keep])
+
+
 @gpu
 @pytest.mark.parametrize("m", [1, 8, 20, 100, 300, 1100])
 def test_a_product_repeats_to_the_bit_and_a_row_does_not_see_the_others(m):

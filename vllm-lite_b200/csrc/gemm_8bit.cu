@@ -796,6 +796,9 @@ static int launch_pair(const void* a, const void* w, const Epilogue& e, int widt
 // a second launch and its bytes.  The numbers were fitted to 311 sizes (17 to 4,096 rows, weights of 16 KB to 178 MB) in every way that this
 // function weighs, calls behind one another and in graphs: the choice is on average 0.9 % slower than the fastest way measured, at worst 16 % (3,200 rows
 // x 320 -> 768: 6.8 us for 5.8).  512 x 4,096 -> 6,144: one SM a tile of 176 rows 14.0 us, pairs with 192 rows 16.4 (14.9 in a graph).
+// overlapped: among launches that start as programmatic dependents with W known as a constant (a decode step) a second launch costs its bytes and little
+// else, and a block that has its SM to itself loses nothing; fitted to 91 sizes of 20 to 64 rows, 0.8 % slower than the fastest way measured, by the numbers
+// above 6.8 % (24 x 4,096 -> 6,144 8.1 us for 9.6, 64 x 12,288 -> 4,096 12.8 for 13.7).
 struct Plan {
     int pair, bt, splits, per_sm;
     long long scratch(int M, int N) const { return splits > 1 ? (long long)splits * M * ((N + ROWS - 1) / ROWS * ROWS) : 0; }
@@ -806,10 +809,11 @@ static int split_stages(int bt, int per_sm) {
     const int fit = (int)(((per_sm == 2 ? 115712u : 232448u) - SPLIT_BESIDE) / (W_BYTES + (unsigned)(bt * KB)));
     return fit < 12 ? fit : 12;
 }
-static Plan plan_of(int M, int N, int k_blocks) {
+static Plan plan_of(int M, int N, int k_blocks, bool overlapped) {
     const int sms = sm_count();
     const double stream = (double)N * k_blocks * KB / 3370;
     const auto longer = [](double a, double b) { return a > b ? a : b; };
+    const double join = overlapped ? 1400 : 3970, join_bytes = overlapped ? 19.6 : 3.48, alone = overlapped ? 0 : 466;
     Plan best{1, 256, 1, 1};
     double least = -1;
     for (int tall : {256, 224, 192, 160, 128, 96, 64, 32}) {
@@ -831,8 +835,8 @@ static Plan plan_of(int M, int N, int k_blocks) {
             for (int per_sm = 1; per_sm <= (bt <= 160 && (rounds > 1 || bt <= 64) ? 2 : 1); ++per_sm) {
                 const int turns = (rounds + per_sm - 1) / per_sm, in_flight = split_stages(bt, per_sm) * (rounds > 1 ? per_sm : 1);
                 const double paced = (double)rounds * ((k_blocks + splits - 1) / splits) * longer(longer(146 + 2.17 * bt, 266), 1230.0 / in_flight);
-                const double cost = 6480 + (per_sm == 1 ? 466 : 0) + sqrt(paced * paced + stream * stream) + 7.91 * bt * turns + 8430 * (turns - 1) +
-                                    (splits > 1 ? 3970 + 3.48 * splits * M * N / 10000 : 0);
+                const double cost = 6480 + (per_sm == 1 ? alone : 0) + sqrt(paced * paced + stream * stream) + 7.91 * bt * turns + 8430 * (turns - 1) +
+                                    (splits > 1 ? join + join_bytes * splits * M * N / 10000 : 0);
                 if (cost < least) { least = cost; best = {0, bt, splits, per_sm}; }
             }
         }
@@ -875,8 +879,9 @@ static int launch_few(const void* a, const void* w, const Epilogue& e, int width
                              width / KB, strips, vl_pdl_enabled() ? 1 : 0, err);
 }
 template <typename TO, int ACT, bool GATED>
-static int launch_many(const void* a, const void* w, const Epilogue& e, int width, float* scratch, long long floats, unsigned* err, cudaStream_t s) {
-    const Plan p = plan_of(e.M, e.N, width / KB);
+static int launch_many(const void* a, const void* w, const Epilogue& e, int width, float* scratch, long long floats, bool overlapped, unsigned* err,
+                       cudaStream_t s) {
+    const Plan p = plan_of(e.M, e.N, width / KB, overlapped);
     if (p.pair) return launch_pair<TO, ACT, GATED>(a, w, e, width, p.bt, err, s);
     if (p.scratch(e.M, e.N) > (scratch ? floats : 0)) return VL_ERR_ARGUMENT;
     return p.per_sm == 2 ? launch_split<TO, ACT, GATED, 2>(a, w, e, width, p.bt, p.splits, scratch, err, s)
@@ -884,46 +889,49 @@ static int launch_many(const void* a, const void* w, const Epilogue& e, int widt
 }
 
 template <typename TO>
-static int launch(const void* a, const void* w, const Epilogue& e, int width, float* scratch, long long floats, unsigned* err, cudaStream_t s) {
+static int launch(const void* a, const void* w, const Epilogue& e, int width, float* scratch, long long floats, bool overlapped, unsigned* err, cudaStream_t s) {
     // Up to 8 rows: strips one by one, four stages of 16 + 8 KB and two blocks an SM.  Up to 16: in twos where that leaves more tiles than SMs (each
     // strip's copy of a is half the bytes then: x 4,096 -> 24,576 19.3 us and 24.8, -> 6,144 6.9 and 9.1), else one by one with two stages and
     // three blocks an SM (x 12,288 -> 4,096 12.2 and 14.6).
     if (e.M <= 8) return launch_few<TO, 1, 1, 4, 2>(a, w, e, width, err, s);
     if (e.M <= 16)
         return (e.N + 2 * STRIP - 1) / (2 * STRIP) > sm_count() ? launch_few<TO, 2, 2, 4, 2>(a, w, e, width, err, s) : launch_few<TO, 2, 1, 2, 3>(a, w, e, width, err, s);
-    if (e.gated) return e.act == ACT_SILU ? launch_many<TO, ACT_SILU, true>(a, w, e, width, scratch, floats, err, s) : launch_many<TO, ACT_RELU, true>(a, w, e, width, scratch, floats, err, s);
+    if (e.gated)
+        return e.act == ACT_SILU ? launch_many<TO, ACT_SILU, true>(a, w, e, width, scratch, floats, overlapped, err, s)
+                                 : launch_many<TO, ACT_RELU, true>(a, w, e, width, scratch, floats, overlapped, err, s);
     switch (e.act) {
-        case ACT_NONE: return launch_many<TO, ACT_NONE, false>(a, w, e, width, scratch, floats, err, s);
-        case ACT_SILU: return launch_many<TO, ACT_SILU, false>(a, w, e, width, scratch, floats, err, s);
-        case ACT_RELU: return launch_many<TO, ACT_RELU, false>(a, w, e, width, scratch, floats, err, s);
-        case ACT_RELU2: return launch_many<TO, ACT_RELU2, false>(a, w, e, width, scratch, floats, err, s);
-        case ACT_TANH: return launch_many<TO, ACT_TANH, false>(a, w, e, width, scratch, floats, err, s);
-        case ACT_GELU: return launch_many<TO, ACT_GELU, false>(a, w, e, width, scratch, floats, err, s);
+        case ACT_NONE: return launch_many<TO, ACT_NONE, false>(a, w, e, width, scratch, floats, overlapped, err, s);
+        case ACT_SILU: return launch_many<TO, ACT_SILU, false>(a, w, e, width, scratch, floats, overlapped, err, s);
+        case ACT_RELU: return launch_many<TO, ACT_RELU, false>(a, w, e, width, scratch, floats, overlapped, err, s);
+        case ACT_RELU2: return launch_many<TO, ACT_RELU2, false>(a, w, e, width, scratch, floats, overlapped, err, s);
+        case ACT_TANH: return launch_many<TO, ACT_TANH, false>(a, w, e, width, scratch, floats, overlapped, err, s);
+        case ACT_GELU: return launch_many<TO, ACT_GELU, false>(a, w, e, width, scratch, floats, overlapped, err, s);
         default: return VL_ERR_UNSUPPORTED;
     }
 }
 
-// What a product of these sizes wants: plan[0] floats of scratch memory; plan[1]: whether it runs as clusters of blocks.
-extern "C" int vl_gemm_8bit_plan(int M, int N, int width, long long* plan) {
+// What a product of these sizes wants: plan[0] floats of scratch memory; plan[1]: whether it runs as clusters of blocks.  overlapped: whether it is among
+// launches that start as programmatic dependents; the launch is told the same.
+extern "C" int vl_gemm_8bit_plan(int M, int N, int width, int overlapped, long long* plan) {
     if (!plan || width <= 0 || width % KB) return VL_ERR_ARGUMENT;
     plan[0] = plan[1] = 0;
     if (M <= 16 || N <= 0) return VL_OK;
-    const Plan p = plan_of(M, N, width / KB);
+    const Plan p = plan_of(M, N, width / KB, overlapped != 0);
     plan[0] = p.scratch(M, N);
     plan[1] = p.pair;
     return VL_OK;
 }
 
 extern "C" int vl_gemm_8bit(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out, int out_dtype, const float* bias,
-                            const void* residual, int act, int gated, int M, int N, int width, float* scratch, long long floats, unsigned* err,
-                            void* stream) {
+                            const void* residual, int act, int gated, int M, int N, int width, float* scratch, long long floats, int overlapped,
+                            unsigned* err, void* stream) {
     if (M <= 0 || N <= 0) return VL_OK;
     if (width <= 0 || width % KB || (gated && N % 16)) return VL_ERR_ARGUMENT;
     if (((uintptr_t)a | (uintptr_t)w) & 15) return VL_ERR_UNSUPPORTED;
     if (gated ? act != ACT_SILU && act != ACT_RELU : act != ACT_NONE && act != ACT_SILU && act != ACT_RELU && act != ACT_RELU2 && act != ACT_TANH && act != ACT_GELU)
         return VL_ERR_UNSUPPORTED;
     const Epilogue e{a_scale, w_scale, bias, residual, out, M, N, act, gated};
-    if (out_dtype == VL_BF16) return launch<bf16>(a, w, e, width, scratch, floats, err, (cudaStream_t)stream);
-    if (out_dtype == VL_F32) return launch<float>(a, w, e, width, scratch, floats, err, (cudaStream_t)stream);
+    if (out_dtype == VL_BF16) return launch<bf16>(a, w, e, width, scratch, floats, overlapped != 0, err, (cudaStream_t)stream);
+    if (out_dtype == VL_F32) return launch<float>(a, w, e, width, scratch, floats, overlapped != 0, err, (cudaStream_t)stream);
     return VL_ERR_UNSUPPORTED;
 }

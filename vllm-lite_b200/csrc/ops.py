@@ -149,8 +149,8 @@ _SIGNATURES = {
     ("rows_8bit", "vl_rows_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     ("rows_8bit", "vl_pack_8bit"): [c_void_p, c_void_p, c_int, c_int, c_void_p],
     ("gemm_8bit", "vl_gemm_8bit"): [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                                    c_int, c_void_p, c_longlong, c_void_p, c_void_p],
-    ("gemm_8bit", "vl_gemm_8bit_plan"): [c_int, c_int, c_int, c_void_p],
+                                    c_int, c_void_p, c_longlong, c_int, c_void_p, c_void_p],
+    ("gemm_8bit", "vl_gemm_8bit_plan"): [c_int, c_int, c_int, c_int, c_void_p],
     ("memprobe", "vl_read_only"): [c_void_p, c_longlong, c_void_p, c_void_p],
     ("sampling", "vl_apply_penalties"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_void_p],
@@ -1614,14 +1614,18 @@ def pack_8bit(w):
 GEMM_8BIT_FEW = 16                                                # most rows of the kernel that streams w alone
 
 
-@functools.lru_cache(maxsize=8192)
-def gemm_8bit_plan(M, N, columns):
+def gemm_8bit_plan(M, N, columns, overlapped=None):
     """(floats of scratch memory that `gemm_8bit` of M rows and N weights of `columns` columns wants, whether it runs as clusters of blocks, which
-    are never launched as programmatic dependents)."""
+    are never launched as programmatic dependents), with dependent launches off or on (`overlapped`; as `set_pdl` left them without it)."""
+    return _gemm_8bit_plan(M, N, columns, _pdl if overlapped is None else overlapped)
+
+
+@functools.lru_cache(maxsize=8192)
+def _gemm_8bit_plan(M, N, columns, overlapped):
     if M <= GEMM_8BIT_FEW:
         return 0, False
     plan = (ctypes.c_longlong * 2)()
-    code = _fn("gemm_8bit", "vl_gemm_8bit_plan")(M, N, columns, ctypes.addressof(plan))
+    code = _fn("gemm_8bit", "vl_gemm_8bit_plan")(M, N, columns, int(overlapped), ctypes.addressof(plan))
     if code:
         raise KernelError(f"vl_gemm_8bit_plan refused {M} rows, {N} weights of {columns} columns: {_ERRORS.get(code, code)}")
     return int(plan[0]), bool(plan[1])
@@ -1657,7 +1661,8 @@ def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, res
         _need(residual, out.dtype, "residual", 2)
         if residual.shape != out.shape:
             raise KernelError(f"gemm_8bit: residual {tuple(residual.shape)} must match out {tuple(out.shape)}")
-    floats = gemm_8bit_plan(M, N, columns)[0] if M > GEMM_8BIT_FEW else 0
+    overlapped = _pdl
+    floats = _gemm_8bit_plan(M, N, columns, overlapped)[0] if M > GEMM_8BIT_FEW else 0
     if floats:
         if scratch is None:
             scratch = torch.empty(floats, dtype=torch.float32, device=a.device)
@@ -1665,7 +1670,7 @@ def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, res
         if scratch.shape[0] < floats:
             raise KernelError(f"gemm_8bit: {floats} floats of scratch memory are wanted, got {scratch.shape[0]}")
     _check(_fn("gemm_8bit", "vl_gemm_8bit")(a, a_scale, w, w_scale, out, dtype_code(out.dtype), bias, residual, _act_code(act), int(gated), M, N,
-                                            columns, scratch if floats else None, floats, err, _stream()), "vl_gemm_8bit")
+                                            columns, scratch if floats else None, floats, int(overlapped), err, _stream()), "vl_gemm_8bit")
     if floats:
         global launch_count
         launch_count += 1                                         # the second kernel, which adds the parts

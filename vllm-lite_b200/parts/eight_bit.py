@@ -56,12 +56,12 @@ class Linear8:
         self.bias = linear.bias
         ctx.clustered.append(self.clusters)
 
-    def _plan(self, M):
-        return ops.gemm_8bit_plan(M, self.out_features, self.weight.shape[1] * 128)
+    def _plan(self, M, overlapped=None):
+        return ops.gemm_8bit_plan(M, self.out_features, self.weight.shape[1] * 128, overlapped)
 
     def clusters(self, M) -> bool:
-        """Whether the product of M rows runs as clusters of blocks."""
-        return self._plan(M)[1]
+        """Whether the product of M rows would run as clusters of blocks among dependent launches."""
+        return self._plan(M, True)[1]
 
     def _product(self, rows, out, step, **how):
         M = rows.values.shape[0]
