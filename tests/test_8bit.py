@@ -271,6 +271,7 @@ def test_epilogues(m, n, k, how):
 
 # sizes that the plan gives to pairs of SMs, and such whose K is shared out among blocks and joined by a second launch
 PAIRED, JOINED = [(1030, 8208, 384), (999, 12001, 200)], [(130, 144, 6000), (50, 99, 5100)]
+LOW = [(64, 20000, 2048), (40, 19001, 2100)]                  # tiles of fewer than 128 rows of w
 
 
 @pytest.fixture(params=[False, True], ids=["", "dependent"])
@@ -295,14 +296,14 @@ def run_product(m, n, k, how, dtype=torch.float32):
 
 @gpu
 @pytest.mark.parametrize("how", EPILOGUES, ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
-@pytest.mark.parametrize("m,n,k", [PAIRED[0], JOINED[0]])
+@pytest.mark.parametrize("m,n,k", [PAIRED[0], JOINED[0], LOW[0]])
 def test_epilogues_of_pairs_and_of_the_join(m, n, k, how, dependent):
     run_product(m, n, k, how)
     run_product(m, n, k, how, torch.bfloat16)
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k", [PAIRED[1], JOINED[1], (24, 2048, 2048), (64, 4096, 1024)])
+@pytest.mark.parametrize("m,n,k", [PAIRED[1], JOINED[1], LOW[1], (24, 2048, 2048), (64, 4096, 1024)])
 def test_odd_sizes_of_pairs_and_of_the_join(m, n, k, dependent):
     run_product(m, n, k, dict(bias=True, act="silu", residual=True))
     run_product(m, n, k, dict(bias=True), torch.bfloat16)
@@ -316,7 +317,7 @@ def test_the_sizes_above_reach_those_kernels():
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k", PAIRED + JOINED)
+@pytest.mark.parametrize("m,n,k", PAIRED + JOINED + LOW)
 def test_pairs_and_the_join_repeat_to_the_bit_and_rows_stay_apart(m, n, k):
     a, sa, w, sw = operands(41, m, n, k)
     p = ops.pack_8bit(w)

@@ -317,7 +317,7 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 }  // namespace pair8
 
 // ---- in between: one SM on a tile of 128 rows of W by bt rows of a, several blocks sharing its K ------------------------
-// A block multiplies a run of the blocks of K (W as the 128-row operand).  Where a tile's K is shared out, the blocks leave their sums in scratch memory,
+// A block multiplies a run of the blocks of K of `height` rows of W (the 128-row operand; 96 or 112 of them where that spreads the tiles better) and bt rows of a.  Where a tile's K is shared out, the blocks leave their sums in scratch memory,
 // [blocks of a tile, rows of a, W's rows rounded up to whole tiles], and a second launch adds them in the order of K and finishes them; it starts behind the
 // first without a gap.  (Joined through the shared memory of a cluster, x 12,288 -> 4,096 took 14.5 us in a graph at 64 rows and 16.4 in calls
 // behind one another, 13.8 and 15.0 so; kernels of clusters are launched the plain way, and a step that holds one has no programmatic launches.)
@@ -327,9 +327,9 @@ constexpr int PARTS = 2, NUM_THREADS = 64 + PARTS * 128;      // (sixteen warps 
 // bt: a multiple of 16 up to 256; ahead: W is a constant, its first copies begin before the kernel in front has ended.
 template <typename TO, int ACT, bool GATED, int PER_SM>
 __global__ void __launch_bounds__(NUM_THREADS, PER_SM)
-gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, Epilogue e, int k_blocks, int bt,
+gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, Epilogue e, int k_blocks, int height, int bt,
                        int tiles_t, int splits, float* scratch, int stages, int ahead, unsigned* err) {
-    const unsigned stage_bytes = W_BYTES + (unsigned)(bt * KB);
+    const unsigned w_bytes = (unsigned)(height * KB), stage_bytes = w_bytes + (unsigned)(bt * KB);
     extern __shared__ __align__(1024) unsigned char smem[];   // (nothing else is shared: it begins on a kilobyte)
     unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(smem + stages * stage_bytes);
     unsigned long long *empty_bar = full_bar + stages, *acc_bar = empty_bar + stages;
@@ -338,14 +338,14 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     float* scales = reinterpret_cast<float*>(((uintptr_t)(failed + 1) + 15) & ~(uintptr_t)15);     // of the tile's rows of a
     const int warp = warp_number(), lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x % splits), tile = (int)(blockIdx.x / splits);
-    const int t0 = (tile % tiles_t) * bt, n0 = (tile / tiles_t) * ROWS;
+    const int t0 = (tile % tiles_t) * bt, n0 = (tile / tiles_t) * height;
     const int kb0 = (int)((long long)k_blocks * rank / splits), kb1 = (int)((long long)k_blocks * (rank + 1) / splits);
     const unsigned tmem_cols = bt <= 32 ? 32 : bt <= 64 ? 64 : bt <= 128 ? 128 : 256;
     auto copy_w = [&](int s, int kb) {
         mbar_arrive_expect_tx(&full_bar[s], stage_bytes);
         tma_load_3d(smem + s * stage_bytes, &map_w, 0, kb * STRIP, n0 / STRIP, &full_bar[s]);
     };
-    auto copy_a = [&](int s, int kb) { tma_load_2d(smem + s * stage_bytes + W_BYTES, &map_a, kb * KB, t0, &full_bar[s]); };
+    auto copy_a = [&](int s, int kb) { tma_load_2d(smem + s * stage_bytes + w_bytes, &map_a, kb * KB, t0, &full_bar[s]); };
     const int early = min(stages, kb1 - kb0);
 
     pdl_launch_dependents();
@@ -368,7 +368,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     }
     if (warp == 1) tc5_alloc(tmem_slot, tmem_cols);
     const int quarter = warp & 3, part = (warp - 2) >> 2;
-    const int row = quarter * 32 + lane, n = n0 + row;
+    const int row = quarter * 32 + lane, n = row < height ? n0 + row : e.N;    // (lanes beyond the tile's height hold products with what lies behind it)
     float sw = 0.f, b = 0.f;
     if (warp >= 2) {
         const int i = threadIdx.x - 64;
@@ -413,7 +413,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             }
             tc5_fence_after();
             const unsigned char* st = smem + s * stage_bytes;
-            const unsigned long long wdesc = make_smem_desc(st), adesc = make_smem_desc(st + W_BYTES);
+            const unsigned long long wdesc = make_smem_desc(st), adesc = make_smem_desc(st + w_bytes);
             if (lead) {
 #pragma unroll
                 for (int k = 0; k < KB / 32; ++k)
@@ -432,7 +432,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         tc5_fence_after();
         return there;
     };
-    if (warp >= 2) {
+    if (warp >= 2 && quarter * 32 < height) {
         if (splits == 1) {
             finish_chunks<TO, ACT, GATED, PARTS>(e, n, scales, sw, b, t0, t0 + bt, part, cols, wait_sums,
                                                  [&](int c0, float (&v)[CHUNK]) { load_tmem(tmem + (unsigned)c0, v); });
@@ -446,7 +446,7 @@ gemm_8bit_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
                 const int rows = min(t0 + bt, e.M) - t0 - c0;
 #pragma unroll
                 for (int c = 0; c < CHUNK; ++c, p += ld)
-                    if (c < rows) *p = v[c];
+                    if (c < rows && n < e.N) *p = v[c];
             }
         }
     }
@@ -734,13 +734,13 @@ static int map_row_blocks(CUtensorMap* map, const void* a, int M, int width, int
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(a), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : VL_ERR_ARGUMENT;
 }
-// packed strips in boxes of 8 strips x 16 rows x 128 bytes: 128 rows of one block of K, already in the swizzle's order
-static int map_strips(CUtensorMap* map, const void* w, int N, int k_blocks) {
+// packed strips in boxes of whole strips x 16 rows x 128 bytes: 128 rows, or fewer, of one block of K, already in the swizzle's order
+static int map_strips(CUtensorMap* map, const void* w, int N, int k_blocks, int rows = ROWS) {
     EncodeTiledFn enc = encode_tiled_fn();
     if (!enc) return VL_ERR_UNSUPPORTED;
     cuuint64_t dims[3] = {(cuuint64_t)KB, (cuuint64_t)STRIP * k_blocks, (cuuint64_t)((N + STRIP - 1) / STRIP)};
     cuuint64_t strides[2] = {(cuuint64_t)KB, (cuuint64_t)STRIP * k_blocks * KB};
-    cuuint32_t box[3] = {(cuuint32_t)KB, (cuuint32_t)STRIP, (cuuint32_t)(ROWS / STRIP)}, estr[3] = {1, 1, 1};
+    cuuint32_t box[3] = {(cuuint32_t)KB, (cuuint32_t)STRIP, (cuuint32_t)(rows / STRIP)}, estr[3] = {1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(w), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : VL_ERR_ARGUMENT;
 }
@@ -797,24 +797,27 @@ static int launch_pair(const void* a, const void* w, const Epilogue& e, int widt
 // function weighs, calls behind one another and in graphs: the choice is on average 0.9 % slower than the fastest way measured, at worst 16 % (3,200 rows
 // x 320 -> 768: 6.8 us for 5.8).  512 x 4,096 -> 6,144: one SM a tile of 176 rows 14.0 us, pairs with 192 rows 16.4 (14.9 in a graph).
 // overlapped: among launches that start as programmatic dependents with W known as a constant (a decode step) a second launch costs its bytes and little
-// else, and a block that has its SM to itself loses nothing; fitted to 91 sizes of 20 to 64 rows, 0.8 % slower than the fastest way measured, by the numbers
-// above 6.8 % (24 x 4,096 -> 6,144 8.1 us for 9.6, 64 x 12,288 -> 4,096 12.8 for 13.7).
+// else, and a block that has its SM to itself loses nothing; fitted to 113 sizes of 17 to 64 rows, 2.2 % slower than the fastest way measured, by the numbers
+// above 6 % (24 x 4,096 -> 6,144 8.1 us for 9.6, 64 x 12,288 -> 4,096 12.8 for 13.7).
+// Lower tiles of W, 96 or 112 rows: where two blocks an SM have room for all of them and 128 rows leave SMs with one block beside SMs with two (64 x 4,096
+// -> 24,576, 256 tiles for 192: 20.0 us for 21.4 overlapped, 96 rows 21.9 for 23.5 in calls); not for a K of a few blocks (20 x 320 -> 20,032 4.8 for 4.6), and
+// tiles of 64 to 16 rows in place of cutting K gain nothing at 20 to 512 rows of twelve weights (a comes in too often).
 struct Plan {
-    int pair, bt, splits, per_sm;
+    int pair, height, bt, splits, per_sm;
     long long scratch(int M, int N) const { return splits > 1 ? (long long)splits * M * ((N + ROWS - 1) / ROWS * ROWS) : 0; }
 };
-// A block's stages: what an SM's 228 KB leave it, less 1 KB that the system keeps of it; behind them barriers, a few words and the scales (SPLIT_BESIDE).
+// A block's stages: what an SM's 228 KB leave it, less 1 KB that the system keeps of it; behind them barriers, a few words and the scales (SPLIT_BESIDE).  A
+// product reads 128 rows of W whatever the tile's height: a stage (96 + 32 rows at least) and what lies behind the last one hold them.
 constexpr unsigned SPLIT_BESIDE = 2048;
-static int split_stages(int bt, int per_sm) {
-    const int fit = (int)(((per_sm == 2 ? 115712u : 232448u) - SPLIT_BESIDE) / (W_BYTES + (unsigned)(bt * KB)));
-    return fit < 12 ? fit : 12;
+static int split_stages(int height, int bt, int per_sm) {
+    return (int)(((per_sm == 2 ? 115712u : 232448u) - SPLIT_BESIDE) / (unsigned)((height + bt) * KB));
 }
 static Plan plan_of(int M, int N, int k_blocks, bool overlapped) {
     const int sms = sm_count();
     const double stream = (double)N * k_blocks * KB / 3370;
     const auto longer = [](double a, double b) { return a > b ? a : b; };
-    const double join = overlapped ? 1400 : 3970, join_bytes = overlapped ? 19.6 : 3.48, alone = overlapped ? 0 : 466;
-    Plan best{1, 256, 1, 1};
+    const double join = overlapped ? 1180 : 3970, join_part = overlapped ? 263 : 0, alone = overlapped ? 0 : 466;
+    Plan best{1, 2 * ROWS, 256, 1, 1};
     double least = -1;
     for (int tall : {256, 224, 192, 160, 128, 96, 64, 32}) {
         const int tiles_t = (M + tall - 1) / tall, each = (M + tiles_t - 1) / tiles_t;
@@ -825,7 +828,7 @@ static Plan plan_of(int M, int N, int k_blocks, bool overlapped) {
             const auto step = [&](int rows) { return longer(85 + 2.41 * rows, 417); };
             const double paced = ((double)(rounds - 1) * step(bt) + step(last)) * k_blocks;
             const double cost = 6950 + 4860 * (double)(rounds - 1) + sqrt(paced * paced + stream * stream) + 12.4 * last;
-            if (least < 0 || cost < least) { least = cost; best = {1, bt, 1, 1}; }
+            if (least < 0 || cost < least) { least = cost; best = {1, 2 * ROWS, bt, 1, 1}; }
         }
         const int bt = (each + 15) / 16 * 16;
         const long long tiles = (long long)tiles_t * ((N + ROWS - 1) / ROWS);
@@ -833,30 +836,37 @@ static Plan plan_of(int M, int N, int k_blocks, bool overlapped) {
             const int rounds = (int)((tiles * splits + sms - 1) / sms);
             // two blocks an SM where there are more blocks than SMs, or little of a in a stage
             for (int per_sm = 1; per_sm <= (bt <= 160 && (rounds > 1 || bt <= 64) ? 2 : 1); ++per_sm) {
-                const int turns = (rounds + per_sm - 1) / per_sm, in_flight = split_stages(bt, per_sm) * (rounds > 1 ? per_sm : 1);
+                const int turns = (rounds + per_sm - 1) / per_sm, in_flight = split_stages(ROWS, bt, per_sm) * (rounds > 1 ? per_sm : 1);
                 const double paced = (double)rounds * ((k_blocks + splits - 1) / splits) * longer(longer(146 + 2.17 * bt, 266), 1230.0 / in_flight);
                 const double cost = 6480 + (per_sm == 1 ? alone : 0) + sqrt(paced * paced + stream * stream) + 7.91 * bt * turns + 8430 * (turns - 1) +
-                                    (splits > 1 ? join + join_bytes * splits * M * N / 10000 : 0);
-                if (cost < least) { least = cost; best = {0, bt, splits, per_sm}; }
+                                    (splits > 1 ? join + join_part * splits + 3.5 * splits * M * N / 10000 : 0);
+                if (cost < least) { least = cost; best = {0, ROWS, bt, splits, per_sm}; }
             }
         }
+    }
+    if (!best.pair && best.splits == 1 && best.per_sm == 2 && k_blocks >= 16) {
+        const long long tiles_t = (M + best.bt - 1) / best.bt;
+        const auto tiles = [&](int height) { return tiles_t * ((N + height - 1) / height); };
+        if (tiles(ROWS) > sms)
+            for (int height : {112, 96})
+                if (tiles(height) <= 2 * sms) best.height = height;
     }
     return best;
 }
 
 template <typename TO, int ACT, bool GATED, int PER_SM>
-static int launch_split(const void* a, const void* w, const Epilogue& e, int width, int bt, int splits, float* scratch, unsigned* err, cudaStream_t s) {
-    const int stages = split_stages(bt, PER_SM);
-    const size_t smem = (size_t)stages * (W_BYTES + (unsigned)(bt * KB)) + SPLIT_BESIDE;
+static int launch_split(const void* a, const void* w, const Epilogue& e, int width, int height, int bt, int splits, float* scratch, unsigned* err, cudaStream_t s) {
+    const int stages = split_stages(height, bt, PER_SM);
+    const size_t smem = (size_t)stages * (unsigned)((height + bt) * KB) + SPLIT_BESIDE;
     auto kern = split8::gemm_8bit_split_kernel<TO, ACT, GATED, PER_SM>;
     cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (ce != cudaSuccess) return (int)ce;
     CUtensorMap map_a, map_w;
     int rc = map_rows(&map_a, a, e.M, width, bt);
-    if (!rc) rc = map_strips(&map_w, w, e.N, width / KB);
+    if (!rc) rc = map_strips(&map_w, w, e.N, width / KB, height);
     if (rc) return rc;
-    const int tiles_t = (e.M + bt - 1) / bt, tiles_n = (e.N + ROWS - 1) / ROWS;
-    rc = vl_launch_waiting(kern, dim3(tiles_t * tiles_n * splits), dim3(split8::NUM_THREADS), smem, s, map_a, map_w, e, width / KB, bt, tiles_t, splits,
+    const int tiles_t = (e.M + bt - 1) / bt, tiles_n = (e.N + height - 1) / height;
+    rc = vl_launch_waiting(kern, dim3(tiles_t * tiles_n * splits), dim3(split8::NUM_THREADS), smem, s, map_a, map_w, e, width / KB, height, bt, tiles_t, splits,
                            scratch, stages, vl_pdl_enabled() ? 1 : 0, err);
     if (rc || splits == 1) return rc;
     const int cols = GATED ? e.N >> 1 : e.N;
@@ -884,8 +894,8 @@ static int launch_many(const void* a, const void* w, const Epilogue& e, int widt
     const Plan p = plan_of(e.M, e.N, width / KB, overlapped);
     if (p.pair) return launch_pair<TO, ACT, GATED>(a, w, e, width, p.bt, err, s);
     if (p.scratch(e.M, e.N) > (scratch ? floats : 0)) return VL_ERR_ARGUMENT;
-    return p.per_sm == 2 ? launch_split<TO, ACT, GATED, 2>(a, w, e, width, p.bt, p.splits, scratch, err, s)
-                         : launch_split<TO, ACT, GATED, 1>(a, w, e, width, p.bt, p.splits, scratch, err, s);
+    return p.per_sm == 2 ? launch_split<TO, ACT, GATED, 2>(a, w, e, width, p.height, p.bt, p.splits, scratch, err, s)
+                         : launch_split<TO, ACT, GATED, 1>(a, w, e, width, p.height, p.bt, p.splits, scratch, err, s);
 }
 
 template <typename TO>
