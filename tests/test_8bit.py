@@ -78,6 +78,19 @@ def test_norm_of_picked_rows_leaves_the_stream(h, with_delta):
 
 
 @gpu
+@pytest.mark.parametrize("h", [96, 2048, 3000, 4096, 5120, 8192, 1001])
+def test_a_norm_does_not_see_how_many_rows_there_are(h):
+    x, w = normal(8, 2500, h).to(DEV), normal(9, h).to(DEV)
+    d = normal(10, 2500, h).to(DEV, torch.bfloat16)
+    many = empty_rows(2500, h)
+    ops.add_rmsnorm_8bit(x, d, w, 1e-6, *many, into=torch.empty_like(x))
+    for r in (0, 1234, 2499):
+        few = empty_rows(1, h)
+        ops.add_rmsnorm_8bit(x[r:r + 1].clone(), d[r:r + 1].clone(), w, 1e-6, *few)
+        assert torch.equal(few[0][0].view(torch.uint8), many[0][r].view(torch.uint8)) and torch.equal(few[1][0], many[1][r])
+
+
+@gpu
 @pytest.mark.parametrize("h", [100, 4096])
 def test_norm_into_other_memory(h):
     x, d, w = normal(7, 6, h), normal(8, 6, h).bfloat16(), torch.ones(h)

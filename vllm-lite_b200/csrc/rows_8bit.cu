@@ -25,6 +25,21 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
     const int lane = threadIdx.x & 31;
     return warp_sum(lane < (int)(blockDim.x >> 5) ? scratch[lane] : 0.f);
 }
+// The same of PIECES values a thread, each of which stands for a thread of a block PIECES times as large: the sum's order, and its bits, are those of that block.
+template <int PIECES>
+__device__ __forceinline__ float row_sum(const float (&v)[PIECES], float* scratch) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const float sum = warp_sum(v[i]);
+        if (lane == 0) scratch[i * warps + (threadIdx.x >> 5)] = sum;
+    }
+    __syncthreads();
+    float all = lane < PIECES * warps ? scratch[lane] : 0.f;
+#pragma unroll
+    for (int i = 32; i < 32 * PIECES; i += 32) all += i + lane < PIECES * warps ? scratch[i + lane] : 0.f;
+    return warp_sum(all);
+}
 __device__ __forceinline__ unsigned row_max(unsigned v, unsigned* scratch) {
     v = __reduce_max_sync(0xffffffffu, v);
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
@@ -90,14 +105,13 @@ __device__ __forceinline__ void store_8bit(unsigned char* p, const float (&v)[8]
 }  // namespace
 
 // One block a row, the row in registers: a thread holds PIECES pieces of eight neighbouring columns, piece by piece over the block's threads.  Bound by
-// the bytes: one read of x (and delta), one write of each result.  The block's shape, and with it the order of the sums, is a function of the
-// row's length alone.
+// the bytes: one read of x (and delta), one write of each result.  The order of the sums is a function of the row's length alone, whatever the block's shape.
 template <typename TX, typename TD, int PIECES, bool NORM, bool ALIGNED>
 __global__ void __launch_bounds__(ALIGNED ? 1024 : 512)
 rows_8bit_kernel(const TX* x, const TD* __restrict__ delta, const int* __restrict__ rows, const float* __restrict__ w, TX* into,
                  unsigned char* __restrict__ out, float* __restrict__ scale, int cols, int width, float eps) {
     constexpr bool APART = !ALIGNED && sizeof(TX) == 4;
-    __shared__ float sums[32];
+    __shared__ float sums[32 * PIECES];
     __shared__ unsigned tops[32];
     pdl_launch_dependents();
     pdl_wait();
@@ -117,11 +131,13 @@ rows_8bit_kernel(const TX* x, const TD* __restrict__ delta, const int* __restric
         float g[PIECES][8];
         if (PIECES == 1) load_pieces<ALIGNED, APART>(w, cols, g);    // few rows: one wait for memory less
         if (delta && !rows) store_stream<ALIGNED>(reinterpret_cast<float*>(into) + (size_t)r * cols, cols, v);
-        float ss = 0.f;
+        float ss[PIECES];
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i)
+        for (int i = 0; i < PIECES; ++i) {
+            ss[i] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+            for (int j = 0; j < 8; ++j) ss[i] += v[i][j] * v[i][j];
+        }
         const float inv = 1.0f / sqrtf(row_sum(ss, sums) / (float)cols + eps);
         if (PIECES > 1) load_pieces<ALIGNED, APART>(w, cols, g);
 #pragma unroll
@@ -252,6 +268,16 @@ pack_8bit_kernel(const uint4* __restrict__ w, uint4* __restrict__ out, int N, in
     }
 }
 
+static int sm_count() {
+    static int num_sms = 0;
+    if (!num_sms) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || num_sms <= 0) num_sms = 148;
+    }
+    return num_sms;
+}
+
 template <typename TX, typename TD, bool NORM>
 static int launch_rows(const void* x, const void* delta, const int* rows, const float* w, void* into, void* out, float* scale, int R, int cols,
                        int width, float eps, cudaStream_t s) {
@@ -259,7 +285,7 @@ static int launch_rows(const void* x, const void* delta, const int* rows, const 
     const bool aligned = cols % 8 == 0 && (((uintptr_t)x | (uintptr_t)delta | (uintptr_t)w | (uintptr_t)into) & 15) == 0;
     if ((uintptr_t)out & 7) return VL_ERR_UNSUPPORTED;
     // Pieces a thread: the longer the row, the fewer threads it is worth (us, one piece / two / four: rows of 4,096 bfloat16, 4,096 of them 13.4 / 10.7 / -,
-    // of 12,288 - / 30.8 / 25.4, of 25,600 - / - / 35.2, eight 28.2; norms of 4,096 34.8 / 35.4 / -, of 8,192 37.2 / 37.0 / 42.6)
+    // of 12,288 - / 30.8 / 25.4, of 25,600 - / - / 35.2, eight 28.2).
     const int pieces = width / 8;
     if (!NORM && sizeof(TX) == 2 && aligned && pieces <= 8192) {
         const int each = pieces <= 256 ? 1 : pieces <= 1024 ? 2 : pieces <= 2048 ? 4 : 8;
@@ -273,7 +299,10 @@ static int launch_rows(const void* x, const void* delta, const int* rows, const 
         }
 #undef ROWS
     }
-    const int each = aligned ? (pieces <= (NORM ? 512 : 256) ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 0)
+    // A norm: one piece while all rows run at once, two where they take turns (us, one piece / two: of 4,096 one row 2.15 / 2.30, 512 rows 6.7 / 6.8, 2,048
+    // 20.0 / 18.0, 4,096 34.5 / 31.7; of 5,120 one row 2.40 / 2.52, 512 rows 8.6 / 7.6, 4,096 42.7 / 39.3; four pieces are slower everywhere).
+    const bool at_once = pieces <= 1024 && (long long)R * ((pieces + 31) / 32 * 32) <= 2048LL * sm_count();
+    const int each = aligned ? ((NORM ? at_once : pieces <= 256) ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 0)
                              : (pieces <= 256 ? 1 : pieces <= 1024 ? 2 : pieces <= 2048 ? 4 : 0);
     const dim3 threads(each ? ((pieces + each - 1) / each + 31) / 32 * 32 : 1024);
 #define ROWS(kernel) vl_launch_waiting(kernel, dim3(R), threads, 0, s, (const TX*)x, (const TD*)delta, rows, w, (TX*)into, (unsigned char*)out, scale, cols, width, eps)
