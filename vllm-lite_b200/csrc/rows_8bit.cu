@@ -284,11 +284,11 @@ static int launch_rows(const void* x, const void* delta, const int* rows, const 
     // whole pieces on 16-byte boundaries: eight values of x are 16 or 32 bytes, of delta and the weight likewise (the results' rows always are)
     const bool aligned = cols % 8 == 0 && (((uintptr_t)x | (uintptr_t)delta | (uintptr_t)w | (uintptr_t)into) & 15) == 0;
     if ((uintptr_t)out & 7) return VL_ERR_UNSUPPORTED;
-    // Pieces a thread: the longer the row, the fewer threads it is worth (us, one piece / two / four: rows of 4,096 bfloat16, 4,096 of them 13.4 / 10.7 / -,
+    // Pieces a thread: the longer the row, the fewer threads it is worth (us, one piece / two / four: rows of 4,096 bfloat16, 4,096 of them 13.4 / 10.7 / -, of 2,048 6.7 / 6.1 / 6.3,
     // of 12,288 - / 30.8 / 25.4, of 25,600 - / - / 35.2, eight 28.2).
     const int pieces = width / 8;
     if (!NORM && sizeof(TX) == 2 && aligned && pieces <= 8192) {
-        const int each = pieces <= 256 ? 1 : pieces <= 1024 ? 2 : pieces <= 2048 ? 4 : 8;
+        const int each = pieces <= 128 ? 1 : pieces <= 1024 ? 2 : pieces <= 2048 ? 4 : 8;
         const dim3 threads(((pieces + each - 1) / each + 31) / 32 * 32);
 #define ROWS(n) vl_launch_waiting(bf16_rows_8bit_kernel<n>, dim3(R), threads, 0, s, (const bf16*)x, (unsigned char*)out, scale, cols, width)
         switch (each) {
