@@ -1,8 +1,9 @@
 // Products of 8-bit rows and 8-bit weights with everything that follows them in one pass:
 //     y[m, n] = f(sa[m] sw[n] sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n]
 // a [M, width] e4m3 with a scale a row (rows_8bit.cu), w packed e4m3 with a scale an output row (vl_pack_8bit), sums,
-// scales, bias, activation and residual in float32, one rounding to out's type.  f: none, a function of one argument, or
-// (gated) f(gate) * up with w's rows in blocks of 8 gates and their 8 ups: out then has N / 2 columns.
+// scales, bias, activation and residual in float32, one rounding to out's type.  A sum is multiplied by w's scale first and by its row's then, in
+// every kernel: times the scale of a row of large numbers alone it may overflow, and the two scales' product alone may be no normal number.
+// f: none, a function of one argument, or (gated) f(gate) * up with w's rows in blocks of 8 gates and their 8 ups: out then has N / 2 columns.
 #include "tc5.cuh"
 #include <cuda_fp8.h>
 #include <math.h>
@@ -106,10 +107,10 @@ __device__ __forceinline__ void finish(float (&v)[CHUNK], TO (&x)[CHUNK / (GATED
 #pragma unroll
     for (int c = 0; c < CHUNK; c += 4) {
         const float4 s = s4[c / 4];
-        v[c] = v[c] * s.x * sw + b;
-        v[c + 1] = v[c + 1] * s.y * sw + b;
-        v[c + 2] = v[c + 2] * s.z * sw + b;
-        v[c + 3] = v[c + 3] * s.w * sw + b;
+        v[c] = v[c] * sw * s.x + b;
+        v[c + 1] = v[c + 1] * sw * s.y + b;
+        v[c + 2] = v[c + 2] * sw * s.z + b;
+        v[c + 3] = v[c + 3] * sw * s.w + b;
     }
     constexpr int STEP = Place<TO, GATED>::STEP, COUNT = Place<TO, GATED>::COUNT;
     if (GATED) {
@@ -486,7 +487,7 @@ gemm_8bit_join_kernel(const float* __restrict__ scratch, Epilogue e, int splits)
             for (int r = 0; r < 4; ++r) v = make_float4(v.x + q[r].x, v.y + q[r].y, v.z + q[r].z, v.w + q[r].w);
         }
         const float4 w = load4<WIDE>(e.w_scale + n + at, left), b = e.bias ? load4<WIDE>(e.bias + n + at, left) : make_float4(0.f, 0.f, 0.f, 0.f);
-        return make_float4(v.x * s * w.x + b.x, v.y * s * w.y + b.y, v.z * s * w.z + b.z, v.w * s * w.w + b.w);
+        return make_float4(v.x * w.x * s + b.x, v.y * w.y * s + b.y, v.z * w.z * s + b.z, v.w * w.w * s + b.w);
     };
     float4 y = scaled(0), r = make_float4(0.f, 0.f, 0.f, 0.f);
     if (e.residual) r = load4<WIDE>(reinterpret_cast<const TO*>(e.residual) + (size_t)m * width + col, left);
@@ -697,11 +698,11 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
             float y = 0.f, u = 0.f;
 #pragma unroll
             for (int v = 0; v < DEEP; ++v) y += red[buf][v][m][place];
-            y = y * (am[o] * ws[o]) + wb[o];
+            y = y * ws[o] * am[o] + wb[o];
             if (e.gated) {
 #pragma unroll
                 for (int v = 0; v < DEEP; ++v) u += red[buf][v][m][place + 8];
-                y = activate(y, e.act) * (u * (am[o] * us[o]) + ub[o]);
+                y = activate(y, e.act) * (u * us[o] * am[o] + ub[o]);
             } else {
                 y = activate(y, e.act);
             }
