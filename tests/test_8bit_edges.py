@@ -36,3 +36,30 @@ def test_gates_and_ups_of_small_rows(m, n, k):
     every = torch.empty(m, n, device=DEV)
     ops.gemm_8bit(a, sa, p, sw, every, act="relu")
     assert ((got.double() - plain.double() * 2.0 ** -117).abs() <= 2.0 ** -149 * (1 + every[:, gate].amax().double())).all()
+
+
+def test_scratch_off_sixteen_bytes_is_refused_before_any_launch():
+    """The entry point itself, which asks before it calls CUDA: the second launch reads the scratch memory 16 bytes at a time."""
+    m, n, k = JOINED[0]
+    columns = ops.eight_bit_columns(k)
+    floats = ops.gemm_8bit_plan(m, n, columns, False)[0]
+    assert floats
+    host = torch.zeros(floats + 8)                            # never read or written
+    at = -host.data_ptr() % 16 + host.data_ptr()
+    for off in (4, 8, 12):
+        code = ops._fn("gemm_8bit", "vl_gemm_8bit")(at, at, at, at, at, ops.F32, None, None, -1, 0, m, n, columns, at + off, floats, 0, None, 0)
+        assert code == -2
+
+
+@gpu
+def test_scratch_of_the_callers_off_sixteen_bytes():
+    m, n, k = JOINED[0]
+    a, sa, w, sw = operands(49, m, n, k)
+    p, floats = ops.pack_8bit(w), ops.gemm_8bit_plan(m, n, ops.eight_bit_columns(k))[0]
+    buf, out = torch.zeros(floats + 8, device=DEV), torch.full((m, n), 3.0, device=DEV)
+    for off in (1, 2, 3):
+        with pytest.raises(ops.KernelError):
+            ops.gemm_8bit(a, sa, p, sw, out, scratch=buf[off:])
+    assert (out == 3).all() and not buf.any()
+    want = ops.gemm_8bit(a, sa, p, sw, torch.empty_like(out))
+    assert torch.equal(ops.gemm_8bit(a, sa, p, sw, out, scratch=buf[4:]), want)

@@ -895,6 +895,7 @@ static int launch_many(const void* a, const void* w, const Epilogue& e, int widt
     const Plan p = plan_of(e.M, e.N, width / KB, overlapped);
     if (p.pair) return launch_pair<TO, ACT, GATED>(a, w, e, width, p.bt, err, s);
     if (p.scratch(e.M, e.N) > (scratch ? floats : 0)) return VL_ERR_ARGUMENT;
+    if (p.splits > 1 && ((uintptr_t)scratch & 15)) return VL_ERR_UNSUPPORTED;      // the second launch reads four sums at a time
     return p.per_sm == 2 ? launch_split<TO, ACT, GATED, 2>(a, w, e, width, p.height, p.bt, p.splits, scratch, err, s)
                          : launch_split<TO, ACT, GATED, 1>(a, w, e, width, p.height, p.bt, p.splits, scratch, err, s);
 }

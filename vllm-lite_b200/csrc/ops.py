@@ -1640,8 +1640,8 @@ def gemm_8bit(a, a_scale, w, w_scale, out, bias=None, act=None, gated=False, res
     `rows_8bit`, `add_rmsnorm_8bit`) and packed weights (w: `pack_8bit`, w_scale float32 [N]); float32 sums, scales, bias (float32 [N]) and
     activation, rounded once to out (bfloat16 or float32 [M, N]).  act: one of GEMM_8BIT_UNARY or None.  gated: w's rows are blocks of
     SWIGLU_GROUP gates and their ups, act one of GEMM_8BIT_ACTIVATIONS, out = f(gate) * up [M, N / 2].  residual: out's shape and type, may
-    be out itself.  scratch: float32, at least `gemm_8bit_plan(M, N, width)[0]` numbers that nobody else on the stream needs; without it the call
-    takes its own."""
+    be out itself.  a, w and scratch begin on 16 bytes.  scratch: float32, at least `gemm_8bit_plan(M, N, width)[0]` numbers that nobody else on the
+    stream needs; without it the call takes its own."""
     _need(a, E4M3, "a", 2); _need(a_scale, torch.float32, "a_scale", 1); _need(w, E4M3, "w", 4); _need(w_scale, torch.float32, "w_scale", 1)
     _need(out, None, "out", 2)
     M, columns = a.shape
