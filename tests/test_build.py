@@ -61,6 +61,44 @@ def test_no_lane_leaves_a_loop_by_itself_when_a_wait_runs_out(name):
     assert "__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity))" in (build.CSRC / "tc5.cuh").read_text()
 
 
+def eight_bit_sources():
+    """The 8-bit product's source without comments, by namespace, and its host side."""
+    code = re.sub(r"//[^\n]*", "", (build.CSRC / "gemm_8bit.cu").read_text())
+    starts = [code.index(f"namespace {n} {{") for n in ("pair8", "split8", "few8")] + [code.index("static int map_rows")]
+    assert starts == sorted(starts)
+    return dict(zip(("pair8", "split8", "few8"), (code[a:b] for a, b in zip(starts, starts[1:]))), host=code[starts[-1]:])
+
+
+def test_the_8bit_product_of_paired_blocks_has_no_path_to_dependent_launch():
+    parts = eight_bit_sources()
+    launcher = parts["host"][parts["host"].index("static int launch_pair("):]
+    launcher = launcher[:launcher.index("\n}\n")]
+    assert "ProgrammaticStreamSerialization" not in parts["host"] and "vl_launch" not in launcher and "vl_pdl_enabled" not in launcher
+    assert re.search(r"cfg\.numAttrs\s*=\s*1\s*;", launcher) and parts["host"].count("numAttrs") == 1
+    assert launcher.count("cudaLaunchKernelEx") == 1 and parts["host"].count("cudaLaunchKernelEx") == 1
+    assert "gemm_8bit_pair_kernel" in launcher and parts["host"].count("gemm_8bit_pair_kernel") == 1
+    # tensor memory and the cluster's barrier are taken behind the wait for the kernels before, by whoever takes them
+    pair, split = parts["pair8"], parts["split8"]
+    assert 0 < pair.index("pdl_wait();") < min(pair.index("alloc_pair("), pair.index("cluster_sync();"))
+    assert "pdl_launch_dependents" not in pair
+    before = split[:split.index("tc5_alloc(")]
+    assert "if (!ahead) pdl_wait();" in before and "if (ahead) pdl_wait();" in before
+
+
+def test_no_lane_of_the_8bit_product_leaves_a_loop_by_itself_when_a_wait_runs_out():
+    """Waits are given up by the vote of a warp, but for the one thread that copies in the kernel of few rows and the waits that note it and go on."""
+    parts = eight_bit_sources()
+    lonely = re.compile(r"if\s*\(\s*!\s*mbar_wait_bounded")
+    assert "warp_wait(" in parts["pair8"] and "warp_wait(" in parts["split8"]
+    assert not lonely.search(parts["pair8"]) and not lonely.search(parts["split8"])
+    few = parts["few8"]
+    copies = few[few.index("if (warp == WARPS) {"):few.index("pdl_wait();\n    const int deep")]
+    assert len(lonely.findall(few)) == len(lonely.findall(copies)) == 1
+    assert copies.index("if (elect_one()) {") < lonely.search(copies).start() < copies.rindex("return;")
+    rest = few[few.index("const int deep"):]
+    assert "wait_or_note(" in rest and "mbar_wait" not in rest and "return" not in rest[:rest.index("if (threadIdx.x == 0 && gave_up")]
+
+
 def test_capped_scores_are_scaled_and_then_capped():
     """The two-at-a-time form of `shape_score` keeps its order: the score times the scale, that times 2 / cap.  The factors' own product first rounds
     elsewhere, which moves last bits of every capped layer."""

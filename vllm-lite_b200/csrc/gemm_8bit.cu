@@ -205,6 +205,9 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         mbar_fence_init();
         failed = 0;
     }
+    // Never launched as a programmatic dependent (see launch_pair); the order is kept all the same: nothing of the SM pair, tensor memory or the
+    // cluster's barrier, is taken while earlier kernels run.
+    pdl_wait();
     __syncthreads();
     cluster_sync();                                          // the other block's mbarriers exist before anything arrives there
     unsigned tmem_base = 0;
