@@ -105,7 +105,8 @@ __device__ __forceinline__ void store_8bit(unsigned char* p, const float (&v)[8]
 }  // namespace
 
 // One block a row, the row in registers: a thread holds PIECES pieces of eight neighbouring columns, piece by piece over the block's threads.  Bound by
-// the bytes: one read of x (and delta), one write of each result.  The order of the sums is a function of the row's length alone, whatever the block's shape.
+// the bytes: one read of x (and delta), one write of each result.  The order of the sums is a function of the row's length and of whether rows
+// lie on 16-byte boundaries, whatever the block's shape and however many rows there are.
 template <typename TX, typename TD, int PIECES, bool NORM, bool ALIGNED>
 __global__ void __launch_bounds__(ALIGNED ? 1024 : 512)
 rows_8bit_kernel(const TX* x, const TD* __restrict__ delta, const int* __restrict__ rows, const float* __restrict__ w, TX* into,
@@ -215,7 +216,8 @@ bf16_rows_8bit_kernel(const bf16* __restrict__ x, unsigned char* __restrict__ ou
     if (threadIdx.x == 0) scale[r] = __uint_as_float(top) / TOP;
 }
 
-// The same for rows that no block's registers hold (more than 32,768 columns, 16,384 off the 16-byte boundaries): three passes, element by element.
+// The same for rows that no block's registers hold (more than 32,768 columns, 65,536 of bfloat16 rows as they are; off the 16-byte boundaries, or where
+// the columns are no multiple of eight, 16,384): three passes, element by element.
 template <typename TX, typename TD>
 __global__ void __launch_bounds__(1024)
 long_rows_8bit_kernel(const TX* x, const TD* __restrict__ delta, const int* __restrict__ rows, const float* __restrict__ w, TX* into,
