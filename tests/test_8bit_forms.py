@@ -6,7 +6,8 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from test_8bit import DEV, F8, JOINED, PAIRED, check_product, check_rows, columns, empty_rows, norm_of, normal, operands
+from test_8bit import (DEV, JOINED, LOW, PAIRED, check_product, check_rows, columns, dependent, empty_rows, norm_of, normal,  # noqa: F401
+                       operands, run_product)
 from vllm_lite_b200.csrc import ops
 
 gpu = pytest.mark.gpu
@@ -156,3 +157,24 @@ def test_a_recorded_step_whose_products_run_on_pairs_of_sms():
     runner.check_device_errors()
     assert runner.graph_replays == 1 and torch.equal(again, first)
     check_gate_up(runner, w, sw, "g2048.1024.", 2048)
+
+
+MIDDLE = [(64, 30000, 2048), (40, 29001, 2100)]              # tiles of 112 rows of w
+
+
+def test_the_sizes_reach_low_tiles():
+    for sizes, height in ((LOW, 96), (MIDDLE, 112), (PAIRED, 256), (JOINED, 128), ([(16, 20000, 2048)], 0)):
+        for m, n, k in sizes:
+            assert [ops.gemm_8bit_tile(m, n, columns(k), overlapped) for overlapped in (False, True)] == [height, height]
+    with pytest.raises(ops.KernelError):
+        ops.gemm_8bit_tile(64, 4096, 100)
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", MIDDLE)
+def test_tiles_of_112_rows(m, n, k, dependent):
+    run_product(m, n, k, dict(bias=True, act="silu", residual=True))
+    run_product(m, n, k, dict(bias=True), torch.bfloat16)
+    if n % 16 == 0:
+        run_product(m, n, k, dict(gated=True, act="silu", residual=True, bias=True))
+        run_product(m, n, k, dict(gated=True, act="silu"), torch.bfloat16)

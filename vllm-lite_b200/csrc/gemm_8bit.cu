@@ -925,15 +925,16 @@ static int launch(const void* a, const void* w, const Epilogue& e, int width, fl
     }
 }
 
-// What a product of these sizes wants: plan[0] floats of scratch memory; plan[1]: whether it runs as clusters of blocks.  overlapped: whether it is among
-// launches that start as programmatic dependents; the launch is told the same.
+// What a product of these sizes wants: plan[0] floats of scratch memory; plan[1]: whether it runs as clusters of blocks; plan[2]: w's rows of a tile, 0 for
+// few rows of a.  overlapped: whether it is among launches that start as programmatic dependents; the launch is told the same.
 extern "C" int vl_gemm_8bit_plan(int M, int N, int width, int overlapped, long long* plan) {
     if (!plan || width <= 0 || width % KB) return VL_ERR_ARGUMENT;
-    plan[0] = plan[1] = 0;
+    plan[0] = plan[1] = plan[2] = 0;
     if (M <= 16 || N <= 0) return VL_OK;
     const Plan p = plan_of(M, N, width / KB, overlapped != 0);
     plan[0] = p.scratch(M, N);
     plan[1] = p.pair;
+    plan[2] = p.height;
     return VL_OK;
 }
 

@@ -1624,11 +1624,22 @@ def gemm_8bit_plan(M, N, columns, overlapped=None):
 def _gemm_8bit_plan(M, N, columns, overlapped):
     if M <= GEMM_8BIT_FEW:
         return 0, False
-    plan = (ctypes.c_longlong * 2)()
+    plan = _plan_of_8bit(M, N, columns, overlapped)
+    return int(plan[0]), bool(plan[1])
+
+
+def _plan_of_8bit(M, N, columns, overlapped):
+    plan = (ctypes.c_longlong * 3)()
     code = _fn("gemm_8bit", "vl_gemm_8bit_plan")(M, N, columns, int(overlapped), ctypes.addressof(plan))
     if code:
         raise KernelError(f"vl_gemm_8bit_plan refused {M} rows, {N} weights of {columns} columns: {_ERRORS.get(code, code)}")
-    return int(plan[0]), bool(plan[1])
+    return plan
+
+
+def gemm_8bit_tile(M, N, columns, overlapped=None):
+    """Rows of w that a tile of `gemm_8bit` takes, arguments as `gemm_8bit_plan` has them: 256 on pairs of SMs, 128, 112 or 96 on one, 0 where few rows of
+    a run without tiles."""
+    return int(_plan_of_8bit(M, N, columns, _pdl if overlapped is None else overlapped)[2])
 
 
 GEMM_8BIT_ACTIVATIONS = ("silu", "relu")                          # f(gate) * up
