@@ -335,3 +335,15 @@ def test_the_library_product_is_torchs_own_in_all_its_forms():
         ops.mm(a, w, torch.empty(1, 3))
     with pytest.raises(TypeError):
         ops.mm(a, w, None)
+
+
+def test_the_blocks_of_the_8bit_product_of_few_rows_fit_the_sms_as_often_as_they_say():
+    """Shared memory of a block (ring, two buffers of sums, barriers) and the kilobyte that the system keeps of each, of an SM's 228 KB."""
+    host = eight_bit_sources()["host"]
+    variants = re.findall(r"launch_few<TO, (\d), (\d), (\d), (\d)>", host)
+    assert len(variants) == 3
+    for mt, ns, stages, per_sm in (map(int, v) for v in variants):
+        deep = 8 // ns
+        stage = ns * deep * 16 * 128 + deep * mt * 8 * 128
+        sums = deep * mt * 8 * (ns * 16 + 1) * 4
+        assert per_sm * (stages * stage + 2 * sums + 16 * stages + 16 + 1024) <= 228 * 1024, (mt, ns, stages, per_sm)

@@ -547,10 +547,9 @@ template <int MT, int NS> struct Shape {
     static constexpr int DEEP = WARPS / NS;                   // blocks of K of a stage
     static constexpr unsigned W_STRIP = DEEP * BLOCK_BYTES, A_OFF = NS * W_STRIP, A_BYTES = DEEP * MT * 8 * KB, STAGE_BYTES = A_OFF + A_BYTES;
     static constexpr int OUTS = MT * NS > 2 ? MT * NS / 2 : 1;       // outputs of a thread
-    // the sums of a tile's warps: twice, so that a tile's are added while the next tile's arrive, where two blocks of an SM leave the room
-    static constexpr int BUFS = MT <= 2 ? 2 : 1;
+    // the sums of a tile's warps: twice, so that a tile's are added while the next tile's arrive
     typedef float Sums[DEEP][MT * 8][NS * STRIP + 1];
-    static constexpr unsigned smem(int stages) { return stages * STAGE_BYTES + BUFS * (unsigned)sizeof(Sums) + 16 * stages + 16; }
+    static constexpr unsigned smem(int stages) { return stages * STAGE_BYTES + 2 * (unsigned)sizeof(Sums) + 16 * stages + 16; }
 };
 
 template <typename TO, int MT, int NS, int STAGES, int PER_SM>
@@ -560,7 +559,7 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
     constexpr int DEEP = S::DEEP, OUTS = S::OUTS;
     extern __shared__ __align__(1024) unsigned char ring[];   // (nothing else is shared: it begins on a kilobyte)
     typename S::Sums* red = reinterpret_cast<typename S::Sums*>(ring + STAGES * S::STAGE_BYTES);
-    unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(red + S::BUFS);
+    unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(red + 2);
     unsigned long long* empty_bar = full_bar + STAGES;
     volatile int& gave_up = *reinterpret_cast<volatile int*>(empty_bar + STAGES);
     const int warp = warp_number(), lane = threadIdx.x & 31;
@@ -635,7 +634,7 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
     const TO* res = reinterpret_cast<const TO*>(e.residual);
     int s = 0, buf = 0;
     unsigned phase = 0;
-    for (int strip = blockIdx.x * NS; strip < strips; strip += gridDim.x * NS, buf = (buf + 1) % S::BUFS) {
+    for (int strip = blockIdx.x * NS; strip < strips; strip += gridDim.x * NS, buf ^= 1) {
         // only asked for here: a use would wait for memory
         float am[OUTS], ws[OUTS], wb[OUTS], us[OUTS], ub[OUTS];
         TO yr[OUTS];
@@ -711,7 +710,6 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
             }
             out[(size_t)m * ld + col] = from_f32<TO>(y + to_f32(yr[o]));
         }
-        if (S::BUFS == 1) asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
     }
     if (threadIdx.x == 0 && gave_up && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_GEMM_8BIT);
 }
@@ -905,12 +903,13 @@ static int launch_many(const void* a, const void* w, const Epilogue& e, int widt
 
 template <typename TO>
 static int launch(const void* a, const void* w, const Epilogue& e, int width, float* scratch, long long floats, bool overlapped, unsigned* err, cudaStream_t s) {
-    // Up to 8 rows: strips one by one, four stages of 16 + 8 KB and two blocks an SM.  Up to 16: in twos where that leaves more tiles than SMs (each
-    // strip's copy of a is half the bytes then: x 4,096 -> 24,576 19.3 us and 24.8, -> 6,144 6.9 and 9.1), else one by one with two stages and
-    // three blocks an SM (x 12,288 -> 4,096 12.2 and 14.6).
+    // Two blocks an SM.  Up to 8 rows: strips one by one, four stages of 16 + 8 KB.  Up to 16: in twos where that leaves more tiles than SMs, each strip's copy of a
+    // being half the bytes then, else one by one with two stages of 16 + 16 KB (a third passes half an SM).  16 rows of 4,096, in twos / one by one, us overlapped:
+    // -> 4,096 6.5 / 4.9, -> 6,144 7.4 / 7.7, -> 8,192 7.6 / 8.1, -> 18,432 13.3 / 14.7; where the last round of the twos holds few tiles they lose: -> 10,240
+    // 11.6 / 9.4, -> 24,576 18.4 / 17.9.
     if (e.M <= 8) return launch_few<TO, 1, 1, 4, 2>(a, w, e, width, err, s);
     if (e.M <= 16)
-        return (e.N + 2 * STRIP - 1) / (2 * STRIP) > sm_count() ? launch_few<TO, 2, 2, 4, 2>(a, w, e, width, err, s) : launch_few<TO, 2, 1, 2, 3>(a, w, e, width, err, s);
+        return (e.N + 2 * STRIP - 1) / (2 * STRIP) > sm_count() ? launch_few<TO, 2, 2, 4, 2>(a, w, e, width, err, s) : launch_few<TO, 2, 1, 2, 2>(a, w, e, width, err, s);
     if (e.gated)
         return e.act == ACT_SILU ? launch_many<TO, ACT_SILU, true>(a, w, e, width, scratch, floats, overlapped, err, s)
                                  : launch_many<TO, ACT_RELU, true>(a, w, e, width, scratch, floats, overlapped, err, s);
