@@ -74,3 +74,32 @@ def test_a_timed_step_records_every_dense_product(monkeypatch):
     got = bench.timed_step(SimpleNamespace(step=step, decode_graphs=True), [])
     assert {k: v[0] for k, v in got.items()} == {n: 1 for n in bench.DENSE_PRODUCTS if n != "gemm_f32"}
     assert before == {n: getattr(ops, bench.OP_OF.get(n, n)) for n in bench.TIMED_OPS}
+
+
+def test_a_prompts_floor_with_products_in_8_bits():
+    """Half the layers' products' time goes; attention and the head stay at the bfloat16 rate.  8B sizes: 28.5 of the prompt's 29.7 TFLOP are products
+    of the layers (36 of 192.9 million elements, 2,048 tokens), 139,000 tokens/s are 0.61 of the floor's rate, not 1.18 of it."""
+    cfg = dict(bench.QWEN3_8B)
+    flops = bench.model_bytes_and_flops(cfg, 36)[2]
+    elements = (32 + 16) * 128 * 4096 + 4096 * 4096 + 3 * 4096 * 12288
+    assert bench.layer_elements(cfg) == elements
+    rate = 1702.9
+    assert abs(bench.prefill_floor_ms(cfg, 36, rate) / (flops / (rate * 1e9)) - 1) < 1e-9
+    floor = bench.prefill_floor_ms(cfg, 36, rate, eight_bit=True)
+    products = 2 * 2048 * 36 * elements
+    assert abs(floor / ((flops - products) / (rate * 1e9) + products / (2 * rate * 1e9)) - 1) < 1e-9
+    assert abs(floor / (2048 / 139000 * 1e3) - 0.615) < 0.01
+    # what stands in the output is this floor over the time, wherever a prompt is timed
+    code = Path(bench.__file__).read_text()
+    main = code[code.index("def main("):]
+    assert "prefill_flops" not in main and main.count("prefill_floor_ms(") == 3
+
+
+def test_bytes_a_decode_step_reads_with_products_in_8_bits():
+    """A byte an element of the layers' matrices and four a row of them; the head stays bfloat16, norms and cache as they were."""
+    cfg = dict(bench.QWEN3_8B)
+    wide, kv, flops = bench.model_bytes_and_flops(cfg, 36)
+    narrow, kv8, flops8 = bench.model_bytes_and_flops(cfg, 36, True)
+    rows = (32 + 2 * 8) * 128 + 4096 + 2 * 12288 + 4096
+    assert (kv8, flops8) == (kv, flops) and wide - narrow == 36 * (bench.layer_elements(cfg) - 4 * rows)
+    assert abs(narrow / 1e9 - 8.198) < 0.02
