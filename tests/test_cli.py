@@ -80,3 +80,29 @@ def test_the_engine_has_no_cpu_path():
     from vllm_lite_b200.engine import ModelRunner, StepError
     with pytest.raises(StepError, match="CUDA device only"):
         ModelRunner(None, {}, device="cpu")
+
+
+@pytest.mark.parametrize("flags,eight_bit", [([], False), (["--eight-bit"], True)])
+def test_the_engine_is_told_whether_products_run_in_8_bits(flags, eight_bit, monkeypatch, capsys):
+    import vllm_lite_b200.engine as engine
+    seen = []
+
+    class Engine:
+        def __init__(self, model, **kw):
+            seen.append(kw)
+
+        def generate(self, prompts, max_tokens, sampling_params):
+            return [[7, 8] for _ in prompts]
+
+        def stats(self):
+            return {}
+
+    monkeypatch.setattr(engine, "LLMEngine", Engine)
+    assert cli.main(["--model", str(H.model_dir("A")), "--prompt-ids", "1,2"] + flags) == 0
+    assert capsys.readouterr().out == "7,8\n" and len(seen) == 1 and seen[0]["eight_bit"] is eight_bit
+
+
+def test_products_in_8_bits_with_float32_activations_are_refused_before_a_model_is_read(capsys):
+    with pytest.raises(SystemExit) as e:
+        cli.main(["--model", str(H.model_dir("A")), "--prompt-ids", "1,2", "--eight-bit", "--dtype", "float32"])
+    assert e.value.code == 2 and "--eight-bit" in capsys.readouterr().err

@@ -107,6 +107,8 @@ def main(argv=None) -> int:
         ap.error("--tensor-parallel-size: this engine runs on one GPU")
     if args.kv_quantization:
         ap.error("--kv-quantization: the cache is not quantized in this engine")
+    if args.eight_bit and args.dtype != "bfloat16":
+        ap.error("--eight-bit: products in 8 bits go with --dtype bfloat16")
     prompts = read_prompts(args.prompt_ids)
     if not prompts:
         ap.error("give at least one prompt with --prompt-ids")
