@@ -82,8 +82,8 @@ class ModelRunner:
         """`num_pages`: pages of every paged group (an int, or one count per group), or None: the pools are
         then sized from the device memory that is free once the model is built (`memory_fraction` of it,
         less a reserve for the activations of steps of up to `max_step_tokens` tokens; cache/sizing.py).
-        `own_weights`: the dict is emptied once the model holds its tensors, so that what the model stacked
-        into new matrices (q/k/v, gate/up) is freed before memory is measured.  `free_memory_bytes` stands
+        `own_weights`: the dict is emptied, layer by layer while the model is built, so that what the model made new
+        matrices of (q/k/v, gate/up, weights in 8 bits) is freed at once and before memory is measured.  `free_memory_bytes` stands
         in for the measurement (tests)."""
         self.device = torch.device(device)
         if self.device.type != "cuda":
@@ -94,7 +94,7 @@ class ModelRunner:
         self.dtype = dtype
         self.page_size = int(page_size)
         torch.cuda.set_device(self.device)
-        self.model = CausalLM(plan, weights, BuildContext(self.device, dtype))
+        self.model = CausalLM(plan, weights, BuildContext(self.device, dtype), own_weights)
         self.layout = CacheLayout.from_needs(cache_needs(plan), cache_sources(plan))
         self.max_context = int(max_context or plan.max_position_embeddings)
         if own_weights:

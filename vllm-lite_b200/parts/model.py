@@ -50,14 +50,21 @@ def cache_sources(plan: ModelPlan) -> list:
 
 
 class CausalLM:
-    def __init__(self, plan: ModelPlan, weights: dict, ctx: BuildContext):
+    def __init__(self, plan: ModelPlan, weights: dict, ctx: BuildContext, own_weights: bool = False):
+        """`own_weights`: a layer's tensors leave the dict once the layer is built, so that what it made of them (stacked matrices, matrices in 8
+        bits) takes their place and the model needs no room for a second copy of all layers."""
         plan.validate()
         self.plan = plan
         self.ctx = ctx
         emb, head = plan.embedding_spec, plan.head_spec
         self.embedding = EMBEDDINGS.get(emb.kind)(emb, sub_weights(weights, plan.embed_prefix), ctx)
-        self.layers = [BLOCKS.get(b.kind)(b, sub_weights(weights, plan.layer_prefix.format(i)), ctx)
-                       for i, b in enumerate(plan.layers)]
+        self.layers = []
+        for i, b in enumerate(plan.layers):
+            block, prefix = BLOCKS.get(b.kind), plan.layer_prefix.format(i)
+            self.layers.append(block(b, sub_weights(weights, prefix), ctx))
+            if own_weights:
+                for name in prefixed(block.declare(b), prefix):
+                    weights.pop(name, None)
         self.final_norm = NORMS.get(plan.final_norm.kind)(plan.final_norm,
                                                           sub_weights(weights, plan.final_norm_prefix), ctx)
         self.head = HEADS.get(head.kind)(head, sub_weights(weights, plan.head_prefix), ctx, embedding=self.embedding)
