@@ -1,5 +1,5 @@
 """Linear layers in 8 bits: rows too long for a block's registers, operands off the 16-byte boundaries, a layer with a bias, and steps of a model
-whose products run on pairs of SMs.  Tolerances as in test_8bit.py; the sum of squares of a long row has up to 33 terms a thread and 10 steps of
+whose products run on pairs of SMs or whose weights are stored in float32.  Tolerances as in test_8bit.py; the sum of squares of a long row has up to 33 terms a thread and 10 steps of
 joining, 1.3e-6 of the norm at worst, within the 2e-6 that a scale is given there."""
 from types import SimpleNamespace
 
@@ -178,3 +178,20 @@ def test_tiles_of_112_rows(m, n, k, dependent):
     if n % 16 == 0:
         run_product(m, n, k, dict(gated=True, act="silu", residual=True, bias=True))
         run_product(m, n, k, dict(gated=True, act="silu"), torch.bfloat16)
+
+
+@gpu
+def test_a_model_stored_in_float32():
+    """Its weights reach 8 bits from float32 rows; error bound of whole rows as in test_8bit_model.py."""
+    import helpers as H
+    from test_8bit_model import TOL_RMS
+    from vllm_lite_b200.engine import ModelRunner, StepEntry, load_model_dir
+    _, plan, weights = load_model_dir(H.model_dir("B", "float32"), "bfloat16", DEV, eight_bit=True)
+    assert weights["model.layers.0.mlp.down_proj.weight"].dtype == torch.float32
+    runner = ModelRunner(plan, weights, dtype=torch.bfloat16, device=DEV, page_size=8, num_pages=32, max_requests=4)
+    tokens = H.tokens_for("B", 40, 9)
+    rows = [runner.step([StepEntry("a", tokens[:30], [0, 29])]).float().cpu(), runner.step([StepEntry("a", tokens[30:], [9])]).float().cpu()]
+    runner.check_device_errors()
+    want = H.plain_logits("B", tokens, "float32")[[0, 29, 39]]
+    got = torch.cat(rows)
+    assert ((got - want).norm(dim=1) <= TOL_RMS * want.norm(dim=1)).all()
