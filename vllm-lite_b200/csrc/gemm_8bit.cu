@@ -172,7 +172,8 @@ constexpr int MOST = 256, STAGES = 6, PARTS = 4, EPILOGUE = PARTS * 128, NUM_THR
 constexpr unsigned STAGE_BYTES = W_BYTES + MOST / 2 * KB, TMEM_COLS = 512;
 
 // Tile `place` of the pairs' order: its corner and its rows of a.  From `whole` on places are halves of tiles: where the last round of the pairs
-// has at most half of them a tile, its tiles are cut in two (4,096 x 12,288 -> 4,096, 256 tiles for 74 pairs: 150.0 us in whole tiles, 144.6 so).
+// has at most half of them a tile, its tiles are cut in two (4,096 x 12,288 -> 4,096, 256 tiles for 74 pairs, in short
+// runs: bfloat16 147 us in whole tiles, 140 so, the float32 stream 159 and 151).
 __device__ __forceinline__ int tile_corner(int place, int whole, int tiles_t, int tiles_n, int bt, int& t0, int& n0) {
     const int beyond = place - whole, tile = beyond < 0 ? place : whole + (beyond >> 1);
     constexpr int BAND = 8;                                  // pairs that run together share W's tiles in L2
@@ -324,7 +325,8 @@ gemm_8bit_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 // A block multiplies a run of the blocks of K of `height` rows of W (the 128-row operand; 96 or 112 of them where that spreads the tiles better) and bt rows of a.  Where a tile's K is shared out, the blocks leave their sums in scratch memory,
 // [blocks of a tile, rows of a, W's rows rounded up to whole tiles], and a second launch adds them in the order of K and finishes them; it starts behind the
 // first without a gap.  (Joined through the shared memory of a cluster, x 12,288 -> 4,096 took 14.5 us in a graph at 64 rows and 16.4 in calls
-// behind one another, 13.8 and 15.0 so; kernels of clusters are launched the plain way, and a step that holds one has no programmatic launches.)
+// behind one another, 13.8 and 15.0 so; kernels of clusters are launched the plain way, and a step that holds one has the engine's switch off:
+// only kernels that touch nothing before their wait keep the attribute in it.)
 namespace split8 {
 constexpr int PARTS = 2, NUM_THREADS = 64 + PARTS * 128;      // (sixteen warps of epilogue, as pairs have, start later: x 12,288 -> 4,096 at 64 rows 14.4 us and 15.1)
 
@@ -590,7 +592,7 @@ gemm_8bit_few_kernel(const __grid_constant__ CUtensorMap map_a, const unsigned c
             if (!ahead) pdl_wait();                            // W may be as young as a
             for (int s = 0; s < early; ++s, step()) copy_w(s, strip, it);
             // What lies AHEAD stages behind the ring is asked for into L2: where half of a stage is a's, the ring alone does not keep memory busy (16
-            // rows x 12,288 -> 4,096 12.3 us without, 10.3 two stages ahead, 11.2 four; up to 8 rows 9.2 either way).
+            // rows x 12,288 -> 4,096 11.9 us without, 10.1 two stages ahead, 10.6 four, overlapped; up to 8 rows 9.1 without, 9.6 four).
             constexpr int AHEAD = MT > 1 ? 2 : 0;
             int next_strip = strip, next_it = it, asked = early;
             auto ask = [&]() {

@@ -79,10 +79,11 @@ gemm_tc5_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         mbar_fence_init();
         failed = 0;
     }
-    // This kernel is never launched as a programmatic dependent (see launch_pair), so both calls below do
-    // nothing today.  They stay ahead of everything that takes a shared resource of the SM pair (tensor
+    // This kernel is never launched as a programmatic dependent (see launch_pair), so the wait does nothing
+    // today.  It stays ahead of everything that takes a shared resource of the SM pair (tensor
     // memory, the cluster's barrier): were the attribute ever given, nothing would be held while earlier
-    // kernels of the stream still run.
+    // kernels of the stream still run.  A kernel behind that always carries the attribute (vl_launch_waiting)
+    // may come onto the SMs from the second call on, where it waits for this one's end before all else.
     pdl_wait();                                              // A is written by the kernel before
     pdl_launch_dependents();
     if (warp == 1) alloc_pair(&tmem_base_slot, TMEM_COLS);

@@ -256,8 +256,8 @@ class ModelRunner:
         return entry[1][:B]
 
     def _launches_dependent(self, tokens: int, recorded: bool) -> bool:
-        """`launches_dependent`, and no kernel of clusters among them: those are launched the plain way and stay among plain launches, as the
-        paired products do."""
+        """`launches_dependent`, and no kernel of clusters among them: those are launched the plain way, with the switch off for their whole step, as
+        the paired products are (kernels that touch nothing before their wait carry the attribute all the same: csrc/common.cuh)."""
         clusters = getattr(self.model, "clusters", None)
         return launches_dependent(tokens, recorded, self.model.may_pair) and not (clusters and clusters(tokens))
 
