@@ -32,6 +32,7 @@
 #define VL_DEV_IN_GEMM_GROUPED 0x100000u
 #define VL_DEV_IN_GEMM_FEW 0x200000u
 #define VL_DEV_IN_GEMM_8BIT 0x400000u
+#define VL_DEV_IN_FLASH_8BIT 0x800000u
 // ... and, in the tcgen05 products, which waits gave up in the block (shifted left by 16):
 // 1 a free stage (copying thread), 2 a free accumulator, 4 a filled stage (both: issuing thread),
 // 8 a complete accumulator (epilogue)

@@ -1,0 +1,481 @@
+// Attention of prompt portions over a cache in 8 bits (csrc/cache_8bit.cuh) on the 5th-generation tensor cores (tcgen05.mma, accumulators in TMEM),
+// compiled for one head size: -DFA_HD, a multiple of 16 up to 256.
+//
+// The function is that of csrc/flash_decode_8bit.cu for every token of a list of tiles: a query at position p reads the keys lo..p of its
+// request (lo = 0 or p - window + 1).  Scores, maxima, sums and the output accumulate in float32.
+//
+// A block owns consecutive tokens of one request and ALL query heads of one KV head (up to 128): rows of its one or two query tiles of 128 are
+// (token, head) pairs, so a short portion fills a tile as a long one does and a tile's mask is as sharp as its few tokens.  It walks that request's
+// keys in tiles of 64, which both query tiles read.  Roles:
+//   warps 0..3 (and 4..7), a thread per row   read the scores of a key tile from TMEM, keep the running maximum and sum of their row, write
+//        P as halves into shared memory (128-byte swizzled rows) and, when a row's maximum has grown by more than 2^8, rescale the row's output in
+//        TMEM.  While one query tile's rows are exponentiated the tensor cores work on the other's products;
+//   four warps           bring keys and values: 16 bytes a load into registers, one tile ahead, e4m3 to halves (exact), times a power of two, into two
+//        stages of 128-byte swizzled rows each for keys and values.  The pages' scales are folded in here: page by page 2^(e - E + 7), E the largest
+//        exponent of all pages that the block reads (found first; 448 * 2^7 is below the largest half), so that scores and outputs of all tiles are in one
+//        unit, which a row's own factor and the end undo.  Exact down to pages 2^15 below the largest, to within 2^-41 of the largest number else.
+//        Rows that no query of the block reads, or that the table does not hold (flagged), are zeros.  A page whose scale is not a number gives
+//        keys of NaN and values of zero: who may read it gets NaN, rows that may not replace the score;
+//   one warp             issues S = Q K^T (both K-major) into one of two score buffers a query tile, one issues O += P V (V as stored: N contiguous).
+// Roundings: queries times a power of two of their row (largest number in [2^14, 2^15)) and the probabilities, 2^7 p with p up to 2^8, are halves.
+// Every wait on an mbarrier is bounded; when one expires the block records VL_DEV_WAIT_EXPIRED, stops, and still frees its TMEM.
+#include "cache_8bit.cuh"
+#include "tc5.cuh"
+
+#ifndef FA_HD
+#define FA_HD 128
+#endif
+
+using namespace tc5;
+using namespace cache8;
+
+namespace {
+constexpr int HD = FA_HD;
+static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head sizes in steps of 16 up to 256");
+constexpr int GROUPS = HD <= 128 ? 2 : 1;              // query tiles of 128 rows
+constexpr int BM = 128, BN = 64, CB = (HD + 63) / 64;  // CB: blocks of 64 columns (one swizzled row) a head
+constexpr int SOFT = 4 * GROUPS, QK_WARP = SOFT, PV_WARP = SOFT + 1, LOAD0 = SOFT + 2, LOADERS = 4;
+constexpr int NTHREADS = 32 * (LOAD0 + LOADERS), LOAD_THREADS = 32 * LOADERS;
+constexpr unsigned ROW_BYTES = 128;
+constexpr unsigned Q_BYTES = BM * CB * ROW_BYTES;      // CB blocks of [128 rows][128 bytes]
+constexpr unsigned KV_STAGE = BN * CB * ROW_BYTES;     // CB blocks of [64 rows][128 bytes]
+constexpr unsigned P_BYTES = BM * ROW_BYTES;
+constexpr unsigned TILE_BYTES = GROUPS * (Q_BYTES + P_BYTES) + 4 * KV_STAGE;
+constexpr int FOUND = 4;                               // key tiles whose rows are looked up at a time
+constexpr unsigned SMEM_BYTES = TILE_BYTES + 512 + GROUPS * BM * 4 + FOUND * BN * 12;
+constexpr unsigned TMEM_COLS = 512;                    // scores 2 x 64 a query tile, behind them the outputs
+constexpr unsigned O_COL = GROUPS * 2 * BN;
+constexpr int PIECES = HD / 16, EACH = (BN * PIECES + LOAD_THREADS - 1) / LOAD_THREADS;   // 16-byte pieces of a row, of a tile a thread
+constexpr float RESCALE_ABOVE = 8.0f, P_SHIFT = 7.0f;
+constexpr int FOLD = 7;
+
+__host__ __device__ constexpr unsigned idesc_f16(int m, int n) {       // float32 sums of halves: bits 4-5 = 1, operand types 0
+    return (1u << 4) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(min(max(e, -126), 127) + 127) << 23); }
+__device__ __forceinline__ unsigned long long pair(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(unsigned long long v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+template <bool ACC>
+__device__ __forceinline__ void mma_lo(unsigned tmem_c, unsigned a_lo, unsigned b_lo, unsigned a_hi, unsigned b_hi, unsigned idesc) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %5, 0;\n mov.b64 da, {%1, %2};\n mov.b64 db, {%3, %4};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %6, p;\n}"
+        ::"r"(tmem_c), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(ACC ? 1u : 0u), "r"(idesc) : "memory");
+}
+// byte offset of the 16-byte chunk `chunk` (0..7) of row `row` in a tile of 128-byte swizzled rows
+__device__ __forceinline__ unsigned swizzled(int row, int chunk) { return (unsigned)row * ROW_BYTES + (unsigned)((chunk ^ (row & 7)) << 4); }
+__device__ __forceinline__ unsigned times(unsigned h2, unsigned f2) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h2), *reinterpret_cast<const __half2*>(&f2));
+    return *reinterpret_cast<const unsigned*>(&r);
+}
+// A barrier of the loading warps, and whether all of them still have what they waited for: one whose wait ran out takes the others along.
+__device__ __forceinline__ bool loaders_agree(bool ok) {
+    int all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((int)ok), "n"(LOAD_THREADS) : "memory");
+    return all != 0;
+}
+}  // namespace
+
+// tiles[i] = {row of the block table, index of the tile's first token in the step, tokens (<= 128), position of the first}
+__global__ void __launch_bounds__(NTHREADS, 1)
+flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict__ out, const unsigned char* __restrict__ kcache,
+                      const unsigned char* __restrict__ vcache, const float* __restrict__ kscale, const float* __restrict__ vscale,
+                      const int* __restrict__ block_table, int max_blocks, const int4* __restrict__ tiles, int num_tiles, int nq, int nkv, int page_size,
+                      int num_pages, float scale_log2, int window, unsigned* err, int heads, int htiles, int tokens, int cuts) {
+    extern __shared__ __align__(1024) unsigned char smem[];              // (the block's only shared memory, so it begins the window)
+    unsigned char* Qs = smem;                                            // GROUPS
+    unsigned char* Ks = Qs + GROUPS * Q_BYTES;                           // 2 stages
+    unsigned char* Vs = Ks + 2 * KV_STAGE;                               // 2 stages
+    unsigned char* Ps = Vs + 2 * KV_STAGE;                               // GROUPS
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + TILE_BYTES);
+    unsigned long long *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;
+    unsigned long long *s_full = bars + 8, *s_free = bars + 12, *p_full = bars + 16, *pv_done = bars + 18;    // [GROUPS][2], [GROUPS]
+    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(bars + 20);
+    int* words = reinterpret_cast<int*>(bars + 21);
+    int &failed = words[0], &top_k = words[1], &top_v = words[2];
+    float* s_row_scale = reinterpret_cast<float*>(smem + TILE_BYTES + 512);                      // [GROUPS * BM]
+    int* s_krow = reinterpret_cast<int*>(s_row_scale + GROUPS * BM);                             // [FOUND][BN] cache rows, -1: zeros
+    int* s_vrow = s_krow + FOUND * BN;
+    unsigned* s_fold = reinterpret_cast<unsigned*>(s_vrow + FOUND * BN);                         // factor of the key (low half) and of the value
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(smem) & 1023u) {                                        // (uniform) never expected; the tiles would be misread
+        if (tid == 0 && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_FLASH_8BIT);
+        return;
+    }
+    pdl_launch_dependents();
+    pdl_wait();                                                          // q and the cache are written by the kernel before
+    // the blocks with the longest rows of keys first
+    const int number = num_tiles * cuts - 1 - (int)blockIdx.y, cut = number % cuts;
+    const int4 tile = tiles[number / cuts];
+    const int skip = cut * GROUPS * tokens, count = min(GROUPS * tokens, tile.z - skip);         // this block's tokens
+    if (count <= 0) return;
+    const int req = tile.x, tok0 = tile.y + skip, pos0 = tile.w + skip;
+    const int kvh = (int)blockIdx.x / htiles, grp = nq / nkv, hbase = ((int)blockIdx.x % htiles) * heads;
+    const int nheads = min(heads, grp - hbase), h0 = kvh * grp + hbase;
+    const int groups = GROUPS == 2 && count > tokens ? 2 : 1;
+    const int hi = pos0 + count - 1;                                     // the last key any row reads
+    const int lo = (window > 0 && pos0 - window + 1 > 0) ? pos0 - window + 1 : 0;                // the first
+    const int jt0 = lo / BN, n_tiles = hi / BN - jt0 + 1;
+    const int* table = block_table + (size_t)req * max_blocks;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], LOAD_THREADS); mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], LOAD_THREADS); mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < 2 * GROUPS; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], BM); }
+        for (int i = 0; i < GROUPS; ++i) { mbar_init(&p_full[i], BM); mbar_init(&pv_done[i], 1); }
+        mbar_fence_init();
+        failed = 0;
+        top_k = top_v = EXP_MIN;
+    }
+    if (warp == QK_WARP) tc5_alloc(&tmem_slot, TMEM_COLS);
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    const unsigned tmem_base = tmem_slot;
+
+    // the largest exponents of the pages that the block reads
+    {
+        int ek = EXP_MIN, ev = EXP_MIN;
+        for (int blk = lo / page_size + tid; blk <= hi / page_size; blk += NTHREADS) {
+            const int page = blk < max_blocks ? table[blk] : -1;
+            if (page < 0 || page >= num_pages) continue;
+            const float ks = kscale[(size_t)page * nkv + kvh], vs = vscale[(size_t)page * nkv + kvh];
+            if (ks == ks) ek = max(ek, (int)(__float_as_uint(ks) >> 23) - 127);
+            if (vs == vs) ev = max(ev, (int)(__float_as_uint(vs) >> 23) - 127);
+        }
+        ek = __reduce_max_sync(0xffffffffu, ek);
+        ev = __reduce_max_sync(0xffffffffu, ev);
+        if (lane == 0) { atomicMax(&top_k, ek); atomicMax(&top_v, ev); }
+    }
+    // the queries as halves, a warp a row (a lane 8 features), several rows on their way; rows of no token are zeros
+    constexpr int AHEAD = 8;
+    for (int r0 = warp; r0 < groups * BM; r0 += AHEAD * (NTHREADS / 32)) {
+        uint4 raw[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int r = r0 + u * (NTHREADS / 32), rr = r & (BM - 1), tk = (r / BM) * tokens + rr / heads, h = rr % heads;
+            const bool live = r < groups * BM && rr < tokens * heads && tk < count && h < nheads && lane < HD / 8;
+            raw[u] = live ? *reinterpret_cast<const uint4*>(q + (size_t)(tok0 + tk) * q_stride + (size_t)(h0 + h) * HD + lane * 8) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int r = r0 + u * (NTHREADS / 32), rr = r & (BM - 1);
+            if (r >= groups * BM) continue;                              // (warp-uniform)
+            unsigned* w = &raw[u].x;
+            unsigned top = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+            top = __reduce_max_sync(0xffffffffu, top);
+            const int e = top == 0 || top >= 0x7f80u ? 0 : max(-112, (int)(top >> 7) - 127 - 14);
+            const float f = power_of_two(-e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack_half(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+            if (lane < HD / 8)
+                *reinterpret_cast<uint4*>(Qs + (r / BM) * Q_BYTES + (unsigned)(lane >> 3) * (BM * ROW_BYTES) + swizzled(rr, lane & 7)) = raw[u];
+            if (lane == 0) s_row_scale[r] = scale_log2 * power_of_two(e);
+        }
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+
+    const int role = warp_number();
+    if (role >= LOAD0) {                                                 // ---- keys and values ----
+        const int ct = tid - LOAD0 * 32;
+        const int EK = top_k, EV = top_v;
+        // Thread k < 64 looks up key k of every tile, in three steps one tile apart, so that no load is waited for: the page, its scales, and what they say.
+        struct Found { int page, at; float ks, vs; };
+        auto page_of = [&](int it) -> Found {
+            Found f = {-1, 0, 0.f, 0.f};
+            const int key = (jt0 + it) * BN + ct;
+            if (ct >= BN || it >= n_tiles || key < lo || key > hi) return f;
+            const int blk = key / page_size;
+            f.at = key - blk * page_size;
+            f.page = blk < max_blocks ? table[blk] : -1;
+            if (f.page < 0 || f.page >= num_pages) { f.page = -1; if (err) atomicOr(err, VL_DEV_BAD_PAGE); }
+            return f;
+        };
+        auto scales_of = [&](Found& f) {
+            if (f.page >= 0) { f.ks = kscale[(size_t)f.page * nkv + kvh]; f.vs = vscale[(size_t)f.page * nkv + kvh]; }
+        };
+        auto note = [&](const Found& f, int it) {
+            if (ct >= BN) return;
+            const int at = (it % FOUND) * BN + ct, row = f.page < 0 ? -1 : (f.page * nkv + kvh) * page_size + f.at;
+            const bool none = f.ks != f.ks || f.vs != f.vs;
+            s_krow[at] = row;
+            s_vrow[at] = f.vs != f.vs ? -1 : row;
+            const __half fk = none ? __ushort_as_half(0x7e00) : __float2half_rn(f.ks * power_of_two(FOLD - EK)), fv = __float2half_rn(f.vs != f.vs ? 0.f : f.vs * power_of_two(FOLD - EV));
+            s_fold[at] = (unsigned)__half_as_ushort(fk) | ((unsigned)__half_as_ushort(fv) << 16);
+        };
+        auto load = [&](uint4 (&x)[EACH], bool v, int it) {
+            const int* rows = (v ? s_vrow : s_krow) + (it % FOUND) * BN;
+            const unsigned char* cache = v ? vcache : kcache;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
+                const int row = idx < BN * PIECES ? rows[r] : -1;
+                x[i] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(cache + (size_t)row * HD + c * 16)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        auto store = [&](const uint4 (&x)[EACH], bool v, int it) {
+            unsigned char* st = (v ? Vs : Ks) + (unsigned)(it & 1) * KV_STAGE;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
+                if (idx >= BN * PIECES) continue;
+                const unsigned both = s_fold[(it % FOUND) * BN + r], f = v ? __byte_perm(both, both, 0x3232) : __byte_perm(both, both, 0x1010);
+                const unsigned* w = &x[i].x;
+                uint4 a, b;
+                a.x = times(half2_low(w[0]), f); a.y = times(half2_high(w[0]), f); a.z = times(half2_low(w[1]), f); a.w = times(half2_high(w[1]), f);
+                b.x = times(half2_low(w[2]), f); b.y = times(half2_high(w[2]), f); b.z = times(half2_low(w[3]), f); b.w = times(half2_high(w[3]), f);
+                unsigned char* blk = st + (unsigned)(c >> 2) * (BN * ROW_BYTES);
+                const int ch = 2 * (c & 3);
+                *reinterpret_cast<uint4*>(blk + swizzled(r, ch)) = a;
+                *reinterpret_cast<uint4*>(blk + swizzled(r, ch + 1)) = b;
+            }
+        };
+        Found f0 = page_of(0), f1 = page_of(1), f2 = page_of(2);
+        scales_of(f0);
+        scales_of(f1);
+        note(f0, 0);
+        note(f1, 1);
+        bool ok = loaders_agree(true);
+        uint4 xk[EACH], xv[EACH];
+        load(xk, false, 0);
+        // keys run one tile ahead of values: the scores of tile i + 1 are issued before the second product of tile i
+        for (int step = 0; step <= n_tiles; ++step) {
+            scales_of(f2);                                               // of tile step + 2
+            const Found f3 = page_of(step + 3);
+            if (step < n_tiles && step >= 2) ok = warp_wait(&k_empty[step & 1], (unsigned)((step / 2 - 1) & 1));
+            if (step < n_tiles && ok) {
+                store(xk, false, step);
+                fence_proxy_async_smem();
+                mbar_arrive(&k_full[step & 1]);
+                if (step + 1 < n_tiles) load(xk, false, step + 1);
+            }
+            const int it = step - 1;
+            if (it >= 2 && ok) ok = warp_wait(&v_empty[it & 1], (unsigned)((it / 2 - 1) & 1));
+            if (it >= 0 && ok) {
+                store(xv, true, it);
+                fence_proxy_async_smem();
+                mbar_arrive(&v_full[it & 1]);
+            }
+            if (step < n_tiles) load(xv, true, step);
+            note(f2, step + 2);
+            f2 = f3;
+            ok = loaders_agree(ok);
+            if (!ok) break;
+        }
+        if (!ok && lane == 0) atomicExch(&failed, 1);
+    } else if (role == QK_WARP) {                                        // ---- issuer of the scores S = Q K^T ----
+        const bool lead = elect_one();
+        constexpr unsigned idesc = idesc_f16(BM, BN);
+        const unsigned long long dq = make_smem_desc(Qs), dk = make_smem_desc(Ks);
+        const unsigned q_lo = (unsigned)dq, k_lo = (unsigned)dk, hi_word = (unsigned)(dq >> 32);
+        bool ok = true;
+        for (int it = 0; it < n_tiles && ok; ++it) {
+            const int s = it & 1;
+            if (!warp_wait(&k_full[s], (unsigned)((it / 2) & 1))) { ok = false; break; }
+            for (int gr = 0; gr < groups; ++gr) {
+                // the score buffer is free once every row of the tile two before has been read
+                if (it >= 2 && !warp_wait(&s_free[gr * 2 + s], (unsigned)((it / 2 - 1) & 1))) { ok = false; break; }
+                tc5_fence_after();
+                const unsigned qb = q_lo + (unsigned)gr * (Q_BYTES >> 4), kb = k_lo + (unsigned)s * (KV_STAGE >> 4);
+                const unsigned tc = tmem_base + (unsigned)((gr * 2 + s) * BN);
+                if (lead) {
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks) {
+                        // 16 columns further on: 32 bytes inside the swizzled row; 64 columns: the next block of rows
+                        const unsigned qo = (unsigned)(ks >> 2) * (BM * ROW_BYTES >> 4) + (unsigned)(ks & 3) * 2;
+                        const unsigned ko = (unsigned)(ks >> 2) * (BN * ROW_BYTES >> 4) + (unsigned)(ks & 3) * 2;
+                        if (ks == 0) mma_lo<false>(tc, qb + qo, kb + ko, hi_word, hi_word, idesc);
+                        else mma_lo<true>(tc, qb + qo, kb + ko, hi_word, hi_word, idesc);
+                    }
+                    if (gr == groups - 1) tc5_commit(&k_empty[s]);
+                    tc5_commit(&s_full[gr * 2 + s]);
+                }
+            }
+        }
+        if (!ok && lead) atomicExch(&failed, 1);
+    } else if (role == PV_WARP) {                                        // ---- issuer of the output O += P V ----
+        const bool lead = elect_one();
+        constexpr unsigned idesc = idesc_f16(BM, HD) | IDESC_B_MN_MAJOR;
+        const unsigned long long dp = make_smem_desc(Ps), dv = make_smem_desc_lbo_sbo(Vs, BN * ROW_BYTES, 8 * ROW_BYTES);
+        const unsigned p_lo = (unsigned)dp, v_lo = (unsigned)dv, p_hi = (unsigned)(dp >> 32), v_hi = (unsigned)(dv >> 32);
+        bool ok = true;
+        for (int it = 0; it < n_tiles && ok; ++it) {
+            const int s = it & 1;
+            if (!warp_wait(&v_full[s], (unsigned)((it / 2) & 1))) { ok = false; break; }
+            for (int gr = 0; gr < groups; ++gr) {
+                if (!warp_wait(&p_full[gr], (unsigned)(it & 1))) { ok = false; break; }
+                tc5_fence_after();
+                const unsigned pb = p_lo + (unsigned)gr * (P_BYTES >> 4), vb = v_lo + (unsigned)s * (KV_STAGE >> 4);
+                const unsigned tc = tmem_base + O_COL + (unsigned)(gr * 128);
+                if (lead) {
+#pragma unroll
+                    for (int k = 0; k < BN / 16; ++k) {
+                        // 16 keys further on: 32 bytes inside a row of P, 16 rows of 128 bytes of V
+                        if (k == 0 && it == 0) mma_lo<false>(tc, pb, vb, p_hi, v_hi, idesc);
+                        else mma_lo<true>(tc, pb + (unsigned)k * 2, vb + (unsigned)k * (16 * ROW_BYTES >> 4), p_hi, v_hi, idesc);
+                    }
+                    if (gr == groups - 1) tc5_commit(&v_empty[s]);
+                    tc5_commit(&pv_done[gr]);
+                }
+            }
+        }
+        if (!ok && lead) atomicExch(&failed, 1);
+    } else if (warp / 4 < groups) {                                      // ---- softmax: a thread per row ----
+        const int gr = warp / 4, row = (warp & 3) * 32 + lane, tk = gr * tokens + row / heads, h = row % heads;
+        const bool live = row < tokens * heads && tk < count && h < nheads;
+        const int qpos = pos0 + min(tk, count - 1);
+        const int first_key = (window > 0 && qpos - window + 1 > 0) ? qpos - window + 1 : 0;
+        // (warp-uniform) a tile that ends behind the first row's position or begins before the last row's window holds keys that some row must not read
+        const int warp_last = __reduce_min_sync(0xffffffffu, qpos), warp_first = __reduce_max_sync(0xffffffffu, first_key);
+        // (positive even where the product is too small for a float32, so that -inf stays -inf: no sum of products reaches 2^40)
+        const float sl2 = fmaxf(s_row_scale[gr * BM + row] * power_of_two(top_k - FOLD), 1.1754944e-38f);
+        const unsigned masked = 0xff800000u;                             // -inf
+        const unsigned lane_base = (unsigned)((warp & 3) * 32) << 16;
+        unsigned char* Pg = Ps + gr * P_BYTES;
+        const unsigned o_col = tmem_base + lane_base + O_COL + (unsigned)(gr * 128);
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int it = 0; it < n_tiles; ++it) {
+            const int s = it & 1;
+            if (!warp_wait(&s_full[gr * 2 + s], (unsigned)((it / 2) & 1))) { ok = false; break; }
+            tc5_fence_after();
+            unsigned sv[BN];
+            tc5_ld32_nowait(tmem_base + lane_base + (unsigned)((gr * 2 + s) * BN), sv);
+            tc5_ld32_nowait(tmem_base + lane_base + (unsigned)((gr * 2 + s) * BN + 32), sv + 32);
+            tc5_wait_ld();
+            tc5_fence_before();
+            mbar_arrive(&s_free[gr * 2 + s]);                            // the scores are in registers: the buffer may be written again
+            const int j0 = (jt0 + it) * BN;
+            if (j0 + BN - 1 > warp_last || j0 < warp_first) {
+#pragma unroll
+                for (int c = 0; c < BN; ++c)
+                    if (j0 + c > qpos || j0 + c < first_key) sv[c] = masked;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < BN; c += 2) mx = max3(mx, __uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
+            const float m_new = fmaxf(m, mx * sl2);
+            const bool bump = (m_new - m) > RESCALE_ABOVE;               // false when both are -inf (NaN compares false)
+            const float corr = bump ? exp2_fast(m - m_new) : 1.0f;
+            if (bump) m = m_new;
+            const float base = m == -INFINITY ? 0.f : m;
+            const unsigned long long scale2 = pair(sl2, sl2), nbase2 = pair(P_SHIFT - base, P_SHIFT - base);
+            unsigned long long sum2 = pair(0.f, 0.f);
+            unsigned pk[BN / 2];
+#pragma unroll
+            for (int c = 0; c < BN; c += 2) {
+                float t0, t1;
+                unpair(fma2(pair(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, nbase2), t0, t1);
+                const float p0 = exp2_fast(t0), p1 = exp2_fast(t1);
+                sum2 = add2(sum2, pair(p0, p1));
+                pk[c >> 1] = pack_half(p0, p1);
+            }
+            float sum, sum_hi;
+            unpair(sum2, sum, sum_hi);
+            l = l * corr + (sum + sum_hi);
+            if (it > 0) {                                                // P of the tile before has been read, O is at rest
+                if (!warp_wait(&pv_done[gr], (unsigned)((it - 1) & 1))) { ok = false; break; }
+                tc5_fence_after();
+                if (__any_sync(0xffffffffu, bump)) {
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD; c0 += 32) {
+                        unsigned ov[32];
+                        tc5_ld32(o_col + (unsigned)c0, ov);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * corr);
+                        tc5_st32(o_col + (unsigned)c0, ov);
+                    }
+                    tc5_wait_st();
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(Pg + swizzled(row, c)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+            fence_proxy_async_smem();
+            tc5_fence_before();
+            mbar_arrive(&p_full[gr]);
+        }
+        if (ok && warp_wait(&pv_done[gr], (unsigned)((n_tiles - 1) & 1))) {
+            tc5_fence_after();
+            const float inv = l == 0.f ? 0.f : 1.0f / l, unit = power_of_two(top_v - FOLD);
+            bf16* dst = out + ((size_t)(tok0 + (live ? tk : 0)) * nq + h0 + (live ? h : 0)) * HD;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+                unsigned ov[32];
+                tc5_ld32(o_col + (unsigned)c0, ov);
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(ov[8 * i + j]) * inv * unit;
+                        if (c0 + 8 * i < HD) store8(dst + c0 + 8 * i, v);
+                    }
+                }
+                __syncwarp();
+            }
+        } else {
+            atomicExch(&failed, 1);
+        }
+    }
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    if (warp == QK_WARP) tc5_dealloc(tmem_base, TMEM_COLS);
+    if (tid == 0 && failed && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_FLASH_8BIT);
+}
+
+extern "C" int vl_flash_prefill_8bit_head_dim() { return HD; }
+
+// q rows and `out` rows begin on 16 bytes; caches [pages, nkv, page_size, hd] e4m3, scales [pages, nkv]; pages of any number of positions.
+extern "C" int vl_flash_prefill_8bit(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const float* kscale,
+                                     const float* vscale, const int* block_table, int max_blocks, const int* tiles, int num_tiles, int nq, int nkv,
+                                     int hd, int page_size, int num_pages, float scale, int window, unsigned* err, void* stream) {
+    if (num_tiles <= 0) return VL_OK;
+    if (hd != HD) return VL_ERR_UNSUPPORTED;
+    if (nq <= 0 || nkv <= 0 || nq % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || window < 0 || q_stride < nq * hd) return VL_ERR_ARGUMENT;
+    if (q_stride % 8 || (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)tiles) & 15)) return VL_ERR_ARGUMENT;
+    if ((long long)num_pages * nkv * page_size >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
+    const int grp = nq / nkv, heads = grp < BM ? grp : BM, htiles = (grp + heads - 1) / heads, tokens = BM / heads;
+    const int cuts = (128 + GROUPS * tokens - 1) / (GROUPS * tokens);
+    if ((long long)num_tiles * cuts > 65535) return VL_ERR_UNSUPPORTED;
+    cudaError_t e = cudaFuncSetAttribute(flash_tc5_8bit_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+    if (e != cudaSuccess) return (int)e;
+    return vl_launch(flash_tc5_8bit_kernel, dim3(nkv * htiles, num_tiles * cuts), dim3(NTHREADS), SMEM_BYTES, (cudaStream_t)stream, (const bf16*)q,
+                     q_stride, (bf16*)out, (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks,
+                     (const int4*)tiles, num_tiles, nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, err, heads, htiles, tokens, cuts);
+}

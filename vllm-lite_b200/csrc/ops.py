@@ -152,6 +152,14 @@ _SIGNATURES = {
                                     c_int, c_void_p, c_longlong, c_int, c_void_p, c_void_p],
     ("gemm_8bit", "vl_gemm_8bit_plan"): [c_int, c_int, c_int, c_int, c_void_p],
     ("memprobe", "vl_read_only"): [c_void_p, c_longlong, c_void_p, c_void_p],
+    ("cache_8bit", "vl_qk_norm_rope_write_8bit"): [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float,
+                                                   c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                                   c_int, c_void_p, c_void_p],
+    ("flash_decode_8bit", "vl_flash_decode_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                                    c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                                    c_void_p, c_void_p, c_void_p],
+    ("flash_tc5_8bit", "vl_flash_prefill_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                                  c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p],
     ("sampling", "vl_apply_penalties"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_void_p],
     ("sampling", "vl_sample"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -910,6 +918,141 @@ def flash_decode(qkv, out, k_cache, v_cache, block_table, req_index, positions, 
     _check(_fn("attention", "vl_decode_attention_merge")(
         _ptr(part_acc), _ptr(part_ml), _ptr(positions), _ptr(out), dtype_code(out.dtype), T, num_heads, head_dim,
         chunk, S, int(window or 0), _ptr(token_index), _ptr(sinks), _stream()), "vl_decode_attention_merge")
+    return out
+
+
+# ---------------------------------------------------------------- a cache in 8 bits
+def attention_8bit_supported(dtype, head_dim) -> bool:
+    """What the three operators below take: bfloat16 activations and head sizes in steps of 16 up to 256; pages of any number of positions."""
+    return dtype == torch.bfloat16 and head_dim % 16 == 0 and 16 <= head_dim <= 256
+
+
+def _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim):
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _need(t, E4M3, n, 4)
+    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        _need(t, torch.float32, n, 2)
+    shape = k_cache.shape
+    if shape != v_cache.shape or shape[1] != num_kv_heads or shape[3] != head_dim or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
+        raise KernelError(f"a cache in 8 bits [pages, {num_kv_heads}, page size, {head_dim}] has scales [pages, {num_kv_heads}]: got {tuple(shape)}, "
+                          f"{tuple(v_cache.shape)} and {tuple(k_scale.shape)}, {tuple(v_scale.shape)}")
+
+
+def _need_heads(num_heads, num_kv_heads, head_dim, name):
+    if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or not attention_8bit_supported(torch.bfloat16, head_dim):
+        raise KernelError(f"{name}: {num_heads} query heads, {num_kv_heads} KV heads of {head_dim}; KV heads divide query heads, heads are of 16 to 256 "
+                          f"features in steps of 16")
+
+
+def qk_norm_rope_write_8bit(qkv, positions, slots, cu_seqlens, q_weight, k_weight, eps, inv_freq, rotary_dim, k_cache, v_cache, k_scale, v_scale,
+                            num_heads, num_kv_heads, head_dim, err, q_out=None):
+    """`qk_norm_rope_write` for a cache in 8 bits: e4m3 [pages, nkv, page_size, hd] with float32 scales [pages, nkv] for keys and for values, so that a row
+    stands for value * scale.  A page's scale is the least power of two, 2^-100 at least, with |x| <= 448 * scale for all x that the page's rows hold; it starts anew with
+    the page's first row and grows as rows join, and the page's earlier rows are moved to a scale that has grown.  A NaN or an infinity makes the scale
+    of its page NaN.  Tokens cu_seqlens[b] to cu_seqlens[b + 1] (int32 [B + 1]) are request b's, at consecutive positions; token t goes to slots[t] =
+    page * page_size + positions[t] % page_size (negative: it is not written; slots None: none is), rows of a page before its request's first new
+    one being the request's own.  One launch writes a page for one request only.  q goes to q_out [T, nq hd], or stays in qkv.  rotary_dim is a
+    multiple of 4.  Angles are those of the exact products position * inv_freq."""
+    _need(qkv, torch.bfloat16, "qkv", 2); _need(positions, torch.int32, "positions", 1)
+    _need_heads(num_heads, num_kv_heads, head_dim, "qk_norm_rope_write_8bit")
+    T = qkv.shape[0]
+    if qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim or positions.shape[0] != T:
+        raise KernelError(f"qkv {tuple(qkv.shape)} does not match heads {num_heads}+2*{num_kv_heads} x {head_dim}")
+    B = pages = page_size = 0
+    if slots is not None:
+        _need(slots, torch.int32, "slots", 1); _need(cu_seqlens, torch.int32, "cu_seqlens", 1)
+        _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim)
+        if slots.shape[0] != T or cu_seqlens.shape[0] < 1:
+            raise KernelError(f"qk_norm_rope_write_8bit: {slots.shape[0]} slots for {T} tokens, {cu_seqlens.shape[0]} bounds of requests")
+        B, pages, page_size = cu_seqlens.shape[0] - 1, k_cache.shape[0], k_cache.shape[2]
+    else:
+        cu_seqlens = k_cache = v_cache = k_scale = v_scale = None
+    for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            _need(w, torch.float32, n, 1)
+            if w.shape[0] != head_dim:
+                raise KernelError(f"{n} must have head_dim={head_dim} entries")
+    if inv_freq is not None:
+        _need(inv_freq, torch.float32, "inv_freq", 1)
+        if inv_freq.shape[0] * 2 != rotary_dim or rotary_dim % 4 or rotary_dim > head_dim:
+            raise KernelError(f"qk_norm_rope_write_8bit: inv_freq has rotary_dim / 2 entries, rotary_dim is a multiple of 4 and at most head_dim; got "
+                              f"{inv_freq.shape[0]}, {rotary_dim}")
+    if q_out is None:
+        q_out = qkv
+    else:
+        _need(q_out, torch.bfloat16, "q_out", 2)
+        if q_out.shape != (T, num_heads * head_dim):
+            raise KernelError(f"q_out {tuple(q_out.shape)} must be [{T}, {num_heads * head_dim}]")
+    _check(_fn("cache_8bit", "vl_qk_norm_rope_write_8bit")(
+        qkv, qkv.shape[1], q_out, q_out.shape[1], positions, slots, cu_seqlens, B, q_weight, k_weight, float(eps), inv_freq,
+        int(rotary_dim if inv_freq is not None else 0), k_cache, v_cache, k_scale, v_scale, T, num_heads, num_kv_heads, head_dim, page_size, pages,
+        err, _stream()), "vl_qk_norm_rope_write_8bit")
+    return q_out
+
+
+def flash_decode_8bit_scratch(num_tokens, num_heads, num_kv_heads, head_dim):
+    """(floats of scratch memory, int32 counters) that `flash_decode_8bit` wants for so many tokens: an item (a token's KV head) may be shared by as many
+    pieces as leave every block of the launch its share of a step of few tokens, and by two at least."""
+    pieces = 2 + -(-600 // max(1, num_tokens * num_kv_heads))
+    return num_tokens * num_heads * pieces * (head_dim + 2), num_tokens * num_heads
+
+
+def _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, name):
+    _need(q, torch.bfloat16, "q", 2); _need(out, torch.bfloat16, "out", 2); _need(block_table, torch.int32, "block_table", 2)
+    _need_heads(num_heads, num_kv_heads, head_dim, name)
+    _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim)
+    if q.shape[1] < num_heads * head_dim or out.shape != (q.shape[0], num_heads * head_dim):
+        raise KernelError(f"{name}: q {tuple(q.shape)}, out {tuple(out.shape)} for {num_heads} heads of {head_dim}")
+    if not scale > 0 or (window or 0) < 0:
+        raise KernelError(f"{name}: scale {scale} and window {window} must be positive (window None or 0: every earlier key)")
+
+
+def flash_decode_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, req_index, positions, num_heads, num_kv_heads, head_dim, scale, window,
+                      max_context, err, token_index=None, scratch=None, arrivals=None):
+    """Attention of single tokens over a cache in 8 bits (`qk_norm_rope_write_8bit`): q bfloat16 [T, >= nq hd] (its first columns are read), out bfloat16
+    [T, nq hd]; token t, at positions[t] of the request whose pages row req_index[t] of block_table names, reads every key up to its own or the last `window`.
+    Tokens at negative positions and (flagged) at max_context or beyond get rows of zeros.  token_index (int32): only these tokens, the others' rows of
+    out are left alone.  scratch (float32) and arrivals (int32, zero before and after each call): at least `flash_decode_8bit_scratch` of them, which nobody
+    else on the stream needs; without them the call takes its own.  Pages may have any number of positions; q begins on 8 bytes."""
+    _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, "flash_decode_8bit")
+    _need(req_index, torch.int32, "req_index", 1); _need(positions, torch.int32, "positions", 1)
+    T = q.shape[0]
+    if req_index.shape[0] != T or positions.shape[0] != T:
+        raise KernelError(f"flash_decode_8bit: {T} tokens, {req_index.shape[0]} request numbers, {positions.shape[0]} positions")
+    if int(max_context) < 1:
+        raise KernelError(f"flash_decode_8bit: max_context {max_context}")
+    if token_index is not None:
+        _need(token_index, torch.int32, "token_index", 1)
+        T = token_index.shape[0]
+    if T == 0:
+        return out
+    floats, counters = flash_decode_8bit_scratch(T, num_heads, num_kv_heads, head_dim)
+    if scratch is None:
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+    if arrivals is None:
+        arrivals = torch.zeros(counters, dtype=torch.int32, device=q.device)
+    _need(scratch, torch.float32, "scratch", 1); _need(arrivals, torch.int32, "arrivals", 1)
+    if scratch.shape[0] < floats or arrivals.shape[0] < counters:
+        raise KernelError(f"flash_decode_8bit: {floats} floats of scratch and {counters} counters are wanted, got {scratch.shape[0]} and {arrivals.shape[0]}")
+    pieces = floats // (T * num_heads * (head_dim + 2))
+    _check(_fn("flash_decode_8bit", "vl_flash_decode_8bit", {"FA_HD": head_dim})(
+        q, q.shape[1], k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], req_index, positions, T, num_heads, num_kv_heads, head_dim,
+        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), int(max_context), pieces, scratch, err, token_index, out, arrivals,
+        _stream()), "vl_flash_decode_8bit")
+    return out
+
+
+def flash_prefill_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, tiles, num_heads, num_kv_heads, head_dim, scale, window, err):
+    """Attention of prompt portions over a cache in 8 bits, q and out as in `flash_decode_8bit`.  tiles int32 [n, 4]: (row of the block table, index of the
+    tile's first token, tokens (<= 128), position of the first); a step's tiles cover once every token that the launch is to serve, the other rows of out are left
+    alone.  q, out and tiles begin on 16 bytes."""
+    _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, "flash_prefill_8bit")
+    _need(tiles, torch.int32, "tiles", 2)
+    if tiles.shape[1] != 4:
+        raise KernelError(f"flash_prefill_8bit: tiles {tuple(tiles.shape)} must be [n, 4]")
+    _check(_fn("flash_tc5_8bit", "vl_flash_prefill_8bit", {"FA_HD": head_dim})(
+        q, q.shape[1], out, k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], tiles, tiles.shape[0], num_heads, num_kv_heads, head_dim,
+        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), err, _stream()), "vl_flash_prefill_8bit")
     return out
 
 
