@@ -163,7 +163,7 @@ _SIGNATURES = {
     ("sampling", "vl_apply_penalties"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_void_p],
     ("sampling", "vl_sample"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-                                c_void_p, c_void_p, c_void_p],
+                                c_void_p, c_void_p, c_void_p, c_void_p],
     ("hyper", "vl_hc_step"): [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                               c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     ("hyper", "vl_dyt_rows"): [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
@@ -1854,18 +1854,24 @@ def apply_penalties(logits, seen_off=None, seen_ids=None, repeat=None, presence=
     return logits
 
 
-def sample(logits, temperature, top_k, top_p, uniform, out_token, out_logprob=None):
+def sample(logits, temperature, top_k, top_p, uniform, out_token, out_logprob=None, min_p=None):
+    """Draws a token for each row of logits float32 [R, V]; one number a row of temperature (0 and below: the first largest logit), top_k (int32, 0: off),
+    top_p (1: off), min_p (in [0, 1], 0: off: tokens less than min_p times as probable as the most probable one are dropped) and uniform (in [0, 1)), each of
+    which may be None: greedy, off, off, off, 0.  Order: temperature, top-k, top-p, min-p, then the inverse distribution at uniform over the
+    kept tokens in index order (csrc/sampling.cu).  out_token int32 [R]; out_logprob: what the draw gave its token."""
     _need(logits, torch.float32, "logits", 2); _need(out_token, torch.int32, "out_token", 1)
     R, V = logits.shape
     for t, dt, n in ((temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"),
-                     (top_p, torch.float32, "top_p"), (uniform, torch.float32, "uniform"),
+                     (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"), (uniform, torch.float32, "uniform"),
                      (out_logprob, torch.float32, "out_logprob")):
         if t is not None:
             _need(t, dt, n, 1)
             if t.shape[0] < R:
                 raise KernelError(f"{n} has fewer entries than rows")
+    if out_token.shape[0] < R:
+        raise KernelError("out_token has fewer entries than rows")
     _check(_fn("sampling", "vl_sample")(
-        _ptr(logits), logits.stride(0), R, V, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(uniform),
+        _ptr(logits), logits.stride(0), R, V, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform),
         _ptr(out_token), _ptr(out_logprob), _stream()), "vl_sample")
     return out_token
 

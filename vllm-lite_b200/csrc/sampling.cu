@@ -10,19 +10,35 @@
 //   (6) T <= 0: argmax (ties: lowest index, NaN counts as -inf); else softmax with the
 //       maximum subtracted; top_p < 1 keeps the most probable tokens, in descending
 //       order, up to and including the one with which the cumulative probability
-//       exceeds top_p; the draw is the inverse CDF at u over the kept tokens.
+//       exceeds top_p; min_p > 0 then drops what is less than min_p times as probable as
+//       the most probable token; the draw is the inverse CDF at u over the kept tokens.
 // Two choices are this engine's own.  The draw walks the kept tokens in index order
 // (the reference walks nucleus tokens in sorted order): same distribution, other
 // token for the same u.  Tokens whose probability equals the nucleus' last one are
-// all kept.  Probabilities are accumulated as 40-bit fixed-point integers, so sums do
-// not depend on the order in which threads add and a draw is reproducible.
+// all kept.  Probabilities are accumulated as 40-bit fixed-point integers, floor(exp(s - max) 2^40), so sums do
+// not depend on the order in which threads add, or on how many blocks share a row, and a draw is reproducible; min_p's bound is one of
+// these integers too, floor(min_p 2^40).
 //
-// vl_apply_penalties works on ragged per-row lists; vl_sample uses one block of 1024
-// threads per row.  Any vocabulary size.
+// vl_apply_penalties works on ragged per-row lists.
+// vl_sample: a cluster of 1 to 8 blocks holds a row in shared memory, so that it is read from memory once, whatever the options.  A row that asks for top-k
+// or top-p is sorted into SMP_BINS bins of its distance from the maximum (a partition that keeps the order of values: subtraction and the cut are
+// monotone), with their counts and masses; each block adds up a share of the bins over the cluster and the bin in which a threshold lies is found by
+// a scan of them.  Inside that bin the threshold's key is found 8 bits at a time, until what is left is kept whole; few values lie there, so these passes
+// count little.  Values 32 and more below the maximum have mass 0 and are in no bin: no threshold need be found among them.  Any vocabulary size; what of
+// a slice shared memory does not hold (rows of more than some 390,000) is read again in each pass.
 #include "common.cuh"
+#include <cooperative_groups.h>
 
-#define SMP_THREADS 1024
+namespace cg = cooperative_groups;
+
+#define SMP_THREADS 512
+#define SMP_WARPS (SMP_THREADS / 32)
 #define SMP_FIX 1099511627776.0f /* 2^40 */
+#define SMP_BINS 2048
+#define SMP_PER_UNIT 64.0f       /* bins per unit of s: 32 units in all, and exp(-27.8) 2^40 is below one */
+#define SMP_CLUSTER 8
+
+typedef unsigned long long u64;
 
 __device__ __forceinline__ unsigned order_key(float v) {
     unsigned k = __float_as_uint(v);
@@ -30,7 +46,7 @@ __device__ __forceinline__ unsigned order_key(float v) {
 }
 __device__ __forceinline__ float clean(float v, float inv_t) {
     v = v * inv_t;
-    return (v != v) ? -INFINITY : v;
+    return (v != v) ? -INFINITY : v + 0.f;                  // (-0 becomes 0: the two are a tie, and their keys differ)
 }
 
 __global__ void apply_penalties_kernel(float* __restrict__ logits, long long row_stride, int V,
@@ -67,254 +83,305 @@ __device__ __forceinline__ ArgBest better(ArgBest a, ArgBest b) {
     return a;
 }
 
-__global__ void __launch_bounds__(SMP_THREADS)
-sample_kernel(const float* __restrict__ logits, long long row_stride, int V,
-              const float* __restrict__ temperature, const int* __restrict__ top_k,
-              const float* __restrict__ top_p, const float* __restrict__ uniform,
-              int* __restrict__ out_token, float* __restrict__ out_logprob) {
-    __shared__ unsigned s_cnt[256];
-    __shared__ unsigned long long s_mass[256];
-    __shared__ float s_f[32];
-    __shared__ int s_i[32];
-    __shared__ unsigned long long s_w[32];
-    __shared__ unsigned s_prefix, s_remaining;
-    __shared__ unsigned long long s_above, s_total;
-    __shared__ float s_max;
-    __shared__ int s_pick;
+struct SampleShared {
+    u64 mass[SMP_BINS];
+    unsigned count[SMP_BINS];
+    u64 fine_mass[2][256];                  // two levels of the search in a bin in turn: one is read by the cluster while the other is filled
+    unsigned fine_count[2][256];
+    u64 warp_sum[SMP_WARPS], all_mass, part_mass;      // part: this block's share of the bins
+    unsigned part_count;
+    ArgBest warp_best[SMP_WARPS], best;
+    int found_bin;
+    u64 found_above_mass, found_mass, found_value;
+    unsigned found_above, found_count;
+};
 
-    pdl_launch_dependents();
-    pdl_wait();
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const float* l = logits + (size_t)r * row_stride;
+__device__ __forceinline__ u64 warp_sum_u64(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// inclusive sums over the block in the order of the threads; all threads call it
+__device__ __forceinline__ u64 block_scan_u64(u64 v, u64* warp_sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 n = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += n;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) v += warp_sums[w];
+    return v;
+}
+
+__global__ void __launch_bounds__(SMP_THREADS)
+sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int slice, int held,
+              const float* __restrict__ temperature, const int* __restrict__ top_k,
+              const float* __restrict__ top_p, const float* __restrict__ min_p, const float* __restrict__ uniform,
+              int* __restrict__ out_token, float* __restrict__ out_logprob) {
+    extern __shared__ __align__(16) float s_val[];          // the block's slice of the row, scaled: `held` values
+    __shared__ SampleShared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int r = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float* l = logits + (size_t)r * row_stride + (size_t)rank * slice;
+    const int n = max(0, min(slice, V - rank * slice)), first = rank * slice;
     const float temp = temperature ? temperature[r] : 0.f;
     const bool greedy = !(temp > 0.f);
     const float inv_t = greedy ? 1.f : 1.f / temp;
-    int k = top_k ? top_k[r] : 0;
-    const float tp = top_p ? top_p[r] : 1.f;
+    const int k = top_k ? top_k[r] : 0;
+    const float tp = top_p ? top_p[r] : 1.f, mp = min_p ? min_p[r] : 0.f;
 
-    // ---- argmax of the cleaned row (also the fallback of a degenerate row) ----
+    // ---- the slice into shared memory, and the row's first largest value ----
     ArgBest best{-INFINITY, 0x7fffffff};
-    // 16 bytes a load, four loads in flight (a row of 152 thousand logits: 20 -> measured below us); a thread
-    // sees its elements in rising order, so the first of equal values stays
-    const int V4 = (((uintptr_t)l & 15) == 0) ? (V & ~3) : 0;
-    for (int i0 = 4 * tid; i0 < V4; i0 += 16 * SMP_THREADS) {
+    auto take = [&](int i, float x) {
+        const float v = clean(x, 1.f);
+        best = better(best, ArgBest{v, first + i});
+        if (i < held) s_val[i] = clean(x, inv_t);
+    };
+    const int n4 = ((uintptr_t)l & 15) == 0 ? (n & ~3) : 0;
+    for (int i0 = 4 * tid; i0 < n4; i0 += 16 * SMP_THREADS) {           // 16 bytes a load, four on their way
         float4 q[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * 4 * SMP_THREADS;
-            q[u] = i < V4 ? *reinterpret_cast<const float4*>(l + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        }
+        for (int u = 0; u < 4; ++u)
+            if (i0 + u * 4 * SMP_THREADS < n4) q[u] = *reinterpret_cast<const float4*>(l + i0 + u * 4 * SMP_THREADS);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int i = i0 + u * 4 * SMP_THREADS;
-            if (i < V4) {
-                const float e[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float v = clean(e[j], 1.f);
-                    if (best.i == 0x7fffffff || v > best.v) best = ArgBest{v, i + j};
-                }
-            }
+            if (i < n4) { take(i, q[u].x); take(i + 1, q[u].y); take(i + 2, q[u].z); take(i + 3, q[u].w); }
         }
     }
-    for (int i = V4 + tid; i < V; i += SMP_THREADS) {
-        const float v = clean(l[i], 1.f);
-        best = better(best, ArgBest{v, i});
-    }
+    for (int i = n4 + tid; i < n; i += SMP_THREADS) take(i, l[i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         ArgBest other{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.i, o)};
         best = better(best, other);
     }
-    if (lane == 0) { s_f[warp] = best.v; s_i[warp] = best.i; }
+    if (lane == 0) sh.warp_best[warp] = best;
     __syncthreads();
     if (tid == 0) {
-        ArgBest b{s_f[0], s_i[0]};
-        for (int w = 1; w < SMP_THREADS / 32; ++w) b = better(b, ArgBest{s_f[w], s_i[w]});
-        s_pick = b.i == 0x7fffffff ? 0 : b.i;
-        s_max = b.v * inv_t;
+        for (int w = 1; w < SMP_WARPS; ++w) best = better(best, sh.warp_best[w]);
+        sh.best = best;
     }
-    __syncthreads();
-    const int arg = s_pick;
-    const float row_max = s_max;               // maximum of the scaled row (top-k keeps it)
+    cluster.sync();
+    best = sh.best;
+    for (int c = 0; c < C; ++c) best = better(best, cluster.map_shared_rank(&sh, c)->best);
+    const int arg = best.i == 0x7fffffff ? 0 : best.i;
+    const float row_max = best.v * inv_t;      // maximum of the scaled row (top-k keeps it)
     const bool degenerate = !(row_max > -INFINITY && row_max < INFINITY);
-    if (greedy && !out_logprob) {
-        if (tid == 0) out_token[r] = arg;
+    auto value = [&](int i) { return i < held ? s_val[i] : clean(l[i], inv_t); };
+    auto mass_of = [&](float s) { return (u64)(expf(s - row_max) * SMP_FIX); };
+    // the bin of a value; SMP_BINS for one without mass
+    auto bin_of = [&](float s) {
+        const float d = (row_max - s) * SMP_PER_UNIT;
+        return d < (float)SMP_BINS ? (int)d : SMP_BINS;
+    };
+    auto finish = [&](int token, float logprob) {
+        out_token[r] = token;
+        if (out_logprob) out_logprob[r] = logprob;
+    };
+    if ((greedy && !out_logprob) || degenerate) {
+        if (rank == 0 && tid == 0) finish(arg, 0.f);
+        cluster.sync();                        // nobody leaves while others read its shared memory
         return;
     }
 
-    // ---- top-k threshold by radix select on order-preserving keys ----
-    unsigned kth_key = 0;                      // keep key >= kth_key
-    if (!greedy && !degenerate && k > 0 && k < V) {
-        if (tid == 0) { s_prefix = 0; s_remaining = (unsigned)k; }
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) s_cnt[tid] = 0;
-            __syncthreads();
-            const unsigned prefix = s_prefix;
-            const unsigned himask = shift == 24 ? 0u : (0xffffffffu << (shift + 8));
-            for (int i = tid; i < V; i += SMP_THREADS) {
-                const unsigned key = order_key(clean(l[i], inv_t));
-                if ((key & himask) == prefix) atomicAdd(&s_cnt[(key >> shift) & 255u], 1u);
+    // A token is kept if its bin lies before `cut_bin`, or in it with at least the key `cut_key`.
+    int cut_bin = SMP_BINS;
+    unsigned cut_key = 0;
+    const bool by_k = !greedy && k > 0 && k < V, by_p = !greedy && tp < 1.f;
+    if (by_k || by_p) {
+        for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { sh.count[i] = 0; sh.mass[i] = 0; }
+        __syncthreads();
+        for (int i = tid; i < n; i += SMP_THREADS) {
+            const float s = value(i);
+            const int b = bin_of(s);
+            if (b < SMP_BINS) {
+                atomicAdd(&sh.count[b], 1u);
+                const u64 q = mass_of(s);
+                if (q) atomicAdd(&sh.mass[b], q);
             }
-            __syncthreads();
-            if (tid == 0) {
-                unsigned rem = s_remaining, cum = 0;
-                int b = 255;
-                for (; b > 0; --b) {
-                    if (cum + s_cnt[b] >= rem) break;
-                    cum += s_cnt[b];
-                }
-                s_remaining = rem - cum;
-                s_prefix = prefix | ((unsigned)b << shift);
-            }
-            __syncthreads();
         }
-        kth_key = s_prefix;
-    }
+        cluster.sync();
+        // this block's share of the bins, summed over the cluster in its own arrays (nobody else reads that share there)
+        const int share = SMP_BINS / C, lo = rank * share;
+        u64 m = 0;
+        unsigned c = 0;
+        for (int i = lo + tid; i < lo + share; i += SMP_THREADS) {
+            unsigned bc = 0;
+            u64 bm = 0;
+            for (int b = 0; b < C; ++b) {
+                const SampleShared* other = cluster.map_shared_rank(&sh, b);
+                bc += other->count[i];
+                bm += other->mass[i];
+            }
+            sh.count[i] = bc;
+            sh.mass[i] = bm;
+            c += bc;
+            m += bm;
+        }
+        c = __reduce_add_sync(0xffffffffu, c);
+        m = warp_sum_u64(m);
+        if (tid == 0) { sh.part_count = 0; sh.part_mass = 0; }
+        __syncthreads();
+        if (lane == 0) { atomicAdd(&sh.part_count, c); atomicAdd(&sh.part_mass, m); }
+        cluster.sync();
 
-    // ---- total mass of the kept tokens (40-bit fixed point of exp(s - max)) ----
-    unsigned long long mass = 0;
-    if (!degenerate) {
-        for (int i = tid; i < V; i += SMP_THREADS) {
-            const float s = clean(l[i], inv_t);
-            if (order_key(s) >= kth_key) mass += (unsigned long long)(expf(s - row_max) * SMP_FIX);
+        // The bin with which the sum, from the largest values on, of counts (masses) reaches `goal`; false if all bins together do not.
+        struct Found { int bin; unsigned above, count; u64 above_mass, mass; } f;
+        auto cross = [&](bool masses, u64 goal) -> bool {
+            int owner = -1;
+            unsigned before_c = 0;
+            u64 before_m = 0;
+            for (int b = 0; b < C && owner < 0; ++b) {
+                const SampleShared* other = cluster.map_shared_rank(&sh, b);
+                const unsigned pc = other->part_count;
+                const u64 pm = other->part_mass;
+                if ((masses ? before_m + pm : (u64)(before_c + pc)) >= goal) owner = b;
+                else { before_c += pc; before_m += pm; }
+            }
+            if (owner < 0) return false;
+            if (owner == rank) {
+                const int each = (share + SMP_THREADS - 1) / SMP_THREADS, i0 = lo + tid * each, i1 = min(lo + share, i0 + each);
+                u64 mine_c = 0, mine_m = 0;
+                for (int i = i0; i < i1; ++i) { mine_c += sh.count[i]; mine_m += sh.mass[i]; }
+                u64 cum_c = before_c + block_scan_u64(mine_c, sh.warp_sum) - mine_c, cum_m = before_m + block_scan_u64(mine_m, sh.warp_sum) - mine_m;
+                for (int i = i0; i < i1; ++i) {
+                    const u64 x = masses ? sh.mass[i] : sh.count[i], cum = masses ? cum_m : cum_c;
+                    if (cum < goal && cum + x >= goal) {
+                        sh.found_bin = i;
+                        sh.found_above = (unsigned)cum_c; sh.found_above_mass = cum_m;
+                        sh.found_count = sh.count[i]; sh.found_mass = sh.mass[i];
+                    }
+                    cum_c += sh.count[i];
+                    cum_m += sh.mass[i];
+                }
+            }
+            cluster.sync();
+            const SampleShared* o = cluster.map_shared_rank(&sh, owner);
+            f.bin = o->found_bin; f.above = o->found_above; f.count = o->found_count; f.above_mass = o->found_above_mass; f.mass = o->found_mass;
+            return true;
+        };
+        // Within bin f.bin, among keys of at least `least`: the key with which the sum of counts (masses) reaches `goal`, all of that key's values kept.
+        // f.mass becomes the mass of the bin's kept values.
+        int level = 0;
+        auto refine = [&](bool masses, u64 goal, unsigned least) -> unsigned {
+            unsigned prefix = 0;
+            u64 kept = 0;                      // mass of the bin's values above the prefix
+            for (int shift = 24; shift >= 0; shift -= 8, ++level) {
+                u64* fm = sh.fine_mass[level & 1];
+                unsigned* fc = sh.fine_count[level & 1];
+                if (tid < 256) { fm[tid] = 0; fc[tid] = 0; }
+                __syncthreads();
+                const unsigned himask = shift == 24 ? 0u : (0xffffffffu << (shift + 8));
+                for (int i = tid; i < n; i += SMP_THREADS) {
+                    const float s = value(i);
+                    const unsigned key = order_key(s);
+                    if (bin_of(s) == f.bin && key >= least && (key & himask) == prefix) {
+                        atomicAdd(&fc[255u - ((key >> shift) & 255u)], 1u);
+                        atomicAdd(&fm[255u - ((key >> shift) & 255u)], mass_of(s));
+                    }
+                }
+                cluster.sync();
+                u64 x = 0, xm = 0;             // every block finds the same digit for itself
+                unsigned xc = 0;
+                if (tid < 256)
+                    for (int b = 0; b < C; ++b) {
+                        const SampleShared* other = cluster.map_shared_rank(&sh, b);
+                        xc += other->fine_count[level & 1][tid];
+                        xm += other->fine_mass[level & 1][tid];
+                    }
+                x = masses ? xm : xc;
+                const u64 upto = block_scan_u64(x, sh.warp_sum), upto_m = block_scan_u64(xm, sh.warp_sum);
+                __syncthreads();
+                if (tid < 256 && upto >= goal && upto - x < goal) {
+                    sh.found_bin = 255 - tid; sh.found_value = upto - x; sh.found_count = xc; sh.found_above_mass = upto_m - xm; sh.found_mass = xm;
+                }
+                __syncthreads();
+                prefix |= (unsigned)sh.found_bin << shift;
+                goal -= sh.found_value;
+                kept += sh.found_above_mass;
+                f.mass = kept + sh.found_mass;
+                const bool whole = masses ? sh.found_count == 1 : goal == sh.found_count;
+                __syncthreads();
+                if (whole) { ++level; break; }
+            }
+            return max(prefix, least);
+        };
+
+        u64 total = 0;                         // mass after top-k
+        for (int b = 0; b < C; ++b) total += cluster.map_shared_rank(&sh, b)->part_mass;
+        if (by_k && cross(false, (u64)k)) {
+            cut_bin = f.bin;
+            if (f.above + f.count > (unsigned)k) cut_key = refine(false, (u64)(k - f.above), 0u);
+            total = f.above_mass + f.mass;
+        }
+        if (by_p && total > 0) {
+            if (by_k) cluster.sync();          // what the search before left has been read
+            const u64 target = (u64)((double)tp * (double)total);
+            if (cross(true, target + 1)) {     // (always: the target is less than the total)
+                const unsigned least = f.bin == cut_bin ? cut_key : 0u;
+                cut_bin = f.bin;
+                cut_key = refine(true, target + 1 - f.above_mass, least);
+            }
         }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-    if (lane == 0) s_w[warp] = mass;
+    // ---- the draw: masses of the kept tokens in index order; a warp owns a contiguous part of the slice ----
+    const u64 floor_mass = greedy ? 0 : (u64)((double)fminf(fmaxf(mp, 0.f), 1.f) * (double)SMP_FIX);
+    auto kept_mass = [&](float s) -> u64 {
+        const int b = bin_of(s);
+        if (b > cut_bin || (b == cut_bin && order_key(s) < cut_key)) return 0;
+        const u64 q = mass_of(s);
+        return q >= floor_mass ? q : 0;
+    };
+    const int span = (n + SMP_WARPS - 1) / SMP_WARPS, from = warp * span, to = min(n, from + span);
+    u64 sum = 0;
+    for (int i = from + lane; i < to; i += 32) sum += kept_mass(value(i));
+    sum = warp_sum_u64(sum);
+    __syncthreads();
+    if (lane == 0) sh.warp_sum[warp] = sum;
     __syncthreads();
     if (tid == 0) {
-        unsigned long long t = 0;
-        for (int w = 0; w < SMP_THREADS / 32; ++w) t += s_w[w];
-        s_total = t;
+        u64 t = 0;
+        for (int w = 0; w < SMP_WARPS; ++w) t += sh.warp_sum[w];
+        sh.all_mass = t;
     }
-    __syncthreads();
-    const unsigned long long total_k = s_total;   // mass after top-k
-
-    if (greedy || degenerate || total_k == 0) {
-        if (tid == 0) {
-            out_token[r] = arg;
-            if (out_logprob) {
-                // log-softmax of the row at the argmax: exp(0) / sum
-                out_logprob[r] = (degenerate || total_k == 0) ? 0.f : -logf((float)((double)total_k / (double)SMP_FIX));
-            }
-        }
+    cluster.sync();
+    u64 total = 0, before = 0;
+    for (int c = 0; c < C; ++c) {
+        const u64 t = cluster.map_shared_rank(&sh, c)->all_mass;
+        if (c < rank) before += t;
+        total += t;
+    }
+    if (greedy) {                              // log-softmax of the row at the argmax: exp(0) / sum
+        if (rank == 0 && tid == 0) finish(arg, -logf((float)((double)total / (double)SMP_FIX)));
+        cluster.sync();
         return;
     }
-
-    // ---- nucleus threshold: radix select on keys weighted by mass ----
-    unsigned nuc_key = kth_key;
-    unsigned long long total = total_k;
-    if (tp < 1.f) {
-        const unsigned long long target = (unsigned long long)((double)tp * (double)total_k);
-        if (tid == 0) { s_prefix = 0; s_above = 0; }
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) s_mass[tid] = 0;
-            __syncthreads();
-            const unsigned prefix = s_prefix;
-            const unsigned himask = shift == 24 ? 0u : (0xffffffffu << (shift + 8));
-            for (int i = tid; i < V; i += SMP_THREADS) {
-                const float s = clean(l[i], inv_t);
-                const unsigned key = order_key(s);
-                if (key >= kth_key && (key & himask) == prefix) {
-                    const unsigned long long q = (unsigned long long)(expf(s - row_max) * SMP_FIX);
-                    if (q) atomicAdd(&s_mass[(key >> shift) & 255u], q);
-                }
-            }
-            __syncthreads();
-            if (tid == 0) {
-                unsigned long long above = s_above;
-                int b = 255;
-                for (; b > 0; --b) {
-                    if (above + s_mass[b] > target) break;   // crossing bin: cumulative exceeds top_p
-                    above += s_mass[b];
-                }
-                s_above = above;
-                s_prefix = prefix | ((unsigned)b << shift);
-            }
-            __syncthreads();
-        }
-        nuc_key = s_prefix > kth_key ? s_prefix : kth_key;
-        // mass of the nucleus
-        unsigned long long nm = 0;
-        for (int i = tid; i < V; i += SMP_THREADS) {
-            const float s = clean(l[i], inv_t);
-            if (order_key(s) >= nuc_key) nm += (unsigned long long)(expf(s - row_max) * SMP_FIX);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) nm += __shfl_xor_sync(0xffffffffu, nm, o);
-        __syncthreads();
-        if (lane == 0) s_w[warp] = nm;
-        __syncthreads();
-        if (tid == 0) {
-            unsigned long long t = 0;
-            for (int w = 0; w < SMP_THREADS / 32; ++w) t += s_w[w];
-            s_total = t;
-        }
-        __syncthreads();
-        total = s_total;
-    }
-
-    // ---- inverse CDF in index order: warp w owns a contiguous span of the row ----
-    const float u = uniform ? uniform[r] : 0.f;
-    unsigned long long target = (unsigned long long)((double)u * (double)total);
+    u64 target = (u64)((double)(uniform ? uniform[r] : 0.f) * (double)total);
     if (target >= total) target = total - 1;
-    const int span = (V + 31) / 32;
-    const int lo = warp * span, hi = min(V, lo + span);
-    unsigned long long wsum = 0;
-    for (int i = lo + lane; i < hi; i += 32) {
-        const float s = clean(l[i], inv_t);
-        if (order_key(s) >= nuc_key) wsum += (unsigned long long)(expf(s - row_max) * SMP_FIX);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) wsum += __shfl_xor_sync(0xffffffffu, wsum, o);
-    __syncthreads();
-    if (lane == 0) s_w[warp] = wsum;
-    __syncthreads();
-    unsigned long long before = 0;
-    int owner = -1;
-    for (int w = 0; w < 32; ++w) {
-        if (owner < 0) {
-            if (before + s_w[w] > target) owner = w; else before += s_w[w];
-        }
-    }
-    if (owner < 0 && tid == 0) {
-        out_token[r] = arg;
-        if (out_logprob) out_logprob[r] = 0.f;
-    }
-    if (warp == owner) {
-        unsigned long long run = before;
-        int pick = -1;
-        unsigned long long pick_q = 0;
-        for (int base = lo; base < hi && pick < 0; base += 32) {
-            const int i = base + lane;
-            unsigned long long q = 0;
-            if (i < hi) {
-                const float s = clean(l[i], inv_t);
-                if (order_key(s) >= nuc_key) q = (unsigned long long)(expf(s - row_max) * SMP_FIX);
-            }
-            unsigned long long inc = q;          // inclusive scan over the warp
+    for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
+    if (target >= before && target - before < sum) {                    // (warp-uniform) the drawn token is this warp's
+        u64 run = before;
+        for (int base = from; base < to; base += 32) {
+            const u64 q = base + lane < to ? kept_mass(value(base + lane)) : 0;
+            u64 inc = q;                       // inclusive scan over the warp
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long n = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += n;
+                const u64 x = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += x;
             }
-            const bool hit = q > 0 && run + inc > target;
-            const unsigned ballot = __ballot_sync(0xffffffffu, hit);
-            if (ballot) {
-                const int first = __ffs(ballot) - 1;
-                pick = base + first;
-                pick_q = __shfl_sync(0xffffffffu, q, first);
+            const unsigned hits = __ballot_sync(0xffffffffu, q > 0 && run + inc > target);
+            if (hits) {
+                if (lane == __ffs(hits) - 1) finish(first + base + lane, logf((float)((double)q / (double)total)));
+                break;
             }
             run += __shfl_sync(0xffffffffu, inc, 31);
         }
-        if (lane == 0) {
-            out_token[r] = pick < 0 ? arg : pick;
-            if (out_logprob)
-                out_logprob[r] = pick < 0 ? 0.f : logf((float)((double)pick_q / (double)total));
-        }
     }
+    cluster.sync();
 }
 
 extern "C" int vl_apply_penalties(float* logits, long long row_stride, int R, int V,
@@ -328,11 +395,31 @@ extern "C" int vl_apply_penalties(float* logits, long long row_stride, int R, in
     return vl_launch_status();
 }
 
+// Values of a slice that a block's shared memory holds beside its tables.
+#define SMP_HELD_MAX ((200 * 1024 - (int)sizeof(SampleShared)) / 4)
+
 extern "C" int vl_sample(const float* logits, long long row_stride, int R, int V,
-                         const float* temperature, const int* top_k, const float* top_p,
+                         const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                          const float* uniform, int* out_token, float* out_logprob, void* stream) {
     if (R <= 0) return VL_OK;
     if (V <= 0) return VL_ERR_ARGUMENT;
-    return vl_launch(sample_kernel, dim3(R), dim3(SMP_THREADS), 0, (cudaStream_t)stream,
-                     logits, row_stride, V, temperature, top_k, top_p, uniform, out_token, out_logprob);
+    if ((long long)R * SMP_CLUSTER >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
+    int C = SMP_CLUSTER;
+    while (C > 1 && V <= 2048 * C / 2) C /= 2;
+    const int slice = ((V + C - 1) / C + 3) & ~3, held = slice < SMP_HELD_MAX ? slice : SMP_HELD_MAX;
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMP_HELD_MAX * 4);
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(R * C));
+    cfg.blockDim = dim3(SMP_THREADS);
+    cfg.dynamicSmemBytes = (size_t)held * 4;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, sample_kernel, logits, row_stride, V, slice, held, temperature, top_k, top_p, min_p, uniform, out_token,
+                                   out_logprob);
 }
