@@ -100,8 +100,8 @@ def prefill_floor_ms(cfg, layers, bf16_tflops, eight_bit=False):
     return (flops - products / 2 if eight_bit else flops) / (bf16_tflops * 1e9)
 
 
-def model_bytes_and_flops(cfg, layers, eight_bit=False):
-    """eight_bit: the layers' matrices are one byte an element and a float32 scale a row."""
+def model_bytes_and_flops(cfg, layers, eight_bit=False, eight_bit_cache=False):
+    """eight_bit: the layers' matrices are one byte an element and a float32 scale a row; eight_bit_cache: so are keys and values (a scale a page)."""
     H, I, V = cfg["hidden_size"], cfg["intermediate_size"], cfg["vocab_size"]
     nq, nkv, hd = cfg["num_attention_heads"], cfg["num_key_value_heads"], cfg["head_dim"]
     per_layer = layer_elements(cfg)
@@ -109,7 +109,7 @@ def model_bytes_and_flops(cfg, layers, eight_bit=False):
     weight_bytes = 2 * (layers * per_layer + V * H) + 4 * norms            # bf16 matrices, every one read once
     if eight_bit:
         weight_bytes -= layers * (per_layer - 4 * ((nq + 2 * nkv) * hd + 2 * H + 2 * I))
-    kv_bytes_per_token = layers * 2 * nkv * hd * 2
+    kv_bytes_per_token = layers * 2 * nkv * hd * (1 if eight_bit_cache else 2)
     T = PREFILL_TOKENS
     prefill_flops = 2 * T * layers * per_layer + layers * 4 * nq * hd * (T * (T + 1) // 2) + 2 * V * H
     return weight_bytes, kv_bytes_per_token, prefill_flops
@@ -1360,6 +1360,7 @@ def main(argv=None):
     ap.add_argument("--size", default="8b", choices=sorted(SIZES), help="layer sizes of Qwen3-8B (default), 14B or 32B")
     ap.add_argument("--layers", type=int, default=None, help="fewer layers than the size has (both numbers are reported)")
     ap.add_argument("--eight-bit", action="store_true", help="the layers' linear products in 8 bits (weights and activations)")
+    ap.add_argument("--eight-bit-cache", action="store_true", help="keys and values in 8 bits, with a scale for each page and head")
     ap.add_argument("--block-size", type=int, default=64, help="positions per page of the cache")
     ap.add_argument("--no-points", action="store_true", help="skip the batch 1 / 64 points and the prefill")
     ap.add_argument("--only-prefill", action="store_true", help="time the 2,048-token prefill alone (for profiling)")
@@ -1430,12 +1431,13 @@ def main(argv=None):
     if args.read_ceiling:
         return read_ceiling(cfg, args.batch, args.context)
     _, plan, weights = random_model(cfg, seed=0, dtype="bfloat16", device="cuda:0")
-    dtype = "bf16, layers' products in e4m3" if args.eight_bit else "bf16"
+    dtype = "bf16" + (", layers' products in e4m3" if args.eight_bit else "") + (", cache in e4m3" if args.eight_bit_cache else "")
     if args.continuous:
         R, out_len, prompt_range = args.continuous, 512, (256, args.context // 2)
         pages = R * (-(-(prompt_range[1] + out_len) // args.block_size) + 1) + 64
         engine = LLMEngine(plan=plan, weights=weights, dtype="bfloat16", kv_blocks=pages, block_size=args.block_size, max_batch_size=R,
-                           max_num_batched_tokens=4096, prefill_chunk_size=512, max_model_len=args.context, eight_bit=args.eight_bit)
+                           max_num_batched_tokens=4096, prefill_chunk_size=512, max_model_len=args.context, eight_bit=args.eight_bit,
+                           eight_bit_cache=args.eight_bit_cache)
         del weights
         continuous_run(engine, min(R, 4), vocab, (256, 512), 16)          # warm-up: builds, graphs of the small buckets
         clocks = ClockSampler().start()
@@ -1462,12 +1464,17 @@ def main(argv=None):
         pages = int(args.kv_blocks)
     engine = LLMEngine(plan=plan, weights=weights, dtype="bfloat16", kv_blocks=pages, block_size=args.block_size, max_batch_size=big,
                        max_num_batched_tokens=PREFILL_TOKENS, prefill_chunk_size=PREFILL_TOKENS,
-                       max_model_len=args.context + slack, eight_bit=args.eight_bit)
+                       max_model_len=args.context + slack, eight_bit=args.eight_bit, eight_bit_cache=args.eight_bit_cache)
     del weights
     runner, sampler = engine.runner, engine.sampler
-    for t in runner.storage.paged:                        # pages that no prompt wrote hold random numbers
-        t.normal_()
-    weight_bytes, kv_per_token, _ = model_bytes_and_flops(cfg, args.layers, args.eight_bit)
+    for t, scales in zip(runner.storage.paged, runner.storage.scales):               # pages that no prompt wrote hold random numbers
+        if scales is None:
+            t.normal_()
+        else:
+            scales.fill_(1.0)
+            for call in t:
+                call.copy_(torch.randn(call.shape, device=call.device))
+    weight_bytes, kv_per_token, _ = model_bytes_and_flops(cfg, args.layers, args.eight_bit, args.eight_bit_cache)
     pk = peaks()
     rate = {"frac_of": "the layers' products at twice the bfloat16 rate, the rest at that rate"} if args.eight_bit else {}
 

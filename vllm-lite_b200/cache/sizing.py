@@ -18,7 +18,7 @@ MIN_RESERVE = 512 << 20
 
 def page_bytes(layout: CacheLayout, page_size: int, itemsize: int) -> List[int]:
     """Bytes of one page in every paged group: keys and values of every call of the group."""
-    return [len(members) * page_size * need.bytes_per_token(itemsize)
+    return [len(members) * (page_size * need.bytes_per_token(itemsize) + getattr(need, "extra_page_bytes", 0))
             for need, members in zip(layout.paged_groups, layout.paged_members)]
 
 

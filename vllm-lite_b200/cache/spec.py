@@ -6,7 +6,8 @@ pages that lie wholly before the window may be given back.  `chunk`, when set,
 means that positions form blocks of that many from the request's first token and
 no query reads a key of an earlier block, so pages that lie wholly before the
 block of the next query may be given back too.  `keep`, when set beside a window, means that the first `keep` tokens
-stay readable however far behind the window they lie.
+stay readable however far behind the window they lie.  `eight_bit`: rows are e4m3 values under a float32 scale a page and head
+(csrc/cache_8bit.cuh).
 `PagedLatent`: one row per token from which keys and values are both derived (a
 compressed latent); paged and windowed like `PagedKV`, but stored once.
 `FixedState`: a tensor of fixed shape per request, stored in a slot.
@@ -28,11 +29,17 @@ class PagedKV:
     window: Optional[int] = None
     chunk: Optional[int] = None
     keep: Optional[int] = None
+    eight_bit: bool = False
 
     planes = 2                      # keys and values are stored apart
 
     def bytes_per_token(self, itemsize: int) -> int:
-        return 2 * self.num_kv_heads * self.head_dim * itemsize
+        return 2 * self.num_kv_heads * self.head_dim * (1 if self.eight_bit else itemsize)
+
+    @property
+    def extra_page_bytes(self) -> int:
+        """What a page holds beside its tokens: the scales of its keys and values."""
+        return 2 * self.num_kv_heads * 4 if self.eight_bit else 0
 
 
 @dataclass(frozen=True)
@@ -67,8 +74,8 @@ def widened(owner, reader):
     """The need of a cache that its owner and another call read: what either of them can still reach stays."""
     if not isinstance(owner, PagedKV) or not isinstance(reader, PagedKV):
         return owner
-    if (owner.num_kv_heads, owner.head_dim) != (reader.num_kv_heads, reader.head_dim):
-        raise ValueError(f"a call that reads another's cache has its heads: {reader} against {owner}")
+    if (owner.num_kv_heads, owner.head_dim, owner.eight_bit) != (reader.num_kv_heads, reader.head_dim, reader.eight_bit):
+        raise ValueError(f"a call that reads another's cache has its heads and its type: {reader} against {owner}")
     both = lambda a, b: None if a is None or b is None else max(a, b)
     chunk = owner.chunk if owner.chunk == reader.chunk else None
     window = both(owner.window, reader.window)

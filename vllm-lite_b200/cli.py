@@ -10,7 +10,7 @@ reference's default is 1024, here the cache is sized from the GPU's free memory 
 is absent, under `--gpu-memory-fraction`), `--max-batch-size` (256, VLLM_MAX_BATCH_SIZE), `--max-model-len`
 (VLLM_MAX_MODEL_LEN), `--tensor-parallel-size` (1) and `--kv-quantization`
 (false), which are accepted only at those values because the engine runs on one
-GPU with an unquantized cache, and `--log-level`.  The server's network and
+GPU and does not quantize its cache in the reference's way, and `--log-level`; `--eight-bit-cache` (bfloat16) keeps keys and values in 8 bits in a form of this engine's own.  The server's network and
 speculative-decoding flags have no counterpart.  Prompts are token ids (the engine
 has no tokenizer): a comma-separated list, or a file with one prompt per line.
 """
@@ -63,6 +63,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--log-level", default=_env("VLLM_LOG_LEVEL", "info"))
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     ap.add_argument("--eight-bit", action="store_true", help="run the layers' linear products in 8 bits (weights and activations)")
+    ap.add_argument("--eight-bit-cache", action="store_true", help="keep keys and values in 8 bits, with a scale for each page and head")
     ap.add_argument("--block-size", type=_bounded(1, 256, "--block-size"), default=64,
                     help="positions per page of the cache (the reference's constant is 16; 64 suits the TMA copies)")
     ap.add_argument("--max-num-batched-tokens", type=int, default=4096)
@@ -73,6 +74,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--top-k", type=int, default=0)
     ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     ap.add_argument("--repeat-penalty", type=float, default=1.0)
     ap.add_argument("--presence-penalty", type=float, default=0.0)
     ap.add_argument("--seed", type=int, default=None)
@@ -106,7 +108,9 @@ def main(argv=None) -> int:
     if args.tensor_parallel_size != 1:
         ap.error("--tensor-parallel-size: this engine runs on one GPU")
     if args.kv_quantization:
-        ap.error("--kv-quantization: the cache is not quantized in this engine")
+        ap.error("--kv-quantization: the reference's form is not here, the cache is not quantized by this flag; --eight-bit-cache keeps it in 8 bits")
+    if args.eight_bit_cache and args.dtype != "bfloat16":
+        ap.error("--eight-bit-cache: a cache in 8 bits goes with --dtype bfloat16")
     if args.eight_bit and args.dtype != "bfloat16":
         ap.error("--eight-bit: products in 8 bits go with --dtype bfloat16")
     prompts = read_prompts(args.prompt_ids)
@@ -119,10 +123,10 @@ def main(argv=None) -> int:
     engine = LLMEngine(args.model, dtype=args.dtype, kv_blocks=args.kv_blocks, block_size=args.block_size,
                        max_batch_size=args.max_batch_size, max_num_batched_tokens=args.max_num_batched_tokens,
                        prefill_chunk_size=args.prefill_chunk_size, max_model_len=args.max_model_len,
-                       gpu_memory_fraction=args.gpu_memory_fraction, eight_bit=args.eight_bit)
+                       gpu_memory_fraction=args.gpu_memory_fraction, eight_bit=args.eight_bit, eight_bit_cache=args.eight_bit_cache)
     if verbose:
         print(f"[vllm-lite_b200] model loaded in {time.time() - t0:.1f} s", file=sys.stderr)
-    params = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
+    params = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p,
                             repeat_penalty=args.repeat_penalty, presence_penalty=args.presence_penalty,
                             seed=args.seed)
     t0 = time.time()

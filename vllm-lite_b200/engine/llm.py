@@ -18,7 +18,7 @@ from typing import Dict, List, Optional, Sequence as Seq
 import torch
 
 from ..sampling import Sampler, SamplingParams
-from .loading import load_model_dir, parse_dtype, plan_in_8_bits
+from .loading import load_model_dir, parse_dtype, plan_in_8_bits, plan_with_8_bit_cache
 from .runner import ModelRunner, StepEntry
 from .scheduler import Scheduler, SchedulerConfig, Sequence
 
@@ -116,7 +116,8 @@ class LLMEngine:
     def __init__(self, model=None, *, dtype="bfloat16", device="cuda:0", kv_blocks: Optional[int] = None,
                  block_size: int = 64, max_batch_size: int = 256, max_num_batched_tokens: int = 4096,
                  prefill_chunk_size: int = 512, max_model_len: Optional[int] = None, plan=None, weights=None,
-                 logprobs: bool = False, lookahead: bool = True, gpu_memory_fraction: float = 0.9, eight_bit: bool = False):
+                 logprobs: bool = False, lookahead: bool = True, gpu_memory_fraction: float = 0.9, eight_bit: bool = False,
+                 eight_bit_cache: bool = False):
         """`model`: a folder with config.json and safetensors (never downloaded).  `kv_blocks`
         and `max_batch_size` carry the reference's names (crates/server/src/cli/args.rs:155-186);
         `block_size` is its BLOCK_SIZE constant (crates/traits/src/types.rs:13: 16) made an option; the
@@ -127,14 +128,17 @@ class LLMEngine:
         reserve for activations (cache/sizing.py).  Alternatively pass `plan` and `weights` of a
         model that is already on the device; the engine takes the dict over and empties it.
         `lookahead`: see `step`.  `eight_bit`: the layers' linear products run in 8 bits, weights and activations
-        (parts/eight_bit.py; dtype bfloat16, models of pre-norm blocks with grouped-query attention and SwiGLU)."""
+        (parts/eight_bit.py; dtype bfloat16, models of pre-norm blocks with grouped-query attention and SwiGLU).
+        `eight_bit_cache`: keys and values are kept in 8 bits, with a scale for each page of `block_size` positions and head (dtype bfloat16,
+        models whose layers all mix by plain grouped-query attention): pages take half the memory, and decoding reads half the bytes."""
         self.dtype = parse_dtype(dtype)
         if plan is None:
             if model is None:
                 raise ValueError("give a model folder (or plan and weights)")
-            _, plan, weights = load_model_dir(model, self.dtype, device, eight_bit)
-        elif eight_bit:
-            plan = plan_in_8_bits(plan, self.dtype)
+            _, plan, weights = load_model_dir(model, self.dtype, device, eight_bit, eight_bit_cache)
+        else:
+            plan = plan_in_8_bits(plan, self.dtype) if eight_bit else plan
+            plan = plan_with_8_bit_cache(plan, self.dtype) if eight_bit_cache else plan
         if max_model_len is None:
             max_model_len = plan.max_position_embeddings
         self.runner = ModelRunner(plan, weights, dtype=self.dtype, device=device, page_size=block_size,

@@ -30,6 +30,13 @@ def plan_in_8_bits(plan, dtype):
     return in_8_bits(plan)
 
 
+def plan_with_8_bit_cache(plan, dtype):
+    from ..parts.eight_bit import cache_in_8_bits
+    if parse_dtype(dtype) != torch.bfloat16:
+        raise ValueError("a cache in 8 bits goes with bfloat16 activations")
+    return cache_in_8_bits(plan)
+
+
 def tensor_shapes(model_dir) -> dict:
     """{tensor name: shape} from the headers of a folder's weight files (no data is read); {} when there are none."""
     from ..weights.loader import WeightError, find_weight_files
@@ -48,13 +55,15 @@ def tensor_shapes(model_dir) -> dict:
     return shapes
 
 
-def load_model_dir(model_dir, dtype, device, eight_bit=False):
+def load_model_dir(model_dir, dtype, device, eight_bit=False, eight_bit_cache=False):
     """(typed configuration, plan, {name: device tensor}).  eight_bit: the plan's linear layers run in 8 bits (parts/eight_bit.py; the
-    tensors are read as they are stored, the parts bring them to 8 bits)."""
+    tensors are read as they are stored, the parts bring them to 8 bits).  eight_bit_cache: its layers keep keys and values in 8 bits."""
     dtype = parse_dtype(dtype)
     cfg, plan = plan_from_config_json(read_config_json(model_dir), shapes=tensor_shapes(model_dir))
     if eight_bit:
         plan = plan_in_8_bits(plan, dtype)
+    if eight_bit_cache:
+        plan = plan_with_8_bit_cache(plan, dtype)
     weights = load_weights(model_dir, declare_model(plan), dtype, device, unused=plan.unused_tensors)
     return cfg, plan, weights
 

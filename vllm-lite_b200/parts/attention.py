@@ -36,6 +36,20 @@ def check_attention_sizes(spec: AttentionSpec):
         raise ValueError(f"window {spec.window} must be positive (None reads every earlier key)")
 
 
+def has_options(spec: AttentionSpec) -> bool:
+    """Whether the attention does more than norm, rotate, and weigh the values by a softmax over its window."""
+    return bool(spec.q_temp is not None or spec.v_norm is not None or spec.whole_norm or spec.head_temp is not None or spec.softcap
+                or spec.distance_bias is not None or spec.unit_sink or spec.sink is not None or spec.keep_first or spec.gate is not None)
+
+
+def check_eight_bit_cache(spec: AttentionSpec):
+    """Raises ValueError for an attention whose cache has no form in 8 bits."""
+    rot = spec.position.dim if hasattr(spec.position, "dim") else 0
+    if has_options(spec) or rot % 4:
+        raise ValueError("a cache in 8 bits goes with plain grouped-query attention: no gate, sink, cap or bias on its scores, no kept keys, no row work, a "
+                         f"rotated part of a multiple of 4 features (got {rot})")
+
+
 def _pad_heads(w, heads, size, padded):
     """Rows (or entries) of `heads` heads of `size` each, every head padded with zeros to `padded`."""
     if size == padded:
@@ -115,7 +129,7 @@ class GqaAttention:
     @staticmethod
     def cache_need(spec: AttentionSpec):
         return PagedKV(spec.num_kv_heads, GqaAttention.padded_head_dim(spec), spec.window,
-                       keep=spec.keep_first if spec.window is not None else None)
+                       keep=spec.keep_first if spec.window is not None else None, eight_bit=spec.eight_bit_cache)
 
     def __init__(self, spec: AttentionSpec, weights: dict, ctx):
         import dataclasses
@@ -127,8 +141,11 @@ class GqaAttention:
         # ... and so is it with a norm over the whole projection or a factor per head (`ops.head_work`: bias, norm, rotation,
         # factor and the cache rows in one pass, from rows of unpadded heads)
         self.row_work = bool(spec.whole_norm or spec.head_temp is not None)
-        self.with_options = bool(self.own_head_work or self.row_work or spec.softcap or spec.distance_bias is not None
-                                 or spec.unit_sink or spec.sink is not None or spec.keep_first or spec.gate is not None)
+        self.with_options = has_options(spec)
+        if spec.eight_bit_cache:
+            check_eight_bit_cache(spec)
+            if ctx.dtype != torch.bfloat16:
+                raise ValueError("a cache in 8 bits goes with bfloat16 activations")
         if self.row_work and (self.own_head_work or (spec.qk_norm is not None and (spec.qk_norm.kind != "rms_norm" or spec.qk_norm.offset
                                                      or spec.qk_norm.scalar or not spec.qk_norm.has_weight))):
             raise ValueError("a whole-row norm or a factor per head goes with plain RMS norms, no query factor and no value norm")
@@ -343,13 +360,19 @@ class GqaAttention:
         slots = group.slots if cache.writes else None
         from . import attention_dispatch
         fold = None
-        if attention_dispatch.folds_head_work(qkv.dtype, step, s, group, qkv.shape[0]):
+        if cache.k_scale is not None:
+            ops.qk_norm_rope_write_8bit(qkv, step.positions, slots, step.cu_seqlens, qw, kw, eps, inv_freq, rot, cache.k, cache.v,
+                                        cache.k_scale, cache.v_scale, s.num_heads, s.num_kv_heads, s.head_dim, step.err)
+        elif attention_dispatch.folds_head_work(qkv.dtype, step, s, group, qkv.shape[0]):
             fold = (qw, kw, eps, inv_freq, rot, slots)          # the attention kernel does it on the way
         else:
             ops.qk_norm_rope_write(qkv, step.positions, slots, qw, kw, eps, inv_freq, rot, cache.k, cache.v,
                                    s.num_heads, s.num_kv_heads, s.head_dim, step.err)
         out = step.workspace.get(step.tag + "attn.out", (qkv.shape[0], s.num_heads * s.head_dim), self.dtype)
-        attention_dispatch.run(qkv, out, cache, group, step, s, self.scale, fold=fold)
+        if cache.k_scale is not None:
+            attention_dispatch.run_8bit(qkv, out, cache, group, step, s, self.scale)
+        else:
+            attention_dispatch.run(qkv, out, cache, group, step, s, self.scale, fold=fold)
         if sink is not None:
             return self.o_proj.into_stream(out, sink, step, "attn.o")
         return self.o_proj(out, step, "attn.o", torch.float32 if sums else None)

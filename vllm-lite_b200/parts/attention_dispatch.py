@@ -145,6 +145,27 @@ def run(qkv, out, cache, group, step, spec, scale, fold=None, sinks=None, weight
     return ops.paged_attention(*args, step.err, sinks=sinks)
 
 
+def run_8bit(qkv, out, cache, group, step, spec, scale):
+    """Attention over a cache in 8 bits: one kernel for single tokens, one for portions of prompts, a mixed step launches both."""
+    common = (qkv, out, cache.k, cache.v, cache.k_scale, cache.v_scale, group.block_table)
+    sizes = (spec.num_heads, spec.num_kv_heads, spec.head_dim, scale, spec.window)
+
+    def single(tokens, context, token_index=None):
+        floats, counters = ops.flash_decode_8bit_scratch(tokens, spec.num_heads, spec.num_kv_heads, spec.head_dim)
+        # one set of counters for all layers of a step shape: every launch leaves them zero
+        ops.flash_decode_8bit(*common, step.req_index, step.positions, *sizes, context, step.err, token_index=token_index,
+                              scratch=step.workspace.get(step.tag + "attn8.scratch", (floats,), torch.float32),
+                              arrivals=step.workspace.zeros(step.tag + "attn8.arrivals", counters, torch.int32))
+
+    if step.max_query_len == 1:
+        single(qkv.shape[0], group.max_context)
+        return out
+    ops.flash_prefill_8bit(*common, step.query_tiles, *sizes, step.err)
+    if step.single_tokens is not None:
+        single(step.single_tokens.shape[0], step.single_context, step.single_tokens)
+    return out
+
+
 def _run_variant(ops, q, out, cache, group, step, spec, scale, weighting, chunk, head_bias, gate, sinks):
     """Attention with another weighting than the softmax, a chunked mask or an output gate: in bfloat16 the tensor-core
     kernels for portions of prompts (tcgen05 for long portions of heads of 64 or 128, else mma.sync) and the

@@ -138,13 +138,15 @@ class CallCache:
 
     Paged: `k`, `v` are [pages, kv_heads, page_size, head_dim]; `group` indexes
     StepBatch.groups; `writes` is False for a call that reads an earlier call's
-    cache.  Fixed state: `state` is [slots, *shape], indexed by StepBatch.state_slots.
+    cache.  In 8 bits: e4m3 pages, and `k_scale`, `v_scale` float32 [pages, kv_heads].  Fixed state: `state` is [slots, *shape], indexed by StepBatch.state_slots.
     """
     group: int = -1
     k: Optional[torch.Tensor] = None
     v: Optional[torch.Tensor] = None
     writes: bool = True
     state: Optional[torch.Tensor] = None
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
     parts: Optional[list] = None              # a call with several needs (cache.spec.Several): one CallCache per need
 
 

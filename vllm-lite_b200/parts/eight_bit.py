@@ -7,7 +7,10 @@ SwiGLU; tensor names and shapes stay, weights are brought to 8 bits when the par
     norm -> gate/up product with SwiGLU -> rows to 8 bits -> down product, which the next norm adds to the stream
 
 where a norm's output is `Rows8` (`ops.add_rmsnorm_8bit`) and the products apply scales, bias, activation and residual themselves
-(`ops.gemm_8bit`).  The stream stays float32; embedding, final norm, output head, attention and its cache stay as they were."""
+(`ops.gemm_8bit`).  The stream stays float32; embedding, final norm, output head, attention and its cache stay as they were.
+
+`cache_in_8_bits(plan)` is about the cache alone, with products in 8 bits or without: keys and values are kept as e4m3 values with a scale for
+each page and head (`AttentionSpec.eight_bit_cache`)."""
 from __future__ import annotations
 
 import dataclasses
@@ -16,7 +19,7 @@ from dataclasses import dataclass
 import torch
 
 from ..csrc import ops
-from .attention import GqaAttention
+from .attention import GqaAttention, check_eight_bit_cache
 from .block import PreNormBlock
 from .linear import Linear
 from .mlp import SwiGLU
@@ -147,6 +150,21 @@ class PreNormBlock8(PreNormBlock):
         h = self.norm1(residual.x, residual.pending, step, tag="norm1")
         self.mixer(h, step, cache, sink=residual.x)
         residual.pending = self.ffn(self.norm2(residual.x, None, step, tag="norm2"), step)
+
+
+def cache_in_8_bits(plan):
+    """The plan with the keys and values of every layer kept in 8 bits.  Raises ValueError for a layer whose cache has no such form."""
+    layers = []
+    for i, block in enumerate(plan.layers):
+        mixer = getattr(block, "mixer", None)
+        if not (isinstance(mixer, AttentionSpec) and mixer.kind in ("gqa_attention", "gqa_attention_8bit")):
+            raise ValueError(f"layer {i} ({getattr(mixer, 'kind', '?')}) keeps nothing that has a form in 8 bits; grouped-query attention does")
+        try:
+            check_eight_bit_cache(mixer)
+        except ValueError as e:
+            raise ValueError(f"layer {i}: {e}") from None
+        layers.append(dataclasses.replace(block, mixer=dataclasses.replace(mixer, eight_bit_cache=True)))
+    return dataclasses.replace(plan, layers=tuple(layers))
 
 
 def in_8_bits(plan):

@@ -118,6 +118,9 @@ class AttentionSpec:
     `sink` (a tensor name, [num_heads]): the softmax denominator of head h holds one more term exp(sink_h), with no key, no
     value and no scale;
     `keep_first`: beside a window, the first that many keys of the sequence stay visible to every query.
+
+    `eight_bit_cache`: keys and values are kept as e4m3 values with a scale a page and head (`ops.qk_norm_rope_write_8bit`); bfloat16, and
+    none of the options above.
     """
     hidden_size: int
     num_heads: int
@@ -146,6 +149,7 @@ class AttentionSpec:
     head_temp: Optional[str] = None
     sink: Optional[str] = None
     keep_first: Optional[int] = None
+    eight_bit_cache: bool = False
 
 
 @dataclass(frozen=True)

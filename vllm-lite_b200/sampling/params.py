@@ -1,7 +1,7 @@
 """Per-request sampling options, with the reference's names, meanings and defaults
 (crates/traits/src/sampling.rs:83-257).  The reference's `beam_width`,
 `length_penalty`, `max_retries` and `top_logprobs` are declared there but are not
-part of what its sampler draws with, and have no counterpart here."""
+part of what its sampler draws with, and have no counterpart here; `min_p` is this engine's own."""
 from __future__ import annotations
 
 from dataclasses import dataclass
@@ -18,6 +18,7 @@ class SamplingParams:
     logit_bias: Optional[Dict[int, float]] = None
     seed: Optional[int] = None          # per-request stream, indexed by the step
     stop_token_sequences: Optional[List[List[int]]] = None
+    min_p: float = 0.0                  # 0 disables; drops what is less than min_p times as probable as the most probable token
 
     def validate(self) -> "SamplingParams":
         if self.temperature < 0 or self.temperature != self.temperature:
@@ -26,6 +27,8 @@ class SamplingParams:
             raise ValueError(f"top_k must be >= 0, got {self.top_k}")
         if not 0 < self.top_p <= 1:
             raise ValueError(f"top_p must lie in (0, 1], got {self.top_p}")
+        if not 0 <= self.min_p <= 1:
+            raise ValueError(f"min_p must lie in [0, 1], got {self.min_p}")
         if self.repeat_penalty <= 0:
             raise ValueError(f"repeat_penalty must be positive, got {self.repeat_penalty}")
         return self

@@ -1,7 +1,7 @@
 """Draws one token per logits row on the device.
 
 Rows that are all greedy need no upload at all.  Otherwise the options of all rows
-(temperature, top-p, the uniform number of the draw; top-k) go up as two small arrays;
+(temperature, top-p, the uniform number of the draw, min-p; top-k) go up as two small arrays;
 penalties and biases go as ragged lists (each distinct generated id once,
 as the reference's set does, crates/core/src/sampling.rs:670-688); the kernels of
 csrc/sampling.cu do the rest and only the chosen ids come back to the host."""
@@ -49,15 +49,15 @@ class Sampler:
             return out_tok, (out_lp if want_logprobs else None)
         if any(p.needs_penalties for p in params):
             self._penalties(logits, params, generated)
-        f = np.zeros((3, R), dtype=np.float32)
+        f = np.zeros((4, R), dtype=np.float32)
         k = np.zeros(R, dtype=np.int32)
         for r, p in enumerate(params):
-            f[0, r], f[1, r] = p.temperature, p.top_p
+            f[0, r], f[1, r], f[3, r] = p.temperature, p.top_p, p.min_p
             f[2, r] = self.uniform_for(p, steps[r] if steps is not None else len(generated[r])) if p.temperature > 0 else 0.0
             k[r] = p.top_k
         fd = torch.from_numpy(f).to(self.device, non_blocking=True)
         kd = torch.from_numpy(k).to(self.device, non_blocking=True)
-        ops.sample(logits, fd[0], kd, fd[1], fd[2], out_tok, out_lp if want_logprobs else None)
+        ops.sample(logits, fd[0], kd, fd[1], fd[2], out_tok, out_lp if want_logprobs else None, min_p=fd[3])
         return out_tok, (out_lp if want_logprobs else None)
 
     def _penalties(self, logits, params, generated):
