@@ -960,6 +960,8 @@ def qk_norm_rope_write_8bit(qkv, positions, slots, cu_seqlens, q_weight, k_weigh
         raise KernelError(f"qkv {tuple(qkv.shape)} does not match heads {num_heads}+2*{num_kv_heads} x {head_dim}")
     B = pages = page_size = 0
     if slots is not None:
+        if any(t is None for t in (cu_seqlens, k_cache, v_cache, k_scale, v_scale)):
+            raise KernelError("qk_norm_rope_write_8bit: slots go with cu_seqlens, a cache and its scales")
         _need(slots, torch.int32, "slots", 1); _need(cu_seqlens, torch.int32, "cu_seqlens", 1)
         _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim)
         if slots.shape[0] != T or cu_seqlens.shape[0] < 1:
