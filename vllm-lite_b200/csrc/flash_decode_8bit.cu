@@ -43,6 +43,9 @@ constexpr bool ODD = HD % 32 != 0;                     // and two features more:
 constexpr int OT = HD / 16;                            // tiles of 16 features
 constexpr float ROOM = 8.f;                            // log2 of what a weight may exceed the base's by
 constexpr int SHIFT = 6;                               // p sv is held times 2^SHIFT
+constexpr int AHEAD = 4;                               // steps whose keys and values are asked for into L2 ahead of their loads
+constexpr int PIECES_MAX = 4 * (HD + 4) < 302 ? 4 * (HD + 4) : 302;     // most pieces of an item: a weight a head and piece in the room of s_o
+constexpr int MIN_RUN = 2;                             // fewest steps of a run
 
 struct Tile { unsigned k[2][KW], v[4][VW > 0 ? VW : 1]; unsigned short v2[4]; };
 
@@ -69,6 +72,9 @@ __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const unsigned*>(&v);
 }
+__device__ __forceinline__ void prefetch_l2(const void* p, unsigned bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(min(max(e, -126), 127) + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float s) { return (int)(__float_as_uint(s) >> 23) - 127; }
 
@@ -82,17 +88,18 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
                          const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ block_table, int max_blocks,
                          const int* __restrict__ req_index, const int* __restrict__ positions, int T, int nq, int nkv, int page_size, int num_pages,
                          float scale_log2, int window, int bound, int S, float* __restrict__ part, unsigned* err, const int* __restrict__ token_index,
-                         bf16* __restrict__ out, int* arrivals) {
+                         bf16* __restrict__ out, int* arrivals, int settled) {
     constexpr int HEADS = 8 * NT;
     constexpr int OLD = HD + 4;
-    __shared__ float s_o[WARPS][HEADS][OLD];
+    __shared__ __align__(16) float s_o[WARPS][HEADS][OLD];
     __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_e[WARPS];
     __shared__ int s_scan[WARPS], s_most, s_z, s_before, s_last[2];
     __shared__ Piece s_partial[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    float* const part_ml = part + (size_t)T * nq * S * HD;   // behind the numerators: (maximum, sum) of each
     pdl_launch_dependents();
     if (tid == 0) { s_most = 0; s_z = T; s_before = 0; s_partial[0].heads = s_partial[1].heads = 0; }
-    pdl_wait();
+    if (!settled) pdl_wait();                                // a kernel before this one may be writing the step's description
     __syncthreads();
     const int grp = nq / nkv, htiles = (grp + HEADS - 1) / HEADS, ny = nkv * htiles;
     // the keys [lo, n) of token z (its number within the launch): none for a padded place or a position beyond the bound
@@ -130,7 +137,7 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
     }
     // (a run as long as S allows leaves no item in more than S runs)
     const int grid = gridDim.x, all_steps = total;
-    const int per = max(max((all_steps + grid - 1) / grid, 1), (s_most + S - 2) / (S - 1));
+    const int per = max(max((all_steps + grid - 1) / grid, MIN_RUN), (s_most + S - 2) / (S - 1));
     const int first = (int)min((long long)blockIdx.x * per, (long long)all_steps), last = (int)min((long long)first + per, (long long)all_steps);
     total = 0;
     for (int z0 = 0; z0 < T; z0 += NTHREADS) {
@@ -139,6 +146,7 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         if (u > first && u - n <= first) { s_z = z0 + tid; s_before = u - n; }
     }
     __syncthreads();
+    pdl_wait();                                              // q and the cache are written by the kernel before
     // the places without keys: rows of zeros, and the ones beyond the bound are flagged
     for (int z = blockIdx.x; z < T; z += grid) {
         int tok, lo;
@@ -230,19 +238,28 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         const int st0 = pc.c0 / BN, st1 = (pc.c1 - 1) / BN;
         // the cache row and the scales of key `lane` (of 16; WIDE: of the first one) of a step's keys: row < 0 for one that is not read
         struct Where { int row; float ks, vs; };
-        auto find = [&](int st) -> Where {
+        auto page_of = [&](int key) -> int {                 // -1 for one that is not read
+            if (key >= pc.c1 || key + (WIDE ? 15 : 0) < pc.c0) return -1;
+            const int blk = key / page_size;
+            return blk < max_blocks ? table[blk] : -2;
+        };
+        auto where_of = [&](int page, int key) -> Where {
             Where w = {-1, 0.f, 0.f};
-            const int key = st * BN + warp * 16 + (WIDE ? 0 : (lane & 15));
-            if (st > st1 || key >= pc.c1 || key + (WIDE ? 15 : 0) < pc.c0) return w;
-            const int blk = key / page_size, page = blk < max_blocks ? table[blk] : -1;
+            if (page == -1 && (key >= pc.c1 || key + (WIDE ? 15 : 0) < pc.c0)) return w;
             if (page < 0 || page >= num_pages) { bad_page = true; return w; }
             const int head = page * nkv + pc.kvh;
-            w.row = head * page_size + (key - blk * page_size);
+            w.row = head * page_size + key % page_size;
             w.ks = kscale[head];
             w.vs = vscale[head];
-            // values under a scale that is none: their keys' scores say so, so that only who reads them gets NaN
+            return w;
+        };
+        // values under a scale that is none: their keys' scores say so, so that only who reads them gets NaN
+        auto settle = [&](Where w) -> Where {
             if (w.vs != w.vs) { w.ks = w.vs; w.vs = 0.f; }
             return w;
+        };
+        auto ask = [&](int row) {                            // 16 keys' rows and their values' into L2
+            if (row >= 0) { prefetch_l2(kcache + (size_t)row * HD, 16 * HD); prefetch_l2(vcache + (size_t)row * HD, 16 * HD); }
         };
         auto load = [&](Tile& x, const Where& w) {
 #pragma unroll
@@ -364,18 +381,56 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         };
         {
             Tile x, y;
-            Where wx = find(st0), wy = find(st0 + 1);
-            load(x, wx);
-            for (int st = st0; st <= st1; st += 2) {
-                load(y, wy);
-                Where next = find(st + 2);
-                work(x, wx, st);
-                wx = next;
-                if (st + 1 > st1) break;
+            if constexpr (WIDE) {
+                // lane i knows the place of step base + i; the next 32 steps' are looked up on the way, a load at a time
+                const int k_of = warp * 16;
+                auto key_of = [&](int st) { return st * BN + k_of; };
+                Where now = where_of(page_of(key_of(st0 + lane)), key_of(st0 + lane)), then = {-1, 0.f, 0.f};
+                int base = st0, page = -1;
+                auto at_step = [&](int st) -> Where {        // (of a step of the present 32)
+                    Where w = {__shfl_sync(0xffffffffu, now.row, st - base), __shfl_sync(0xffffffffu, now.ks, st - base), __shfl_sync(0xffffffffu, now.vs, st - base)};
+                    return settle(w);
+                };
+                if (lane <= AHEAD) ask(now.row);
+                auto advance = [&](int st) {                 // before step st's work: what lies ahead of it
+                    const int i = st - base;
+                    if (i == 0) page = page_of(key_of(base + 32 + lane));
+                    if (i == 16) then = where_of(page, key_of(base + 32 + lane));
+                    const int j = i + 1 + AHEAD;             // step st + 1 + AHEAD
+                    if (lane == (j & 31)) ask(j < 32 ? now.row : then.row);
+                };
+                auto next_of = [&](int st) -> Where {        // step st + 1
+                    if (st + 1 - base == 32) { now = then; base += 32; }
+                    return at_step(st + 1);
+                };
+                Where wx = at_step(st0), wy;
                 load(x, wx);
-                next = find(st + 3);
-                work(y, wy, st + 1);
-                wy = next;
+                for (int st = st0; st <= st1; st += 2) {
+                    advance(st);
+                    wy = next_of(st);
+                    load(y, wy);
+                    work(x, wx, st);
+                    if (st + 1 > st1) break;
+                    advance(st + 1);
+                    wx = next_of(st + 1);
+                    load(x, wx);
+                    work(y, wy, st + 1);
+                }
+            } else {
+                auto find = [&](int st) -> Where { return settle(where_of(page_of(st * BN + warp * 16 + (lane & 15)), st * BN + warp * 16 + (lane & 15))); };
+                Where wx = find(st0), wy = find(st0 + 1);
+                load(x, wx);
+                for (int st = st0; st <= st1; st += 2) {
+                    load(y, wy);
+                    Where next = find(st + 2);
+                    work(x, wx, st);
+                    wx = next;
+                    if (st + 1 > st1) break;
+                    load(x, wx);
+                    next = find(st + 3);
+                    work(y, wy, st + 1);
+                    wy = next;
+                }
             }
         }
 
@@ -416,9 +471,9 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
             if (pc.pieces == 1) {
                 out[((size_t)pc.tok * nq + pc.h0 + h) * HD + d] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
             } else {
-                float* mine = part + (((size_t)pc.place * nq + pc.h0 + h) * S + pc.piece) * (HD + 2);
-                __stcg(mine + d, acc);
-                if (d == 0) { __stcg(mine + HD, M); __stcg(mine + HD + 1, L); }
+                const size_t row = ((size_t)pc.place * nq + pc.h0 + h) * S + pc.piece;
+                __stcg(part + row * HD + d, acc);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(part_ml) + row, make_float2(M, L));
             }
         }
         if (pc.pieces > 1 && tid == 0) s_partial[number > 0] = pc;
@@ -437,21 +492,40 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
     for (int k = 0; k < 2; ++k) {
         if (!s_last[k]) continue;
         const Piece pc = s_partial[k];
-        for (int i = tid; i < pc.heads * HD; i += NTHREADS) {
-            const int h = i / HD, d = i - h * HD;
-            const float* all = part + ((size_t)pc.place * nq + pc.h0 + h) * S * (HD + 2);
-            float M = -INFINITY, acc = 0.f, L = 0.f;
-            for (int p = 0; p < pc.pieces; ++p) M = fmaxf(M, __ldcg(all + (size_t)p * (HD + 2) + HD));
+        // the pieces' weights and the sums' quotient, in the memory of the warps' shares
+        float* weight = &s_o[0][0][0];                       // [heads][pieces]
+        const float2* ml = reinterpret_cast<const float2*>(part_ml) + ((size_t)pc.place * nq + pc.h0) * S;
+        for (int h = warp; h < pc.heads; h += WARPS) {
+            float M = -INFINITY, L = 0.f;
+            for (int p = lane; p < pc.pieces; p += 32) M = fmaxf(M, __ldcg(ml + (size_t)h * S + p).x);
+            M = warp_max(M);
             const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
-            for (int p = 0; p < pc.pieces; ++p) {
-                const float* one = all + (size_t)p * (HD + 2);
-                const float mp = __ldcg(one + HD), f = mp == -INFINITY ? 1.f : exp2_fast(mp - base);
-                acc += __ldcg(one + d) * f;
-                L += __ldcg(one + HD + 1) * f;
+            for (int p = lane; p < pc.pieces; p += 32) {
+                const float2 x = __ldcg(ml + (size_t)h * S + p);
+                const float f = x.x == -INFINITY ? 1.f : exp2_fast(x.x - base);
+                L += x.y * f;
+                weight[h * pc.pieces + p] = f;
             }
-            out[((size_t)pc.tok * nq + pc.h0 + h) * HD + d] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
+            L = warp_sum(L);
+            if (lane == 0) s_l[0][h] = L;
         }
+        __syncthreads();
+        for (int i = tid; i < pc.heads * (HD / 4); i += NTHREADS) {
+            const int h = i / (HD / 4), d = (i - h * (HD / 4)) * 4;
+            const float* row = part + ((size_t)pc.place * nq + pc.h0 + h) * S * HD + d;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int p = 0; p < pc.pieces; ++p) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(row + (size_t)p * HD));
+                const float f = weight[h * pc.pieces + p];
+                acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+            }
+            const float L = s_l[0][h], inv = L == 0.f ? 0.f : 1.f / L;
+            bf16* dst = out + ((size_t)pc.tok * nq + pc.h0 + h) * HD + d;
+            dst[0] = __float2bfloat16(acc.x * inv); dst[1] = __float2bfloat16(acc.y * inv);
+            dst[2] = __float2bfloat16(acc.z * inv); dst[3] = __float2bfloat16(acc.w * inv);
+        }
+        __syncthreads();                                     // the weights may be written again
         if (tid == 0) arrivals[pc.counter] = 0;              // as the next launch finds it
     }
 }
@@ -464,12 +538,12 @@ extern "C" int vl_flash_decode_8bit_head_dim() { return HD; }
 extern "C" int vl_flash_decode_8bit(const void* q, int q_stride, const void* kcache, const void* vcache, const float* kscale, const float* vscale,
                                     const int* block_table, int max_blocks, const int* req_index, const int* positions, int T, int nq, int nkv, int hd,
                                     int page_size, int num_pages, float scale, int window, int bound, int S, float* part, unsigned* err,
-                                    const int* token_index, void* out, int* arrivals, void* stream) {
+                                    const int* token_index, void* out, int* arrivals, int settled, void* stream) {
     if (T <= 0) return VL_OK;
     if (hd != HD) return VL_ERR_UNSUPPORTED;
     if (nq <= 0 || nkv <= 0 || nq % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || q_stride < nq * hd || q_stride % 4) return VL_ERR_ARGUMENT;
-    if (bound <= 0 || S < 2 || !out || !arrivals || !part) return VL_ERR_ARGUMENT;
-    if (((uintptr_t)q & 7) || (((uintptr_t)kcache | (uintptr_t)vcache) & 15)) return VL_ERR_ARGUMENT;
+    if (bound <= 0 || S < 2 || S > PIECES_MAX || !out || !arrivals || !part) return VL_ERR_ARGUMENT;
+    if (((uintptr_t)q & 7) || (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)part) & 15)) return VL_ERR_ARGUMENT;
     const int grp = nq / nkv, wide_heads = grp > 8 && HD <= 128 ? 16 : 8, htiles = (grp + wide_heads - 1) / wide_heads;
     const long long most = (long long)T * nkv * htiles * ((bound + BN - 1) / BN);
     if ((long long)num_pages * nkv * page_size >= (1ll << 31) || most >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
@@ -482,7 +556,7 @@ extern "C" int vl_flash_decode_8bit(const void* q, int q_stride, const void* kca
         const long long grid = (long long)sms * blocks_an_sm;
         return vl_launch(kernel, dim3((unsigned)(most < grid ? most : grid)), dim3(NTHREADS), 0, (cudaStream_t)stream, (const bf16*)q, q_stride,
                          (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks, req_index, positions, T,
-                         nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, bound, S, part, err, token_index, (bf16*)out, arrivals);
+                         nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, bound, S, part, err, token_index, (bf16*)out, arrivals, settled);
     };
     if constexpr (HD <= 128) {
         if (wide_heads == 16) return wide ? launch(flash_decode_8bit_kernel<2, true>, 2) : launch(flash_decode_8bit_kernel<2, false>, 2);

@@ -157,7 +157,7 @@ _SIGNATURES = {
                                                    c_int, c_void_p, c_void_p],
     ("flash_decode_8bit", "vl_flash_decode_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                                                     c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
-                                                    c_void_p, c_void_p, c_void_p],
+                                                    c_void_p, c_void_p, c_int, c_void_p],
     ("flash_tc5_8bit", "vl_flash_prefill_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                                   c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p],
     ("sampling", "vl_apply_penalties"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -993,10 +993,14 @@ def qk_norm_rope_write_8bit(qkv, positions, slots, cu_seqlens, q_weight, k_weigh
 
 
 def flash_decode_8bit_scratch(num_tokens, num_heads, num_kv_heads, head_dim):
-    """(floats of scratch memory, int32 counters) that `flash_decode_8bit` wants for so many tokens: an item (a token's KV head) may be shared by as many
-    pieces as leave every block of the launch its share of a step of few tokens, and by two at least."""
-    pieces = 2 + -(-600 // max(1, num_tokens * num_kv_heads))
-    return num_tokens * num_heads * pieces * (head_dim + 2), num_tokens * num_heads
+    """(floats of scratch memory, int32 counters) that `flash_decode_8bit` wants for so many tokens."""
+    return num_tokens * num_heads * _pieces_8bit(num_tokens, num_kv_heads, head_dim) * (head_dim + 2), num_tokens * num_heads
+
+
+def _pieces_8bit(num_tokens, num_kv_heads, head_dim):
+    """How many pieces an item (a token's KV head) may be shared by: as many as leave every block of the launch its share of a step of few tokens, two at
+    least, and no more than a block can add up."""
+    return min(2 + -(-600 // max(1, num_tokens * num_kv_heads)), 302, 4 * (head_dim + 4))
 
 
 def _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, name):
@@ -1010,12 +1014,13 @@ def _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table
 
 
 def flash_decode_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, req_index, positions, num_heads, num_kv_heads, head_dim, scale, window,
-                      max_context, err, token_index=None, scratch=None, arrivals=None):
+                      max_context, err, token_index=None, scratch=None, arrivals=None, settled=False):
     """Attention of single tokens over a cache in 8 bits (`qk_norm_rope_write_8bit`): q bfloat16 [T, >= nq hd] (its first columns are read), out bfloat16
     [T, nq hd]; token t, at positions[t] of the request whose pages row req_index[t] of block_table names, reads every key up to its own or the last `window`.
     Tokens at negative positions and (flagged) at max_context or beyond get rows of zeros.  token_index (int32): only these tokens, the others' rows of
     out are left alone.  scratch (float32) and arrivals (int32, zero before and after each call): at least `flash_decode_8bit_scratch` of them, which nobody
-    else on the stream needs; without them the call takes its own.  Pages may have any number of positions; q begins on 8 bytes."""
+    else on the stream needs; without them the call takes its own.  Pages may have any number of positions; q begins on 8 bytes, scratch on 16.
+    `settled`: as in `flash_decode`."""
     _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, "flash_decode_8bit")
     _need(req_index, torch.int32, "req_index", 1); _need(positions, torch.int32, "positions", 1)
     T = q.shape[0]
@@ -1036,11 +1041,10 @@ def flash_decode_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, r
     _need(scratch, torch.float32, "scratch", 1); _need(arrivals, torch.int32, "arrivals", 1)
     if scratch.shape[0] < floats or arrivals.shape[0] < counters:
         raise KernelError(f"flash_decode_8bit: {floats} floats of scratch and {counters} counters are wanted, got {scratch.shape[0]} and {arrivals.shape[0]}")
-    pieces = floats // (T * num_heads * (head_dim + 2))
     _check(_fn("flash_decode_8bit", "vl_flash_decode_8bit", {"FA_HD": head_dim})(
         q, q.shape[1], k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], req_index, positions, T, num_heads, num_kv_heads, head_dim,
-        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), int(max_context), pieces, scratch, err, token_index, out, arrivals,
-        _stream()), "vl_flash_decode_8bit")
+        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), int(max_context), _pieces_8bit(T, num_kv_heads, head_dim), scratch, err,
+        token_index, out, arrivals, int(settled), _stream()), "vl_flash_decode_8bit")
     return out
 
 

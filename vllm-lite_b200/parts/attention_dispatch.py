@@ -155,7 +155,8 @@ def run_8bit(qkv, out, cache, group, step, spec, scale):
         # one set of counters for all layers of a step shape: every launch leaves them zero
         ops.flash_decode_8bit(*common, step.req_index, step.positions, *sizes, context, step.err, token_index=token_index,
                               scratch=step.workspace.get(step.tag + "attn8.scratch", (floats,), torch.float32),
-                              arrivals=step.workspace.zeros(step.tag + "attn8.arrivals", counters, torch.int32))
+                              arrivals=step.workspace.zeros(step.tag + "attn8.arrivals", counters, torch.int32),
+                              settled=getattr(step, "settled", False))
 
     if step.max_query_len == 1:
         single(qkv.shape[0], group.max_context)
