@@ -591,15 +591,15 @@ def test_the_write_refuses_before_any_launch(change, code):
 
 @pytest.mark.parametrize("change,code", [
     (dict(hd=64), -2), (dict(nq=3), -3), (dict(nkv=0), -3), (dict(ps=0), -3), (dict(pages=0), -3), (dict(blocks=0), -3), (dict(stride=250), -3), (dict(stride=258), -3),
-    (dict(bound=0), -3), (dict(S=1), -3), (dict(q=4), -3), (dict(k=8), -3), (dict(v=8), -3), (dict(part=None), -3), (dict(S=303), -3), (dict(part=8), -3), (dict(arrivals=None), -3), (dict(pages=1 << 30), -2),
+    (dict(bound=0), -3), (dict(floats=700), -3), (dict(q=4), -3), (dict(k=8), -3), (dict(v=8), -3), (dict(part=None), -3), (dict(part=8), -3), (dict(arrivals=None), -3), (dict(pages=1 << 30), -2),
     (dict(T=1 << 30), -2), (dict(T=0), 0)])
 def test_single_tokens_are_refused_before_any_launch(change, code):
     host, at = entry_args()
-    c = dict(q=0, k=0, v=0, stride=256, blocks=2, T=1, nq=2, nkv=1, hd=128, ps=64, pages=4, bound=100, S=4, part=at, arrivals=at)
+    c = dict(q=0, k=0, v=0, stride=256, blocks=2, T=1, nq=2, nkv=1, hd=128, ps=64, pages=4, bound=100, floats=780, part=at, arrivals=at)
     c.update(change)
     got = ops._fn("flash_decode_8bit", "vl_flash_decode_8bit", {"FA_HD": 128})(
-        at + c["q"], c["stride"], at + c["k"], at + c["v"], at, at, at, c["blocks"], at, at, c["T"], c["nq"], c["nkv"], c["hd"], c["ps"], c["pages"], 0.1, 0, c["bound"], c["S"],
-        c["part"], None, None, at, c["arrivals"], 0, 0)
+        at + c["q"], c["stride"], at + c["k"], at + c["v"], at, at, at, c["blocks"], at, at, c["T"], c["nq"], c["nkv"], c["hd"], c["ps"], c["pages"], 0.1, 0, c["bound"],
+        c["part"], c["floats"], None, None, at, c["arrivals"], 0, 0)
     assert got == code
 
 

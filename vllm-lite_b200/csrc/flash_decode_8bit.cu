@@ -24,6 +24,7 @@
 // Keys outside lo..p, or on pages that the table does not hold (flagged), weigh nothing whatever their bytes and scales are; a page whose scale is not a
 // number makes the result NaN where one of its keys is read.
 #include "cache_8bit.cuh"
+#include <type_traits>
 
 #ifndef FA_HD
 #define FA_HD 128
@@ -34,7 +35,8 @@ using namespace cache8;
 namespace {
 constexpr int HD = FA_HD;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head sizes in steps of 16 up to 256");
-constexpr int BN = 64, WARPS = 4, NTHREADS = 32 * WARPS;
+constexpr int SUB = HD <= 192 ? 2 : 1, WARPS = 4, BN = 16 * SUB * WARPS;   // a step: SUB tiles of 16 keys a warp
+constexpr int NTHREADS = 32 * WARPS, OLD = HD + 4;
 constexpr int KW = HD / 16;                            // words (4 features) of a key that a lane takes: lanes t of a quad, piece j -> words (4j + t) KL ..
 constexpr int KL = KW % 4 == 0 ? 4 : (KW % 2 == 0 ? 2 : 1);      // words a load
 constexpr int VW = HD / 32;                            // ... of a value: lanes g of eight, piece j -> words (8j + g) VL ..
@@ -43,16 +45,40 @@ constexpr bool ODD = HD % 32 != 0;                     // and two features more:
 constexpr int OT = HD / 16;                            // tiles of 16 features
 constexpr float ROOM = 8.f;                            // log2 of what a weight may exceed the base's by
 constexpr int SHIFT = 6;                               // p sv is held times 2^SHIFT
-constexpr int AHEAD = 4;                               // steps whose keys and values are asked for into L2 ahead of their loads
-constexpr int PIECES_MAX = 4 * (HD + 4) < 302 ? 4 * (HD + 4) : 302;     // most pieces of an item: a weight a head and piece in the room of s_o
-constexpr int MIN_RUN = 2;                             // fewest steps of a run
+#ifndef T_MIN
+#define T_MIN 2
+#define T_WAVES 3
+#define T_SHORT 4
+#define T_APART 64
+#endif
+constexpr int SHORTER = T_SHORT;                       // the later runs are so many times shorter
+constexpr int MIN_RUN = T_MIN;                             // fewest steps of a run
 
-struct Tile { unsigned k[2][KW], v[4][VW > 0 ? VW : 1]; unsigned short v2[4]; };
+// A warp's ring: NS stages of 16 keys' rows and 16 values' rows, in strides with which the lanes' loads meet in no bank: a quad of lanes takes
+// 16 KL bytes of a key's row side by side, four rows apart in the lanes' groups of eight, and values are taken two rows apart.
+constexpr int stride_of(int at_least, int want, int mod) { return at_least % mod == want ? at_least : stride_of(at_least + 16, want, mod); }
+constexpr int KS = stride_of(HD, 16 * KL, 128), VS = stride_of(HD, 16, 64), TILE = 16 * (KS + VS), STAGE = SUB * TILE;
+constexpr int RESIDENT = 2;                            // blocks an SM
+constexpr int NS = 2;
+constexpr int PIECES = HD / 16;                        // 16-byte pieces of a row
 
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, int bytes) {       // bytes 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// N copies of 16 bytes, TO and FROM bytes apart (offsets within the instructions: an addition for each would cost more than the copies)
+template <int TO, int FROM, int N, int I = 0> __device__ __forceinline__ void copies16(unsigned dst, const void* src) {
+    if constexpr (I < N) {
+        asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(dst), "l"(src), "n"(I * TO), "n"(I * FROM) : "memory");
+        copies16<TO, FROM, N, I + 1>(dst, src);
+    }
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 template <int N> __device__ __forceinline__ void load_words(const unsigned char* p, unsigned* w) {
-    if constexpr (N == 4) { const uint4 x = __ldg(reinterpret_cast<const uint4*>(p)); w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; }
-    else if constexpr (N == 2) { const uint2 x = __ldg(reinterpret_cast<const uint2*>(p)); w[0] = x.x; w[1] = x.y; }
-    else w[0] = __ldg(reinterpret_cast<const unsigned*>(p));
+    if constexpr (N == 4) { const uint4 x = *reinterpret_cast<const uint4*>(p); w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; }
+    else if constexpr (N == 2) { const uint2 x = *reinterpret_cast<const uint2*>(p); w[0] = x.x; w[1] = x.y; }
+    else w[0] = *reinterpret_cast<const unsigned*>(p);
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -72,43 +98,111 @@ __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const unsigned*>(&v);
 }
-__device__ __forceinline__ void prefetch_l2(const void* p, unsigned bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(min(max(e, -126), 127) + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float s) { return (int)(__float_as_uint(s) >> 23) - 127; }
 
-struct Piece { int tok, place, kvh, h0, heads, c0, c1, piece, pieces, counter, stop; };   // heads 0: the end of the run
+struct Piece { int tok, req, kvh, h0, heads, c0, c1, piece, pieces, item, slot, slot0, stop; };   // heads 0: the end of the run
+
+// The runs: as many of a steps as the GPU holds at once, then equally many of about a / SHORTER and a / SHORTER^2, which the blocks that finish first take.
+struct Runs {
+    int most, more, a, b, c;
+    __device__ __forceinline__ Runs(int all, int resident, int count) : most(min(resident, count)), more((count - most) / 2) {
+        const int in_first = SHORTER * SHORTER * most + (SHORTER + 1) * more;    // steps of all, were a = SHORTER^2
+        a = max((int)(((long long)all * SHORTER * SHORTER + in_first - 1) / in_first), MIN_RUN);
+        b = max((a + SHORTER - 1) / SHORTER, MIN_RUN);
+        c = max((b + SHORTER - 1) / SHORTER, MIN_RUN);
+    }
+    __device__ __forceinline__ long long begin(int r) const {
+        return (long long)min(r, most) * a + (long long)min(max(r - most, 0), more) * b + (long long)max(r - most - more, 0) * c;
+    }
+    __device__ __forceinline__ int of(int step) const {
+        const long long one = (long long)most * a, two = one + (long long)more * b;
+        return step < one ? step / a : (step < two ? most + (int)((step - one) / b) : most + more + (int)((step - two) / c));
+    }
+};
+
+// Adds up an item's pieces for one head: numerators at part + (slot of piece p) * stride, (maximum, sum) at ml + (slot of piece p) * heads.  The slots: `first`,
+// then every second one from `next` on.  A thread takes 4 features at d; 8 pieces' numbers are on their way together.
+__device__ __forceinline__ void add_pieces(const float* part, const float2* ml, size_t stride, int heads, int first, int next, int pieces, int d, bf16* dst) {
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < pieces; p0 += 8) {
+        float2 x[8];
+        float4 a[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            const int i = min(p0 + p, pieces - 1);
+            const size_t slot = i == 0 ? first : next + 2 * (i - 1);
+            x[p] = __ldcg(ml + slot * heads);
+            a[p] = __ldcg(reinterpret_cast<const float4*>(part + slot * stride + d));
+        }
+        float top = M;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) top = fmaxf(top, x[p].x);
+        const float base = top == -INFINITY ? 0.f : top, old = M == -INFINITY ? 1.f : exp2_fast(M - base);
+        M = top;
+        L *= old;
+        acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            if (p0 + p >= pieces) continue;
+            const float f = x[p].x == -INFINITY ? 1.f : exp2_fast(x[p].x - base);         // (a piece of NaN keeps its sums)
+            L += x[p].y * f;
+            acc.x += a[p].x * f; acc.y += a[p].y * f; acc.z += a[p].z * f; acc.w += a[p].w * f;
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    dst[d] = __float2bfloat16(acc.x * inv); dst[d + 1] = __float2bfloat16(acc.y * inv);
+    dst[d + 2] = __float2bfloat16(acc.z * inv); dst[d + 3] = __float2bfloat16(acc.w * inv);
+}
 }  // namespace
+
+// What of the scratch memory holds what: `runs` runs leave two pieces at most (of the item that a run begins in, of the one that it ends in), each of `heads` rows of
+// HD numerators; behind them (maximum, sum) of each row; behind those four words for each item.
+struct Scratch {
+    float* part;
+    float2* ml;
+    int4* info;                                        // of an item in pieces: slot of the first, of the second, how many (0: none), token
+    __host__ __device__ Scratch(float* p, long long runs, int heads)
+        : part(p), ml(reinterpret_cast<float2*>(p + 2 * runs * heads * HD)), info(reinterpret_cast<int4*>(p + (2 * runs * heads * (HD + 2) + 3) / 4 * 4)) {}
+    static __host__ __device__ long long floats(long long runs, int heads, long long items) { return (2 * runs * heads * (HD + 2) + 3) / 4 * 4 + 4 * items; }
+};
 
 // WIDE: pages of a multiple of 16 positions, so that 16 keys lie on one page.
 template <int NT, bool WIDE>
-__global__ void __launch_bounds__(NTHREADS, NT == 1 && HD <= 128 ? 3 : 2)
+__global__ void __launch_bounds__(NTHREADS, RESIDENT)
 flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigned char* __restrict__ kcache, const unsigned char* __restrict__ vcache,
                          const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ block_table, int max_blocks,
                          const int* __restrict__ req_index, const int* __restrict__ positions, int T, int nq, int nkv, int page_size, int num_pages,
-                         float scale_log2, int window, int bound, int S, float* __restrict__ part, unsigned* err, const int* __restrict__ token_index,
-                         bf16* __restrict__ out, int* arrivals, int settled) {
+                         float scale_log2, int window, int bound, int resident, float* scratch, unsigned* err, const int* __restrict__ token_index,
+                         bf16* __restrict__ out, int* arrivals, int settled) {      // arrivals null: another launch adds the pieces up
     constexpr int HEADS = 8 * NT;
-    constexpr int OLD = HD + 4;
-    __shared__ __align__(16) float s_o[WARPS][HEADS][OLD];
+    extern __shared__ __align__(16) unsigned char smem[];    // the warps' rings; where those are at rest, the warps' shares of a piece
+    float (*s_o)[HEADS][OLD] = reinterpret_cast<float (*)[HEADS][OLD]>(smem);
+    __shared__ float2 s_scale[WARPS][NS][SUB][WIDE ? 1 : 16];     // scales of a stage's keys and values
     __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_e[WARPS];
-    __shared__ int s_scan[WARPS], s_most, s_z, s_before, s_last[2];
+    __shared__ int s_scan[WARPS], s_z, s_before, s_last[2];
+    __shared__ int s_tok[NTHREADS], s_pos[NTHREADS], s_req[NTHREADS];            // of the launch's first tokens
     __shared__ Piece s_partial[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    float* const part_ml = part + (size_t)T * nq * S * HD;   // behind the numerators: (maximum, sum) of each
     pdl_launch_dependents();
-    if (tid == 0) { s_most = 0; s_z = T; s_before = 0; s_partial[0].heads = s_partial[1].heads = 0; }
+    if (tid == 0) { s_z = T; s_before = 0; s_partial[0].heads = s_partial[1].heads = 0; }
     if (!settled) pdl_wait();                                // a kernel before this one may be writing the step's description
-    __syncthreads();
     const int grp = nq / nkv, htiles = (grp + HEADS - 1) / HEADS, ny = nkv * htiles;
     // the keys [lo, n) of token z (its number within the launch): none for a padded place or a position beyond the bound
     auto keys_of = [&](int z, int* tok, int* lo) -> int {
-        const int k = token_index ? token_index[z] : z, pos = positions[k];
+        const int k = token_index ? (z < NTHREADS ? s_tok[z] : token_index[z]) : z, pos = z < NTHREADS ? s_pos[z] : positions[k];
         if (tok) *tok = k;
         *lo = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
         return pos >= 0 && pos < bound ? pos + 1 : 0;
     };
+    if (tid < T) {
+        const int k = token_index ? token_index[tid] : tid;
+        s_tok[tid] = k;
+        s_pos[tid] = positions[k];
+        s_req[tid] = req_index[k];
+    }
+    __syncthreads();
     auto steps_of = [&](int lo, int keys) { return keys > 0 ? (keys - 1) / BN - lo / BN + 1 : 0; };
     // Where this block's run lies: the number of steps, the longest item, and the token in which the run begins.  A round is a token a thread.
     int total = 0;
@@ -119,8 +213,6 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         int x = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
-        const int longest = __reduce_max_sync(0xffffffffu, most);
-        if (lane == 0) atomicMax(&s_most, longest);
         if (lane == 31) s_scan[warp] = x;
         __syncthreads();
         int all = 0;
@@ -135,10 +227,11 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         const int u = round(z0, n);
         if (z0 == 0) { n0 = n; u0 = u; }
     }
-    // (a run as long as S allows leaves no item in more than S runs)
-    const int grid = gridDim.x, all_steps = total;
-    const int per = max(max((all_steps + grid - 1) / grid, MIN_RUN), (s_most + S - 2) / (S - 1));
-    const int first = (int)min((long long)blockIdx.x * per, (long long)all_steps), last = (int)min((long long)first + per, (long long)all_steps);
+    const int grid = gridDim.x, all_steps = total, run = blockIdx.x;
+    const Runs runs(all_steps, resident, grid);
+    const int first = (int)min(runs.begin(run), (long long)all_steps), last = (int)min(runs.begin(run + 1), (long long)all_steps);
+    const int held = min(HEADS, grp);                        // rows that a piece leaves
+    const Scratch left(scratch, grid, held);
     total = 0;
     for (int z0 = 0; z0 < T; z0 += NTHREADS) {
         int n = n0, u = u0;
@@ -153,6 +246,8 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         if (keys_of(z, &tok, &lo) > 0) continue;
         if (tid == 0 && err && positions[tok] >= 0) atomicOr(err, VL_DEV_BEYOND_BOUND);
         for (int i = tid; i < nq * HD; i += NTHREADS) out[(size_t)tok * nq * HD + i] = __float2bfloat16(0.f);
+        if (!arrivals)
+            for (int y = tid; y < ny; y += NTHREADS) __stcg(left.info + z * ny + y, make_int4(0, 0, 0, 0));
     }
 
     int z = s_z, before = s_before;
@@ -170,17 +265,20 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         }
         if (at >= last || z >= T) return p;
         const int y = (at - before) / tz, start = before + y * tz, htile = y % htiles;       // the item's first step
+        p.req = z < NTHREADS ? s_req[z] : req_index[p.tok];
         p.kvh = y / htiles;
-        p.place = z;
         p.stop = min(last, start + tz);
         p.h0 = p.kvh * grp + htile * HEADS;
         p.heads = min(HEADS, grp - htile * HEADS);
         const int step0 = lo / BN - start;                   // + a step's number in the launch = its number in the request
         p.c0 = max((at + step0) * BN, lo);
         p.c1 = min((p.stop + step0) * BN, keys);
-        p.piece = (int)blockIdx.x - start / per;
-        p.pieces = (start + tz - 1) / per - start / per + 1;
-        p.counter = z * ny + y;
+        const int run0 = runs.of(start);
+        p.piece = run - run0;
+        p.pieces = runs.of(start + tz - 1) - run0 + 1;
+        p.item = z * ny + y;
+        p.slot = 2 * run + (at > first ? 1 : 0);             // the item that the run begins in, or the one that it ends in
+        p.slot0 = 2 * run0 + (start > runs.begin(run0) ? 1 : 0);                 // where its first piece is
         return p;
     };
 
@@ -190,53 +288,59 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         const Piece pc = piece_at(at);
         if (pc.heads == 0) break;
         at = pc.stop;
-        const int* table = block_table + (size_t)req_index[pc.tok] * max_blocks;
+        const int* table = block_table + (size_t)pc.req * max_blocks;
 
-        // the queries as the second operand of S^T: head n0 + g, the features of this lane's words
-        unsigned qf[NT][KW][2];
-        float qs[NT][2];                                     // scale * log2(e) * what head 2t (+ 1) was divided by
+        float o[NT][OT][4], less[NT][2], l[NT][2];           // less: SHIFT less the base, a maximum of the scores so far
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int h = n * 8 + g;
-            const bf16* row = q + (size_t)pc.tok * q_stride + (size_t)(pc.h0 + h) * HD;
-            uint2 raw[KW];
+#pragma unroll
+            for (int i = 0; i < OT; ++i) { o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f; }
+            less[n][0] = less[n][1] = INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+        }
+        int E = EXP_MIN;
+        float in_units = power_of_two(-EXP_MIN);             // 2^-E
+
+        unsigned qf[NT][KW][2];
+        float qs[NT][2];                                     // scale * log2(e) * what head 2t (+ 1) was divided by
+        // the queries as the second operand of S^T: head 8 n + g, the features of this lane's words, as halves
+        uint2 raw_q[NT][KW];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                const bf16* row = q + (size_t)pc.tok * q_stride + (size_t)(pc.h0 + n * 8 + g) * HD;
+                raw_q[n][w] = n * 8 + g < pc.heads ? *reinterpret_cast<const uint2*>(row + ((w / KL * 4 + t) * KL + w % KL) * 4) : make_uint2(0u, 0u);
+            }
+        auto queries = [&]() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint2 (&raw)[KW] = raw_q[n];
             unsigned top = 0;
 #pragma unroll
             for (int j = 0; j < KW / KL; ++j)
 #pragma unroll
                 for (int i = 0; i < KL; ++i) {
                     const int w = j * KL + i;
-                    raw[w] = h < pc.heads ? *reinterpret_cast<const uint2*>(row + ((j * 4 + t) * KL + i) * 4) : make_uint2(0u, 0u);
                     top = max(top, max(max(raw[w].x & 0x7fffu, (raw[w].x >> 16) & 0x7fffu), max(raw[w].y & 0x7fffu, (raw[w].y >> 16) & 0x7fffu)));
                 }
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // to [2^14, 2^15); a row of zeros, a NaN or an infinity stays as it is
-            const int e = top == 0 || top >= 0x7f80u ? 0 : max(-112, (int)(top >> 7) - 127 - 14);
+            // to [2^14, 2^15); a row of zeros stays as it is, one with a NaN or an infinity has a factor that says so
+            const int e = top == 0 ? 0 : max(-112, (int)(top >> 7) - 127 - 14);
             const float f = power_of_two(-e);
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
                 qf[n][w][0] = pack_half(__uint_as_float(raw[w].x << 16) * f, __uint_as_float(raw[w].x & 0xffff0000u) * f);
                 qf[n][w][1] = pack_half(__uint_as_float(raw[w].y << 16) * f, __uint_as_float(raw[w].y & 0xffff0000u) * f);
             }
-            const float back = scale_log2 * power_of_two(e);
+            const float back = top >= 0x7f80u ? __uint_as_float(0x7fc00000u) : scale_log2 * power_of_two(e);
             qs[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);
             qs[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
         }
-
-        float o[NT][OT][4], m[NT][2], l[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int i = 0; i < OT; ++i) { o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f; }
-            m[n][0] = m[n][1] = -INFINITY;
-            l[n][0] = l[n][1] = 0.f;
-        }
-        int E = EXP_MIN;
-
-        // this warp's 16 keys of step st begin at st * 64 + warp * 16
+        };
         const int st0 = pc.c0 / BN, st1 = (pc.c1 - 1) / BN;
-        // the cache row and the scales of key `lane` (of 16; WIDE: of the first one) of a step's keys: row < 0 for one that is not read
+        // a cache row and its page's scales: of the key of this lane (of 16), or, WIDE, of the first key of a step's 16; row < 0: not read
         struct Where { int row; float ks, vs; };
         auto page_of = [&](int key) -> int {                 // -1 for one that is not read
             if (key >= pc.c1 || key + (WIDE ? 15 : 0) < pc.c0) return -1;
@@ -253,84 +357,100 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
             w.vs = vscale[head];
             return w;
         };
-        // values under a scale that is none: their keys' scores say so, so that only who reads them gets NaN
-        auto settle = [&](Where w) -> Where {
-            if (w.vs != w.vs) { w.ks = w.vs; w.vs = 0.f; }
-            return w;
-        };
-        auto ask = [&](int row) {                            // 16 keys' rows and their values' into L2
-            if (row >= 0) { prefetch_l2(kcache + (size_t)row * HD, 16 * HD); prefetch_l2(vcache + (size_t)row * HD, 16 * HD); }
-        };
-        auto load = [&](Tile& x, const Where& w) {
+        unsigned char* const ring = smem + warp * NS * STAGE;
+        const unsigned ring_u32 = smem_u32(ring);
+        // the keys of this warp's tile `tile`, of SUB a step, begin here
+        auto first_key = [&](int tile) { return tile / SUB * BN + (warp * SUB + tile % SUB) * 16; };
+        auto fetch = [&](const Where& w, int tile, int stage) {  // a tile's keys and values on their way; a row that is not read: zeros
+            const int k0 = first_key(tile);
+            const unsigned to = ring_u32 + stage * STAGE + tile % SUB * TILE;
+            constexpr int COPIES = (16 * PIECES + 31) / 32;
+            const bool whole = WIDE && w.row >= 0 && k0 >= pc.c0 && k0 + 16 <= pc.c1;             // (warp-uniform)
+            if (whole) {                                     // 16 rows of a page lie side by side
+                const unsigned char* const k = kcache + (size_t)w.row * HD + lane * 16;
+                const unsigned char* const v = vcache + (size_t)w.row * HD + lane * 16;
+                if constexpr (32 % PIECES == 0) {            // 32 / PIECES rows a round
+                    copies16<32 / PIECES * KS, 512, COPIES>(to + lane / PIECES * KS + lane % PIECES * 16, k);
+                    copies16<32 / PIECES * VS, 512, COPIES>(to + 16 * KS + lane / PIECES * VS + lane % PIECES * 16, v);
+                } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int row = WIDE ? (w.row < 0 ? -1 : w.row + g + 8 * i) : __shfl_sync(0xffffffffu, w.row, g + 8 * i);
-                const unsigned char* p = kcache + (size_t)max(row, 0) * HD;
-#pragma unroll
-                for (int j = 0; j < KW / KL; ++j) {
-                    if (row >= 0) load_words<KL>(p + (j * 4 + t) * KL * 4, &x.k[i][j * KL]);
-                    else {
-#pragma unroll
-                        for (int c = 0; c < KL; ++c) x.k[i][j * KL + c] = 0u;
+                    for (int j = 0; j < COPIES; ++j) {
+                        const int i = j * 32 + lane, r = i / PIECES, c = i - r * PIECES;
+                        if (16 * PIECES % 32 && i >= 16 * PIECES) continue;
+                        copies16<0, 0, 1>(to + r * KS + c * 16, k + j * 512);
+                        copies16<0, 0, 1>(to + 16 * KS + r * VS + c * 16, v + j * 512);
                     }
                 }
-            }
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = 2 * t + (i & 1) + 8 * (i >> 1);
-                const int row = WIDE ? (w.row < 0 ? -1 : w.row + key) : __shfl_sync(0xffffffffu, w.row, key);
-                const unsigned char* p = vcache + (size_t)max(row, 0) * HD;
-                if constexpr (VW > 0) {
-#pragma unroll
-                    for (int j = 0; j < VW / VL; ++j) {
-                        if (row >= 0) load_words<VL>(p + (j * 8 + g) * VL * 4, &x.v[i][j * VL]);
-                        else {
-#pragma unroll
-                            for (int c = 0; c < VL; ++c) x.v[i][j * VL + c] = 0u;
-                        }
-                    }
+                for (int j = 0; j < COPIES; ++j) {
+                    const int i = j * 32 + lane, r = i / PIECES, c = i - r * PIECES;
+                    const int first_row = WIDE ? w.row : __shfl_sync(0xffffffffu, w.row, r & 15), row = WIDE ? first_row + r : first_row;
+                    if (16 * PIECES % 32 && i >= 16 * PIECES) continue;
+                    const int bytes = first_row >= 0 && k0 + r >= pc.c0 && k0 + r < pc.c1 ? 16 : 0;
+                    const size_t at = (size_t)max(row, 0) * HD + c * 16;
+                    copy16(to + r * KS + c * 16, kcache + at, bytes);
+                    copy16(to + 16 * KS + r * VS + c * 16, vcache + at, bytes);
                 }
-                if constexpr (ODD) x.v2[i] = row >= 0 ? __ldg(reinterpret_cast<const unsigned short*>(p + HD - 16 + 2 * g)) : (unsigned short)0;
             }
+            // values under a scale that is none: their keys' scores say so, so that only who reads them gets NaN
+            if (lane < (WIDE ? 1 : 16)) s_scale[warp][stage][tile % SUB][lane] = w.vs != w.vs ? make_float2(w.vs, 0.f) : make_float2(w.ks, w.vs);
         };
-        auto work = [&](Tile& x, const Where& w, int st) {
-            const int k0 = st * BN + warp * 16;              // the tile's first key
-            float s[NT][4];
+        // PART: a step with keys that are not read.  The step's tiles side by side, so that one's chain of products, exponentials and conversions
+        // runs beside another's.
+        auto work = [&](auto partly, int st, int stage) {
+            constexpr bool PART = decltype(partly)::value;
+            const unsigned char* const keys = ring + stage * STAGE + g * KS + t * KL * 4;
+            const unsigned char* const values = ring + stage * STAGE + 16 * KS + 2 * t * VS + g * VL * 4;
+            float2 scale0[SUB], scale1[SUB];
+            float s[SUB][NT][4], x[SUB][NT][4], top = -INFINITY;
+            bool none0[SUB], none1[SUB];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) { s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f; }
+            for (int u = 0; u < SUB; ++u) {
+                scale0[u] = s_scale[warp][stage][u][WIDE ? 0 : g];
+                scale1[u] = WIDE ? scale0[u] : s_scale[warp][stage][u][WIDE ? 0 : g + 8];
+                unsigned k[2][KW];
 #pragma unroll
-            for (int i = 0; i < KW; ++i) {
-                const unsigned a0 = half2_low(x.k[0][i]), a2 = half2_high(x.k[0][i]), a1 = half2_low(x.k[1][i]), a3 = half2_high(x.k[1][i]);
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+                    for (int j = 0; j < KW / KL; ++j) load_words<KL>(keys + u * TILE + i * 8 * KS + j * 16 * KL, &k[i][j * KL]);
+                float odd[NT][4];                            // two chains a tile
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) s[u][n][c] = odd[n][c] = 0.f;
+#pragma unroll
+                for (int i = 0; i < KW; ++i) {
+                    const unsigned a0 = half2_low(k[0][i]), a1 = half2_low(k[1][i]), a2 = half2_high(k[0][i]), a3 = half2_high(k[1][i]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_f16(i & 1 ? odd[n] : s[u][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) s[u][n][c] += odd[n][c];
             }
-            const float ks0 = WIDE ? w.ks : __shfl_sync(0xffffffffu, w.ks, g), ks1 = WIDE ? w.ks : __shfl_sync(0xffffffffu, w.ks, g + 8);
-            const float vs0 = WIDE ? w.vs : __shfl_sync(0xffffffffu, w.vs, g), vs1 = WIDE ? w.vs : __shfl_sync(0xffffffffu, w.vs, g + 8);
-            const bool edge = k0 < pc.c0 || k0 + 16 > pc.c1;                     // (warp-uniform)
-            const bool in0 = !edge || (k0 + g >= pc.c0 && k0 + g < pc.c1), in1 = !edge || (k0 + g + 8 >= pc.c0 && k0 + g + 8 < pc.c1);
-            const int row0 = WIDE ? w.row : __shfl_sync(0xffffffffu, w.row, g), row1 = WIDE ? w.row : __shfl_sync(0xffffffffu, w.row, g + 8);
-            const bool r0 = in0 && row0 >= 0, r1 = in1 && row1 >= 0;
-            if (edge) {                                      // values that are not read may be anything, and 0 * NaN is NaN
+            // a score less its base, in units of log2, and SHIFT more: what the halves of the weights are the powers of
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = k0 + 2 * t + (i & 1) + 8 * (i >> 1);
-                    if (key < pc.c0 || key >= pc.c1) {
+            for (int u = 0; u < SUB; ++u) {
+                const int k0 = st * BN + (warp * SUB + u) * 16;
+                // keys that are not read weigh nothing: those outside the piece, and those without a page, whose scale is left 0
+                none0[u] = PART && (scale0[u].x == 0.f || k0 + g < pc.c0 || k0 + g >= pc.c1);
+                none1[u] = PART && (scale1[u].x == 0.f || k0 + g + 8 < pc.c0 || k0 + g + 8 >= pc.c1);
 #pragma unroll
-                        for (int c = 0; c < (VW > 0 ? VW : 1); ++c) x.v[i][c] = 0u;
-                        x.v2[i] = 0;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        x[u][n][c] = fmaf(s[u][n][c], (c < 2 ? scale0[u].x : scale1[u].x) * qs[n][c & 1], less[n][c & 1]);
+                        if (PART && (c < 2 ? none0[u] : none1[u])) x[u][n][c] = -INFINITY;
+                        top = fmaxf(top, x[u][n][c]);        // (no base yet: +inf)
                     }
-                }
             }
-            bool over = false;
+            int tile_e = -128;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    s[n][c] = (c < 2 ? r0 : r1) ? s[n][c] * (c < 2 ? ks0 : ks1) * qs[n][c & 1] : -INFINITY;
-                    over |= s[n][c] > m[n][c & 1] + ROOM;
-                }
-            const int ev = max(exponent_of(vs0), exponent_of(vs1)), tile_e = WIDE ? ev : __reduce_max_sync(0xffffffffu, ev);
-            if (__any_sync(0xffffffffu, over) || tile_e > E) {
+            for (int u = 0; u < SUB; ++u) tile_e = max(tile_e, max(exponent_of(scale0[u].y), exponent_of(scale1[u].y)));
+            if (!WIDE) tile_e = __reduce_max_sync(0xffffffffu, tile_e);
+            if (__any_sync(0xffffffffu, top > ROOM + SHIFT) || tile_e > E) {
                 const int grown = max(E, tile_e);
                 const float lower = power_of_two(E - grown);
                 E = grown;
@@ -338,101 +458,132 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        float mx = fmaxf(s[n][c], s[n][c + 2]);
+                        const float was = SHIFT - less[n][c];
+                        float mx = was, sc[SUB][2];
+#pragma unroll
+                        for (int u = 0; u < SUB; ++u) {
+                            sc[u][0] = none0[u] ? -INFINITY : s[u][n][c] * (scale0[u].x * qs[n][c]);
+                            sc[u][1] = none1[u] ? -INFINITY : s[u][n][c + 2] * (scale1[u].x * qs[n][c]);
+                            mx = fmaxf(mx, fmaxf(sc[u][0], sc[u][1]));
+                        }
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[n][c]);
-                        const float corr = mx == -INFINITY ? 1.f : exp2_fast(m[n][c] - mx), both = corr * lower;
-                        m[n][c] = mx;
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float corr = mx == -INFINITY ? 1.f : exp2_fast(was - mx), both = corr * lower, base = mx == -INFINITY ? 0.f : mx;
+                        less[n][c] = SHIFT - mx;
                         l[n][c] *= corr;
+#pragma unroll
+                        for (int u = 0; u < SUB; ++u) {
+                            x[u][n][c] = sc[u][0] - base + SHIFT;
+                            x[u][n][c + 2] = sc[u][1] - base + SHIFT;
+                        }
 #pragma unroll
                         for (int i = 0; i < OT; ++i) { o[n][i][c] *= both; o[n][i][c + 2] *= both; }
                     }
+                in_units = power_of_two(-E);
             }
-            const float in_units = power_of_two(SHIFT - E), f0 = vs0 * in_units, f1 = vs1 * in_units;
-            unsigned pf[NT][2];
+            unsigned pf[SUB][NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float b0 = m[n][0] == -INFINITY ? 0.f : m[n][0], b1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-                const float p00 = exp2_fast(s[n][0] - b0), p01 = exp2_fast(s[n][1] - b1), p10 = exp2_fast(s[n][2] - b0), p11 = exp2_fast(s[n][3] - b1);
-                l[n][0] += p00 + p10;
-                l[n][1] += p01 + p11;
-                pf[n][0] = turned(pack_half(p00 * f0, p01 * f0));
-                pf[n][1] = turned(pack_half(p10 * f1, p11 * f1));
-            }
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                const unsigned lo01 = __byte_perm(x.v[0][i], x.v[1][i], 0x5140), hi01 = __byte_perm(x.v[0][i], x.v[1][i], 0x7362);
-                const unsigned lo23 = __byte_perm(x.v[2][i], x.v[3][i], 0x5140), hi23 = __byte_perm(x.v[2][i], x.v[3][i], 0x7362);
-                const unsigned a0 = half2_low(lo01), a1 = half2_high(lo01), a2 = half2_low(lo23), a3 = half2_high(lo23);
-                const unsigned c0 = half2_low(hi01), c1 = half2_high(hi01), c2 = half2_low(hi23), c3 = half2_high(hi23);
+            for (int u = 0; u < SUB; ++u) {
+                const float f0 = scale0[u].y * in_units, f1 = scale1[u].y * in_units;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    mma_f16(o[n][2 * i], a0, a1, a2, a3, pf[n][0], pf[n][1]);
-                    mma_f16(o[n][2 * i + 1], c0, c1, c2, c3, pf[n][0], pf[n][1]);
+                    float p[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) p[c] = exp2_fast(x[u][n][c]);
+                    l[n][0] += p[0] + p[2];
+                    l[n][1] += p[1] + p[3];
+                    pf[u][n][0] = turned(pack_half(p[0] * f0, p[1] * f0));
+                    pf[u][n][1] = turned(pack_half(p[2] * f1, p[3] * f1));
                 }
             }
-            if constexpr (ODD) {
-                const unsigned lo01 = __byte_perm(x.v2[0], x.v2[1], 0x5140), lo23 = __byte_perm(x.v2[2], x.v2[3], 0x5140);
-                const unsigned a0 = half2_low(lo01), a1 = half2_high(lo01), a2 = half2_low(lo23), a3 = half2_high(lo23);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(o[n][OT - 1], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+            for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+                for (int j = 0; j < VW / VL; ++j) {
+                    unsigned v[4][VL];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) load_words<VL>(values + u * TILE + ((i & 1) + 8 * (i >> 1)) * VS + j * 32 * VL, v[i]);
+#pragma unroll
+                    for (int c = 0; c < VL; ++c) {
+                        const int i = j * VL + c;
+                        const unsigned lo01 = __byte_perm(v[0][c], v[1][c], 0x5140), hi01 = __byte_perm(v[0][c], v[1][c], 0x7362);
+                        const unsigned lo23 = __byte_perm(v[2][c], v[3][c], 0x5140), hi23 = __byte_perm(v[2][c], v[3][c], 0x7362);
+                        const unsigned a0 = half2_low(lo01), a1 = half2_high(lo01), a2 = half2_low(lo23), a3 = half2_high(lo23);
+                        const unsigned c0 = half2_low(hi01), c1 = half2_high(hi01), c2 = half2_low(hi23), c3 = half2_high(hi23);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma_f16(o[n][2 * i], a0, a1, a2, a3, pf[u][n][0], pf[u][n][1]);
+                            mma_f16(o[n][2 * i + 1], c0, c1, c2, c3, pf[u][n][0], pf[u][n][1]);
+                        }
+                    }
+                }
+                if constexpr (ODD) {
+                    unsigned v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        v[i] = *reinterpret_cast<const unsigned short*>(values + u * TILE + ((i & 1) + 8 * (i >> 1)) * VS - g * VL * 4 + HD - 16 + 2 * g);
+                    const unsigned lo01 = __byte_perm(v[0], v[1], 0x5140), lo23 = __byte_perm(v[2], v[3], 0x5140);
+                    const unsigned a0 = half2_low(lo01), a1 = half2_high(lo01), a2 = half2_low(lo23), a3 = half2_high(lo23);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_f16(o[n][OT - 1], a0, a1, a2, a3, pf[u][n][0], pf[u][n][1]);
+                }
             }
         };
-        {
-            Tile x, y;
-            if constexpr (WIDE) {
-                // lane i knows the place of step base + i; the next 32 steps' are looked up on the way, a load at a time
-                const int k_of = warp * 16;
-                auto key_of = [&](int st) { return st * BN + k_of; };
-                Where now = where_of(page_of(key_of(st0 + lane)), key_of(st0 + lane)), then = {-1, 0.f, 0.f};
-                int base = st0, page = -1;
-                auto at_step = [&](int st) -> Where {        // (of a step of the present 32)
-                    Where w = {__shfl_sync(0xffffffffu, now.row, st - base), __shfl_sync(0xffffffffu, now.ks, st - base), __shfl_sync(0xffffffffu, now.vs, st - base)};
-                    return settle(w);
-                };
-                if (lane <= AHEAD) ask(now.row);
-                auto advance = [&](int st) {                 // before step st's work: what lies ahead of it
-                    const int i = st - base;
-                    if (i == 0) page = page_of(key_of(base + 32 + lane));
-                    if (i == 16) then = where_of(page, key_of(base + 32 + lane));
-                    const int j = i + 1 + AHEAD;             // step st + 1 + AHEAD
-                    if (lane == (j & 31)) ask(j < 32 ? now.row : then.row);
-                };
-                auto next_of = [&](int st) -> Where {        // step st + 1
-                    if (st + 1 - base == 32) { now = then; base += 32; }
-                    return at_step(st + 1);
-                };
-                Where wx = at_step(st0), wy;
-                load(x, wx);
-                for (int st = st0; st <= st1; st += 2) {
-                    advance(st);
-                    wy = next_of(st);
-                    load(y, wy);
-                    work(x, wx, st);
-                    if (st + 1 > st1) break;
-                    advance(st + 1);
-                    wx = next_of(st + 1);
-                    load(x, wx);
-                    work(y, wy, st + 1);
-                }
-            } else {
-                auto find = [&](int st) -> Where { return settle(where_of(page_of(st * BN + warp * 16 + (lane & 15)), st * BN + warp * 16 + (lane & 15))); };
-                Where wx = find(st0), wy = find(st0 + 1);
-                load(x, wx);
-                for (int st = st0; st <= st1; st += 2) {
-                    load(y, wy);
-                    Where next = find(st + 2);
-                    work(x, wx, st);
-                    wx = next;
-                    if (st + 1 > st1) break;
-                    load(x, wx);
-                    next = find(st + 3);
-                    work(y, wy, st + 1);
-                    wy = next;
-                }
+        if constexpr (WIDE) {
+            // lane i knows the place of tile base + i; the next 32 tiles' are looked up on the way, a load at a time
+            Where now = where_of(page_of(first_key(st0 * SUB + lane)), first_key(st0 * SUB + lane)), then = {-1, 0.f, 0.f};
+            int from = 0, base = st0 * SUB, page = -1;
+            auto next = [&](int stage) {                     // the step that begins with tile base + from
+                if (from == 32) { now = then; base += 32; from = 0; }
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
+                    fetch(Where{__shfl_sync(0xffffffffu, now.row, from + u), __shfl_sync(0xffffffffu, now.ks, from + u), __shfl_sync(0xffffffffu, now.vs, from + u)},
+                          base + from + u, stage);
+                copies_commit();
+                if (from == 8) page = page_of(first_key(base + 32 + lane));
+                if (from == 20) then = where_of(page, first_key(base + 32 + lane));
+                from += SUB;
+            };
+            next(0);
+            queries();                                       // (while the first keys are on their way)
+            int stage = 0;
+            for (int st = st0; st <= st1; ++st, stage ^= 1) {
+                next(stage ^ 1);
+                copies_wait<1>();
+                __syncwarp();                                // every lane's copies have landed
+                const int k0 = st * BN + warp * SUB * 16;
+                bool whole = k0 >= pc.c0 && k0 + 16 * SUB <= pc.c1;
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) whole = whole && s_scale[warp][stage][u][0].x != 0.f;
+                if (whole) work(std::false_type(), st, stage);
+                else work(std::true_type(), st, stage);
+                __syncwarp();                                // the stage has been read
+            }
+        } else {
+            auto find = [&](int tile) { return where_of(page_of(first_key(tile) + (lane & 15)), first_key(tile) + (lane & 15)); };
+            Where w[SUB];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) fetch(find(st0 * SUB + u), st0 * SUB + u, 0);
+            copies_commit();
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) w[u] = find((st0 + 1) * SUB + u);
+            queries();
+            int stage = 0;
+            for (int st = st0; st <= st1; ++st, stage ^= 1) {
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) fetch(w[u], (st + 1) * SUB + u, stage ^ 1);
+                copies_commit();
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) w[u] = find((st + 2) * SUB + u);             // (used a step later)
+                copies_wait<1>();
+                __syncwarp();
+                work(std::true_type(), st, stage);
+                __syncwarp();
             }
         }
+        copies_wait<0>();
+        __syncthreads();                                     // all rings are at rest
 
         // the four warps' shares, put together in warp order
 #pragma unroll
@@ -443,107 +594,105 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
                 x += __shfl_xor_sync(0xffffffffu, x, 4);
                 x += __shfl_xor_sync(0xffffffffu, x, 8);
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
-                if (g == 0) { s_m[warp][n * 8 + 2 * t + c] = m[n][c]; s_l[warp][n * 8 + 2 * t + c] = x; }
+                if (g == 0) { s_m[warp][n * 8 + 2 * t + c] = SHIFT - less[n][c]; s_l[warp][n * 8 + 2 * t + c] = x; }
             }
-        if (lane == 0) s_e[warp] = power_of_two(E - SHIFT);
+        if (lane == 0) s_e[warp] = power_of_two(E);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < OT; ++i) {
-                const int w = i / 2;
-                const int d = (ODD && i == OT - 1) ? HD - 16 + 2 * g : (((w / VL) * 8 + g) * VL + w % VL) * 4 + 2 * (i & 1);
+            for (int c = 0; c < 2; ++c) {
+                float* row = &s_o[warp][n * 8 + 2 * t + c][0];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s_o[warp][n * 8 + 2 * t + (c & 1)][d + (c >> 1)] = o[n][i][c];
+                for (int w = 0; w < VW; ++w)
+                    *reinterpret_cast<float4*>(row + (((w / VL) * 8 + g) * VL + w % VL) * 4) =
+                        make_float4(o[n][2 * w][c], o[n][2 * w][c + 2], o[n][2 * w + 1][c], o[n][2 * w + 1][c + 2]);
+                if constexpr (ODD) *reinterpret_cast<float2*>(row + HD - 16 + 2 * g) = make_float2(o[n][OT - 1][c], o[n][OT - 1][c + 2]);
             }
         __syncthreads();
-        for (int i = tid; i < pc.heads * HD; i += NTHREADS) {
-            const int h = i / HD, d = i - h * HD;
-            float M = -INFINITY, acc = 0.f, L = 0.f;
+        for (int i = tid; i < pc.heads * (HD / 4); i += NTHREADS) {
+            const int h = i / (HD / 4), d = (i - h * (HD / 4)) * 4;
+            float M = -INFINITY, L = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][h]);
             const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {                // (a warp without a key has sums of zero; one of NaN keeps them)
-                const float f = s_m[w][h] == -INFINITY ? 1.f : exp2_fast(s_m[w][h] - base);
-                acc += s_o[w][h][d] * f * s_e[w];
+                const float f = s_m[w][h] == -INFINITY ? 1.f : exp2_fast(s_m[w][h] - base), e = s_e[w];
+                const float4 x = *reinterpret_cast<const float4*>(&s_o[w][h][d]);
+                acc.x += x.x * f * e; acc.y += x.y * f * e; acc.z += x.z * f * e; acc.w += x.w * f * e;
                 L += s_l[w][h] * f;
             }
             if (pc.pieces == 1) {
-                out[((size_t)pc.tok * nq + pc.h0 + h) * HD + d] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+                bf16* dst = out + ((size_t)pc.tok * nq + pc.h0 + h) * HD + d;
+                dst[0] = __float2bfloat16(acc.x * inv); dst[1] = __float2bfloat16(acc.y * inv);
+                dst[2] = __float2bfloat16(acc.z * inv); dst[3] = __float2bfloat16(acc.w * inv);
             } else {
-                const size_t row = ((size_t)pc.place * nq + pc.h0 + h) * S + pc.piece;
-                __stcg(part + row * HD + d, acc);
-                if (d == 0) __stcg(reinterpret_cast<float2*>(part_ml) + row, make_float2(M, L));
+                const size_t row = (size_t)pc.slot * held + h;
+                __stcg(reinterpret_cast<float4*>(left.part + row * HD + d), acc);
+                if (d == 0) __stcg(left.ml + row, make_float2(M, L));
             }
         }
-        if (pc.pieces > 1 && tid == 0) s_partial[number > 0] = pc;
+        if (tid == 0) {
+            if (pc.pieces > 1) s_partial[number > 0] = pc;
+            if (!arrivals && pc.piece == 0)
+                __stcg(left.info + pc.item, make_int4(pc.slot0, 2 * (run + 1), pc.pieces > 1 ? pc.pieces : 0, pc.tok));
+        }
         __syncthreads();                                     // the shares may be written again
     }
     if (bad_page && err) atomicOr(err, VL_DEV_BAD_PAGE);
     // The items shared with other blocks (the run's first and last), at its end so that the stream does not wait for them: this block's pieces are
     // counted; whoever comes last adds up all of an item's, in their order.
-    if (s_partial[0].heads == 0 && s_partial[1].heads == 0) return;
+    if (!arrivals || (s_partial[0].heads == 0 && s_partial[1].heads == 0)) return;
     __threadfence();                                         // this thread's parts, before the block's arrivals are counted
     __syncthreads();
-    if (tid < 2) s_last[tid] = s_partial[tid].heads && atomicAdd(&arrivals[s_partial[tid].counter], 1) == s_partial[tid].pieces - 1;
+    if (tid < 2) s_last[tid] = s_partial[tid].heads && atomicAdd(&arrivals[s_partial[tid].item], 1) == s_partial[tid].pieces - 1;
     __syncthreads();
     if (!s_last[0] && !s_last[1]) return;
     __threadfence();
     for (int k = 0; k < 2; ++k) {
         if (!s_last[k]) continue;
         const Piece pc = s_partial[k];
-        // the pieces' weights and the sums' quotient, in the memory of the warps' shares
-        float* weight = &s_o[0][0][0];                       // [heads][pieces]
-        const float2* ml = reinterpret_cast<const float2*>(part_ml) + ((size_t)pc.place * nq + pc.h0) * S;
-        for (int h = warp; h < pc.heads; h += WARPS) {
-            float M = -INFINITY, L = 0.f;
-            for (int p = lane; p < pc.pieces; p += 32) M = fmaxf(M, __ldcg(ml + (size_t)h * S + p).x);
-            M = warp_max(M);
-            const float base = M == -INFINITY ? 0.f : M;
-            for (int p = lane; p < pc.pieces; p += 32) {
-                const float2 x = __ldcg(ml + (size_t)h * S + p);
-                const float f = x.x == -INFINITY ? 1.f : exp2_fast(x.x - base);
-                L += x.y * f;
-                weight[h * pc.pieces + p] = f;
-            }
-            L = warp_sum(L);
-            if (lane == 0) s_l[0][h] = L;
-        }
-        __syncthreads();
+        const int run0 = run - pc.piece, slot0 = pc.slot0;
         for (int i = tid; i < pc.heads * (HD / 4); i += NTHREADS) {
-            const int h = i / (HD / 4), d = (i - h * (HD / 4)) * 4;
-            const float* row = part + ((size_t)pc.place * nq + pc.h0 + h) * S * HD + d;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int p = 0; p < pc.pieces; ++p) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(row + (size_t)p * HD));
-                const float f = weight[h * pc.pieces + p];
-                acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
-            }
-            const float L = s_l[0][h], inv = L == 0.f ? 0.f : 1.f / L;
-            bf16* dst = out + ((size_t)pc.tok * nq + pc.h0 + h) * HD + d;
-            dst[0] = __float2bfloat16(acc.x * inv); dst[1] = __float2bfloat16(acc.y * inv);
-            dst[2] = __float2bfloat16(acc.z * inv); dst[3] = __float2bfloat16(acc.w * inv);
+            const int h = i / (HD / 4);
+            add_pieces(left.part + (size_t)h * HD, left.ml + h, (size_t)held * HD, held, slot0, 2 * (run0 + 1), pc.pieces, (i - h * (HD / 4)) * 4,
+                       out + ((size_t)pc.tok * nq + pc.h0 + h) * HD);
         }
-        __syncthreads();                                     // the weights may be written again
-        if (tid == 0) arrivals[pc.counter] = 0;              // as the next launch finds it
+        if (tid == 0) arrivals[pc.item] = 0;               // as the next launch finds it
     }
+}
+
+// The pieces of one head of one item, where a block of the launch above would take longer over all of an item's.
+__global__ void __launch_bounds__(HD / 4 < 32 ? 32 : HD / 4)
+flash_decode_8bit_merge_kernel(float* scratch, int runs, int held, int grp, int nq, int nkv, bf16* __restrict__ out) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const Scratch left(scratch, runs, held);
+    const int htiles = (grp + held - 1) / held, item = blockIdx.x / held, h = blockIdx.x % held, y = item % (nkv * htiles);
+    const int head = (y % htiles) * held + h;                // within the KV head's group
+    if ((int)threadIdx.x >= HD / 4 || head >= grp) return;
+    const int4 info = __ldcg(left.info + item);
+    if (info.z == 0) return;
+    add_pieces(left.part + (size_t)h * HD, left.ml + h, (size_t)held * HD, held, info.x, info.y, info.z, (int)threadIdx.x * 4,
+               out + ((size_t)info.w * nq + (y / htiles) * grp + head) * HD);
 }
 
 extern "C" int vl_flash_decode_8bit_head_dim() { return HD; }
 
 // q [T, q_stride] bfloat16, out [.., nq * hd]; caches [pages, nkv, page_size, hd] e4m3, scales [pages, nkv]; positions from `bound` on are
-// flagged and get rows of zeros.  part: T * nq * S * (hd + 2) floats (T: tokens of the launch), S > 1 pieces an item; arrivals: T * nq counters,
-// zero before and after.
+// flagged and get rows of zeros.  scratch: `floats` of them, the more the shorter the runs may be, 3 * T * nq * (hd + 2) at least; arrivals: T * nq counters, zero
+// before and after.
 extern "C" int vl_flash_decode_8bit(const void* q, int q_stride, const void* kcache, const void* vcache, const float* kscale, const float* vscale,
                                     const int* block_table, int max_blocks, const int* req_index, const int* positions, int T, int nq, int nkv, int hd,
-                                    int page_size, int num_pages, float scale, int window, int bound, int S, float* part, unsigned* err,
+                                    int page_size, int num_pages, float scale, int window, int bound, float* scratch, long long floats, unsigned* err,
                                     const int* token_index, void* out, int* arrivals, int settled, void* stream) {
     if (T <= 0) return VL_OK;
     if (hd != HD) return VL_ERR_UNSUPPORTED;
     if (nq <= 0 || nkv <= 0 || nq % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || q_stride < nq * hd || q_stride % 4) return VL_ERR_ARGUMENT;
-    if (bound <= 0 || S < 2 || S > PIECES_MAX || !out || !arrivals || !part) return VL_ERR_ARGUMENT;
-    if (((uintptr_t)q & 7) || (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)part) & 15)) return VL_ERR_ARGUMENT;
+    if (bound <= 0 || !out || !arrivals || !scratch || floats < 3ll * T * nq * (hd + 2)) return VL_ERR_ARGUMENT;
+    if (((uintptr_t)q & 7) || (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)scratch) & 15)) return VL_ERR_ARGUMENT;
     const int grp = nq / nkv, wide_heads = grp > 8 && HD <= 128 ? 16 : 8, htiles = (grp + wide_heads - 1) / wide_heads;
     const long long most = (long long)T * nkv * htiles * ((bound + BN - 1) / BN);
     if ((long long)num_pages * nkv * page_size >= (1ll << 31) || most >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
@@ -552,14 +701,32 @@ extern "C" int vl_flash_decode_8bit(const void* q, int q_stride, const void* kca
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return (int)e;
     const bool wide = page_size % 16 == 0;
-    auto launch = [&](auto kernel, int blocks_an_sm) {
-        const long long grid = (long long)sms * blocks_an_sm;
-        return vl_launch(kernel, dim3((unsigned)(most < grid ? most : grid)), dim3(NTHREADS), 0, (cudaStream_t)stream, (const bf16*)q, q_stride,
-                         (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks, req_index, positions, T,
-                         nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, bound, S, part, err, token_index, (bf16*)out, arrivals, settled);
+    const int held = grp < wide_heads ? grp : wide_heads;
+    const long long items = (long long)T * nkv * htiles, reach = window > 0 && window < bound ? window + BN : bound, steps = (reach + BN - 1) / BN;
+    auto launch = [&](auto kernel) {
+        const long long resident = (long long)sms * RESIDENT;
+        long long runs = (floats - 8 - 4 * items) / (2ll * held * (HD + 2));
+        if (runs > T_WAVES * resident) runs = T_WAVES * resident;
+        if (runs > sms) runs -= runs % sms;                  // as many on every SM
+        if (runs > most) runs = most;
+        if (runs < 1) runs = 1;
+        // pieces that an item may come in, were every place full, and what a block would read to add them up: above 64 KB another launch, a block a head, does
+        const long long run = (most + resident - 1) / resident > MIN_RUN ? (most + resident - 1) / resident : MIN_RUN, pieces = (steps + run - 1) / run + 1;
+        const bool apart = pieces * held * HD * 4 > T_APART * 1024;
+        const int rings = WARPS * NS * STAGE, shares = WARPS * wide_heads * OLD * 4, smem = rings > shares ? rings : shares;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return (int)e;
+        int rc = vl_launch(kernel, dim3((unsigned)runs), dim3(NTHREADS), (size_t)smem, (cudaStream_t)stream, (const bf16*)q, q_stride,
+                           (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks, req_index, positions, T,
+                           nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, bound, (int)resident, scratch, err, token_index, (bf16*)out,
+                           apart ? (int*)nullptr : arrivals, settled);
+        if (rc == VL_OK && apart)
+            rc = vl_launch(flash_decode_8bit_merge_kernel, dim3((unsigned)(items * held)), dim3(HD / 4 < 32 ? 32 : HD / 4), 0, (cudaStream_t)stream, scratch,
+                           (int)runs, held, grp, nq, nkv, (bf16*)out);
+        return rc;
     };
     if constexpr (HD <= 128) {
-        if (wide_heads == 16) return wide ? launch(flash_decode_8bit_kernel<2, true>, 2) : launch(flash_decode_8bit_kernel<2, false>, 2);
+        if (wide_heads == 16) return wide ? launch(flash_decode_8bit_kernel<2, true>) : launch(flash_decode_8bit_kernel<2, false>);
     }
-    return wide ? launch(flash_decode_8bit_kernel<1, true>, HD <= 128 ? 3 : 2) : launch(flash_decode_8bit_kernel<1, false>, HD <= 128 ? 3 : 2);
+    return wide ? launch(flash_decode_8bit_kernel<1, true>) : launch(flash_decode_8bit_kernel<1, false>);
 }

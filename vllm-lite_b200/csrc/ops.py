@@ -156,7 +156,7 @@ _SIGNATURES = {
                                                    c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                                    c_int, c_void_p, c_void_p],
     ("flash_decode_8bit", "vl_flash_decode_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
-                                                    c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                                    c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p,
                                                     c_void_p, c_void_p, c_int, c_void_p],
     ("flash_tc5_8bit", "vl_flash_prefill_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                                   c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p],
@@ -993,14 +993,10 @@ def qk_norm_rope_write_8bit(qkv, positions, slots, cu_seqlens, q_weight, k_weigh
 
 
 def flash_decode_8bit_scratch(num_tokens, num_heads, num_kv_heads, head_dim):
-    """(floats of scratch memory, int32 counters) that `flash_decode_8bit` wants for so many tokens."""
-    return num_tokens * num_heads * _pieces_8bit(num_tokens, num_kv_heads, head_dim) * (head_dim + 2), num_tokens * num_heads
-
-
-def _pieces_8bit(num_tokens, num_kv_heads, head_dim):
-    """How many pieces an item (a token's KV head) may be shared by: as many as leave every block of the launch its share of a step of few tokens, two at
-    least, and no more than a block can add up."""
-    return min(2 + -(-600 // max(1, num_tokens * num_kv_heads)), 302, 4 * (head_dim + 4))
+    """(floats of scratch memory, int32 counters) that `flash_decode_8bit` wants for so many tokens: as many pieces for each item (a token's KV head) as leave
+    every block of the launch its share of a step of few tokens, and three at least."""
+    pieces = 2 + -(-600 // max(1, num_tokens * num_kv_heads))
+    return num_tokens * num_heads * pieces * (head_dim + 2), num_tokens * num_heads
 
 
 def _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, name):
@@ -1043,8 +1039,8 @@ def flash_decode_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, r
         raise KernelError(f"flash_decode_8bit: {floats} floats of scratch and {counters} counters are wanted, got {scratch.shape[0]} and {arrivals.shape[0]}")
     _check(_fn("flash_decode_8bit", "vl_flash_decode_8bit", {"FA_HD": head_dim})(
         q, q.shape[1], k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], req_index, positions, T, num_heads, num_kv_heads, head_dim,
-        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), int(max_context), _pieces_8bit(T, num_kv_heads, head_dim), scratch, err,
-        token_index, out, arrivals, int(settled), _stream()), "vl_flash_decode_8bit")
+        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), int(max_context), scratch, floats, err, token_index, out,
+        arrivals, int(settled), _stream()), "vl_flash_decode_8bit")
     return out
 
 
