@@ -13,7 +13,7 @@
 //
 // Angles: pos * inv_freq in float32 is off by up to 2^-24 of itself, at position 100,000 by 0.006; the product's error, which one fma
 // gives, is added to first order, so that sines and cosines are those of the exact product.
-// Positions and slots are read before the wait for the kernel ahead, as the other head work does (csrc/common.cuh).
+// While dependent launches are on, positions and slots are read before the wait for the kernel ahead, as the other head work does (csrc/common.cuh).
 #include "cache_8bit.cuh"
 
 using namespace cache8;
@@ -141,10 +141,11 @@ qk_norm_rope_write_8bit_kernel(const bf16* qkv, int row_stride, bf16* q_out, int
                                const int* __restrict__ slots, const int* __restrict__ cu, int B, const float* __restrict__ qw,
                                const float* __restrict__ kw, float eps, const float* __restrict__ inv_freq, int rot, unsigned char* kcache,
                                unsigned char* vcache, float* kscale, float* vscale, int T, int nq, int nkv, int hd, int page_size, int num_pages,
-                               unsigned* err, int page_blocks, int heads_a_warp) {
+                               unsigned* err, int page_blocks, int heads_a_warp, int early) {
     constexpr int ROWS = MAXHD <= 128 ? 8 : 4;               // rows a warp holds
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
+    if (!early) pdl_wait();
     if ((int)blockIdx.x >= page_blocks) {                    // ---- queries ----
         const int groups = (nq + heads_a_warp - 1) / heads_a_warp;
         const long long unit = (long long)((int)blockIdx.x - page_blocks) * WARPS + warp;
@@ -301,7 +302,7 @@ extern "C" int vl_qk_norm_rope_write_8bit(const void* qkv, int row_stride, void*
     const long long units = (long long)T * ((nq + heads_a_warp - 1) / heads_a_warp), blocks = pages * nkv * 2 + (units + WARPS - 1) / WARPS;
     if (blocks >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
     auto kernel = hd <= 128 ? qk_norm_rope_write_8bit_kernel<128> : qk_norm_rope_write_8bit_kernel<256>;
-    return vl_launch(kernel, dim3((unsigned)blocks), dim3(NT), 0, (cudaStream_t)stream, (const bf16*)qkv, row_stride, (bf16*)q_out, q_stride,
+    return vl_launch_waiting(kernel, dim3((unsigned)blocks), dim3(NT), 0, (cudaStream_t)stream, (const bf16*)qkv, row_stride, (bf16*)q_out, q_stride,
                      positions, slots, cu, B, qw, kw, eps, inv_freq, rot, (unsigned char*)kcache, (unsigned char*)vcache, kscale, vscale, T, nq, nkv,
-                     hd, page_size, num_pages, err, (int)(pages * nkv * 2), heads_a_warp);
+                     hd, page_size, num_pages, err, (int)(pages * nkv * 2), heads_a_warp, (int)vl_pdl_enabled());
 }

@@ -45,14 +45,7 @@ constexpr bool ODD = HD % 32 != 0;                     // and two features more:
 constexpr int OT = HD / 16;                            // tiles of 16 features
 constexpr float ROOM = 8.f;                            // log2 of what a weight may exceed the base's by
 constexpr int SHIFT = 6;                               // p sv is held times 2^SHIFT
-#ifndef T_MIN
-#define T_MIN 2
-#define T_WAVES 3
-#define T_SHORT 4
-#define T_APART 64
-#endif
-constexpr int SHORTER = T_SHORT;                       // the later runs are so many times shorter
-constexpr int MIN_RUN = T_MIN;                             // fewest steps of a run
+constexpr int MIN_RUN = 2;                             // fewest steps of a run
 
 // A warp's ring: NS stages of 16 keys' rows and 16 values' rows, in strides with which the lanes' loads meet in no bank: a quad of lanes takes
 // 16 KL bytes of a key's row side by side, four rows apart in the lanes' groups of eight, and values are taken two rows apart.
@@ -102,24 +95,6 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 __device__ __forceinline__ int exponent_of(float s) { return (int)(__float_as_uint(s) >> 23) - 127; }
 
 struct Piece { int tok, req, kvh, h0, heads, c0, c1, piece, pieces, item, slot, slot0, stop; };   // heads 0: the end of the run
-
-// The runs: as many of a steps as the GPU holds at once, then equally many of about a / SHORTER and a / SHORTER^2, which the blocks that finish first take.
-struct Runs {
-    int most, more, a, b, c;
-    __device__ __forceinline__ Runs(int all, int resident, int count) : most(min(resident, count)), more((count - most) / 2) {
-        const int in_first = SHORTER * SHORTER * most + (SHORTER + 1) * more;    // steps of all, were a = SHORTER^2
-        a = max((int)(((long long)all * SHORTER * SHORTER + in_first - 1) / in_first), MIN_RUN);
-        b = max((a + SHORTER - 1) / SHORTER, MIN_RUN);
-        c = max((b + SHORTER - 1) / SHORTER, MIN_RUN);
-    }
-    __device__ __forceinline__ long long begin(int r) const {
-        return (long long)min(r, most) * a + (long long)min(max(r - most, 0), more) * b + (long long)max(r - most - more, 0) * c;
-    }
-    __device__ __forceinline__ int of(int step) const {
-        const long long one = (long long)most * a, two = one + (long long)more * b;
-        return step < one ? step / a : (step < two ? most + (int)((step - one) / b) : most + more + (int)((step - two) / c));
-    }
-};
 
 // Adds up an item's pieces for one head: numerators at part + (slot of piece p) * stride, (maximum, sum) at ml + (slot of piece p) * heads.  The slots: `first`,
 // then every second one from `next` on.  A thread takes 4 features at d; 8 pieces' numbers are on their way together.
@@ -174,7 +149,7 @@ __global__ void __launch_bounds__(NTHREADS, RESIDENT)
 flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigned char* __restrict__ kcache, const unsigned char* __restrict__ vcache,
                          const float* __restrict__ kscale, const float* __restrict__ vscale, const int* __restrict__ block_table, int max_blocks,
                          const int* __restrict__ req_index, const int* __restrict__ positions, int T, int nq, int nkv, int page_size, int num_pages,
-                         float scale_log2, int window, int bound, int resident, float* scratch, unsigned* err, const int* __restrict__ token_index,
+                         float scale_log2, int window, int bound, float* scratch, unsigned* err, const int* __restrict__ token_index,
                          bf16* __restrict__ out, int* arrivals, int settled) {      // arrivals null: another launch adds the pieces up
     constexpr int HEADS = 8 * NT;
     extern __shared__ __align__(16) unsigned char smem[];    // the warps' rings; where those are at rest, the warps' shares of a piece
@@ -228,8 +203,8 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         if (z0 == 0) { n0 = n; u0 = u; }
     }
     const int grid = gridDim.x, all_steps = total, run = blockIdx.x;
-    const Runs runs(all_steps, resident, grid);
-    const int first = (int)min(runs.begin(run), (long long)all_steps), last = (int)min(runs.begin(run + 1), (long long)all_steps);
+    const int per = max((all_steps + grid - 1) / grid, MIN_RUN);
+    const int first = (int)min((long long)run * per, (long long)all_steps), last = min(first + per, all_steps);
     const int held = min(HEADS, grp);                        // rows that a piece leaves
     const Scratch left(scratch, grid, held);
     total = 0;
@@ -273,12 +248,12 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         const int step0 = lo / BN - start;                   // + a step's number in the launch = its number in the request
         p.c0 = max((at + step0) * BN, lo);
         p.c1 = min((p.stop + step0) * BN, keys);
-        const int run0 = runs.of(start);
+        const int run0 = start / per;
         p.piece = run - run0;
-        p.pieces = runs.of(start + tz - 1) - run0 + 1;
+        p.pieces = (start + tz - 1) / per - run0 + 1;
         p.item = z * ny + y;
         p.slot = 2 * run + (at > first ? 1 : 0);             // the item that the run begins in, or the one that it ends in
-        p.slot0 = 2 * run0 + (start > runs.begin(run0) ? 1 : 0);                 // where its first piece is
+        p.slot0 = 2 * run0 + (start > run0 * per ? 1 : 0);                 // where its first piece is
         return p;
     };
 
@@ -369,7 +344,7 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
             if (whole) {                                     // 16 rows of a page lie side by side
                 const unsigned char* const k = kcache + (size_t)w.row * HD + lane * 16;
                 const unsigned char* const v = vcache + (size_t)w.row * HD + lane * 16;
-                if constexpr (32 % PIECES == 0) {            // 32 / PIECES rows a round
+                if constexpr (PIECES > 1 && 32 % PIECES == 0) {            // 32 / PIECES rows a round (one piece a row leaves half of the lanes without)
                     copies16<32 / PIECES * KS, 512, COPIES>(to + lane / PIECES * KS + lane % PIECES * 16, k);
                     copies16<32 / PIECES * VS, 512, COPIES>(to + 16 * KS + lane / PIECES * VS + lane % PIECES * 16, v);
                 } else {
@@ -393,8 +368,10 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
                     copy16(to + 16 * KS + r * VS + c * 16, vcache + at, bytes);
                 }
             }
-            // values under a scale that is none: their keys' scores say so, so that only who reads them gets NaN
-            if (lane < (WIDE ? 1 : 16)) s_scale[warp][stage][tile % SUB][lane] = w.vs != w.vs ? make_float2(w.vs, 0.f) : make_float2(w.ks, w.vs);
+        };
+        // values under a scale that is none: their keys' scores say so, so that only who reads them gets NaN
+        auto note = [&](const Where& w, int u, int stage) {
+            if (lane < (WIDE ? 1 : 16)) s_scale[warp][stage][u][lane] = w.vs != w.vs ? make_float2(w.vs, 0.f) : make_float2(w.ks, w.vs);
         };
         // PART: a step with keys that are not read.  The step's tiles side by side, so that one's chain of products, exponentials and conversions
         // runs beside another's.
@@ -534,22 +511,30 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
             // lane i knows the place of tile base + i; the next 32 tiles' are looked up on the way, a load at a time
             Where now = where_of(page_of(first_key(st0 * SUB + lane)), first_key(st0 * SUB + lane)), then = {-1, 0.f, 0.f};
             int from = 0, base = st0 * SUB, page = -1;
-            auto next = [&](int stage) {                     // the step that begins with tile base + from
-                if (from == 32) { now = then; base += 32; from = 0; }
+            auto ask = [&](int stage) {                      // the step that begins with tile base + from
 #pragma unroll
-                for (int u = 0; u < SUB; ++u)
-                    fetch(Where{__shfl_sync(0xffffffffu, now.row, from + u), __shfl_sync(0xffffffffu, now.ks, from + u), __shfl_sync(0xffffffffu, now.vs, from + u)},
-                          base + from + u, stage);
+                for (int u = 0; u < SUB; ++u) fetch(Where{__shfl_sync(0xffffffffu, now.row, from + u), 0.f, 0.f}, base + from + u, stage);
                 copies_commit();
+            };
+            auto tell = [&](int stage) {                     // its scales
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) note(Where{0, __shfl_sync(0xffffffffu, now.ks, from + u), __shfl_sync(0xffffffffu, now.vs, from + u)}, u, stage);
+            };
+            auto advance = [&]() {
                 if (from == 8) page = page_of(first_key(base + 32 + lane));
                 if (from == 20) then = where_of(page, first_key(base + 32 + lane));
                 from += SUB;
+                if (from == 32) { now = then; base += 32; from = 0; }
             };
-            next(0);
-            queries();                                       // (while the first keys are on their way)
+            ask(0);
+            queries();                                       // (while the first keys and their scales are on their way)
+            tell(0);
+            advance();
             int stage = 0;
             for (int st = st0; st <= st1; ++st, stage ^= 1) {
-                next(stage ^ 1);
+                ask(stage ^ 1);
+                tell(stage ^ 1);
+                advance();
                 copies_wait<1>();
                 __syncwarp();                                // every lane's copies have landed
                 const int k0 = st * BN + warp * SUB * 16;
@@ -564,7 +549,7 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
             auto find = [&](int tile) { return where_of(page_of(first_key(tile) + (lane & 15)), first_key(tile) + (lane & 15)); };
             Where w[SUB];
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) fetch(find(st0 * SUB + u), st0 * SUB + u, 0);
+            for (int u = 0; u < SUB; ++u) { w[u] = find(st0 * SUB + u); fetch(w[u], st0 * SUB + u, 0); note(w[u], u, 0); }
             copies_commit();
 #pragma unroll
             for (int u = 0; u < SUB; ++u) w[u] = find((st0 + 1) * SUB + u);
@@ -572,7 +557,7 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
             int stage = 0;
             for (int st = st0; st <= st1; ++st, stage ^= 1) {
 #pragma unroll
-                for (int u = 0; u < SUB; ++u) fetch(w[u], (st + 1) * SUB + u, stage ^ 1);
+                for (int u = 0; u < SUB; ++u) { fetch(w[u], (st + 1) * SUB + u, stage ^ 1); note(w[u], u, stage ^ 1); }
                 copies_commit();
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) w[u] = find((st + 2) * SUB + u);             // (used a step later)
@@ -706,22 +691,23 @@ extern "C" int vl_flash_decode_8bit(const void* q, int q_stride, const void* kca
     auto launch = [&](auto kernel) {
         const long long resident = (long long)sms * RESIDENT;
         long long runs = (floats - 8 - 4 * items) / (2ll * held * (HD + 2));
-        if (runs > T_WAVES * resident) runs = T_WAVES * resident;
+        if (runs > resident) runs = resident;
         if (runs > sms) runs -= runs % sms;                  // as many on every SM
         if (runs > most) runs = most;
         if (runs < 1) runs = 1;
         // pieces that an item may come in, were every place full, and what a block would read to add them up: above 64 KB another launch, a block a head, does
         const long long run = (most + resident - 1) / resident > MIN_RUN ? (most + resident - 1) / resident : MIN_RUN, pieces = (steps + run - 1) / run + 1;
-        const bool apart = pieces * held * HD * 4 > T_APART * 1024;
+        const bool apart = pieces * held * HD * 4 > 64 * 1024;
         const int rings = WARPS * NS * STAGE, shares = WARPS * wide_heads * OLD * 4, smem = rings > shares ? rings : shares;
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return (int)e;
-        int rc = vl_launch(kernel, dim3((unsigned)runs), dim3(NTHREADS), (size_t)smem, (cudaStream_t)stream, (const bf16*)q, q_stride,
+        // (unless it may read the step's description early it touches no memory before its wait)
+        int rc = vl_launch_as(settled ? vl_pdl_enabled() : !vl_pdl_forbidden(), kernel, dim3((unsigned)runs), dim3(NTHREADS), (size_t)smem, (cudaStream_t)stream, (const bf16*)q, q_stride,
                            (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks, req_index, positions, T,
-                           nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, bound, (int)resident, scratch, err, token_index, (bf16*)out,
+                           nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, bound, scratch, err, token_index, (bf16*)out,
                            apart ? (int*)nullptr : arrivals, settled);
         if (rc == VL_OK && apart)
-            rc = vl_launch(flash_decode_8bit_merge_kernel, dim3((unsigned)(items * held)), dim3(HD / 4 < 32 ? 32 : HD / 4), 0, (cudaStream_t)stream, scratch,
+            rc = vl_launch_waiting(flash_decode_8bit_merge_kernel, dim3((unsigned)(items * held)), dim3(HD / 4 < 32 ? 32 : HD / 4), 0, (cudaStream_t)stream, scratch,
                            (int)runs, held, grp, nq, nkv, (bf16*)out);
         return rc;
     };

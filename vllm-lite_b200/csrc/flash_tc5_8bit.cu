@@ -475,7 +475,7 @@ extern "C" int vl_flash_prefill_8bit(const void* q, int q_stride, void* out, con
     if ((long long)num_tiles * cuts > 65535) return VL_ERR_UNSUPPORTED;
     cudaError_t e = cudaFuncSetAttribute(flash_tc5_8bit_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
     if (e != cudaSuccess) return (int)e;
-    return vl_launch(flash_tc5_8bit_kernel, dim3(nkv * htiles, num_tiles * cuts), dim3(NTHREADS), SMEM_BYTES, (cudaStream_t)stream, (const bf16*)q,
+    return vl_launch_waiting(flash_tc5_8bit_kernel, dim3(nkv * htiles, num_tiles * cuts), dim3(NTHREADS), SMEM_BYTES, (cudaStream_t)stream, (const bf16*)q,
                      q_stride, (bf16*)out, (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks,
                      (const int4*)tiles, num_tiles, nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, err, heads, htiles, tokens, cuts);
 }
