@@ -20,12 +20,13 @@
 // these integers too, floor(min_p 2^40).
 //
 // vl_apply_penalties works on ragged per-row lists.
-// vl_sample: a cluster of 1 to 8 blocks holds a row in shared memory, so that it is read from memory once, whatever the options.  A row that asks for top-k
-// or top-p is sorted into SMP_BINS bins of its distance from the maximum (a partition that keeps the order of values: subtraction and the cut are
-// monotone), with their counts and masses; each block adds up a share of the bins over the cluster and the bin in which a threshold lies is found by
-// a scan of them.  Inside that bin the threshold's key is found 8 bits at a time, until what is left is kept whole; few values lie there, so these passes
-// count little.  Values 32 and more below the maximum have mass 0 and are in no bin: no threshold need be found among them.  Any vocabulary size; what of
-// a slice shared memory does not hold (rows of more than some 390,000) is read again in each pass.
+// vl_sample: a cluster of 1 to 8 blocks holds a row in shared memory, so that it is read from memory once, whatever the options.  A threshold (top-k's by
+// counts, top-p's by masses) is found in three steps.  All values are sorted into SMP_BINS bins of their distance from the maximum, a partition that keeps
+// their order (subtraction and the cut are monotone); the blocks add up a share of the bins each and a scan finds the bin with which the sum is reached.
+// The few values of that bin are brought together in every block, and there the threshold's key is found 8 bits at a time, until what is left
+// is kept whole.  (Should they be more than SMP_LIST, as in a row of one value, the 8 bits at a time go over the cluster's whole row.)  Behind top-k, top-p's sum runs over
+// what top-k left.  Values 32 and more below the maximum have mass 0 and are in no bin: no threshold need be found among them.  Any vocabulary
+// size; what of a slice shared memory does not hold (rows of more than some 390,000) is read again in each pass.
 #include "common.cuh"
 #include <cooperative_groups.h>
 
@@ -37,6 +38,8 @@ namespace cg = cooperative_groups;
 #define SMP_BINS 2048
 #define SMP_PER_UNIT 64.0f       /* bins per unit of s: 32 units in all, and exp(-27.8) 2^40 is below one */
 #define SMP_CLUSTER 8
+#define SMP_LIST 2048            /* values of one bin that a block brings together */
+#define SMP_OWN 512              /* ... of them its own */
 
 typedef unsigned long long u64;
 
@@ -83,17 +86,28 @@ __device__ __forceinline__ ArgBest better(ArgBest a, ArgBest b) {
     return a;
 }
 
+// Adds to a 64-bit sum in shared memory, low word at p: 32-bit atomics are the hardware's own, and the high word is seldom touched.
+__device__ __forceinline__ void add_mass(u64* p, u64 q) {
+    unsigned* w = reinterpret_cast<unsigned*>(p);
+    const unsigned lo = (unsigned)q, old = atomicAdd(w, lo), hi = (unsigned)(q >> 32) + (old + lo < old ? 1u : 0u);
+    if (hi) atomicAdd(w + 1, hi);
+}
+
+__device__ __forceinline__ float from_key(unsigned k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+
 struct SampleShared {
-    u64 mass[SMP_BINS];
-    unsigned count[SMP_BINS];
+    union {                                 // (the bins are at rest when values are brought together)
+        struct { u64 mass[SMP_BINS]; unsigned count[SMP_BINS]; };
+        unsigned list[SMP_LIST];
+    };
+    unsigned own[SMP_OWN], own_count;       // this block's values of a bin, by their keys
     u64 fine_mass[2][256];                  // two levels of the search in a bin in turn: one is read by the cluster while the other is filled
     unsigned fine_count[2][256];
-    u64 warp_sum[SMP_WARPS], all_mass, part_mass;      // part: this block's share of the bins
-    unsigned part_count;
+    u64 warp_sum[SMP_WARPS], all_mass, part_mass;      // part: of this block's share of the bins
     ArgBest warp_best[SMP_WARPS], best;
-    int found_bin;
-    u64 found_above_mass, found_mass, found_value;
-    unsigned found_above, found_count;
+    int found_bin, found_digit;
+    u64 found_value, found_before;
+    unsigned found_count, found_key;
 };
 
 __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
@@ -114,6 +128,19 @@ __device__ __forceinline__ u64 block_scan_u64(u64 v, u64* warp_sums) {
     __syncthreads();
     for (int w = 0; w < warp; ++w) v += warp_sums[w];
     return v;
+}
+
+// Sums of one number of each block of a cluster (x: this lane's block's, 0 beyond the last): all of them, and those of the blocks before each lane's.
+__device__ __forceinline__ void cluster_sums(u64 x, u64* total, u64* before) {
+    const int lane = threadIdx.x & 31;
+    u64 upto = x;
+#pragma unroll
+    for (int o = 1; o < SMP_CLUSTER; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    *total = __shfl_sync(0xffffffffu, upto, SMP_CLUSTER - 1);
+    *before = upto - x;
 }
 
 __global__ void __launch_bounds__(SMP_THREADS)
@@ -154,6 +181,7 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
         }
     }
     for (int i = n4 + tid; i < n; i += SMP_THREADS) take(i, l[i]);
+    for (int i = n + tid; i < held; i += SMP_THREADS) s_val[i] = -INFINITY;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         ArgBest other{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.i, o)};
@@ -166,17 +194,28 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
         sh.best = best;
     }
     cluster.sync();
-    best = sh.best;
-    for (int c = 0; c < C; ++c) best = better(best, cluster.map_shared_rank(&sh, c)->best);
+    const SampleShared* const peer = cluster.map_shared_rank(&sh, lane < C ? lane : rank);        // a lane a block
+    best = peer->best;
+#pragma unroll
+    for (int o = SMP_CLUSTER / 2; o > 0; o >>= 1) {
+        ArgBest other{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.i, o)};
+        best = better(best, other);
+    }
+    best = ArgBest{__shfl_sync(0xffffffffu, best.v, 0), __shfl_sync(0xffffffffu, best.i, 0)};
     const int arg = best.i == 0x7fffffff ? 0 : best.i;
     const float row_max = best.v * inv_t;      // maximum of the scaled row (top-k keeps it)
     const bool degenerate = !(row_max > -INFINITY && row_max < INFINITY);
     auto value = [&](int i) { return i < held ? s_val[i] : clean(l[i], inv_t); };
-    auto mass_of = [&](float s) { return (u64)(expf(s - row_max) * SMP_FIX); };
-    // the bin of a value; SMP_BINS for one without mass
+    // floor(exp(s - max) 2^40), the number's own digits shifted (a conversion takes as long as the exponential)
+    auto mass_of = [&](float s) -> u64 {
+        const unsigned e = __float_as_uint(expf(s - row_max)), shift = e >> 23;                  // of 2^(shift - 127), at most 2^0
+        const u64 digits = (e & 0x7fffffu) | 0x800000u;
+        return shift >= 110 ? digits << (shift - 110) : (shift >= 87 ? digits >> (110 - shift) : 0);
+    };
+    // the bin of a value, by an addition that leaves the nearest whole number in a float's low bits; SMP_BINS for one without mass
     auto bin_of = [&](float s) {
-        const float d = (row_max - s) * SMP_PER_UNIT;
-        return d < (float)SMP_BINS ? (int)d : SMP_BINS;
+        const float d = row_max - s;
+        return d < (SMP_BINS - 1) / SMP_PER_UNIT ? (int)(__float_as_uint(fmaf(d, SMP_PER_UNIT, 8388608.f)) & (SMP_BINS - 1)) : SMP_BINS;
     };
     auto finish = [&](int token, float logprob) {
         out_token[r] = token;
@@ -188,173 +227,177 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
         return;
     }
 
-    // A token is kept if its bin lies before `cut_bin`, or in it with at least the key `cut_key`.
-    int cut_bin = SMP_BINS;
-    unsigned cut_key = 0;
-    const bool by_k = !greedy && k > 0 && k < V, by_p = !greedy && tp < 1.f;
-    if (by_k || by_p) {
-        for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { sh.count[i] = 0; sh.mass[i] = 0; }
-        __syncthreads();
-        for (int i = tid; i < n; i += SMP_THREADS) {
-            const float s = value(i);
-            const int b = bin_of(s);
-            if (b < SMP_BINS) {
-                atomicAdd(&sh.count[b], 1u);
-                const u64 q = mass_of(s);
-                if (q) atomicAdd(&sh.mass[b], q);
-            }
+    // every value of the slice, in no order; shared memory holds a multiple of four, filled up with values without mass
+    auto each = [&](auto f) {
+        for (int i = 4 * tid; i < held; i += 4 * SMP_THREADS) {
+            const float4 v = *reinterpret_cast<const float4*>(s_val + i);
+            f(v.x); f(v.y); f(v.z); f(v.w);
         }
+        for (int i = held + tid; i < n; i += SMP_THREADS) f(clean(l[i], inv_t));
+    };
+    float cut = -INFINITY;                     // a token is kept by top-k and top-p if its value is at least this
+    const bool by_k = !greedy && k > 0 && k < V, by_p = !greedy && tp < 1.f;
+    int level = 0;
+
+    // The value with which the sum, from the largest values on, of counts (masses) of all values from `cut` on reaches goal(their sum); -inf if all together do not.
+    auto threshold = [&](bool masses, auto goal_of) -> float {
+        for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { sh.count[i] = 0; sh.mass[i] = 0; }
+        if (tid == 0) { sh.part_mass = 0; sh.own_count = 0; }
+        __syncthreads();
+        each([&](float s) {
+            const int b = bin_of(s);
+            if (b >= SMP_BINS || s < cut) return;
+            if (!masses) atomicAdd(&sh.count[b], 1u);
+            else {
+                const u64 q = mass_of(s);
+                if (q) add_mass(&sh.mass[b], q);
+            }
+        });
         cluster.sync();
-        // this block's share of the bins, summed over the cluster in its own arrays (nobody else reads that share there)
+        // this block's share of the bins, summed over the cluster in its own array (nobody else reads that share there)
         const int share = SMP_BINS / C, lo = rank * share;
         u64 m = 0;
-        unsigned c = 0;
         for (int i = lo + tid; i < lo + share; i += SMP_THREADS) {
-            unsigned bc = 0;
             u64 bm = 0;
-            for (int b = 0; b < C; ++b) {
-                const SampleShared* other = cluster.map_shared_rank(&sh, b);
-                bc += other->count[i];
-                bm += other->mass[i];
+#pragma unroll
+            for (int b = 0; b < SMP_CLUSTER; ++b) {          // (all on their way together)
+                const SampleShared* other = cluster.map_shared_rank(&sh, b < C ? b : rank);
+                const u64 x = masses ? other->mass[i] : (u64)other->count[i];
+                bm += b < C ? x : 0;
             }
-            sh.count[i] = bc;
             sh.mass[i] = bm;
-            c += bc;
             m += bm;
         }
-        c = __reduce_add_sync(0xffffffffu, c);
         m = warp_sum_u64(m);
-        if (tid == 0) { sh.part_count = 0; sh.part_mass = 0; }
-        __syncthreads();
-        if (lane == 0) { atomicAdd(&sh.part_count, c); atomicAdd(&sh.part_mass, m); }
+        if (lane == 0 && m) atomicAdd(&sh.part_mass, m);
         cluster.sync();
+        u64 total, before;
+        const u64 part = lane < C ? peer->part_mass : 0;
+        cluster_sums(part, &total, &before);
+        const u64 goal = goal_of(total);
+        if (goal > total) return -INFINITY;    // (everything that has a mass is kept)
+        const int owner = __ffs(__ballot_sync(0xffffffffu, lane < C && before + part >= goal)) - 1;
+        before = __shfl_sync(0xffffffffu, before, owner);
+        if (owner == rank) {
+            const int per = (share + SMP_THREADS - 1) / SMP_THREADS, i0 = lo + tid * per, i1 = min(lo + share, i0 + per);
+            u64 mine = 0;
+            for (int i = i0; i < i1; ++i) mine += sh.mass[i];
+            u64 cum = before + block_scan_u64(mine, sh.warp_sum) - mine;
+            for (int i = i0; i < i1; ++i) {
+                const u64 x = sh.mass[i];
+                if (cum < goal && cum + x >= goal) { sh.found_bin = i; sh.found_value = cum; }
+                cum += x;
+            }
+        }
+        cluster.sync();
+        const SampleShared* o = cluster.map_shared_rank(&sh, owner);
+        const int bin = o->found_bin;
+        u64 left = goal - o->found_value;
 
-        // The bin with which the sum, from the largest values on, of counts (masses) reaches `goal`; false if all bins together do not.
-        struct Found { int bin; unsigned above, count; u64 above_mass, mass; } f;
-        auto cross = [&](bool masses, u64 goal) -> bool {
-            int owner = -1;
-            unsigned before_c = 0;
-            u64 before_m = 0;
-            for (int b = 0; b < C && owner < 0; ++b) {
-                const SampleShared* other = cluster.map_shared_rank(&sh, b);
-                const unsigned pc = other->part_count;
-                const u64 pm = other->part_mass;
-                if ((masses ? before_m + pm : (u64)(before_c + pc)) >= goal) owner = b;
-                else { before_c += pc; before_m += pm; }
+        // the bin's values, each block's own first
+        each([&](float s) {
+            if (bin_of(s) == bin && s >= cut) {
+                const unsigned at = atomicAdd(&sh.own_count, 1u);
+                if (at < SMP_OWN) sh.own[at] = order_key(s);
             }
-            if (owner < 0) return false;
-            if (owner == rank) {
-                const int each = (share + SMP_THREADS - 1) / SMP_THREADS, i0 = lo + tid * each, i1 = min(lo + share, i0 + each);
-                u64 mine_c = 0, mine_m = 0;
-                for (int i = i0; i < i1; ++i) { mine_c += sh.count[i]; mine_m += sh.mass[i]; }
-                u64 cum_c = before_c + block_scan_u64(mine_c, sh.warp_sum) - mine_c, cum_m = before_m + block_scan_u64(mine_m, sh.warp_sum) - mine_m;
-                for (int i = i0; i < i1; ++i) {
-                    const u64 x = masses ? sh.mass[i] : sh.count[i], cum = masses ? cum_m : cum_c;
-                    if (cum < goal && cum + x >= goal) {
-                        sh.found_bin = i;
-                        sh.found_above = (unsigned)cum_c; sh.found_above_mass = cum_m;
-                        sh.found_count = sh.count[i]; sh.found_mass = sh.mass[i];
-                    }
-                    cum_c += sh.count[i];
-                    cum_m += sh.mass[i];
-                }
+        });
+        cluster.sync();
+        u64 all, place;
+        const unsigned found = lane < C ? peer->own_count : 0;
+        cluster_sums(found, &all, &place);
+        const bool few = all <= SMP_LIST && __all_sync(0xffffffffu, found <= SMP_OWN);
+        if (few) {
+#pragma unroll
+            for (int b = 0; b < SMP_CLUSTER; ++b) {
+                const unsigned c = __shfl_sync(0xffffffffu, found, b), at = (unsigned)__shfl_sync(0xffffffffu, place, b);
+                for (unsigned i = tid; i < c; i += SMP_THREADS) sh.list[at + i] = cluster.map_shared_rank(&sh, b < C ? b : rank)->own[i];
             }
-            cluster.sync();
-            const SampleShared* o = cluster.map_shared_rank(&sh, owner);
-            f.bin = o->found_bin; f.above = o->found_above; f.count = o->found_count; f.above_mass = o->found_above_mass; f.mass = o->found_mass;
-            return true;
-        };
-        // Within bin f.bin, among keys of at least `least`: the key with which the sum of counts (masses) reaches `goal`, all of that key's values kept.
-        // f.mass becomes the mass of the bin's kept values.
-        int level = 0;
-        auto refine = [&](bool masses, u64 goal, unsigned least) -> unsigned {
-            unsigned prefix = 0;
-            u64 kept = 0;                      // mass of the bin's values above the prefix
-            for (int shift = 24; shift >= 0; shift -= 8, ++level) {
-                u64* fm = sh.fine_mass[level & 1];
-                unsigned* fc = sh.fine_count[level & 1];
-                if (tid < 256) { fm[tid] = 0; fc[tid] = 0; }
+        }
+        unsigned prefix = 0;
+        for (int shift = 24; shift >= 0; shift -= 8, ++level) {
+            u64* fm = sh.fine_mass[level & 1];
+            if (tid < 256) { fm[tid] = 0; sh.fine_count[level & 1][tid] = 0; }
+            __syncthreads();
+            const unsigned himask = shift == 24 ? 0u : (0xffffffffu << (shift + 8));
+            auto sort = [&](unsigned key) {
+                if ((key & himask) != prefix) return;
+                const unsigned d = 255u - ((key >> shift) & 255u);
+                atomicAdd(&sh.fine_count[level & 1][d], 1u);
+                if (masses) add_mass(&fm[d], mass_of(from_key(key)));
+            };
+            if (few) {
+                for (unsigned i = tid; i < all; i += SMP_THREADS) sort(sh.list[i]);
                 __syncthreads();
-                const unsigned himask = shift == 24 ? 0u : (0xffffffffu << (shift + 8));
-                for (int i = tid; i < n; i += SMP_THREADS) {
-                    const float s = value(i);
-                    const unsigned key = order_key(s);
-                    if (bin_of(s) == f.bin && key >= least && (key & himask) == prefix) {
-                        atomicAdd(&fc[255u - ((key >> shift) & 255u)], 1u);
-                        atomicAdd(&fm[255u - ((key >> shift) & 255u)], mass_of(s));
-                    }
-                }
+            } else {
+                each([&](float s) { if (bin_of(s) == bin && s >= cut) sort(order_key(s)); });
                 cluster.sync();
-                u64 x = 0, xm = 0;             // every block finds the same digit for itself
-                unsigned xc = 0;
-                if (tid < 256)
-                    for (int b = 0; b < C; ++b) {
-                        const SampleShared* other = cluster.map_shared_rank(&sh, b);
-                        xc += other->fine_count[level & 1][tid];
-                        xm += other->fine_mass[level & 1][tid];
-                    }
-                x = masses ? xm : xc;
-                const u64 upto = block_scan_u64(x, sh.warp_sum), upto_m = block_scan_u64(xm, sh.warp_sum);
-                __syncthreads();
-                if (tid < 256 && upto >= goal && upto - x < goal) {
-                    sh.found_bin = 255 - tid; sh.found_value = upto - x; sh.found_count = xc; sh.found_above_mass = upto_m - xm; sh.found_mass = xm;
+            }
+            u64 x = 0;                         // every block finds the same digit for itself
+            unsigned c = 0;
+            if (tid < 256)
+                for (int b = few ? rank : 0; b < (few ? rank + 1 : C); ++b) {
+                    const SampleShared* other = cluster.map_shared_rank(&sh, b);
+                    c += other->fine_count[level & 1][tid];
+                    x += masses ? other->fine_mass[level & 1][tid] : (u64)other->fine_count[level & 1][tid];
                 }
+            const u64 upto = block_scan_u64(x, sh.warp_sum);
+            if (tid < 256 && upto >= left && upto - x < left) { sh.found_digit = 255 - tid; sh.found_before = upto - x; sh.found_count = c; }
+            __syncthreads();
+            prefix |= (unsigned)sh.found_digit << shift;
+            left -= sh.found_before;
+            const bool whole = few && (sh.found_count == 1 || (!masses && left == sh.found_count));
+            __syncthreads();
+            if (whole && shift > 0) {          // all of them are kept: the least of them is the threshold
+                if (tid == 0) sh.found_key = 0xffffffffu;
                 __syncthreads();
-                prefix |= (unsigned)sh.found_bin << shift;
-                goal -= sh.found_value;
-                kept += sh.found_above_mass;
-                f.mass = kept + sh.found_mass;
-                const bool whole = masses ? sh.found_count == 1 : goal == sh.found_count;
+                for (unsigned i = tid; i < all; i += SMP_THREADS)
+                    if (sh.list[i] >> shift == prefix >> shift) atomicMin(&sh.found_key, sh.list[i]);
                 __syncthreads();
-                if (whole) { ++level; break; }
-            }
-            return max(prefix, least);
-        };
-
-        u64 total = 0;                         // mass after top-k
-        for (int b = 0; b < C; ++b) total += cluster.map_shared_rank(&sh, b)->part_mass;
-        if (by_k && cross(false, (u64)k)) {
-            cut_bin = f.bin;
-            if (f.above + f.count > (unsigned)k) cut_key = refine(false, (u64)(k - f.above), 0u);
-            total = f.above_mass + f.mass;
-        }
-        if (by_p && total > 0) {
-            if (by_k) cluster.sync();          // what the search before left has been read
-            const u64 target = (u64)((double)tp * (double)total);
-            if (cross(true, target + 1)) {     // (always: the target is less than the total)
-                const unsigned least = f.bin == cut_bin ? cut_key : 0u;
-                cut_bin = f.bin;
-                cut_key = refine(true, target + 1 - f.above_mass, least);
+                prefix = sh.found_key;
+                ++level;
+                break;
             }
         }
+        return from_key(prefix);
+    };
+    if (by_k) cut = threshold(false, [&](u64) { return (u64)k; });
+    if (by_p) {
+        if (by_k) cluster.sync();              // what the search before left has been read
+        // (the target is less than the sum, so that there is such a value)
+        cut = fmaxf(cut, threshold(true, [&](u64 total) { return (u64)((double)tp * (double)total) + 1; }));
     }
     // ---- the draw: masses of the kept tokens in index order; a warp owns a contiguous part of the slice ----
     const u64 floor_mass = greedy ? 0 : (u64)((double)fminf(fmaxf(mp, 0.f), 1.f) * (double)SMP_FIX);
     auto kept_mass = [&](float s) -> u64 {
-        const int b = bin_of(s);
-        if (b > cut_bin || (b == cut_bin && order_key(s) < cut_key)) return 0;
+        if (!(s >= cut)) return 0;
         const u64 q = mass_of(s);
         return q >= floor_mass ? q : 0;
     };
-    const int span = (n + SMP_WARPS - 1) / SMP_WARPS, from = warp * span, to = min(n, from + span);
-    u64 sum = 0;
-    for (int i = from + lane; i < to; i += 32) sum += kept_mass(value(i));
+    constexpr int GROUP = 128;                 // neighbouring values that a warp takes at once, four a lane
+    const int span = (n + SMP_WARPS * GROUP - 1) / (SMP_WARPS * GROUP) * GROUP, from = min(n, warp * span), to = min(n, from + span);
+    auto four = [&](int i, u64 (&q)[4]) {      // the masses of values i .. i + 3, and their sum
+        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (i + 4 <= held) v = *reinterpret_cast<const float4*>(s_val + i);
+        else
+            for (int j = 0; j < 4; ++j)
+                if (i + j < n) (&v.x)[j] = value(i + j);
+        q[0] = kept_mass(v.x); q[1] = kept_mass(v.y); q[2] = kept_mass(v.z); q[3] = kept_mass(v.w);
+        return q[0] + q[1] + q[2] + q[3];
+    };
+    u64 sum = 0, q[4];
+    for (int i = from + 4 * lane; i < to; i += GROUP) sum += four(i, q);
     sum = warp_sum_u64(sum);
     __syncthreads();
     if (lane == 0) sh.warp_sum[warp] = sum;
     __syncthreads();
-    if (tid == 0) {
-        u64 t = 0;
-        for (int w = 0; w < SMP_WARPS; ++w) t += sh.warp_sum[w];
-        sh.all_mass = t;
+    if (warp == 0) {
+        const u64 t = warp_sum_u64(lane < SMP_WARPS ? sh.warp_sum[lane] : 0);
+        if (lane == 0) sh.all_mass = t;
     }
     cluster.sync();
-    u64 total = 0, before = 0;
-    for (int c = 0; c < C; ++c) {
-        const u64 t = cluster.map_shared_rank(&sh, c)->all_mass;
-        if (c < rank) before += t;
-        total += t;
-    }
+    u64 total, before;
+    cluster_sums(lane < C ? peer->all_mass : 0, &total, &before);
+    before = __shfl_sync(0xffffffffu, before, rank);
     if (greedy) {                              // log-softmax of the row at the argmax: exp(0) / sum
         if (rank == 0 && tid == 0) finish(arg, -logf((float)((double)total / (double)SMP_FIX)));
         cluster.sync();
@@ -362,20 +405,29 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
     }
     u64 target = (u64)((double)(uniform ? uniform[r] : 0.f) * (double)total);
     if (target >= total) target = total - 1;
-    for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
+    before += warp_sum_u64(lane < warp ? sh.warp_sum[lane] : 0);
     if (target >= before && target - before < sum) {                    // (warp-uniform) the drawn token is this warp's
         u64 run = before;
-        for (int base = from; base < to; base += 32) {
-            const u64 q = base + lane < to ? kept_mass(value(base + lane)) : 0;
-            u64 inc = q;                       // inclusive scan over the warp
+        for (int base = from; base < to; base += GROUP) {
+            const u64 mine = base + 4 * lane < to ? four(base + 4 * lane, q) : 0;
+            u64 inc = mine;                    // inclusive scan over the warp
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const u64 x = __shfl_up_sync(0xffffffffu, inc, o);
                 if (lane >= o) inc += x;
             }
-            const unsigned hits = __ballot_sync(0xffffffffu, q > 0 && run + inc > target);
+            const unsigned hits = __ballot_sync(0xffffffffu, mine > 0 && run + inc > target);
             if (hits) {
-                if (lane == __ffs(hits) - 1) finish(first + base + lane, logf((float)((double)q / (double)total)));
+                if (lane == __ffs(hits) - 1) {
+                    u64 upto = run + inc - mine;
+                    for (int j = 0; j < 4; ++j) {
+                        upto += q[j];
+                        if (q[j] > 0 && upto > target) {
+                            finish(first + base + 4 * lane + j, logf((float)((double)q[j] / (double)total)));
+                            break;
+                        }
+                    }
+                }
                 break;
             }
             run += __shfl_sync(0xffffffffu, inc, 31);
