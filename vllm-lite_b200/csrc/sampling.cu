@@ -40,6 +40,9 @@ namespace cg = cooperative_groups;
 #define SMP_CLUSTER 8
 #define SMP_LIST 2048            /* values of one bin that a block brings together */
 #define SMP_OWN 512              /* ... of them its own */
+#define SMP_COARSE 32            /* bins of the first look at a row, half a unit each: what lies 15.5 and more below the maximum is in none */
+#define SMP_RANKED 256           /* most of those tokens that are compared each with each */
+#define SMP_FEW 3072             /* most tokens that one block finishes a row with */
 
 typedef unsigned long long u64;
 
@@ -99,11 +102,14 @@ struct SampleShared {
     union {                                 // (the bins are at rest when values are brought together)
         struct { u64 mass[SMP_BINS]; unsigned count[SMP_BINS]; };
         unsigned list[SMP_LIST];
+        unsigned coarse[SMP_COARSE * 32];   // a column a lane, so that a warp's additions meet nowhere
+        uint2 near[SMP_FEW];                // this block's tokens that may be kept: key, place in the row
     };
+    unsigned coarse_count[SMP_COARSE], row_count[SMP_COARSE];
     unsigned own[SMP_OWN], own_count;       // this block's values of a bin, by their keys
     u64 fine_mass[2][256];                  // two levels of the search in a bin in turn: one is read by the cluster while the other is filled
     unsigned fine_count[2][256];
-    u64 warp_sum[SMP_WARPS], all_mass, part_mass;      // part: of this block's share of the bins
+    u64 warp_sum[SMP_WARPS], all_mass, part_mass, near_mass;       // part: of this block, of its share of the bins; near: of its tokens that may be kept
     ArgBest warp_best[SMP_WARPS], best;
     int found_bin, found_digit;
     u64 found_value, found_before;
@@ -144,7 +150,7 @@ __device__ __forceinline__ void cluster_sums(u64 x, u64* total, u64* before) {
 }
 
 __global__ void __launch_bounds__(SMP_THREADS)
-sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int slice, int held,
+sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int slice, int held, int room,
               const float* __restrict__ temperature, const int* __restrict__ top_k,
               const float* __restrict__ top_p, const float* __restrict__ min_p, const float* __restrict__ uniform,
               int* __restrict__ out_token, float* __restrict__ out_logprob) {
@@ -169,13 +175,14 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
         if (i < held) s_val[i] = clean(x, inv_t);
     };
     const int n4 = ((uintptr_t)l & 15) == 0 ? (n & ~3) : 0;
-    for (int i0 = 4 * tid; i0 < n4; i0 += 16 * SMP_THREADS) {           // 16 bytes a load, four on their way
-        float4 q[4];
+    constexpr int LOADS = 8;                                            // 16 bytes each, on their way together
+    for (int i0 = 4 * tid; i0 < n4; i0 += LOADS * 4 * SMP_THREADS) {
+        float4 q[LOADS];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < LOADS; ++u)
             if (i0 + u * 4 * SMP_THREADS < n4) q[u] = *reinterpret_cast<const float4*>(l + i0 + u * 4 * SMP_THREADS);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < LOADS; ++u) {
             const int i = i0 + u * 4 * SMP_THREADS;
             if (i < n4) { take(i, q[u].x); take(i + 1, q[u].y); take(i + 2, q[u].z); take(i + 3, q[u].w); }
         }
@@ -227,24 +234,217 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
         return;
     }
 
-    // every value of the slice, in no order; shared memory holds a multiple of four, filled up with values without mass
+    // every value of the slice and its place in it, in no order; shared memory holds a multiple of four, filled up with values without mass
     auto each = [&](auto f) {
         for (int i = 4 * tid; i < held; i += 4 * SMP_THREADS) {
             const float4 v = *reinterpret_cast<const float4*>(s_val + i);
-            f(v.x); f(v.y); f(v.z); f(v.w);
+            f(v.x, i); f(v.y, i + 1); f(v.z, i + 2); f(v.w, i + 3);
         }
-        for (int i = held + tid; i < n; i += SMP_THREADS) f(clean(l[i], inv_t));
+        for (int i = held + tid; i < n; i += SMP_THREADS) f(clean(l[i], inv_t), i);
+    };
+    int level = 0;
+    // Of `all` weighted keys: the key with which the sum of weights, from the largest key on, reaches `left`; this block alone.
+    auto search = [&](unsigned all, auto key_of, auto weight_of, u64 left) -> unsigned {
+        unsigned prefix = 0;
+        for (int shift = 24; shift >= 0; shift -= 8, ++level) {
+            u64* fm = sh.fine_mass[level & 1];
+            unsigned* fc = sh.fine_count[level & 1];
+            if (tid < 256) { fm[tid] = 0; fc[tid] = 0; }
+            if (tid == 0) sh.found_key = 0xffffffffu;
+            __syncthreads();
+            const unsigned himask = shift == 24 ? 0u : (0xffffffffu << (shift + 8));
+            for (unsigned i = tid; i < all; i += SMP_THREADS) {
+                const unsigned key = key_of(i);
+                if ((key & himask) != prefix) continue;
+                const u64 q = weight_of(i);
+                if (!q) continue;
+                const unsigned d = 255u - ((key >> shift) & 255u);
+                atomicAdd(&fc[d], 1u);
+                add_mass(&fm[d], q);
+            }
+            __syncthreads();
+            const u64 x = tid < 256 ? fm[tid] : 0, upto = block_scan_u64(x, sh.warp_sum);
+            if (tid < 256 && upto >= left && upto - x < left) { sh.found_digit = 255 - tid; sh.found_before = upto - x; sh.found_count = fc[tid]; }
+            __syncthreads();
+            prefix |= (unsigned)sh.found_digit << shift;
+            left -= sh.found_before;
+            const bool one = sh.found_count == 1;
+            __syncthreads();
+            if (one && shift > 0) {            // the only one left
+                for (unsigned i = tid; i < all; i += SMP_THREADS) {
+                    const unsigned key = key_of(i);
+                    if (key >> shift == prefix >> shift && weight_of(i)) sh.found_key = key;
+                }
+                __syncthreads();
+                prefix = sh.found_key;
+                ++level;
+                break;
+            }
+        }
+        return prefix;
     };
     float cut = -INFINITY;                     // a token is kept by top-k and top-p if its value is at least this
-    const bool by_k = !greedy && k > 0 && k < V, by_p = !greedy && tp < 1.f;
-    int level = 0;
+    const bool by_k = !greedy && k > 0 && k < V, by_p = !greedy && tp < 1.f, by_m = !greedy && mp > 0.f;
+    const u64 floor_mass = by_m ? (u64)((double)fminf(mp, 1.f) * (double)SMP_FIX) : 0;
+    const float u_draw = uniform ? uniform[r] : 0.f;
+
+    // ---- a row of which few tokens can be kept: those are brought together, and one block finishes ----
+    if (by_k || by_p || by_m) {
+        const bool weigh = by_p && !by_k;      // top-p's sum runs over the whole row
+        for (int i = tid; i < SMP_COARSE * 32; i += SMP_THREADS) sh.coarse[i] = 0;
+        if (tid == 0) { sh.part_mass = 0; sh.near_mass = 0; sh.own_count = 0; }
+        __syncthreads();
+        auto coarse_of = [&](float s) {        // a bin of half a unit of the distance; SMP_COARSE for one that lies far off
+            const float d = row_max - s;
+            return d < (SMP_COARSE - 1) / 2.f ? (int)(__float_as_uint(fmaf(d, 2.f, 8388608.f)) & (SMP_COARSE - 1)) : SMP_COARSE;
+        };
+        u64 mine = 0;
+        each([&](float s, int) {
+            const int b = coarse_of(s);
+            if (b < SMP_COARSE) atomicAdd(&sh.coarse[b * 32 + lane], 1u);
+            if (weigh) mine += mass_of(s);
+        });
+        if (weigh) {
+            mine = warp_sum_u64(mine);
+            if (lane == 0) atomicAdd(&sh.part_mass, mine);
+        }
+        __syncthreads();
+        for (int b = warp; b < SMP_COARSE; b += SMP_WARPS) {
+            const unsigned c = __reduce_add_sync(0xffffffffu, sh.coarse[b * 32 + lane]);
+            if (lane == 0) sh.coarse_count[b] = c;
+        }
+        cluster.sync();
+        static_assert(SMP_COARSE * SMP_CLUSTER <= SMP_THREADS, "a thread a bin and block");
+        if (tid < SMP_COARSE * SMP_CLUSTER) {
+            const int b = tid / SMP_CLUSTER, other = tid % SMP_CLUSTER;
+            unsigned c = other < C ? cluster.map_shared_rank(&sh, other)->coarse_count[b] : 0;
+#pragma unroll
+            for (int o = 1; o < SMP_CLUSTER; o <<= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+            if (other == 0) sh.row_count[b] = c;
+        }
+        u64 row_mass, unused;
+        cluster_sums(weigh && lane < C ? peer->part_mass : 0, &row_mass, &unused);
+        __syncthreads();
+        // the last bin that can hold a kept token: exactly for top-k, by its bins' middles and two more for top-p (checked below), by the bound for min-p
+        unsigned upto = sh.row_count[lane];
+        float guess = upto * __expf(-0.5f * lane);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
+            const float y = __shfl_up_sync(0xffffffffu, guess, o);
+            if (lane >= o) { upto += x; guess += y; }
+        }
+        unsigned reach = 0;
+        if (by_k) reach = __ballot_sync(0xffffffffu, upto >= (unsigned)k);
+        else if (by_p) reach = __ballot_sync(0xffffffffu, guess >= tp * __shfl_sync(0xffffffffu, guess, 31)) << 2;
+        else reach = 1u << (int)fminf(-2.f * logf(mp) + 2.f, 31.f);
+        const int last = __ffs(reach) - 1;     // (-1: none)
+        const unsigned count = last >= 0 && last < SMP_COARSE - 1 ? __shfl_sync(0xffffffffu, upto, max(last, 0)) : SMP_FEW + 1;
+        if (count <= SMP_FEW && count <= (unsigned)room) {
+            u64 near = 0;
+            each([&](float s, int i) {
+                if (coarse_of(s) <= last) {
+                    sh.near[atomicAdd(&sh.own_count, 1u)] = make_uint2(order_key(s), (unsigned)(first + i));
+                    if (weigh) near += mass_of(s);
+                }
+            });
+            if (weigh) {
+                near = warp_sum_u64(near);
+                if (lane == 0) atomicAdd(&sh.near_mass, near);
+            }
+            cluster.sync();
+            u64 near_mass, all, place;
+            cluster_sums(weigh && lane < C ? peer->near_mass : 0, &near_mass, &unused);
+            const u64 target = (u64)((double)tp * (double)row_mass);
+            if (!weigh || near_mass > target) {
+                const unsigned found = lane < C ? peer->own_count : 0;
+                cluster_sums(found, &all, &place);
+                unsigned* const keys = reinterpret_cast<unsigned*>(s_val);         // the slice is at rest: its room holds keys, places and masses
+                unsigned* const places = keys + room;
+                u64* const weights = reinterpret_cast<u64*>(places + room);
+                if (rank == 0) {
+                    unsigned begin[SMP_CLUSTER];
+#pragma unroll
+                    for (int b = 0; b < SMP_CLUSTER; ++b) begin[b] = (unsigned)__shfl_sync(0xffffffffu, place, b);
+                    for (unsigned i = tid; i < (unsigned)all; i += SMP_THREADS) {
+                        int b = 0;
+                        unsigned at = 0;
+#pragma unroll
+                        for (int o = 1; o < SMP_CLUSTER; ++o)
+                            if (i >= begin[o] && o < C) { b = o; at = begin[o]; }
+                        const uint2 x = cluster.map_shared_rank(&sh, b)->near[i - at];
+                        keys[i] = x.x;
+                        places[i] = x.y;
+                        weights[i] = mass_of(from_key(x.x));
+                    }
+                }
+                cluster.sync();                // nobody leaves while others read its shared memory
+                if (rank != 0) return;
+                const unsigned L = (unsigned)all;
+                auto sum_of = [&](auto weight_of) -> u64 {
+                    u64 t = 0;
+                    for (unsigned i = tid; i < L; i += SMP_THREADS) t += weight_of(i);
+                    t = warp_sum_u64(t);
+                    __syncthreads();
+                    if (lane == 0) sh.warp_sum[warp] = t;
+                    __syncthreads();
+                    return warp_sum_u64(lane < SMP_WARPS ? sh.warp_sum[lane] : 0);
+                };
+                if (L <= SMP_RANKED) {         // few enough to be compared each with each: a thread a token
+                    const unsigned key = tid < L ? keys[tid] : 0, mine_at = tid < L ? places[tid] : 0;
+                    u64 w = tid < L ? weights[tid] : 0, above = 0;
+                    unsigned greater = 0;
+                    if (tid < (int)L)
+                        for (unsigned i = 0; i < L; ++i)
+                            if (keys[i] > key) { ++greater; above += weights[i]; }
+                    if (by_k && greater >= (unsigned)k) w = 0;                     // (ties at the threshold stay)
+                    auto sum = [&](u64 x) -> u64 {
+                        x = warp_sum_u64(x);
+                        __syncthreads();
+                        if (lane == 0) sh.warp_sum[warp] = x;
+                        __syncthreads();
+                        return warp_sum_u64(lane < SMP_WARPS ? sh.warp_sum[lane] : 0);
+                    };
+                    if (by_p && above > (by_k ? (u64)((double)tp * (double)sum(w)) : target)) w = 0;
+                    if (w < floor_mass) w = 0;
+                    const u64 kept = sum(w);
+                    if (tid < L) weights[tid] = w;
+                    __syncthreads();
+                    u64 goal = (u64)((double)u_draw * (double)kept), before = 0;
+                    if (goal >= kept) goal = kept - 1;
+                    if (tid < (int)L)
+                        for (unsigned i = 0; i < L; ++i)
+                            if (places[i] < mine_at) before += weights[i];
+                    if (w && before <= goal && goal - before < w) finish((int)mine_at, logf((float)((double)w / (double)kept)));
+                    return;
+                }
+                auto key_of = [&](unsigned i) { return keys[i]; };
+                unsigned least = 0;            // the threshold's key
+                if (by_k) least = search(L, key_of, [&](unsigned) -> u64 { return 1; }, (u64)k);
+                if (by_p) {
+                    auto weight_of = [&](unsigned i) { return keys[i] >= least ? weights[i] : 0; };
+                    const u64 goal = (by_k ? (u64)((double)tp * (double)sum_of(weight_of)) : target) + 1;
+                    least = max(least, search(L, key_of, weight_of, goal));
+                }
+                auto kept_of = [&](unsigned i) { return keys[i] >= least && weights[i] >= floor_mass ? weights[i] : 0; };
+                const u64 kept = sum_of(kept_of);
+                u64 goal = (u64)((double)u_draw * (double)kept);
+                if (goal >= kept) goal = kept - 1;
+                const unsigned token = ~search(L, [&](unsigned i) { return ~places[i]; }, kept_of, goal + 1);
+                for (unsigned i = tid; i < L; i += SMP_THREADS)
+                    if (places[i] == token) finish((int)token, logf((float)((double)weights[i] / (double)kept)));
+                return;
+            }
+        }
+        cluster.sync();                        // what was read of others has been read
+    }
 
     // The value with which the sum, from the largest values on, of counts (masses) of all values from `cut` on reaches goal(their sum); -inf if all together do not.
     auto threshold = [&](bool masses, auto goal_of) -> float {
         for (int i = tid; i < SMP_BINS; i += SMP_THREADS) { sh.count[i] = 0; sh.mass[i] = 0; }
         if (tid == 0) { sh.part_mass = 0; sh.own_count = 0; }
         __syncthreads();
-        each([&](float s) {
+        each([&](float s, int) {
             const int b = bin_of(s);
             if (b >= SMP_BINS || s < cut) return;
             if (!masses) atomicAdd(&sh.count[b], 1u);
@@ -295,7 +495,7 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
         u64 left = goal - o->found_value;
 
         // the bin's values, each block's own first
-        each([&](float s) {
+        each([&](float s, int) {
             if (bin_of(s) == bin && s >= cut) {
                 const unsigned at = atomicAdd(&sh.own_count, 1u);
                 if (at < SMP_OWN) sh.own[at] = order_key(s);
@@ -313,50 +513,31 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
                 for (unsigned i = tid; i < c; i += SMP_THREADS) sh.list[at + i] = cluster.map_shared_rank(&sh, b < C ? b : rank)->own[i];
             }
         }
+        if (few) {
+            __syncthreads();
+            return from_key(search((unsigned)all, [&](unsigned i) { return sh.list[i]; }, [&](unsigned i) -> u64 { return masses ? mass_of(from_key(sh.list[i])) : 1; },
+                                   left));
+        }
         unsigned prefix = 0;
         for (int shift = 24; shift >= 0; shift -= 8, ++level) {
             u64* fm = sh.fine_mass[level & 1];
-            if (tid < 256) { fm[tid] = 0; sh.fine_count[level & 1][tid] = 0; }
+            if (tid < 256) fm[tid] = 0;
             __syncthreads();
             const unsigned himask = shift == 24 ? 0u : (0xffffffffu << (shift + 8));
-            auto sort = [&](unsigned key) {
-                if ((key & himask) != prefix) return;
-                const unsigned d = 255u - ((key >> shift) & 255u);
-                atomicAdd(&sh.fine_count[level & 1][d], 1u);
-                if (masses) add_mass(&fm[d], mass_of(from_key(key)));
-            };
-            if (few) {
-                for (unsigned i = tid; i < all; i += SMP_THREADS) sort(sh.list[i]);
-                __syncthreads();
-            } else {
-                each([&](float s) { if (bin_of(s) == bin && s >= cut) sort(order_key(s)); });
-                cluster.sync();
-            }
+            each([&](float s, int) {
+                const unsigned key = order_key(s);
+                if (bin_of(s) == bin && s >= cut && (key & himask) == prefix) add_mass(&fm[255u - ((key >> shift) & 255u)], masses ? mass_of(s) : 1);
+            });
+            cluster.sync();
             u64 x = 0;                         // every block finds the same digit for itself
-            unsigned c = 0;
             if (tid < 256)
-                for (int b = few ? rank : 0; b < (few ? rank + 1 : C); ++b) {
-                    const SampleShared* other = cluster.map_shared_rank(&sh, b);
-                    c += other->fine_count[level & 1][tid];
-                    x += masses ? other->fine_mass[level & 1][tid] : (u64)other->fine_count[level & 1][tid];
-                }
+                for (int b = 0; b < C; ++b) x += cluster.map_shared_rank(&sh, b)->fine_mass[level & 1][tid];
             const u64 upto = block_scan_u64(x, sh.warp_sum);
-            if (tid < 256 && upto >= left && upto - x < left) { sh.found_digit = 255 - tid; sh.found_before = upto - x; sh.found_count = c; }
+            if (tid < 256 && upto >= left && upto - x < left) { sh.found_digit = 255 - tid; sh.found_before = upto - x; }
             __syncthreads();
             prefix |= (unsigned)sh.found_digit << shift;
             left -= sh.found_before;
-            const bool whole = few && (sh.found_count == 1 || (!masses && left == sh.found_count));
             __syncthreads();
-            if (whole && shift > 0) {          // all of them are kept: the least of them is the threshold
-                if (tid == 0) sh.found_key = 0xffffffffu;
-                __syncthreads();
-                for (unsigned i = tid; i < all; i += SMP_THREADS)
-                    if (sh.list[i] >> shift == prefix >> shift) atomicMin(&sh.found_key, sh.list[i]);
-                __syncthreads();
-                prefix = sh.found_key;
-                ++level;
-                break;
-            }
         }
         return from_key(prefix);
     };
@@ -367,7 +548,6 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
         cut = fmaxf(cut, threshold(true, [&](u64 total) { return (u64)((double)tp * (double)total) + 1; }));
     }
     // ---- the draw: masses of the kept tokens in index order; a warp owns a contiguous part of the slice ----
-    const u64 floor_mass = greedy ? 0 : (u64)((double)fminf(fmaxf(mp, 0.f), 1.f) * (double)SMP_FIX);
     auto kept_mass = [&](float s) -> u64 {
         if (!(s >= cut)) return 0;
         const u64 q = mass_of(s);
@@ -403,7 +583,7 @@ sample_kernel(const float* __restrict__ logits, long long row_stride, int V, int
         cluster.sync();
         return;
     }
-    u64 target = (u64)((double)(uniform ? uniform[r] : 0.f) * (double)total);
+    u64 target = (u64)((double)u_draw * (double)total);
     if (target >= total) target = total - 1;
     before += warp_sum_u64(lane < warp ? sh.warp_sum[lane] : 0);
     if (target >= before && target - before < sum) {                    // (warp-uniform) the drawn token is this warp's
@@ -464,7 +644,9 @@ extern "C" int vl_sample(const float* logits, long long row_stride, int R, int V
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(R * C));
     cfg.blockDim = dim3(SMP_THREADS);
-    cfg.dynamicSmemBytes = (size_t)held * 4;
+    // room for the tokens that a block finishes a row with: 16 bytes each, a multiple of 2 of them
+    const int few = (V < SMP_FEW ? V : SMP_FEW) + 1 & ~1, bytes = held * 4 > few * 16 ? held * 4 : few * 16;
+    cfg.dynamicSmemBytes = (size_t)bytes;
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -472,6 +654,6 @@ extern "C" int vl_sample(const float* logits, long long row_stride, int R, int V
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, sample_kernel, logits, row_stride, V, slice, held, temperature, top_k, top_p, min_p, uniform, out_token,
+    return (int)cudaLaunchKernelEx(&cfg, sample_kernel, logits, row_stride, V, slice, held, few, temperature, top_k, top_p, min_p, uniform, out_token,
                                    out_logprob);
 }
