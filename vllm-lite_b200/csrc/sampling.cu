@@ -42,7 +42,7 @@ namespace cg = cooperative_groups;
 #define SMP_OWN 512              /* ... of them its own */
 #define SMP_COARSE 32            /* bins of the first look at a row, half a unit each: what lies 15.5 and more below the maximum is in none */
 #define SMP_RANKED 256           /* most of those tokens that are compared each with each */
-#define SMP_FEW 3072             /* most tokens that one block finishes a row with */
+#define SMP_FEW 3000             /* most tokens that one block finishes a row with */
 
 typedef unsigned long long u64;
 
