@@ -10,7 +10,7 @@
 //   warps 0..3 (and 4..7), a thread per row   read the scores of a key tile from TMEM, keep the running maximum and sum of their row, write
 //        P as halves into shared memory (128-byte swizzled rows) and, when a row's maximum has grown by more than 2^8, rescale the row's output in
 //        TMEM.  While one query tile's rows are exponentiated the tensor cores work on the other's products;
-//   four warps           bring keys and values: 16 bytes a load into registers, one tile ahead, e4m3 to halves (exact), times a power of two, into two
+//   four warps each      bring keys and values: 16 bytes a load into registers, one tile ahead, e4m3 to halves (exact), times a power of two, into two
 //        stages of 128-byte swizzled rows each for keys and values.  The pages' scales are folded in here: page by page 2^(e - E + 7), E the largest
 //        exponent of all pages that the block reads (found first; 448 * 2^7 is below the largest half), so that scores and outputs of all tiles are in one
 //        unit, which a row's own factor and the end undo.  Exact down to pages 2^15 below the largest, to within 2^-41 of the largest number else.
@@ -34,15 +34,15 @@ constexpr int HD = FA_HD;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head sizes in steps of 16 up to 256");
 constexpr int GROUPS = HD <= 128 ? 2 : 1;              // query tiles of 128 rows
 constexpr int BM = 128, BN = 64, CB = (HD + 63) / 64;  // CB: blocks of 64 columns (one swizzled row) a head
-constexpr int SOFT = 4 * GROUPS, QK_WARP = SOFT, PV_WARP = SOFT + 1, LOAD0 = SOFT + 2, LOADERS = 4;
-constexpr int NTHREADS = 32 * (LOAD0 + LOADERS), LOAD_THREADS = 32 * LOADERS;
+constexpr int SOFT = 4 * GROUPS, QK_WARP = SOFT, PV_WARP = SOFT + 1, LOAD0 = SOFT + 2, LOADERS = 4;   // (loaders of keys, and as many of values)
+constexpr int NTHREADS = 32 * (LOAD0 + 2 * LOADERS), LOAD_THREADS = 32 * LOADERS;
 constexpr unsigned ROW_BYTES = 128;
 constexpr unsigned Q_BYTES = BM * CB * ROW_BYTES;      // CB blocks of [128 rows][128 bytes]
 constexpr unsigned KV_STAGE = BN * CB * ROW_BYTES;     // CB blocks of [64 rows][128 bytes]
 constexpr unsigned P_BYTES = BM * ROW_BYTES;
 constexpr unsigned TILE_BYTES = GROUPS * (Q_BYTES + P_BYTES) + 4 * KV_STAGE;
 constexpr int FOUND = 4;                               // key tiles whose rows are looked up at a time
-constexpr unsigned SMEM_BYTES = TILE_BYTES + 512 + GROUPS * BM * 4 + FOUND * BN * 12;
+constexpr unsigned SMEM_BYTES = TILE_BYTES + 512 + GROUPS * BM * 4 + 2 * FOUND * BN * 8;
 constexpr unsigned TMEM_COLS = 512;                    // scores 2 x 64 a query tile, behind them the outputs
 constexpr unsigned O_COL = GROUPS * 2 * BN;
 constexpr int PIECES = HD / 16, EACH = (BN * PIECES + LOAD_THREADS - 1) / LOAD_THREADS;   // 16-byte pieces of a row, of a tile a thread
@@ -97,10 +97,10 @@ __device__ __forceinline__ unsigned times(unsigned h2, unsigned f2) {
     return *reinterpret_cast<const unsigned*>(&r);
 }
 // A barrier of the loading warps, and whether all of them still have what they waited for: one whose wait ran out takes the others along.
-__device__ __forceinline__ bool loaders_agree(bool ok) {
+__device__ __forceinline__ bool loaders_agree(bool ok, int barrier) {
     int all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-                 : "=r"(all) : "r"((int)ok), "n"(LOAD_THREADS) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all) : "r"((int)ok), "r"(barrier), "n"(LOAD_THREADS) : "memory");
     return all != 0;
 }
 }  // namespace
@@ -123,9 +123,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     int* words = reinterpret_cast<int*>(bars + 21);
     int &failed = words[0], &top_k = words[1], &top_v = words[2];
     float* s_row_scale = reinterpret_cast<float*>(smem + TILE_BYTES + 512);                      // [GROUPS * BM]
-    int* s_krow = reinterpret_cast<int*>(s_row_scale + GROUPS * BM);                             // [FOUND][BN] cache rows, -1: zeros
-    int* s_vrow = s_krow + FOUND * BN;
-    unsigned* s_fold = reinterpret_cast<unsigned*>(s_vrow + FOUND * BN);                         // factor of the key (low half) and of the value
+    int2* s_found = reinterpret_cast<int2*>(s_row_scale + GROUPS * BM);                          // keys, values: [FOUND][BN] cache row (-1: zeros) and factor
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (smem_u32(smem) & 1023u) {                                        // (uniform) never expected; the tiles would be misread
         if (tid == 0 && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_FLASH_8BIT);
@@ -211,49 +209,56 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
 
     const int role = warp_number();
     if (role >= LOAD0) {                                                 // ---- keys and values ----
-        const int ct = tid - LOAD0 * 32;
-        const int EK = top_k, EV = top_v;
-        // Thread k < 64 looks up key k of every tile, in three steps one tile apart, so that no load is waited for: the page, its scales, and what they say.
+        const bool values = role >= LOAD0 + LOADERS;
+        const int ct = (tid - LOAD0 * 32) % LOAD_THREADS, E = values ? top_v : top_k, barrier = 1 + (int)values;
+        const unsigned char* cache = values ? vcache : kcache;
+        unsigned char* stages = values ? Vs : Ks;
+        unsigned long long *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
+        int2* found = s_found + (values ? FOUND * BN : 0);
+        // Thread k < 64 looks up key k of every tile, in three steps a tile apart, so that no load is waited for: the page, its scales, and what they say.
         struct Found { int page, at; float ks, vs; };
         auto page_of = [&](int it) -> Found {
-            Found f = {-1, 0, 0.f, 0.f};
+            Found f = {-1, -1, 0.f, 0.f};
             const int key = (jt0 + it) * BN + ct;
             if (ct >= BN || it >= n_tiles || key < lo || key > hi) return f;
             const int blk = key / page_size;
             f.at = key - blk * page_size;
-            f.page = blk < max_blocks ? table[blk] : -1;
-            if (f.page < 0 || f.page >= num_pages) { f.page = -1; if (err) atomicOr(err, VL_DEV_BAD_PAGE); }
+            if (blk < max_blocks) f.page = table[blk];
             return f;
         };
         auto scales_of = [&](Found& f) {
-            if (f.page >= 0) { f.ks = kscale[(size_t)f.page * nkv + kvh]; f.vs = vscale[(size_t)f.page * nkv + kvh]; }
+            if (f.at < 0) return;
+            if (f.page < 0 || f.page >= num_pages) {
+                f.page = -1;
+                if (err) atomicOr(err, VL_DEV_BAD_PAGE);
+                return;
+            }
+            f.ks = kscale[(size_t)f.page * nkv + kvh];
+            f.vs = vscale[(size_t)f.page * nkv + kvh];
         };
         auto note = [&](const Found& f, int it) {
             if (ct >= BN) return;
-            const int at = (it % FOUND) * BN + ct, row = f.page < 0 ? -1 : (f.page * nkv + kvh) * page_size + f.at;
-            const bool none = f.ks != f.ks || f.vs != f.vs;
-            s_krow[at] = row;
-            s_vrow[at] = f.vs != f.vs ? -1 : row;
-            const __half fk = none ? __ushort_as_half(0x7e00) : __float2half_rn(f.ks * power_of_two(FOLD - EK)), fv = __float2half_rn(f.vs != f.vs ? 0.f : f.vs * power_of_two(FOLD - EV));
-            s_fold[at] = (unsigned)__half_as_ushort(fk) | ((unsigned)__half_as_ushort(fv) << 16);
+            const bool no_value = f.vs != f.vs, none = f.ks != f.ks || no_value;
+            const __half factor = values ? __float2half_rn(no_value ? 0.f : f.vs * power_of_two(FOLD - E))
+                                         : (none ? __ushort_as_half(0x7e00) : __float2half_rn(f.ks * power_of_two(FOLD - E)));
+            found[(it % FOUND) * BN + ct] = make_int2(f.page < 0 || (values && no_value) ? -1 : (f.page * nkv + kvh) * page_size + f.at,
+                                                      (int)(0x10001u * __half_as_ushort(factor)));
         };
-        auto load = [&](uint4 (&x)[EACH], bool v, int it) {
-            const int* rows = (v ? s_vrow : s_krow) + (it % FOUND) * BN;
-            const unsigned char* cache = v ? vcache : kcache;
+        auto load = [&](uint4 (&x)[EACH], int it) {
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
-                const int row = idx < BN * PIECES ? rows[r] : -1;
+                const int row = idx < BN * PIECES ? found[(it % FOUND) * BN + r].x : -1;
                 x[i] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(cache + (size_t)row * HD + c * 16)) : make_uint4(0u, 0u, 0u, 0u);
             }
         };
-        auto store = [&](const uint4 (&x)[EACH], bool v, int it) {
-            unsigned char* st = (v ? Vs : Ks) + (unsigned)(it & 1) * KV_STAGE;
+        auto store = [&](const uint4 (&x)[EACH], int it) {
+            unsigned char* st = stages + (unsigned)(it & 1) * KV_STAGE;
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
                 if (idx >= BN * PIECES) continue;
-                const unsigned both = s_fold[(it % FOUND) * BN + r], f = v ? __byte_perm(both, both, 0x3232) : __byte_perm(both, both, 0x1010);
+                const unsigned f = (unsigned)found[(it % FOUND) * BN + r].y;
                 const unsigned* w = &x[i].x;
                 uint4 a, b;
                 a.x = times(half2_low(w[0]), f); a.y = times(half2_high(w[0]), f); a.z = times(half2_low(w[1]), f); a.w = times(half2_high(w[1]), f);
@@ -264,36 +269,28 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                 *reinterpret_cast<uint4*>(blk + swizzled(r, ch + 1)) = b;
             }
         };
-        Found f0 = page_of(0), f1 = page_of(1), f2 = page_of(2);
+        Found f0 = page_of(0), f1 = page_of(1), f2 = page_of(2), f3 = page_of(3);
         scales_of(f0);
         scales_of(f1);
+        scales_of(f2);
         note(f0, 0);
         note(f1, 1);
-        bool ok = loaders_agree(true);
-        uint4 xk[EACH], xv[EACH];
-        load(xk, false, 0);
-        // keys run one tile ahead of values: the scores of tile i + 1 are issued before the second product of tile i
-        for (int step = 0; step <= n_tiles; ++step) {
-            scales_of(f2);                                               // of tile step + 2
-            const Found f3 = page_of(step + 3);
-            if (step < n_tiles && step >= 2) ok = warp_wait(&k_empty[step & 1], (unsigned)((step / 2 - 1) & 1));
-            if (step < n_tiles && ok) {
-                store(xk, false, step);
-                fence_proxy_async_smem();
-                mbar_arrive(&k_full[step & 1]);
-                if (step + 1 < n_tiles) load(xk, false, step + 1);
-            }
-            const int it = step - 1;
-            if (it >= 2 && ok) ok = warp_wait(&v_empty[it & 1], (unsigned)((it / 2 - 1) & 1));
-            if (it >= 0 && ok) {
-                store(xv, true, it);
-                fence_proxy_async_smem();
-                mbar_arrive(&v_full[it & 1]);
-            }
-            if (step < n_tiles) load(xv, true, step);
-            note(f2, step + 2);
+        bool ok = loaders_agree(true, barrier);
+        uint4 x[EACH];
+        load(x, 0);
+        for (int it = 0; it < n_tiles; ++it) {
+            note(f2, it + 2);
             f2 = f3;
-            ok = loaders_agree(ok);
+            scales_of(f2);                                               // of tile it + 3
+            f3 = page_of(it + 4);
+            if (it >= 2) ok = warp_wait(&empty[it & 1], (unsigned)((it / 2 - 1) & 1));
+            if (ok) {
+                store(x, it);
+                fence_proxy_async_smem();
+                mbar_arrive(&full[it & 1]);
+                if (it + 1 < n_tiles) load(x, it + 1);
+            }
+            ok = loaders_agree(ok, barrier);
             if (!ok) break;
         }
         if (!ok && lane == 0) atomicExch(&failed, 1);
