@@ -8,15 +8,15 @@
 // (token, head) pairs, so a short portion fills a tile as a long one does and a tile's mask is as sharp as its few tokens.  It walks that request's
 // keys in tiles of 64, which both query tiles read.  Roles:
 //   warps 0..3 (and 4..7), a thread per row   read the scores of a key tile from TMEM, keep the running maximum and sum of their row, write
-//        P as halves into shared memory (128-byte swizzled rows) and, when a row's maximum has grown by more than 2^8, rescale the row's output in
-//        TMEM.  While one query tile's rows are exponentiated the tensor cores work on the other's products;
+//        P as halves into TMEM, where the scores were, and, when a row's maximum has grown by more than 2^8, rescale the row's output there.
+//        While one query tile's rows are exponentiated the tensor cores work on the other's products;
 //   four warps each      bring keys and values: 16 bytes a load into registers, one tile ahead, e4m3 to halves (exact), times a power of two, into two
 //        stages of 128-byte swizzled rows each for keys and values.  The pages' scales are folded in here: page by page 2^(e - E + 7), E the largest
 //        exponent of all pages that the block reads (found first; 448 * 2^7 is below the largest half), so that scores and outputs of all tiles are in one
 //        unit, which a row's own factor and the end undo.  Exact down to pages 2^15 below the largest, to within 2^-41 of the largest number else.
 //        Rows that no query of the block reads, or that the table does not hold (flagged), are zeros.  A page whose scale is not a number gives
 //        keys of NaN and values of zero: who may read it gets NaN, rows that may not replace the score;
-//   one warp             issues S = Q K^T (both K-major) into one of two score buffers a query tile, one issues O += P V (V as stored: N contiguous).
+//   one warp             issues S = Q K^T (both K-major) into one of two score buffers a query tile, one issues O += P V (P from TMEM, V as stored: N contiguous).
 // Roundings: queries times a power of two of their row (largest number in [2^14, 2^15)) and the probabilities, 2^7 p with p up to 2^8, are halves.
 // Every wait on an mbarrier is bounded; when one expires the block records VL_DEV_WAIT_EXPIRED, stops, and still frees its TMEM.
 #include "cache_8bit.cuh"
@@ -39,8 +39,8 @@ constexpr int NTHREADS = 32 * (LOAD0 + 2 * LOADERS), LOAD_THREADS = 32 * LOADERS
 constexpr unsigned ROW_BYTES = 128;
 constexpr unsigned Q_BYTES = BM * CB * ROW_BYTES;      // CB blocks of [128 rows][128 bytes]
 constexpr unsigned KV_STAGE = BN * CB * ROW_BYTES;     // CB blocks of [64 rows][128 bytes]
-constexpr unsigned P_BYTES = BM * ROW_BYTES;
-constexpr unsigned TILE_BYTES = GROUPS * (Q_BYTES + P_BYTES) + 4 * KV_STAGE;
+constexpr int STAGES = HD <= 128 ? 3 : 2;              // of keys, and of values
+constexpr unsigned TILE_BYTES = GROUPS * Q_BYTES + 2 * STAGES * KV_STAGE;
 constexpr int FOUND = 4;                               // key tiles whose rows are looked up at a time
 constexpr unsigned SMEM_BYTES = TILE_BYTES + 512 + GROUPS * BM * 4 + 2 * FOUND * BN * 8;
 constexpr unsigned TMEM_COLS = 512;                    // scores 2 x 64 a query tile, behind them the outputs
@@ -90,6 +90,14 @@ __device__ __forceinline__ void mma_lo(unsigned tmem_c, unsigned a_lo, unsigned 
         " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %6, p;\n}"
         ::"r"(tmem_c), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(ACC ? 1u : 0u), "r"(idesc) : "memory");
 }
+// the same with A in TMEM: a row a lane, two halves a column
+template <bool ACC>
+__device__ __forceinline__ void mma_tmem(unsigned tmem_c, unsigned tmem_a, unsigned b_lo, unsigned b_hi, unsigned idesc) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %3};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %5, p;\n}"
+        ::"r"(tmem_c), "r"(tmem_a), "r"(b_lo), "r"(b_hi), "r"(ACC ? 1u : 0u), "r"(idesc) : "memory");
+}
 // byte offset of the 16-byte chunk `chunk` (0..7) of row `row` in a tile of 128-byte swizzled rows
 __device__ __forceinline__ unsigned swizzled(int row, int chunk) { return (unsigned)row * ROW_BYTES + (unsigned)((chunk ^ (row & 7)) << 4); }
 __device__ __forceinline__ unsigned times(unsigned h2, unsigned f2) {
@@ -113,14 +121,13 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                       int num_pages, float scale_log2, int window, unsigned* err, int heads, int htiles, int tokens, int cuts) {
     extern __shared__ __align__(1024) unsigned char smem[];              // (the block's only shared memory, so it begins the window)
     unsigned char* Qs = smem;                                            // GROUPS
-    unsigned char* Ks = Qs + GROUPS * Q_BYTES;                           // 2 stages
-    unsigned char* Vs = Ks + 2 * KV_STAGE;                               // 2 stages
-    unsigned char* Ps = Vs + 2 * KV_STAGE;                               // GROUPS
+    unsigned char* Ks = Qs + GROUPS * Q_BYTES;                           // STAGES
+    unsigned char* Vs = Ks + STAGES * KV_STAGE;                          // STAGES
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + TILE_BYTES);
-    unsigned long long *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;
-    unsigned long long *s_full = bars + 8, *s_free = bars + 12, *p_full = bars + 16, *pv_done = bars + 18;    // [GROUPS][2], [GROUPS]
-    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(bars + 20);
-    int* words = reinterpret_cast<int*>(bars + 21);
+    unsigned long long *k_full = bars, *k_empty = bars + 3, *v_full = bars + 6, *v_empty = bars + 9;
+    unsigned long long *s_full = bars + 12, *p_full = bars + 16, *pv_done = bars + 20;           // [GROUPS][2 buffers]
+    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(bars + 24);
+    int* words = reinterpret_cast<int*>(bars + 25);
     int &failed = words[0], &top_k = words[1], &top_v = words[2];
     float* s_row_scale = reinterpret_cast<float*>(smem + TILE_BYTES + 512);                      // [GROUPS * BM]
     int2* s_found = reinterpret_cast<int2*>(s_row_scale + GROUPS * BM);                          // keys, values: [FOUND][BN] cache row (-1: zeros) and factor
@@ -146,12 +153,11 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     const int* table = block_table + (size_t)req * max_blocks;
 
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < STAGES; ++i) {
             mbar_init(&k_full[i], LOAD_THREADS); mbar_init(&k_empty[i], 1);
             mbar_init(&v_full[i], LOAD_THREADS); mbar_init(&v_empty[i], 1);
         }
-        for (int i = 0; i < 2 * GROUPS; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_free[i], BM); }
-        for (int i = 0; i < GROUPS; ++i) { mbar_init(&p_full[i], BM); mbar_init(&pv_done[i], 1); }
+        for (int i = 0; i < 2 * GROUPS; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], BM); mbar_init(&pv_done[i], 1); }
         mbar_fence_init();
         failed = 0;
         top_k = top_v = EXP_MIN;
@@ -253,7 +259,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             }
         };
         auto store = [&](const uint4 (&x)[EACH], int it) {
-            unsigned char* st = stages + (unsigned)(it & 1) * KV_STAGE;
+            unsigned char* st = stages + (unsigned)(it % STAGES) * KV_STAGE;
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
@@ -283,11 +289,11 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             f2 = f3;
             scales_of(f2);                                               // of tile it + 3
             f3 = page_of(it + 4);
-            if (it >= 2) ok = warp_wait(&empty[it & 1], (unsigned)((it / 2 - 1) & 1));
+            if (it >= STAGES) ok = warp_wait(&empty[it % STAGES], (unsigned)((it / STAGES - 1) & 1));
             if (ok) {
                 store(x, it);
                 fence_proxy_async_smem();
-                mbar_arrive(&full[it & 1]);
+                mbar_arrive(&full[it % STAGES]);
                 if (it + 1 < n_tiles) load(x, it + 1);
             }
             ok = loaders_agree(ok, barrier);
@@ -301,13 +307,13 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         const unsigned q_lo = (unsigned)dq, k_lo = (unsigned)dk, hi_word = (unsigned)(dq >> 32);
         bool ok = true;
         for (int it = 0; it < n_tiles && ok; ++it) {
-            const int s = it & 1;
-            if (!warp_wait(&k_full[s], (unsigned)((it / 2) & 1))) { ok = false; break; }
+            const int s = it & 1, stage = it % STAGES;
+            if (!warp_wait(&k_full[stage], (unsigned)((it / STAGES) & 1))) { ok = false; break; }
             for (int gr = 0; gr < groups; ++gr) {
-                // the score buffer is free once every row of the tile two before has been read
-                if (it >= 2 && !warp_wait(&s_free[gr * 2 + s], (unsigned)((it / 2 - 1) & 1))) { ok = false; break; }
+                // the buffer is free once the product with the probabilities of the tile two before is done
+                if (it >= 2 && !warp_wait(&pv_done[gr * 2 + s], (unsigned)((it / 2 - 1) & 1))) { ok = false; break; }
                 tc5_fence_after();
-                const unsigned qb = q_lo + (unsigned)gr * (Q_BYTES >> 4), kb = k_lo + (unsigned)s * (KV_STAGE >> 4);
+                const unsigned qb = q_lo + (unsigned)gr * (Q_BYTES >> 4), kb = k_lo + (unsigned)stage * (KV_STAGE >> 4);
                 const unsigned tc = tmem_base + (unsigned)((gr * 2 + s) * BN);
                 if (lead) {
 #pragma unroll
@@ -318,7 +324,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                         if (ks == 0) mma_lo<false>(tc, qb + qo, kb + ko, hi_word, hi_word, idesc);
                         else mma_lo<true>(tc, qb + qo, kb + ko, hi_word, hi_word, idesc);
                     }
-                    if (gr == groups - 1) tc5_commit(&k_empty[s]);
+                    if (gr == groups - 1) tc5_commit(&k_empty[stage]);
                     tc5_commit(&s_full[gr * 2 + s]);
                 }
             }
@@ -327,26 +333,26 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     } else if (role == PV_WARP) {                                        // ---- issuer of the output O += P V ----
         const bool lead = elect_one();
         constexpr unsigned idesc = idesc_f16(BM, HD) | IDESC_B_MN_MAJOR;
-        const unsigned long long dp = make_smem_desc(Ps), dv = make_smem_desc_lbo_sbo(Vs, BN * ROW_BYTES, 8 * ROW_BYTES);
-        const unsigned p_lo = (unsigned)dp, v_lo = (unsigned)dv, p_hi = (unsigned)(dp >> 32), v_hi = (unsigned)(dv >> 32);
+        const unsigned long long dv = make_smem_desc_lbo_sbo(Vs, BN * ROW_BYTES, 8 * ROW_BYTES);
+        const unsigned v_lo = (unsigned)dv, v_hi = (unsigned)(dv >> 32);
         bool ok = true;
         for (int it = 0; it < n_tiles && ok; ++it) {
-            const int s = it & 1;
-            if (!warp_wait(&v_full[s], (unsigned)((it / 2) & 1))) { ok = false; break; }
+            const int s = it & 1, stage = it % STAGES;
+            if (!warp_wait(&v_full[stage], (unsigned)((it / STAGES) & 1))) { ok = false; break; }
             for (int gr = 0; gr < groups; ++gr) {
-                if (!warp_wait(&p_full[gr], (unsigned)(it & 1))) { ok = false; break; }
+                if (!warp_wait(&p_full[gr * 2 + s], (unsigned)((it / 2) & 1))) { ok = false; break; }
                 tc5_fence_after();
-                const unsigned pb = p_lo + (unsigned)gr * (P_BYTES >> 4), vb = v_lo + (unsigned)s * (KV_STAGE >> 4);
+                const unsigned pb = tmem_base + (unsigned)((gr * 2 + s) * BN), vb = v_lo + (unsigned)stage * (KV_STAGE >> 4);
                 const unsigned tc = tmem_base + O_COL + (unsigned)(gr * 128);
                 if (lead) {
 #pragma unroll
                     for (int k = 0; k < BN / 16; ++k) {
-                        // 16 keys further on: 32 bytes inside a row of P, 16 rows of 128 bytes of V
-                        if (k == 0 && it == 0) mma_lo<false>(tc, pb, vb, p_hi, v_hi, idesc);
-                        else mma_lo<true>(tc, pb + (unsigned)k * 2, vb + (unsigned)k * (16 * ROW_BYTES >> 4), p_hi, v_hi, idesc);
+                        // 16 keys further on: 8 columns of P, 16 rows of 128 bytes of V
+                        if (k == 0 && it == 0) mma_tmem<false>(tc, pb, vb, v_hi, idesc);
+                        else mma_tmem<true>(tc, pb + (unsigned)k * 8, vb + (unsigned)k * (16 * ROW_BYTES >> 4), v_hi, idesc);
                     }
-                    if (gr == groups - 1) tc5_commit(&v_empty[s]);
-                    tc5_commit(&pv_done[gr]);
+                    if (gr == groups - 1) tc5_commit(&v_empty[stage]);
+                    tc5_commit(&pv_done[gr * 2 + s]);
                 }
             }
         }
@@ -362,7 +368,6 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         const float sl2 = fmaxf(s_row_scale[gr * BM + row] * power_of_two(top_k - FOLD), 1.1754944e-38f);
         const unsigned masked = 0xff800000u;                             // -inf
         const unsigned lane_base = (unsigned)((warp & 3) * 32) << 16;
-        unsigned char* Pg = Ps + gr * P_BYTES;
         const unsigned o_col = tmem_base + lane_base + O_COL + (unsigned)(gr * 128);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
@@ -371,11 +376,10 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             if (!warp_wait(&s_full[gr * 2 + s], (unsigned)((it / 2) & 1))) { ok = false; break; }
             tc5_fence_after();
             unsigned sv[BN];
-            tc5_ld32_nowait(tmem_base + lane_base + (unsigned)((gr * 2 + s) * BN), sv);
-            tc5_ld32_nowait(tmem_base + lane_base + (unsigned)((gr * 2 + s) * BN + 32), sv + 32);
+            const unsigned buffer = tmem_base + lane_base + (unsigned)((gr * 2 + s) * BN);
+            tc5_ld32_nowait(buffer, sv);
+            tc5_ld32_nowait(buffer + 32, sv + 32);
             tc5_wait_ld();
-            tc5_fence_before();
-            mbar_arrive(&s_free[gr * 2 + s]);                            // the scores are in registers: the buffer may be written again
             const int j0 = (jt0 + it) * BN;
             if (j0 + BN - 1 > warp_last || j0 < warp_first) {
 #pragma unroll
@@ -404,29 +408,24 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             float sum, sum_hi;
             unpair(sum2, sum, sum_hi);
             l = l * corr + (sum + sum_hi);
-            if (it > 0) {                                                // P of the tile before has been read, O is at rest
-                if (!warp_wait(&pv_done[gr], (unsigned)((it - 1) & 1))) { ok = false; break; }
-                tc5_fence_after();
-                if (__any_sync(0xffffffffu, bump)) {
+            tc5_st32(buffer, pk);                                        // where the scores were
+            if (it > 0 && __any_sync(0xffffffffu, bump)) {
+                if (!warp_wait(&pv_done[gr * 2 + (s ^ 1)], (unsigned)(((it - 1) / 2) & 1))) { ok = false; break; }
+                tc5_fence_after();                                       // O is at rest
 #pragma unroll 1
-                    for (int c0 = 0; c0 < HD; c0 += 32) {
-                        unsigned ov[32];
-                        tc5_ld32(o_col + (unsigned)c0, ov);
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    unsigned ov[32];
+                    tc5_ld32(o_col + (unsigned)c0, ov);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * corr);
-                        tc5_st32(o_col + (unsigned)c0, ov);
-                    }
-                    tc5_wait_st();
+                    for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * corr);
+                    tc5_st32(o_col + (unsigned)c0, ov);
                 }
             }
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<uint4*>(Pg + swizzled(row, c)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-            fence_proxy_async_smem();
+            tc5_wait_st();
             tc5_fence_before();
-            mbar_arrive(&p_full[gr]);
+            mbar_arrive(&p_full[gr * 2 + s]);
         }
-        if (ok && warp_wait(&pv_done[gr], (unsigned)((n_tiles - 1) & 1))) {
+        if (ok && warp_wait(&pv_done[gr * 2 + ((n_tiles - 1) & 1)], (unsigned)(((n_tiles - 1) / 2) & 1))) {
             tc5_fence_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l, unit = power_of_two(top_v - FOLD);
             bf16* dst = out + ((size_t)(tok0 + (live ? tk : 0)) * nq + h0 + (live ? h : 0)) * HD;
