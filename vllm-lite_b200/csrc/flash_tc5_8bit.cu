@@ -16,7 +16,8 @@
 //        unit, which a row's own factor and the end undo.  Exact down to pages 2^15 below the largest, to within 2^-41 of the largest number else.
 //        Rows that no query of the block reads, or that the table does not hold (flagged), are zeros.  A page whose scale is not a number gives
 //        keys of NaN and values of zero: who may read it gets NaN, rows that may not replace the score;
-//   one warp             issues S = Q K^T (both K-major) into one of two score buffers a query tile, one issues O += P V (P from TMEM, V as stored: N contiguous).
+//   one warp             looks up where the keys' rows are and their pages' scales, up to 8 tiles ahead;
+//   one warp             issues S = Q K^T (both K-major) into one of two score buffers a query tile, and one a query tile O += P V (P from TMEM, V as stored: N contiguous).
 // Roundings: queries times a power of two of their row (largest number in [2^14, 2^15)) and the probabilities, 2^7 p with p up to 2^8, are halves.
 // Every wait on an mbarrier is bounded; when one expires the block records VL_DEV_WAIT_EXPIRED, stops, and still frees its TMEM.
 #include "cache_8bit.cuh"
@@ -34,14 +35,14 @@ constexpr int HD = FA_HD;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head sizes in steps of 16 up to 256");
 constexpr int GROUPS = HD <= 128 ? 2 : 1;              // query tiles of 128 rows
 constexpr int BM = 128, BN = 64, CB = (HD + 63) / 64;  // CB: blocks of 64 columns (one swizzled row) a head
-constexpr int SOFT = 4 * GROUPS, QK_WARP = SOFT, PV_WARP = SOFT + 1, LOAD0 = SOFT + 2, LOADERS = 4;   // (loaders of keys, and as many of values)
+constexpr int SOFT = 4 * GROUPS, FIND_WARP = SOFT, QK_WARP = SOFT + 1, PV_WARP = SOFT + 2, LOAD0 = PV_WARP + GROUPS, LOADERS = 4;   // (loaders of keys, and as many of values)
 constexpr int NTHREADS = 32 * (LOAD0 + 2 * LOADERS), LOAD_THREADS = 32 * LOADERS;
 constexpr unsigned ROW_BYTES = 128;
 constexpr unsigned Q_BYTES = BM * CB * ROW_BYTES;      // CB blocks of [128 rows][128 bytes]
 constexpr unsigned KV_STAGE = BN * CB * ROW_BYTES;     // CB blocks of [64 rows][128 bytes]
 constexpr int STAGES = HD <= 128 ? 3 : 2;              // of keys, and of values
 constexpr unsigned TILE_BYTES = GROUPS * Q_BYTES + 2 * STAGES * KV_STAGE;
-constexpr int FOUND = 4;                               // key tiles whose rows are looked up at a time
+constexpr int FOUND = 8;                               // key tiles whose rows are looked up ahead
 constexpr unsigned SMEM_BYTES = TILE_BYTES + 512 + GROUPS * BM * 4 + 2 * FOUND * BN * 8;
 constexpr unsigned TMEM_COLS = 512;                    // scores 2 x 64 a query tile, behind them the outputs
 constexpr unsigned O_COL = GROUPS * 2 * BN;
@@ -104,13 +105,6 @@ __device__ __forceinline__ unsigned times(unsigned h2, unsigned f2) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h2), *reinterpret_cast<const __half2*>(&f2));
     return *reinterpret_cast<const unsigned*>(&r);
 }
-// A barrier of the loading warps, and whether all of them still have what they waited for: one whose wait ran out takes the others along.
-__device__ __forceinline__ bool loaders_agree(bool ok, int barrier) {
-    int all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-                 : "=r"(all) : "r"((int)ok), "r"(barrier), "n"(LOAD_THREADS) : "memory");
-    return all != 0;
-}
 }  // namespace
 
 // tiles[i] = {row of the block table, index of the tile's first token in the step, tokens (<= 128), position of the first}
@@ -126,8 +120,9 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + TILE_BYTES);
     unsigned long long *k_full = bars, *k_empty = bars + 3, *v_full = bars + 6, *v_empty = bars + 9;
     unsigned long long *s_full = bars + 12, *p_full = bars + 16, *pv_done = bars + 20;           // [GROUPS][2 buffers]
-    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(bars + 24);
-    int* words = reinterpret_cast<int*>(bars + 25);
+    unsigned long long *found_full = bars + 24, *found_empty = bars + 24 + FOUND;
+    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(bars + 24 + 2 * FOUND);
+    int* words = reinterpret_cast<int*>(bars + 25 + 2 * FOUND);
     int &failed = words[0], &top_k = words[1], &top_v = words[2];
     float* s_row_scale = reinterpret_cast<float*>(smem + TILE_BYTES + 512);                      // [GROUPS * BM]
     int2* s_found = reinterpret_cast<int2*>(s_row_scale + GROUPS * BM);                          // keys, values: [FOUND][BN] cache row (-1: zeros) and factor
@@ -155,8 +150,9 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&k_full[i], LOAD_THREADS); mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], LOAD_THREADS); mbar_init(&v_empty[i], 1);
+            mbar_init(&v_full[i], LOAD_THREADS); mbar_init(&v_empty[i], groups);
         }
+        for (int i = 0; i < FOUND; ++i) { mbar_init(&found_full[i], 1); mbar_init(&found_empty[i], 2 * LOADERS); }
         for (int i = 0; i < 2 * GROUPS; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], BM); mbar_init(&pv_done[i], 1); }
         mbar_fence_init();
         failed = 0;
@@ -216,40 +212,11 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     const int role = warp_number();
     if (role >= LOAD0) {                                                 // ---- keys and values ----
         const bool values = role >= LOAD0 + LOADERS;
-        const int ct = (tid - LOAD0 * 32) % LOAD_THREADS, E = values ? top_v : top_k, barrier = 1 + (int)values;
+        const int ct = (tid - LOAD0 * 32) % LOAD_THREADS;
         const unsigned char* cache = values ? vcache : kcache;
         unsigned char* stages = values ? Vs : Ks;
         unsigned long long *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
-        int2* found = s_found + (values ? FOUND * BN : 0);
-        // Thread k < 64 looks up key k of every tile, in three steps a tile apart, so that no load is waited for: the page, its scales, and what they say.
-        struct Found { int page, at; float ks, vs; };
-        auto page_of = [&](int it) -> Found {
-            Found f = {-1, -1, 0.f, 0.f};
-            const int key = (jt0 + it) * BN + ct;
-            if (ct >= BN || it >= n_tiles || key < lo || key > hi) return f;
-            const int blk = key / page_size;
-            f.at = key - blk * page_size;
-            if (blk < max_blocks) f.page = table[blk];
-            return f;
-        };
-        auto scales_of = [&](Found& f) {
-            if (f.at < 0) return;
-            if (f.page < 0 || f.page >= num_pages) {
-                f.page = -1;
-                if (err) atomicOr(err, VL_DEV_BAD_PAGE);
-                return;
-            }
-            f.ks = kscale[(size_t)f.page * nkv + kvh];
-            f.vs = vscale[(size_t)f.page * nkv + kvh];
-        };
-        auto note = [&](const Found& f, int it) {
-            if (ct >= BN) return;
-            const bool no_value = f.vs != f.vs, none = f.ks != f.ks || no_value;
-            const __half factor = values ? __float2half_rn(no_value ? 0.f : f.vs * power_of_two(FOLD - E))
-                                         : (none ? __ushort_as_half(0x7e00) : __float2half_rn(f.ks * power_of_two(FOLD - E)));
-            found[(it % FOUND) * BN + ct] = make_int2(f.page < 0 || (values && no_value) ? -1 : (f.page * nkv + kvh) * page_size + f.at,
-                                                      (int)(0x10001u * __half_as_ushort(factor)));
-        };
+        const int2* found = s_found + (values ? FOUND * BN : 0);
         auto load = [&](uint4 (&x)[EACH], int it) {
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
@@ -275,31 +242,100 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                 *reinterpret_cast<uint4*>(blk + swizzled(r, ch + 1)) = b;
             }
         };
-        Found f0 = page_of(0), f1 = page_of(1), f2 = page_of(2), f3 = page_of(3);
-        scales_of(f0);
-        scales_of(f1);
-        scales_of(f2);
-        note(f0, 0);
-        note(f1, 1);
-        bool ok = loaders_agree(true, barrier);
         uint4 x[EACH];
-        load(x, 0);
-        for (int it = 0; it < n_tiles; ++it) {
-            note(f2, it + 2);
-            f2 = f3;
-            scales_of(f2);                                               // of tile it + 3
-            f3 = page_of(it + 4);
-            if (it >= STAGES) ok = warp_wait(&empty[it % STAGES], (unsigned)((it / STAGES - 1) & 1));
-            if (ok) {
-                store(x, it);
-                fence_proxy_async_smem();
-                mbar_arrive(&full[it % STAGES]);
-                if (it + 1 < n_tiles) load(x, it + 1);
-            }
-            ok = loaders_agree(ok, barrier);
+        bool ok = warp_wait(&found_full[0], 0u);
+        if (ok) load(x, 0);
+        for (int it = 0; it < n_tiles && ok; ++it) {
+            ok = it < STAGES || warp_wait(&empty[it % STAGES], (unsigned)((it / STAGES - 1) & 1));
             if (!ok) break;
+            store(x, it);
+            fence_proxy_async_smem();
+            mbar_arrive(&full[it % STAGES]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&found_empty[it % FOUND]);
+            if (it + 1 == n_tiles) break;
+            ok = warp_wait(&found_full[(it + 1) % FOUND], (unsigned)(((it + 1) / FOUND) & 1));
+            if (ok) load(x, it + 1);
         }
         if (!ok && lane == 0) atomicExch(&failed, 1);
+    } else if (role == FIND_WARP) {                                      // ---- where the keys are ----
+        // A lane looks up keys `lane` and lane + 32 of every tile, in three steps a tile apart, so that no load is waited for: the page, its
+        // scales, and what they say.
+        struct Found { int page, at; float ks, vs; };
+        const int EK = top_k, EV = top_v;
+        auto page_of = [&](int it, int u) -> Found {
+            Found f = {-1, -1, 0.f, 0.f};
+            const int key = (jt0 + it) * BN + u * 32 + lane;
+            if (it >= n_tiles || key < lo || key > hi) return f;
+            const int blk = key / page_size;
+            f.at = key - blk * page_size;
+            if (blk < max_blocks) f.page = table[blk];
+            return f;
+        };
+        auto scales_of = [&](Found& f) {
+            if (f.at < 0) return;
+            if (f.page < 0 || f.page >= num_pages) {
+                f.page = -1;
+                if (err) atomicOr(err, VL_DEV_BAD_PAGE);
+                return;
+            }
+            f.ks = kscale[(size_t)f.page * nkv + kvh];
+            f.vs = vscale[(size_t)f.page * nkv + kvh];
+        };
+        auto note = [&](const Found& f, int it, int u) {
+            const bool no_value = f.vs != f.vs, none = f.ks != f.ks || no_value;
+            const __half fk = none ? __ushort_as_half(0x7e00) : __float2half_rn(f.ks * power_of_two(FOLD - EK));
+            const __half fv = __float2half_rn(no_value ? 0.f : f.vs * power_of_two(FOLD - EV));
+            const int at = (it % FOUND) * BN + u * 32 + lane, row = f.page < 0 ? -1 : (f.page * nkv + kvh) * page_size + f.at;
+            s_found[at] = make_int2(row, (int)(0x10001u * __half_as_ushort(fk)));
+            s_found[FOUND * BN + at] = make_int2(no_value ? -1 : row, (int)(0x10001u * __half_as_ushort(fv)));
+        };
+        Found a[BN / 32], b[BN / 32];
+#pragma unroll
+        for (int u = 0; u < BN / 32; ++u) { a[u] = page_of(0, u); b[u] = page_of(1, u); }
+#pragma unroll
+        for (int u = 0; u < BN / 32; ++u) scales_of(a[u]);
+        bool ok = true;
+        for (int it = 0; it < n_tiles; ++it) {
+            ok = it < FOUND || warp_wait(&found_empty[it % FOUND], (unsigned)((it / FOUND - 1) & 1));
+            if (!ok) break;
+#pragma unroll
+            for (int u = 0; u < BN / 32; ++u) {
+                scales_of(b[u]);
+                const Found c = page_of(it + 2, u);
+                note(a[u], it, u);
+                a[u] = b[u];
+                b[u] = c;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&found_full[it % FOUND]);
+        }
+        if (!ok && lane == 0) atomicExch(&failed, 1);
+    } else if (role >= PV_WARP && role - PV_WARP < groups) {             // ---- issuer of a query tile's output O += P V ----
+        const int gr = role - PV_WARP;
+        const bool lead = elect_one();
+        constexpr unsigned idesc = idesc_f16(BM, HD) | IDESC_B_MN_MAJOR;
+        const unsigned long long dv = make_smem_desc_lbo_sbo(Vs, BN * ROW_BYTES, 8 * ROW_BYTES);
+        const unsigned v_lo = (unsigned)dv, v_hi = (unsigned)(dv >> 32), tc = tmem_base + O_COL + (unsigned)(gr * 128);
+        bool ok = true;
+        for (int it = 0; it < n_tiles && ok; ++it) {
+            const int s = gr * 2 + (it & 1), stage = it % STAGES;
+            ok = warp_wait(&v_full[stage], (unsigned)((it / STAGES) & 1)) && warp_wait(&p_full[s], (unsigned)((it / 2) & 1));
+            if (!ok) break;
+            tc5_fence_after();
+            const unsigned pb = tmem_base + (unsigned)(s * BN), vb = v_lo + (unsigned)stage * (KV_STAGE >> 4);
+            if (lead) {
+#pragma unroll
+                for (int k = 0; k < BN / 16; ++k) {
+                    // 16 keys further on: 8 columns of P, 16 rows of 128 bytes of V
+                    if (k == 0 && it == 0) mma_tmem<false>(tc, pb, vb, v_hi, idesc);
+                    else mma_tmem<true>(tc, pb + (unsigned)k * 8, vb + (unsigned)k * (16 * ROW_BYTES >> 4), v_hi, idesc);
+                }
+                tc5_commit(&v_empty[stage]);
+                tc5_commit(&pv_done[s]);
+            }
+        }
+        if (!ok && lead) atomicExch(&failed, 1);
     } else if (role == QK_WARP) {                                        // ---- issuer of the scores S = Q K^T ----
         const bool lead = elect_one();
         constexpr unsigned idesc = idesc_f16(BM, BN);
@@ -307,14 +343,15 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         const unsigned q_lo = (unsigned)dq, k_lo = (unsigned)dk, hi_word = (unsigned)(dq >> 32);
         bool ok = true;
         for (int it = 0; it < n_tiles && ok; ++it) {
-            const int s = it & 1, stage = it % STAGES;
-            if (!warp_wait(&k_full[stage], (unsigned)((it / STAGES) & 1))) { ok = false; break; }
-            for (int gr = 0; gr < groups; ++gr) {
+            const int stage = it % STAGES;
+            ok = warp_wait(&k_full[stage], (unsigned)((it / STAGES) & 1));
+            for (int gr = 0; gr < groups && ok; ++gr) {
+                const int s = gr * 2 + (it & 1);
                 // the buffer is free once the product with the probabilities of the tile two before is done
-                if (it >= 2 && !warp_wait(&pv_done[gr * 2 + s], (unsigned)((it / 2 - 1) & 1))) { ok = false; break; }
+                ok = it < 2 || warp_wait(&pv_done[s], (unsigned)((it / 2 - 1) & 1));
+                if (!ok) break;
                 tc5_fence_after();
-                const unsigned qb = q_lo + (unsigned)gr * (Q_BYTES >> 4), kb = k_lo + (unsigned)stage * (KV_STAGE >> 4);
-                const unsigned tc = tmem_base + (unsigned)((gr * 2 + s) * BN);
+                const unsigned qb = q_lo + (unsigned)gr * (Q_BYTES >> 4), kb = k_lo + (unsigned)stage * (KV_STAGE >> 4), tc = tmem_base + (unsigned)(s * BN);
                 if (lead) {
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks) {
@@ -325,39 +362,12 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                         else mma_lo<true>(tc, qb + qo, kb + ko, hi_word, hi_word, idesc);
                     }
                     if (gr == groups - 1) tc5_commit(&k_empty[stage]);
-                    tc5_commit(&s_full[gr * 2 + s]);
+                    tc5_commit(&s_full[s]);
                 }
             }
         }
         if (!ok && lead) atomicExch(&failed, 1);
-    } else if (role == PV_WARP) {                                        // ---- issuer of the output O += P V ----
-        const bool lead = elect_one();
-        constexpr unsigned idesc = idesc_f16(BM, HD) | IDESC_B_MN_MAJOR;
-        const unsigned long long dv = make_smem_desc_lbo_sbo(Vs, BN * ROW_BYTES, 8 * ROW_BYTES);
-        const unsigned v_lo = (unsigned)dv, v_hi = (unsigned)(dv >> 32);
-        bool ok = true;
-        for (int it = 0; it < n_tiles && ok; ++it) {
-            const int s = it & 1, stage = it % STAGES;
-            if (!warp_wait(&v_full[stage], (unsigned)((it / STAGES) & 1))) { ok = false; break; }
-            for (int gr = 0; gr < groups; ++gr) {
-                if (!warp_wait(&p_full[gr * 2 + s], (unsigned)((it / 2) & 1))) { ok = false; break; }
-                tc5_fence_after();
-                const unsigned pb = tmem_base + (unsigned)((gr * 2 + s) * BN), vb = v_lo + (unsigned)stage * (KV_STAGE >> 4);
-                const unsigned tc = tmem_base + O_COL + (unsigned)(gr * 128);
-                if (lead) {
-#pragma unroll
-                    for (int k = 0; k < BN / 16; ++k) {
-                        // 16 keys further on: 8 columns of P, 16 rows of 128 bytes of V
-                        if (k == 0 && it == 0) mma_tmem<false>(tc, pb, vb, v_hi, idesc);
-                        else mma_tmem<true>(tc, pb + (unsigned)k * 8, vb + (unsigned)k * (16 * ROW_BYTES >> 4), v_hi, idesc);
-                    }
-                    if (gr == groups - 1) tc5_commit(&v_empty[stage]);
-                    tc5_commit(&pv_done[gr * 2 + s]);
-                }
-            }
-        }
-        if (!ok && lead) atomicExch(&failed, 1);
-    } else if (warp / 4 < groups) {                                      // ---- softmax: a thread per row ----
+    } else if (role < SOFT && warp / 4 < groups) {                                      // ---- softmax: a thread per row ----
         const int gr = warp / 4, row = (warp & 3) * 32 + lane, tk = gr * tokens + row / heads, h = row % heads;
         const bool live = row < tokens * heads && tk < count && h < nheads;
         const int qpos = pos0 + min(tk, count - 1);
