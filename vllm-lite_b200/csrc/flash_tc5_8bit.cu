@@ -242,20 +242,31 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                 *reinterpret_cast<uint4*>(blk + swizzled(r, ch + 1)) = b;
             }
         };
-        uint4 x[EACH];
-        bool ok = warp_wait(&found_full[0], 0u);
-        if (ok) load(x, 0);
-        for (int it = 0; it < n_tiles && ok; ++it) {
+        // two tiles on their way: the loads of tile it + 2 are issued when those of tile it have been used
+        bool ok = true;
+        auto ask = [&](uint4 (&x)[EACH], int it) {
+            if (it >= n_tiles || !ok) return;
+            ok = warp_wait(&found_full[it % FOUND], (unsigned)((it / FOUND) & 1));
+            if (ok) load(x, it);
+        };
+        auto bring = [&](uint4 (&x)[EACH], int it) {
+            if (it >= n_tiles || !ok) return;
             ok = it < STAGES || warp_wait(&empty[it % STAGES], (unsigned)((it / STAGES - 1) & 1));
-            if (!ok) break;
+            if (!ok) return;
             store(x, it);
             fence_proxy_async_smem();
             mbar_arrive(&full[it % STAGES]);
             __syncwarp();
             if (lane == 0) mbar_arrive(&found_empty[it % FOUND]);
-            if (it + 1 == n_tiles) break;
-            ok = warp_wait(&found_full[(it + 1) % FOUND], (unsigned)(((it + 1) / FOUND) & 1));
-            if (ok) load(x, it + 1);
+        };
+        uint4 x[EACH], y[EACH];
+        ask(x, 0);
+        ask(y, 1);
+        for (int it = 0; it < n_tiles && ok; it += 2) {
+            bring(x, it);
+            ask(x, it + 2);
+            bring(y, it + 1);
+            ask(y, it + 3);
         }
         if (!ok && lane == 0) atomicExch(&failed, 1);
     } else if (role == FIND_WARP) {                                      // ---- where the keys are ----
@@ -290,25 +301,28 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             s_found[at] = make_int2(row, (int)(0x10001u * __half_as_ushort(fk)));
             s_found[FOUND * BN + at] = make_int2(no_value ? -1 : row, (int)(0x10001u * __half_as_ushort(fv)));
         };
+        bool ok = true;
+        // `now`, whose scales are on their way, is said and takes up the tile two further on; `next`, whose pages are, asks for its scales.  (Two
+        // names that change places every step: a copy of one into the other would wait for its loads.)
+        auto step = [&](Found (&now)[BN / 32], Found (&next)[BN / 32], int it) {
+            if (it >= n_tiles || !ok) return;
+            ok = it < FOUND || warp_wait(&found_empty[it % FOUND], (unsigned)((it / FOUND - 1) & 1));
+            if (!ok) return;
+#pragma unroll
+            for (int u = 0; u < BN / 32; ++u) note(now[u], it, u);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&found_full[it % FOUND]);
+#pragma unroll
+            for (int u = 0; u < BN / 32; ++u) { now[u] = page_of(it + 2, u); scales_of(next[u]); }
+        };
         Found a[BN / 32], b[BN / 32];
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u) { a[u] = page_of(0, u); b[u] = page_of(1, u); }
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u) scales_of(a[u]);
-        bool ok = true;
-        for (int it = 0; it < n_tiles; ++it) {
-            ok = it < FOUND || warp_wait(&found_empty[it % FOUND], (unsigned)((it / FOUND - 1) & 1));
-            if (!ok) break;
-#pragma unroll
-            for (int u = 0; u < BN / 32; ++u) {
-                scales_of(b[u]);
-                const Found c = page_of(it + 2, u);
-                note(a[u], it, u);
-                a[u] = b[u];
-                b[u] = c;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&found_full[it % FOUND]);
+        for (int it = 0; it < n_tiles && ok; it += 2) {
+            step(a, b, it);
+            step(b, a, it + 1);
         }
         if (!ok && lane == 0) atomicExch(&failed, 1);
     } else if (role >= PV_WARP && role - PV_WARP < groups) {             // ---- issuer of a query tile's output O += P V ----
