@@ -17,7 +17,7 @@
 //        Rows that no query of the block reads, or that the table does not hold (flagged), are zeros.  A page whose scale is not a number gives
 //        keys of NaN and values of zero: who may read it gets NaN, rows that may not replace the score;
 //   one warp             looks up where the keys' rows are and their pages' scales, up to 8 tiles ahead;
-//   one warp             issues S = Q K^T (both K-major) into one of two score buffers a query tile, and one a query tile O += P V (P from TMEM, V as stored: N contiguous).
+//   one warp a query tile   issues S = Q K^T (both K-major) into one of two score buffers and O += P V (P from TMEM, V as stored: N contiguous).
 // Roundings: queries times a power of two of their row (largest number in [2^14, 2^15)) and the probabilities, 2^7 p with p up to 2^8, are halves.
 // Every wait on an mbarrier is bounded; when one expires the block records VL_DEV_WAIT_EXPIRED, stops, and still frees its TMEM.
 #include "cache_8bit.cuh"
@@ -35,8 +35,8 @@ constexpr int HD = FA_HD;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head sizes in steps of 16 up to 256");
 constexpr int GROUPS = HD <= 128 ? 2 : 1;              // query tiles of 128 rows
 constexpr int BM = 128, BN = 64, CB = (HD + 63) / 64;  // CB: blocks of 64 columns (one swizzled row) a head
-constexpr int SOFT = 4 * GROUPS, FIND_WARP = SOFT, QK_WARP = SOFT + 1, PV_WARP = SOFT + 2, LOAD0 = PV_WARP + GROUPS, LOADERS = 4;   // (loaders of keys, and as many of values)
-constexpr int NTHREADS = 32 * (LOAD0 + 2 * LOADERS), LOAD_THREADS = 32 * LOADERS;
+constexpr int SOFT = 4 * GROUPS, FIND_WARP = SOFT, MMA_WARP = SOFT + 1, LOAD0 = MMA_WARP + GROUPS, LOADERS = 4;   // (loaders of keys, and as many of values)
+constexpr int NTHREADS = 32 * (LOAD0 + 2 * LOADERS), LOAD_THREADS = 32 * LOADERS, WORKERS = 32 * (SOFT + 2 * LOADERS);
 constexpr unsigned ROW_BYTES = 128;
 constexpr unsigned Q_BYTES = BM * CB * ROW_BYTES;      // CB blocks of [128 rows][128 bytes]
 constexpr unsigned KV_STAGE = BN * CB * ROW_BYTES;     // CB blocks of [64 rows][128 bytes]
@@ -132,12 +132,11 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         return;
     }
     pdl_launch_dependents();
-    pdl_wait();                                                          // q and the cache are written by the kernel before
     // the blocks with the longest rows of keys first
     const int number = num_tiles * cuts - 1 - (int)blockIdx.y, cut = number % cuts;
     const int4 tile = tiles[number / cuts];
     const int skip = cut * GROUPS * tokens, count = min(GROUPS * tokens, tile.z - skip);         // this block's tokens
-    if (count <= 0) return;
+    if (count <= 0) return;                                              // (the whole block)
     const int req = tile.x, tok0 = tile.y + skip, pos0 = tile.w + skip;
     const int kvh = (int)blockIdx.x / htiles, grp = nq / nkv, hbase = ((int)blockIdx.x % htiles) * heads;
     const int nheads = min(heads, grp - hbase), h0 = kvh * grp + hbase;
@@ -149,7 +148,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
 
     if (tid == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            mbar_init(&k_full[i], LOAD_THREADS); mbar_init(&k_empty[i], 1);
+            mbar_init(&k_full[i], LOAD_THREADS); mbar_init(&k_empty[i], groups);
             mbar_init(&v_full[i], LOAD_THREADS); mbar_init(&v_empty[i], groups);
         }
         for (int i = 0; i < FOUND; ++i) { mbar_init(&found_full[i], 1); mbar_init(&found_empty[i], 2 * LOADERS); }
@@ -158,56 +157,103 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         failed = 0;
         top_k = top_v = EXP_MIN;
     }
-    if (warp == QK_WARP) tc5_alloc(&tmem_slot, TMEM_COLS);
-    tc5_fence_before();
     __syncthreads();
-    tc5_fence_after();
-    const unsigned tmem_base = tmem_slot;
 
-    // the largest exponents of the pages that the block reads
-    {
-        int ek = EXP_MIN, ev = EXP_MIN;
-        for (int blk = lo / page_size + tid; blk <= hi / page_size; blk += NTHREADS) {
-            const int page = blk < max_blocks ? table[blk] : -1;
-            if (page < 0 || page >= num_pages) continue;
-            const float ks = kscale[(size_t)page * nkv + kvh], vs = vscale[(size_t)page * nkv + kvh];
-            if (ks == ks) ek = max(ek, (int)(__float_as_uint(ks) >> 23) - 127);
-            if (vs == vs) ev = max(ev, (int)(__float_as_uint(vs) >> 23) - 127);
+    // The finder: a lane looks up keys `lane` and lane + 32 of every tile, in three steps a tile apart, so that no load is waited for: the page, its
+    // scales, and what they say.
+    struct Found { int page, at; float ks, vs; };
+    auto page_of = [&](int it, int u) -> Found {
+        Found f = {-1, -1, 0.f, 0.f};
+        const int key = (jt0 + it) * BN + u * 32 + lane;
+        if (it >= n_tiles || key < lo || key > hi) return f;
+        const int blk = key / page_size;
+        f.at = key - blk * page_size;
+        if (blk < max_blocks) f.page = table[blk];
+        return f;
+    };
+    auto scales_of = [&](Found& f) {
+        if (f.at < 0) return;
+        if (f.page < 0 || f.page >= num_pages) {
+            f.page = -1;
+            if (err) atomicOr(err, VL_DEV_BAD_PAGE);
+            return;
         }
-        ek = __reduce_max_sync(0xffffffffu, ek);
-        ev = __reduce_max_sync(0xffffffffu, ev);
-        if (lane == 0) { atomicMax(&top_k, ek); atomicMax(&top_v, ev); }
-    }
-    // the queries as halves, a warp a row (a lane 8 features), several rows on their way; rows of no token are zeros
-    constexpr int AHEAD = 8;
-    for (int r0 = warp; r0 < groups * BM; r0 += AHEAD * (NTHREADS / 32)) {
+        f.ks = kscale[(size_t)f.page * nkv + kvh];
+        f.vs = vscale[(size_t)f.page * nkv + kvh];
+    };
+    Found a[BN / 32], b[BN / 32];
+    // The largest exponents of the pages that the block reads, and the queries as halves; the first loads of both are on their way at once.
+    // QL lanes a query row, 8 features each; rows of no token are zeros.
+    const int worker = warp < SOFT ? tid : tid - 32 * (LOAD0 - SOFT);
+    if (warp < SOFT || warp >= LOAD0) {
+        const int first = lo / page_size, last = hi / page_size;
+        auto page_at = [&](int blk) -> int {
+            const int page = blk <= last && blk < max_blocks ? table[blk] : -1;
+            return page < num_pages ? page : -1;
+        };
+        int page = page_at(first + worker), ek = EXP_MIN, ev = EXP_MIN;     // (the table is the step's description: no kernel writes it)
+        pdl_wait();
+        constexpr int QL = HD <= 16 ? 2 : HD <= 32 ? 4 : HD <= 64 ? 8 : HD <= 128 ? 16 : 32, AT_ONCE = WORKERS / QL;
+        constexpr int AHEAD = (GROUPS * BM + AT_ONCE - 1) / AT_ONCE;
+        const int r0 = worker / QL, c = worker - r0 * QL, per_head = 65536 / heads + 1;      // (rr * per_head) >> 16 is rr / heads
         uint4 raw[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const int r = r0 + u * (NTHREADS / 32), rr = r & (BM - 1), tk = (r / BM) * tokens + rr / heads, h = rr % heads;
-            const bool live = r < groups * BM && rr < tokens * heads && tk < count && h < nheads && lane < HD / 8;
-            raw[u] = live ? *reinterpret_cast<const uint4*>(q + (size_t)(tok0 + tk) * q_stride + (size_t)(h0 + h) * HD + lane * 8) : make_uint4(0u, 0u, 0u, 0u);
+            const int r = r0 + u * AT_ONCE, rr = r & (BM - 1), t = (rr * per_head) >> 16, tk = (r / BM) * tokens + t, h = rr - t * heads;
+            const bool live = r < groups * BM && t < tokens && tk < count && h < nheads && c < HD / 8;
+            raw[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (live) raw[u] = *reinterpret_cast<const uint4*>(q + (size_t)(tok0 + tk) * q_stride + (size_t)(h0 + h) * HD + c * 8);
+        }
+        for (int blk = first + worker;;) {
+            if (page >= 0) {
+                const float ks = kscale[(size_t)page * nkv + kvh], vs = vscale[(size_t)page * nkv + kvh];
+                if (ks == ks) ek = max(ek, (int)(__float_as_uint(ks) >> 23) - 127);
+                if (vs == vs) ev = max(ev, (int)(__float_as_uint(vs) >> 23) - 127);
+            }
+            blk += WORKERS;
+            if (blk > last) break;
+            page = page_at(blk);
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const int r = r0 + u * (NTHREADS / 32), rr = r & (BM - 1);
-            if (r >= groups * BM) continue;                              // (warp-uniform)
+            const int r = r0 + u * AT_ONCE, rr = r & (BM - 1);
             unsigned* w = &raw[u].x;
-            unsigned top = 0;
+            __nv_bfloat162 most = __habs2(*reinterpret_cast<__nv_bfloat162*>(&w[0]));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-            top = __reduce_max_sync(0xffffffffu, top);
+            for (int i = 1; i < 4; ++i) most = __hmax2(most, __habs2(*reinterpret_cast<__nv_bfloat162*>(&w[i])));
+#pragma unroll
+            for (int o = 1; o < QL; o <<= 1) most = __hmax2(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const unsigned both = *reinterpret_cast<unsigned*>(&most), top = max(both & 0x7fffu, both >> 16);
             const int e = top == 0 || top >= 0x7f80u ? 0 : max(-112, (int)(top >> 7) - 127 - 14);
             const float f = power_of_two(-e);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = pack_half(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
-            if (lane < HD / 8)
-                *reinterpret_cast<uint4*>(Qs + (r / BM) * Q_BYTES + (unsigned)(lane >> 3) * (BM * ROW_BYTES) + swizzled(rr, lane & 7)) = raw[u];
-            if (lane == 0) s_row_scale[r] = scale_log2 * power_of_two(e);
+            if (r < groups * BM && c < HD / 8) {
+                *reinterpret_cast<uint4*>(Qs + (r / BM) * Q_BYTES + (unsigned)(c >> 3) * (BM * ROW_BYTES) + swizzled(rr, c & 7)) = raw[u];
+                if (c == 0) s_row_scale[r] = scale_log2 * power_of_two(e);
+            }
+        }
+        ek = __reduce_max_sync(0xffffffffu, ek);
+        ev = __reduce_max_sync(0xffffffffu, ev);
+        if (lane == 0) { atomicMax(&top_k, ek); atomicMax(&top_v, ev); }
+    } else {
+        if (warp == FIND_WARP) {
+#pragma unroll
+            for (int u = 0; u < BN / 32; ++u) { a[u] = page_of(0, u); b[u] = page_of(1, u); }
+        }
+        pdl_wait();                                                      // q, the cache and its scales are written by the kernel before
+        if (warp == FIND_WARP) {
+            __syncwarp();
+            tc5_alloc(&tmem_slot, TMEM_COLS);                            // (not earlier: a block of that kernel may be about to take its own)
+#pragma unroll
+            for (int u = 0; u < BN / 32; ++u) scales_of(a[u]);
         }
     }
+    tc5_fence_before();
     fence_proxy_async_smem();
     __syncthreads();
+    tc5_fence_after();
+    const unsigned tmem_base = tmem_slot;
 
     const int role = warp_number();
     if (role >= LOAD0) {                                                 // ---- keys and values ----
@@ -217,29 +263,49 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         unsigned char* stages = values ? Vs : Ks;
         unsigned long long *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
         const int2* found = s_found + (values ? FOUND * BN : 0);
+        // Piece i of this thread: row r, 16-byte piece c.  Head sizes of a power of two have c and the row's place in the swizzle the same for all of
+        // a thread's pieces, whose places are then a constant apart.
+        constexpr int APART = LOAD_THREADS / PIECES;
+        constexpr bool EVEN = LOAD_THREADS % PIECES == 0 && APART % 8 == 0 && BN % APART == 0;
+        const int r0 = ct / PIECES, c0 = ct - r0 * PIECES;
+        const unsigned char* my_cache = cache + c0 * 16;
+        const int2* my_found = found + r0;
+        auto place = [&](int r, int c, int half) { return (unsigned)(c >> 2) * (BN * ROW_BYTES) + swizzled(r, 2 * (c & 3) + half); };
+        unsigned char *my_a = stages + place(r0, c0, 0), *my_b = stages + place(r0, c0, 1);
         auto load = [&](uint4 (&x)[EACH], int it) {
+            const int2* f = my_found + (it % FOUND) * BN;
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
-                const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
-                const int row = idx < BN * PIECES ? found[(it % FOUND) * BN + r].x : -1;
-                x[i] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(cache + (size_t)row * HD + c * 16)) : make_uint4(0u, 0u, 0u, 0u);
+                x[i] = make_uint4(0u, 0u, 0u, 0u);
+                if constexpr (EVEN) {
+                    const int row = f[i * APART].x;
+                    if (row >= 0) x[i] = __ldg(reinterpret_cast<const uint4*>(my_cache + (size_t)row * HD));
+                } else {
+                    const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
+                    const int row = idx < BN * PIECES ? f[r - r0].x : -1;
+                    if (row >= 0) x[i] = __ldg(reinterpret_cast<const uint4*>(cache + (size_t)row * HD + c * 16));
+                }
             }
         };
         auto store = [&](const uint4 (&x)[EACH], int it) {
-            unsigned char* st = stages + (unsigned)(it % STAGES) * KV_STAGE;
+            const int2* fold = my_found + (it % FOUND) * BN;
+            const unsigned stage = (unsigned)(it % STAGES) * KV_STAGE;
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
-                if (idx >= BN * PIECES) continue;
-                const unsigned f = (unsigned)found[(it % FOUND) * BN + r].y;
+                if (!EVEN && idx >= BN * PIECES) continue;
+                const unsigned f = (unsigned)fold[EVEN ? i * APART : r - r0].y;
                 const unsigned* w = &x[i].x;
                 uint4 a, b;
                 a.x = times(half2_low(w[0]), f); a.y = times(half2_high(w[0]), f); a.z = times(half2_low(w[1]), f); a.w = times(half2_high(w[1]), f);
                 b.x = times(half2_low(w[2]), f); b.y = times(half2_high(w[2]), f); b.z = times(half2_low(w[3]), f); b.w = times(half2_high(w[3]), f);
-                unsigned char* blk = st + (unsigned)(c >> 2) * (BN * ROW_BYTES);
-                const int ch = 2 * (c & 3);
-                *reinterpret_cast<uint4*>(blk + swizzled(r, ch)) = a;
-                *reinterpret_cast<uint4*>(blk + swizzled(r, ch + 1)) = b;
+                if constexpr (EVEN) {
+                    *reinterpret_cast<uint4*>(my_a + stage + i * (APART * ROW_BYTES)) = a;
+                    *reinterpret_cast<uint4*>(my_b + stage + i * (APART * ROW_BYTES)) = b;
+                } else {
+                    *reinterpret_cast<uint4*>(stages + stage + place(r, c, 0)) = a;
+                    *reinterpret_cast<uint4*>(stages + stage + place(r, c, 1)) = b;
+                }
             }
         };
         // two tiles on their way: the loads of tile it + 2 are issued when those of tile it have been used
@@ -270,29 +336,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         }
         if (!ok && lane == 0) atomicExch(&failed, 1);
     } else if (role == FIND_WARP) {                                      // ---- where the keys are ----
-        // A lane looks up keys `lane` and lane + 32 of every tile, in three steps a tile apart, so that no load is waited for: the page, its
-        // scales, and what they say.
-        struct Found { int page, at; float ks, vs; };
         const int EK = top_k, EV = top_v;
-        auto page_of = [&](int it, int u) -> Found {
-            Found f = {-1, -1, 0.f, 0.f};
-            const int key = (jt0 + it) * BN + u * 32 + lane;
-            if (it >= n_tiles || key < lo || key > hi) return f;
-            const int blk = key / page_size;
-            f.at = key - blk * page_size;
-            if (blk < max_blocks) f.page = table[blk];
-            return f;
-        };
-        auto scales_of = [&](Found& f) {
-            if (f.at < 0) return;
-            if (f.page < 0 || f.page >= num_pages) {
-                f.page = -1;
-                if (err) atomicOr(err, VL_DEV_BAD_PAGE);
-                return;
-            }
-            f.ks = kscale[(size_t)f.page * nkv + kvh];
-            f.vs = vscale[(size_t)f.page * nkv + kvh];
-        };
         auto note = [&](const Found& f, int it, int u) {
             const bool no_value = f.vs != f.vs, none = f.ks != f.ks || no_value;
             const __half fk = none ? __ushort_as_half(0x7e00) : __float2half_rn(f.ks * power_of_two(FOLD - EK));
@@ -315,69 +359,61 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
 #pragma unroll
             for (int u = 0; u < BN / 32; ++u) { now[u] = page_of(it + 2, u); scales_of(next[u]); }
         };
-        Found a[BN / 32], b[BN / 32];
-#pragma unroll
-        for (int u = 0; u < BN / 32; ++u) { a[u] = page_of(0, u); b[u] = page_of(1, u); }
-#pragma unroll
-        for (int u = 0; u < BN / 32; ++u) scales_of(a[u]);
         for (int it = 0; it < n_tiles && ok; it += 2) {
             step(a, b, it);
             step(b, a, it + 1);
         }
         if (!ok && lane == 0) atomicExch(&failed, 1);
-    } else if (role >= PV_WARP && role - PV_WARP < groups) {             // ---- issuer of a query tile's output O += P V ----
-        const int gr = role - PV_WARP;
+    } else if (role >= MMA_WARP && role - MMA_WARP < groups) {           // ---- issuer of a query tile's products ----
+        const int gr = role - MMA_WARP;
         const bool lead = elect_one();
-        constexpr unsigned idesc = idesc_f16(BM, HD) | IDESC_B_MN_MAJOR;
+        const unsigned tmem = __shfl_sync(0xffffffffu, tmem_base, 0);    // (the warp's own, like everything an instruction is issued with)
+        constexpr unsigned s_idesc = idesc_f16(BM, BN), o_idesc = idesc_f16(BM, HD) | IDESC_B_MN_MAJOR;
+        const unsigned long long dq = make_smem_desc(Qs + gr * Q_BYTES), dk = make_smem_desc(Ks);
         const unsigned long long dv = make_smem_desc_lbo_sbo(Vs, BN * ROW_BYTES, 8 * ROW_BYTES);
-        const unsigned v_lo = (unsigned)dv, v_hi = (unsigned)(dv >> 32), tc = tmem_base + O_COL + (unsigned)(gr * 128);
+        const unsigned q_lo = (unsigned)dq, k_lo = (unsigned)dk, k_hi = (unsigned)(dq >> 32), v_lo = (unsigned)dv, v_hi = (unsigned)(dv >> 32);
+        const unsigned to = tmem + O_COL + (unsigned)(gr * 128);
         bool ok = true;
+        auto scores = [&](int it) {                                      // S = Q K^T
+            const int s = gr * 2 + (it & 1), stage = it % STAGES;
+            ok = warp_wait(&k_full[stage], (unsigned)((it / STAGES) & 1));
+            if (!ok) return;
+            tc5_fence_after();
+            const unsigned kb = k_lo + (unsigned)stage * (KV_STAGE >> 4), tc = tmem + (unsigned)(s * BN);
+            if (lead) {
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    // 16 columns further on: 32 bytes inside the swizzled row; 64 columns: the next block of rows
+                    const unsigned qo = (unsigned)(ks >> 2) * (BM * ROW_BYTES >> 4) + (unsigned)(ks & 3) * 2;
+                    const unsigned ko = (unsigned)(ks >> 2) * (BN * ROW_BYTES >> 4) + (unsigned)(ks & 3) * 2;
+                    if (ks == 0) mma_lo<false>(tc, q_lo + qo, kb + ko, k_hi, k_hi, s_idesc);
+                    else mma_lo<true>(tc, q_lo + qo, kb + ko, k_hi, k_hi, s_idesc);
+                }
+                tc5_commit(&k_empty[stage]);
+                tc5_commit(&s_full[s]);
+            }
+        };
+        scores(0);
+        if (ok && n_tiles > 1) scores(1);
         for (int it = 0; it < n_tiles && ok; ++it) {
             const int s = gr * 2 + (it & 1), stage = it % STAGES;
             ok = warp_wait(&v_full[stage], (unsigned)((it / STAGES) & 1)) && warp_wait(&p_full[s], (unsigned)((it / 2) & 1));
             if (!ok) break;
             tc5_fence_after();
-            const unsigned pb = tmem_base + (unsigned)(s * BN), vb = v_lo + (unsigned)stage * (KV_STAGE >> 4);
-            if (lead) {
+            const unsigned pb = tmem + (unsigned)(s * BN), vb = v_lo + (unsigned)stage * (KV_STAGE >> 4);
+            if (lead) {                                                  // O += P V
 #pragma unroll
                 for (int k = 0; k < BN / 16; ++k) {
                     // 16 keys further on: 8 columns of P, 16 rows of 128 bytes of V
-                    if (k == 0 && it == 0) mma_tmem<false>(tc, pb, vb, v_hi, idesc);
-                    else mma_tmem<true>(tc, pb + (unsigned)k * 8, vb + (unsigned)k * (16 * ROW_BYTES >> 4), v_hi, idesc);
+                    if (k == 0 && it == 0) mma_tmem<false>(to, pb, vb, v_hi, o_idesc);
+                    else mma_tmem<true>(to, pb + (unsigned)k * 8, vb + (unsigned)k * (16 * ROW_BYTES >> 4), v_hi, o_idesc);
                 }
                 tc5_commit(&v_empty[stage]);
                 tc5_commit(&pv_done[s]);
             }
-        }
-        if (!ok && lead) atomicExch(&failed, 1);
-    } else if (role == QK_WARP) {                                        // ---- issuer of the scores S = Q K^T ----
-        const bool lead = elect_one();
-        constexpr unsigned idesc = idesc_f16(BM, BN);
-        const unsigned long long dq = make_smem_desc(Qs), dk = make_smem_desc(Ks);
-        const unsigned q_lo = (unsigned)dq, k_lo = (unsigned)dk, hi_word = (unsigned)(dq >> 32);
-        bool ok = true;
-        for (int it = 0; it < n_tiles && ok; ++it) {
-            const int stage = it % STAGES;
-            ok = warp_wait(&k_full[stage], (unsigned)((it / STAGES) & 1));
-            for (int gr = 0; gr < groups && ok; ++gr) {
-                const int s = gr * 2 + (it & 1);
-                // the buffer is free once the product with the probabilities of the tile two before is done
-                ok = it < 2 || warp_wait(&pv_done[s], (unsigned)((it / 2 - 1) & 1));
-                if (!ok) break;
-                tc5_fence_after();
-                const unsigned qb = q_lo + (unsigned)gr * (Q_BYTES >> 4), kb = k_lo + (unsigned)stage * (KV_STAGE >> 4), tc = tmem_base + (unsigned)(s * BN);
-                if (lead) {
-#pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks) {
-                        // 16 columns further on: 32 bytes inside the swizzled row; 64 columns: the next block of rows
-                        const unsigned qo = (unsigned)(ks >> 2) * (BM * ROW_BYTES >> 4) + (unsigned)(ks & 3) * 2;
-                        const unsigned ko = (unsigned)(ks >> 2) * (BN * ROW_BYTES >> 4) + (unsigned)(ks & 3) * 2;
-                        if (ks == 0) mma_lo<false>(tc, qb + qo, kb + ko, hi_word, hi_word, idesc);
-                        else mma_lo<true>(tc, qb + qo, kb + ko, hi_word, hi_word, idesc);
-                    }
-                    if (gr == groups - 1) tc5_commit(&k_empty[stage]);
-                    tc5_commit(&s_full[s]);
-                }
+            if (it + 2 < n_tiles) {                                      // (the scores take the place of P, once it has been read)
+                ok = warp_wait(&pv_done[s], (unsigned)((it / 2) & 1));
+                if (ok) scores(it + 2);
             }
         }
         if (!ok && lead) atomicExch(&failed, 1);
@@ -399,41 +435,65 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             const int s = it & 1;
             if (!warp_wait(&s_full[gr * 2 + s], (unsigned)((it / 2) & 1))) { ok = false; break; }
             tc5_fence_after();
-            unsigned sv[BN];
             const unsigned buffer = tmem_base + lane_base + (unsigned)((gr * 2 + s) * BN);
-            tc5_ld32_nowait(buffer, sv);
-            tc5_ld32_nowait(buffer + 32, sv + 32);
-            tc5_wait_ld();
             const int j0 = (jt0 + it) * BN;
-            if (j0 + BN - 1 > warp_last || j0 < warp_first) {
-#pragma unroll
-                for (int c = 0; c < BN; ++c)
-                    if (j0 + c > qpos || j0 + c < first_key) sv[c] = masked;
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < BN; c += 2) mx = max3(mx, __uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
-            const float m_new = fmaxf(m, mx * sl2);
-            const bool bump = (m_new - m) > RESCALE_ABOVE;               // false when both are -inf (NaN compares false)
-            const float corr = bump ? exp2_fast(m - m_new) : 1.0f;
-            if (bump) m = m_new;
-            const float base = m == -INFINITY ? 0.f : m;
-            const unsigned long long scale2 = pair(sl2, sl2), nbase2 = pair(P_SHIFT - base, P_SHIFT - base);
-            unsigned long long sum2 = pair(0.f, 0.f);
+            const bool edge = j0 + BN - 1 > warp_last || j0 < warp_first;
             unsigned pk[BN / 2];
+            float sum, most;
+            auto scores = [&](unsigned (&sv)[BN]) {
+                tc5_ld32_nowait(buffer, sv);
+                tc5_ld32_nowait(buffer + 32, sv + 32);
+                tc5_wait_ld();
+                if (edge) {
 #pragma unroll
-            for (int c = 0; c < BN; c += 2) {
-                float t0, t1;
-                unpair(fma2(pair(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, nbase2), t0, t1);
-                const float p0 = exp2_fast(t0), p1 = exp2_fast(t1);
-                sum2 = add2(sum2, pair(p0, p1));
-                pk[c >> 1] = pack_half(p0, p1);
+                    for (int c = 0; c < BN; ++c)
+                        if (j0 + c > qpos || j0 + c < first_key) sv[c] = masked;
+                }
+            };
+            auto peek = [&]() -> float {                                 // the largest score
+                unsigned sv[BN];
+                scores(sv);
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < BN; c += 2) top[c / 2 % 4] = max3(top[c / 2 % 4], __uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
+                return max3(fmaxf(top[0], top[1]), top[2], top[3]) * sl2;
+            };
+            auto weigh = [&] {                                           // P and its sum relative to the row's base, and the largest score
+                unsigned sv[BN];
+                scores(sv);
+                const float base = m == -INFINITY ? 0.f : m;
+                const unsigned long long scale2 = pair(sl2, sl2), nbase2 = pair(P_SHIFT - base, P_SHIFT - base);
+                unsigned long long sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < BN; c += 2) {
+                    float t0, t1;
+                    top[c / 2 % 4] = max3(top[c / 2 % 4], __uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
+                    unpair(fma2(pair(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, nbase2), t0, t1);
+                    const float p0 = exp2_fast(t0), p1 = exp2_fast(t1);
+                    sums[c / 2 % 2] = add2(sums[c / 2 % 2], pair(p0, p1));
+                    pk[c >> 1] = pack_half(p0, p1);
+                }
+                float sum_hi;
+                unpair(add2(sums[0], sums[1]), sum, sum_hi);
+                sum += sum_hi;
+                most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * sl2;
+            };
+            // The largest score is found beside the exponentials and not before them: a row's base is an older maximum, good until it has been passed by 2^8.
+            // Then it is moved and the scores, still where they were, are weighed again.
+            if (it == 0) m = peek();
+            weigh();
+            const float m_new = fmaxf(m, most);
+            const bool bump = (m_new - m) > RESCALE_ABOVE;               // false when both are -inf (NaN compares false)
+            const bool any_bump = __any_sync(0xffffffffu, bump);
+            const float corr = bump ? exp2_fast(m - m_new) : 1.0f;
+            if (any_bump) {
+                if (bump) m = m_new;
+                weigh();
             }
-            float sum, sum_hi;
-            unpair(sum2, sum, sum_hi);
-            l = l * corr + (sum + sum_hi);
+            l = l * corr + sum;
             tc5_st32(buffer, pk);                                        // where the scores were
-            if (it > 0 && __any_sync(0xffffffffu, bump)) {
+            if (it > 0 && any_bump) {
                 if (!warp_wait(&pv_done[gr * 2 + (s ^ 1)], (unsigned)(((it - 1) / 2) & 1))) { ok = false; break; }
                 tc5_fence_after();                                       // O is at rest
 #pragma unroll 1
@@ -453,13 +513,16 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             tc5_fence_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l, unit = power_of_two(top_v - FOLD);
             bf16* dst = out + ((size_t)(tok0 + (live ? tk : 0)) * nq + h0 + (live ? h : 0)) * HD;
-#pragma unroll 1
-            for (int c0 = 0; c0 < HD; c0 += 32) {
-                unsigned ov[32];
-                tc5_ld32(o_col + (unsigned)c0, ov);
+            constexpr int STEP = HD <= 32 ? 32 : 64;
+#pragma unroll
+            for (int c0 = 0; c0 < HD; c0 += STEP) {
+                unsigned ov[STEP];
+#pragma unroll
+                for (int i = 0; i < STEP; i += 32) tc5_ld32_nowait(o_col + (unsigned)(c0 + i), ov + i);
+                tc5_wait_ld();
                 if (live) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < STEP / 8; ++i) {
                         float v[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(ov[8 * i + j]) * inv * unit;
@@ -475,7 +538,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     tc5_fence_before();
     __syncthreads();
     tc5_fence_after();
-    if (warp == QK_WARP) tc5_dealloc(tmem_base, TMEM_COLS);
+    if (warp == FIND_WARP) tc5_dealloc(tmem_base, TMEM_COLS);
     if (tid == 0 && failed && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_FLASH_8BIT);
 }
 
