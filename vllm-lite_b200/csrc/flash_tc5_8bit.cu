@@ -47,6 +47,7 @@ constexpr unsigned SMEM_BYTES = TILE_BYTES + 512 + GROUPS * BM * 4 + 2 * FOUND *
 constexpr unsigned TMEM_COLS = 512;                    // scores 2 x 64 a query tile, behind them the outputs
 constexpr unsigned O_COL = GROUPS * 2 * BN;
 constexpr int PIECES = HD / 16, EACH = (BN * PIECES + LOAD_THREADS - 1) / LOAD_THREADS;   // 16-byte pieces of a row, of a tile a thread
+constexpr int QL = HD <= 16 ? 2 : HD <= 32 ? 4 : HD <= 64 ? 8 : HD <= 128 ? 16 : 32;      // lanes a row of queries or of the output, 8 features each
 constexpr float RESCALE_ABOVE = 8.0f, P_SHIFT = 7.0f;
 constexpr int FOLD = 7;
 
@@ -145,18 +146,24 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     const int lo = (window > 0 && pos0 - window + 1 > 0) ? pos0 - window + 1 : 0;                // the first
     const int jt0 = lo / BN, n_tiles = hi / BN - jt0 + 1;
     const int* table = block_table + (size_t)req * max_blocks;
+    const int per_head = 65536 / heads + 1;                              // (r * per_head) >> 16 is r / heads for rows of a tile
 
-    if (tid == 0) {
-        for (int i = 0; i < STAGES; ++i) {
-            mbar_init(&k_full[i], LOAD_THREADS); mbar_init(&k_empty[i], groups);
-            mbar_init(&v_full[i], LOAD_THREADS); mbar_init(&v_empty[i], groups);
-        }
-        for (int i = 0; i < FOUND; ++i) { mbar_init(&found_full[i], 1); mbar_init(&found_empty[i], 2 * LOADERS); }
-        for (int i = 0; i < 2 * GROUPS; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], BM); mbar_init(&pv_done[i], 1); }
+    // (barrier i by thread i; the numbers of arrivals in the order of `bars`)
+    if (tid < 24 + 2 * FOUND) {
+        const int i = tid;
+        const int count = i < 12 ? (i / 3 % 2 ? groups : LOAD_THREADS) : i < 16 ? 1 : i < 20 ? BM : i < 24 + FOUND ? 1 : 2 * LOADERS;
+        mbar_init(&bars[i], count);
         mbar_fence_init();
+    } else if (tid == NTHREADS - 1) {
         failed = 0;
         top_k = top_v = EXP_MIN;
     }
+    const int worker = warp < SOFT ? tid : tid - 32 * (LOAD0 - SOFT), first_page = lo / page_size, last_page = hi / page_size;
+    auto page_at = [&](int blk) -> int {                                 // (the table is the step's description: no kernel writes it)
+        const int page = blk <= last_page && blk < max_blocks ? table[blk] : -1;
+        return page < num_pages ? page : -1;
+    };
+    int page = page_at(first_page + worker);
     __syncthreads();
 
     // The finder: a lane looks up keys `lane` and lane + 32 of every tile, in three steps a tile apart, so that no load is waited for: the page, its
@@ -184,18 +191,12 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     Found a[BN / 32], b[BN / 32];
     // The largest exponents of the pages that the block reads, and the queries as halves; the first loads of both are on their way at once.
     // QL lanes a query row, 8 features each; rows of no token are zeros.
-    const int worker = warp < SOFT ? tid : tid - 32 * (LOAD0 - SOFT);
     if (warp < SOFT || warp >= LOAD0) {
-        const int first = lo / page_size, last = hi / page_size;
-        auto page_at = [&](int blk) -> int {
-            const int page = blk <= last && blk < max_blocks ? table[blk] : -1;
-            return page < num_pages ? page : -1;
-        };
-        int page = page_at(first + worker), ek = EXP_MIN, ev = EXP_MIN;     // (the table is the step's description: no kernel writes it)
+        int ek = EXP_MIN, ev = EXP_MIN;
         pdl_wait();
-        constexpr int QL = HD <= 16 ? 2 : HD <= 32 ? 4 : HD <= 64 ? 8 : HD <= 128 ? 16 : 32, AT_ONCE = WORKERS / QL;
+        constexpr int AT_ONCE = WORKERS / QL;
         constexpr int AHEAD = (GROUPS * BM + AT_ONCE - 1) / AT_ONCE;
-        const int r0 = worker / QL, c = worker - r0 * QL, per_head = 65536 / heads + 1;      // (rr * per_head) >> 16 is rr / heads
+        const int r0 = worker / QL, c = worker - r0 * QL;
         uint4 raw[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
@@ -204,15 +205,14 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             raw[u] = make_uint4(0u, 0u, 0u, 0u);
             if (live) raw[u] = *reinterpret_cast<const uint4*>(q + (size_t)(tok0 + tk) * q_stride + (size_t)(h0 + h) * HD + c * 8);
         }
-        for (int blk = first + worker;;) {
-            if (page >= 0) {
-                const float ks = kscale[(size_t)page * nkv + kvh], vs = vscale[(size_t)page * nkv + kvh];
-                if (ks == ks) ek = max(ek, (int)(__float_as_uint(ks) >> 23) - 127);
-                if (vs == vs) ev = max(ev, (int)(__float_as_uint(vs) >> 23) - 127);
-            }
-            blk += WORKERS;
-            if (blk > last) break;
+        auto exponents = [&](float ks, float vs) {
+            if (ks == ks) ek = max(ek, (int)(__float_as_uint(ks) >> 23) - 127);
+            if (vs == vs) ev = max(ev, (int)(__float_as_uint(vs) >> 23) - 127);
+        };
+        const float ks = page >= 0 ? kscale[(size_t)page * nkv + kvh] : 0.f, vs = page >= 0 ? vscale[(size_t)page * nkv + kvh] : 0.f;
+        for (int blk = first_page + worker + WORKERS; blk <= last_page; blk += WORKERS) {
             page = page_at(blk);
+            if (page >= 0) exponents(kscale[(size_t)page * nkv + kvh], vscale[(size_t)page * nkv + kvh]);
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
@@ -233,6 +233,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                 if (c == 0) s_row_scale[r] = scale_log2 * power_of_two(e);
             }
         }
+        exponents(ks, vs);
         ek = __reduce_max_sync(0xffffffffu, ek);
         ev = __reduce_max_sync(0xffffffffu, ev);
         if (lane == 0) { atomicMax(&top_k, ek); atomicMax(&top_v, ev); }
@@ -418,8 +419,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         }
         if (!ok && lead) atomicExch(&failed, 1);
     } else if (role < SOFT && warp / 4 < groups) {                                      // ---- softmax: a thread per row ----
-        const int gr = warp / 4, row = (warp & 3) * 32 + lane, tk = gr * tokens + row / heads, h = row % heads;
-        const bool live = row < tokens * heads && tk < count && h < nheads;
+        const int gr = warp / 4, row = (warp & 3) * 32 + lane, tk = gr * tokens + row / heads;
         const int qpos = pos0 + min(tk, count - 1);
         const int first_key = (window > 0 && qpos - window + 1 > 0) ? qpos - window + 1 : 0;
         // (warp-uniform) a tile that ends behind the first row's position or begins before the last row's window holds keys that some row must not read
@@ -512,7 +512,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         if (ok && warp_wait(&pv_done[gr * 2 + ((n_tiles - 1) & 1)], (unsigned)(((n_tiles - 1) / 2) & 1))) {
             tc5_fence_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l, unit = power_of_two(top_v - FOLD);
-            bf16* dst = out + ((size_t)(tok0 + (live ? tk : 0)) * nq + h0 + (live ? h : 0)) * HD;
+            unsigned char* turn = Qs + gr * Q_BYTES;                     // (all products with the queries are done)
             constexpr int STEP = HD <= 32 ? 32 : 64;
 #pragma unroll
             for (int c0 = 0; c0 < HD; c0 += STEP) {
@@ -520,16 +520,25 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
 #pragma unroll
                 for (int i = 0; i < STEP; i += 32) tc5_ld32_nowait(o_col + (unsigned)(c0 + i), ov + i);
                 tc5_wait_ld();
-                if (live) {
 #pragma unroll
-                    for (int i = 0; i < STEP / 8; ++i) {
-                        float v[8];
+                for (int i = 0; i < STEP / 8; ++i) {
+                    if (c0 + 8 * i >= HD) continue;
+                    float v[8];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(ov[8 * i + j]) * inv * unit;
-                        if (c0 + 8 * i < HD) store8(dst + c0 + 8 * i, v);
-                    }
+                    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(ov[8 * i + j]) * inv * unit;
+                    const int c = c0 / 8 + i;
+                    store8(reinterpret_cast<bf16*>(turn + (unsigned)(c >> 3) * (BM * ROW_BYTES) + swizzled(row, c & 7)), v);
                 }
-                __syncwarp();
+            }
+            __syncwarp();
+            // this warp's 32 rows, QL lanes a row: neighbouring lanes write neighbouring bytes
+            const int c = lane % QL;
+#pragma unroll 4
+            for (int r = (warp & 3) * 32 + lane / QL; r < (warp & 3) * 32 + 32; r += 32 / QL) {
+                const int t = (r * per_head) >> 16, tk = gr * tokens + t, h = r - t * heads;
+                if (t < tokens && tk < count && h < nheads && c < HD / 8)
+                    *reinterpret_cast<uint4*>(out + ((size_t)(tok0 + tk) * nq + h0 + h) * HD + c * 8) =
+                        *reinterpret_cast<const uint4*>(turn + (unsigned)(c >> 3) * (BM * ROW_BYTES) + swizzled(r, c & 7));
             }
         } else {
             atomicExch(&failed, 1);
