@@ -360,6 +360,45 @@ def test_prompt_portions(nq, nkv, hd, ps, window):
 
 
 @gpu
+@pytest.mark.parametrize("nq,nkv,hd,ps,window", [(8, 2, 128, 64, None), (4, 1, 64, 16, None), (6, 2, 80, 40, 900), (4, 1, 256, 64, None), (32, 1, 128, 128, 1500)])
+@pytest.mark.parametrize("own", [True, False])
+def test_few_tokens_with_many_keys(nq, nkv, hd, ps, window, own):
+    """Keys shared out among blocks and joined (a weight, a product and a sum a share in float32: 2^-20 of the sums as they are allowed anyway holds 16 of them)."""
+    before, new = [1900, 0, 700, 1337, 511], [3, 1, 40, 64, 1]
+    cache = Cache(len(new), 1984, nkv, ps, hd, seed=4).fill([b + n for b, n in zip(before, new)], seed=hd + 1)
+    pos, req, _, _ = batch(cache, before, new)
+    q = queries(sum(new), nq, hd, 9, extra=16)
+    out = torch.full((sum(new) + 1, nq * hd), 3.0, dtype=torch.bfloat16, device=DEV)
+    floats = ops.flash_prefill_8bit_scratch(hd, DEV)
+    scratch = torch.full((floats + 64,), float("nan"), device=DEV) if own else None
+    for _ in range(2):
+        ops.flash_prefill_8bit(q, out[:-1], *cache.tensors, cache.table, tiles_of(before, new), nq, nkv, hd, hd ** -0.5, window, cache.err,
+                               scratch=scratch[:floats] if own else None)
+    assert int(cache.err) == 0 and (out[-1] == 3.0).all()
+    assert not own or torch.isnan(scratch[floats:]).all()
+    check_attention(cache, q, out[:-1], pos, req, nq, window, hd ** -0.5, [0, 1, 2, 3, 4, 20, 43, 44, 60, 107, 108])
+
+
+@gpu
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_a_lost_page_among_shared_keys(which):
+    """One share of the keys is none: so is the result of those who read it, whatever share it is, and nobody else's."""
+    nq, nkv, hd, ps, n = 4, 2, 64, 64, 1600
+    cache = Cache(1, n, nkv, ps, hd).fill([n])
+    q = queries(4, nq, hd, 5)
+    for lost in (0, 12, 24):
+        scale = getattr(cache, which)
+        page, kept = int(cache.table[0, lost]), scale.clone()
+        scale[page, 1] = float("nan")
+        out = ops.flash_prefill_8bit(q, torch.empty_like(q), *cache.tensors, cache.table, tiles_of([n - 4], [4]), nq, nkv, hd, hd ** -0.5, None, cache.err).view(4, nq, hd)
+        assert torch.isfinite(out[:, :2]).all() and torch.isnan(out[:, 2:]).all()
+        out = ops.flash_prefill_8bit(q, torch.empty_like(q), *cache.tensors, cache.table, tiles_of([n - 4], [4]), nq, nkv, hd, hd ** -0.5, 700, cache.err).view(4, nq, hd)
+        assert torch.isfinite(out[:, :2]).all() and torch.isnan(out[:, 2:]).all() == (lost == 24) and torch.isfinite(out[:, 2:]).all() == (lost != 24)
+        scale.copy_(kept)
+    assert int(cache.err) == 0
+
+
+@gpu
 def test_pages_of_very_different_scales():
     """Values of a page 2^14 below the largest page's, which alone is looked at (its key is the only one near the query), keep their bits."""
     nq, nkv, hd, ps = 4, 1, 64, 64
@@ -605,14 +644,14 @@ def test_single_tokens_are_refused_before_any_launch(change, code):
 
 @pytest.mark.parametrize("change,code", [
     (dict(hd=64), -2), (dict(nq=3), -3), (dict(nkv=0), -3), (dict(ps=0), -3), (dict(pages=0), -3), (dict(blocks=0), -3), (dict(stride=250), -3), (dict(stride=260), -3),
-    (dict(window=-1), -3), (dict(q=8), -3), (dict(out=8), -3), (dict(k=8), -3), (dict(tiles=4), -3), (dict(pages=1 << 30), -2), (dict(n=1 << 16), -2), (dict(n=0), 0)])
+    (dict(window=-1), -3), (dict(scratch=4), -3), (dict(floats=10), -3), (dict(q=8), -3), (dict(out=8), -3), (dict(k=8), -3), (dict(tiles=4), -3), (dict(pages=1 << 30), -2), (dict(n=1 << 16), -2), (dict(n=0), 0)])
 def test_prompt_portions_are_refused_before_any_launch(change, code):
     host, at = entry_args()
-    c = dict(q=0, out=0, k=0, v=0, tiles=0, stride=256, blocks=2, n=1, nq=2, nkv=1, hd=128, ps=64, pages=4, window=0)
+    c = dict(q=0, out=0, k=0, v=0, tiles=0, stride=256, blocks=2, n=1, nq=2, nkv=1, hd=128, ps=64, pages=4, window=0, scratch=0, floats=1 << 30)
     c.update(change)
     got = ops._fn("flash_tc5_8bit", "vl_flash_prefill_8bit", {"FA_HD": 128})(
         at + c["q"], c["stride"], at + c["out"], at + c["k"], at + c["v"], at, at, at, c["blocks"], at + c["tiles"], c["n"], c["nq"], c["nkv"], c["hd"], c["ps"], c["pages"], 0.1,
-        c["window"], None, 0)
+        c["window"], at + c["scratch"], c["floats"], None, 0)
     assert got == code
 
 
@@ -654,7 +693,8 @@ def test_refusals():
         with pytest.raises(ops.KernelError):
             ops.flash_decode_8bit(**{**good, **single, **bad})
     tiles = tiles_of([0], [4])
-    for bad in common + [dict(tiles=tiles[:, :3].contiguous()), dict(tiles=tiles.long()), dict(tiles=tiles[0])]:
+    for bad in common + [dict(tiles=tiles[:, :3].contiguous()), dict(tiles=tiles.long()), dict(tiles=tiles[0]), dict(scratch=torch.empty(8, device=DEV)),
+                         dict(scratch=torch.empty(1 << 24, device=DEV)[1:]), dict(scratch=torch.empty(1 << 24, device=DEV).double())]:
         with pytest.raises(ops.KernelError):
             ops.flash_prefill_8bit(**{**good, "tiles": tiles, **bad})
     off = torch.empty(4 * (nq + 2 * nkv) * hd + 1, dtype=torch.bfloat16, device=DEV)[1:].view(4, -1)     # rows that begin on two bytes

@@ -680,7 +680,7 @@ extern "C" int vl_flash_decode_8bit(const void* q, int q_stride, const void* kca
     if (((uintptr_t)q & 7) || (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)scratch) & 15)) return VL_ERR_ARGUMENT;
     const int grp = nq / nkv, wide_heads = grp > 8 && HD <= 128 ? 16 : 8, htiles = (grp + wide_heads - 1) / wide_heads;
     const long long most = (long long)T * nkv * htiles * ((bound + BN - 1) / BN);
-    if ((long long)num_pages * nkv * page_size >= (1ll << 31) || most >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
+    if ((long long)num_pages * nkv * page_size >= (1ll << 31) || most >= (1ll << 30)) return VL_ERR_UNSUPPORTED;
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -42,6 +42,8 @@ constexpr unsigned Q_BYTES = BM * CB * ROW_BYTES;      // CB blocks of [128 rows
 constexpr unsigned KV_STAGE = BN * CB * ROW_BYTES;     // CB blocks of [64 rows][128 bytes]
 constexpr int STAGES = HD <= 128 ? 3 : 2;              // of keys, and of values
 constexpr unsigned TILE_BYTES = GROUPS * Q_BYTES + 2 * STAGES * KV_STAGE;
+constexpr int ROWS = GROUPS * BM;
+constexpr int MIN_PART = 4, MOST_ITEMS = 160;          // splitting of keys: key tiles of a block at least, items a head at most
 constexpr int FOUND = 8;                               // key tiles whose rows are looked up ahead
 constexpr unsigned SMEM_BYTES = TILE_BYTES + 512 + GROUPS * BM * 4 + 2 * FOUND * BN * 8;
 constexpr unsigned TMEM_COLS = 512;                    // scores 2 x 64 a query tile, behind them the outputs
@@ -106,6 +108,58 @@ __device__ __forceinline__ unsigned times(unsigned h2, unsigned f2) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h2), *reinterpret_cast<const __half2*>(&f2));
     return *reinterpret_cast<const unsigned*>(&r);
 }
+// Items of the list: cut i % cuts of tile i / cuts, the tokens that a block takes for one KV head (or a part of its query heads).
+struct List { const int4* tiles; int num_tiles, cuts, tokens, window; };
+struct Item {
+    int req, tok0, pos0, count, lo, jt0, n;                              // tokens, the first key, the first key tile, key tiles (0: no tokens)
+    __device__ __forceinline__ Item(const List& list, int i) {
+        const int4 tile = list.tiles[i / list.cuts];
+        const int skip = i % list.cuts * GROUPS * list.tokens;
+        req = tile.x; tok0 = tile.y + skip; pos0 = tile.w + skip;
+        count = min(GROUPS * list.tokens, tile.z - skip);
+        lo = list.window > 0 && pos0 - list.window + 1 > 0 ? pos0 - list.window + 1 : 0;
+        jt0 = lo / BN;
+        n = count > 0 ? (pos0 + count - 1) / BN - jt0 + 1 : 0;
+    }
+};
+// Splitting of keys: item i's key tiles go to parts[i] blocks in equal shares, of as few tiles as there are blocks for (MIN_PART at least).
+// The blocks of a head are numbered from item 0's on; a lane holds items lane, lane + 32, ...
+struct Split {
+    static constexpr int U = MOST_ITEMS / 32;
+    int n[U], parts[U], before[U], blocks;                               // `before`: blocks of the items ahead; `blocks`: of a head
+    __device__ __forceinline__ Split(const List& list, int most) {       // (all lanes of a warp)
+        const int lane = threadIdx.x & 31, in_list = list.num_tiles * list.cuts;
+        int all = 0, longest = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            n[u] = u * 32 + lane < in_list ? Item(list, u * 32 + lane).n : 0;
+            all += n[u];
+            longest = max(longest, n[u]);
+        }
+        all = __reduce_add_sync(0xffffffffu, all);
+        longest = max(1, __reduce_max_sync(0xffffffffu, longest));
+        int share = min(longest, max(MIN_PART, (all + most - 1) / most)), enough = longest;
+        while (share < enough) {                                         // the smallest share for which the blocks are enough
+            const int mid = (share + enough) / 2;
+            int sum = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) sum += (n[u] + mid - 1) / mid;
+            if (__reduce_add_sync(0xffffffffu, sum) <= most) enough = mid;
+            else share = mid + 1;
+        }
+        blocks = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            parts[u] = (n[u] + enough - 1) / enough;
+            int x = parts[u];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+            before[u] = blocks + x - parts[u];
+            blocks += __shfl_sync(0xffffffffu, x, 31);
+        }
+    }
+};
+struct Partial { float4* out; float2* ml; };                             // out [blocks][HD / 4][ROWS], ml (base, sum) [blocks][ROWS]
 }  // namespace
 
 // tiles[i] = {row of the block table, index of the tile's first token in the step, tokens (<= 128), position of the first}
@@ -113,7 +167,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict__ out, const unsigned char* __restrict__ kcache,
                       const unsigned char* __restrict__ vcache, const float* __restrict__ kscale, const float* __restrict__ vscale,
                       const int* __restrict__ block_table, int max_blocks, const int4* __restrict__ tiles, int num_tiles, int nq, int nkv, int page_size,
-                      int num_pages, float scale_log2, int window, unsigned* err, int heads, int htiles, int tokens, int cuts) {
+                      int num_pages, float scale_log2, int window, unsigned* err, int heads, int htiles, int tokens, int cuts, int split, Partial partial) {
     extern __shared__ __align__(1024) unsigned char smem[];              // (the block's only shared memory, so it begins the window)
     unsigned char* Qs = smem;                                            // GROUPS
     unsigned char* Ks = Qs + GROUPS * Q_BYTES;                           // STAGES
@@ -133,18 +187,36 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         return;
     }
     pdl_launch_dependents();
-    // the blocks with the longest rows of keys first
-    const int number = num_tiles * cuts - 1 - (int)blockIdx.y, cut = number % cuts;
-    const int4 tile = tiles[number / cuts];
-    const int skip = cut * GROUPS * tokens, count = min(GROUPS * tokens, tile.z - skip);         // this block's tokens
-    if (count <= 0) return;                                              // (the whole block)
-    const int req = tile.x, tok0 = tile.y + skip, pos0 = tile.w + skip;
-    const int kvh = (int)blockIdx.x / htiles, grp = nq / nkv, hbase = ((int)blockIdx.x % htiles) * heads;
+    // This block's item and its key tiles from .. to; the items with the longest rows of keys first, or a share of an item's keys.
+    const List list = {tiles, num_tiles, cuts, tokens, window};
+    int head = (int)blockIdx.x, number = num_tiles * cuts - 1 - (int)blockIdx.y, part = 0, parts = 1;
+    if (split) {
+        const Split plan(list, split / (nkv * htiles));
+        if (plan.blocks == 0) return;
+        head = (int)blockIdx.x / plan.blocks;
+        if (head >= nkv * htiles) return;
+        const int x = (int)blockIdx.x - head * plan.blocks;
+        number = -1;
+#pragma unroll
+        for (int u = 0; u < Split::U; ++u) {
+            const unsigned here = __ballot_sync(0xffffffffu, x >= plan.before[u] && x < plan.before[u] + plan.parts[u]);
+            if (here) {
+                const int from = __ffs(here) - 1;
+                number = u * 32 + from;
+                part = x - __shfl_sync(0xffffffffu, plan.before[u], from);
+                parts = __shfl_sync(0xffffffffu, plan.parts[u], from);
+            }
+        }
+    }
+    const Item item(list, number);
+    if (item.n == 0) return;                                             // (the whole block)
+    const int from = (int)((long long)item.n * part / parts), n_tiles = (int)((long long)item.n * (part + 1) / parts) - from;
+    const int req = item.req, tok0 = item.tok0, pos0 = item.pos0, count = item.count, jt0 = item.jt0 + from;
+    const int kvh = head / htiles, grp = nq / nkv, hbase = (head - kvh * htiles) * heads;
     const int nheads = min(heads, grp - hbase), h0 = kvh * grp + hbase;
     const int groups = GROUPS == 2 && count > tokens ? 2 : 1;
-    const int hi = pos0 + count - 1;                                     // the last key any row reads
-    const int lo = (window > 0 && pos0 - window + 1 > 0) ? pos0 - window + 1 : 0;                // the first
-    const int jt0 = lo / BN, n_tiles = hi / BN - jt0 + 1;
+    // the keys that this block reads for any of its rows
+    const int lo = max(item.lo, jt0 * BN), hi = min(pos0 + count - 1, (jt0 + n_tiles) * BN - 1);
     const int* table = block_table + (size_t)req * max_blocks;
     const int per_head = 65536 / heads + 1;                              // (r * per_head) >> 16 is r / heads for rows of a tile
 
@@ -509,7 +581,25 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             tc5_fence_before();
             mbar_arrive(&p_full[gr * 2 + s]);
         }
-        if (ok && warp_wait(&pv_done[gr * 2 + ((n_tiles - 1) & 1)], (unsigned)(((n_tiles - 1) / 2) & 1))) {
+        if (!ok || !warp_wait(&pv_done[gr * 2 + ((n_tiles - 1) & 1)], (unsigned)(((n_tiles - 1) / 2) & 1))) {
+            atomicExch(&failed, 1);
+        } else if (parts > 1) {                                          // a share of the item's keys: sums and base as they are
+            tc5_fence_after();
+            const float unit = power_of_two(top_v - FOLD);
+            const bool live = row < tokens * heads && tk < count;
+            float4* dst = partial.out + (size_t)blockIdx.x * (HD / 4) * ROWS + gr * BM + row;
+#pragma unroll
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+                unsigned ov[32];
+                tc5_ld32(o_col + (unsigned)c0, ov);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (live && c0 + 4 * i < HD)
+                        dst[(size_t)(c0 / 4 + i) * ROWS] = make_float4(__uint_as_float(ov[4 * i]) * unit, __uint_as_float(ov[4 * i + 1]) * unit,
+                                                                       __uint_as_float(ov[4 * i + 2]) * unit, __uint_as_float(ov[4 * i + 3]) * unit);
+            }
+            if (live) partial.ml[(size_t)blockIdx.x * ROWS + gr * BM + row] = make_float2(m, l);
+        } else {
             tc5_fence_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l, unit = power_of_two(top_v - FOLD);
             unsigned char* turn = Qs + gr * Q_BYTES;                     // (all products with the queries are done)
@@ -540,8 +630,6 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                     *reinterpret_cast<uint4*>(out + ((size_t)(tok0 + tk) * nq + h0 + h) * HD + c * 8) =
                         *reinterpret_cast<const uint4*>(turn + (unsigned)(c >> 3) * (BM * ROW_BYTES) + swizzled(r, c & 7));
             }
-        } else {
-            atomicExch(&failed, 1);
         }
     }
     tc5_fence_before();
@@ -551,23 +639,91 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     if (tid == 0 && failed && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_FLASH_8BIT);
 }
 
+// The shares of an item whose keys several blocks have walked: out = sum_r 2^(m_r - M) o_r / sum_r 2^(m_r - M) l_r, M the largest base.  A block an
+// item and 16 columns, a thread a row.
+__global__ void __launch_bounds__(ROWS)
+flash_tc5_8bit_join_kernel(const int4* __restrict__ tiles, int num_tiles, int cuts, int tokens, int window, int nq, int nkv, int heads, int htiles, int split,
+                           Partial partial, bf16* __restrict__ out) {
+    pdl_launch_dependents();
+    const List list = {tiles, num_tiles, cuts, tokens, window};
+    const int in_list = num_tiles * cuts, head = (int)blockIdx.x / in_list, number = (int)blockIdx.x - head * in_list;
+    const Item item(list, number);
+    if (item.n <= MIN_PART) return;
+    const Split plan(list, split / (nkv * htiles));
+    int first = 0, parts = 0;
+#pragma unroll
+    for (int u = 0; u < Split::U; ++u)
+        if (number / 32 == u) {
+            first = head * plan.blocks + __shfl_sync(0xffffffffu, plan.before[u], number % 32);
+            parts = __shfl_sync(0xffffffffu, plan.parts[u], number % 32);
+        }
+    if (parts <= 1) return;                                              // (one block had them all)
+    const int grp = nq / nkv, kvh = head / htiles, hbase = (head - kvh * htiles) * heads, nheads = min(heads, grp - hbase);
+    const int row = threadIdx.x, rr = row & (BM - 1), t = rr / heads, tk = row / BM * tokens + t, h = rr - t * heads;
+    if (t >= tokens || tk >= item.count || h >= nheads) return;
+    pdl_wait();
+    const float2* ml = partial.ml + (size_t)first * ROWS + row;
+    float top = -INFINITY;
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, ml[(size_t)k * ROWS].x);
+    float sum = 0.f, o[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) o[c] = 0.f;
+#pragma unroll 2
+    for (int k = 0; k < parts; ++k) {
+        const float2 b = ml[(size_t)k * ROWS];
+        const float w = b.x == -INFINITY ? 0.f : exp2f(b.x - top);
+        const float4* src = partial.out + ((size_t)(first + k) * (HD / 4) + blockIdx.y * 4) * ROWS + row;
+        sum += w * b.y;                                                  // (also where w is 0: NaN stays NaN)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float4 v = src[c * ROWS];
+            o[4 * c] += w * v.x; o[4 * c + 1] += w * v.y; o[4 * c + 2] += w * v.z; o[4 * c + 3] += w * v.w;
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    bf16* dst = out + ((size_t)(item.tok0 + tk) * nq + kvh * grp + hbase + h) * HD + blockIdx.y * 16;
+#pragma unroll
+    for (int c = 0; c < 16; c += 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = o[c + j] * inv;
+        store8(dst + c, v);
+    }
+}
+
 extern "C" int vl_flash_prefill_8bit_head_dim() { return HD; }
 
-// q rows and `out` rows begin on 16 bytes; caches [pages, nkv, page_size, hd] e4m3, scales [pages, nkv]; pages of any number of positions.
+// scratch (may be null: no keys are split): SMs * ROWS * (hd + 2) floats from a 16-byte boundary.  q rows and `out` rows begin on 16 bytes; caches [pages, nkv, page_size, hd] e4m3, scales [pages, nkv]; pages of any number of positions.
 extern "C" int vl_flash_prefill_8bit(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const float* kscale,
                                      const float* vscale, const int* block_table, int max_blocks, const int* tiles, int num_tiles, int nq, int nkv,
-                                     int hd, int page_size, int num_pages, float scale, int window, unsigned* err, void* stream) {
+                                     int hd, int page_size, int num_pages, float scale, int window, float* scratch, long long floats, unsigned* err, void* stream) {
     if (num_tiles <= 0) return VL_OK;
     if (hd != HD) return VL_ERR_UNSUPPORTED;
     if (nq <= 0 || nkv <= 0 || nq % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || window < 0 || q_stride < nq * hd) return VL_ERR_ARGUMENT;
     if (q_stride % 8 || (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)tiles) & 15)) return VL_ERR_ARGUMENT;
+    if (scratch && (((uintptr_t)scratch & 15) || floats < (long long)ROWS * (HD + 2))) return VL_ERR_ARGUMENT;
     if ((long long)num_pages * nkv * page_size >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
     const int grp = nq / nkv, heads = grp < BM ? grp : BM, htiles = (grp + heads - 1) / heads, tokens = BM / heads;
     const int cuts = (128 + GROUPS * tokens - 1) / (GROUPS * tokens);
     if ((long long)num_tiles * cuts > 65535) return VL_ERR_UNSUPPORTED;
-    cudaError_t e = cudaFuncSetAttribute(flash_tc5_8bit_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+    int device, sms;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(flash_tc5_8bit_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
     if (e != cudaSuccess) return (int)e;
-    return vl_launch_waiting(flash_tc5_8bit_kernel, dim3(nkv * htiles, num_tiles * cuts), dim3(NTHREADS), SMEM_BYTES, (cudaStream_t)stream, (const bf16*)q,
-                     q_stride, (bf16*)out, (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks,
-                     (const int4*)tiles, num_tiles, nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, err, heads, htiles, tokens, cuts);
+    // Keys are split where the rows of keys may be long and at least every second SM would be without a block.
+    const int in_list = num_tiles * cuts;
+    const long long blocks = (long long)in_list * nkv * htiles, reach = (long long)max_blocks * page_size;
+    const long long keys = window > 0 && window + GROUPS * tokens < reach ? window + GROUPS * tokens : reach;
+    const int split = scratch && in_list <= MOST_ITEMS && 2 * blocks <= sms && keys >= 2 * MIN_PART * BN ? sms : 0;
+    if (split && floats < (long long)sms * ROWS * (HD + 2)) return VL_ERR_ARGUMENT;
+    const Partial partial = {(float4*)scratch, split ? (float2*)(scratch + (long long)sms * ROWS * HD) : nullptr};
+    cudaStream_t s = (cudaStream_t)stream;
+    const int rc = vl_launch_waiting(flash_tc5_8bit_kernel, split ? dim3(sms) : dim3(nkv * htiles, in_list), dim3(NTHREADS), SMEM_BYTES, s, (const bf16*)q, q_stride,
+                                     (bf16*)out, (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks,
+                                     (const int4*)tiles, num_tiles, nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, err, heads, htiles, tokens,
+                                     cuts, split, partial);
+    if (rc != VL_OK || !split) return rc;
+    return vl_launch_waiting(flash_tc5_8bit_join_kernel, dim3((unsigned)blocks, HD / 16), dim3(ROWS), 0, s, (const int4*)tiles, num_tiles, cuts, tokens, window, nq,
+                             nkv, heads, htiles, split, partial, (bf16*)out);
 }

@@ -159,7 +159,7 @@ _SIGNATURES = {
                                                     c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p,
                                                     c_void_p, c_void_p, c_int, c_void_p],
     ("flash_tc5_8bit", "vl_flash_prefill_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
-                                                  c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p],
+                                                  c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_longlong, c_void_p, c_void_p],
     ("sampling", "vl_apply_penalties"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_void_p],
     ("sampling", "vl_sample"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -1044,17 +1044,29 @@ def flash_decode_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, r
     return out
 
 
-def flash_prefill_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, tiles, num_heads, num_kv_heads, head_dim, scale, window, err):
+def flash_prefill_8bit_scratch(head_dim, device=None):
+    """Floats of scratch memory that `flash_prefill_8bit` wants on a device: a partial output for every SM."""
+    return torch.cuda.get_device_properties(device).multi_processor_count * (256 if head_dim <= 128 else 128) * (head_dim + 2)
+
+
+def flash_prefill_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, tiles, num_heads, num_kv_heads, head_dim, scale, window, err, scratch=None):
     """Attention of prompt portions over a cache in 8 bits, q and out as in `flash_decode_8bit`.  tiles int32 [n, 4]: (row of the block table, index of the
     tile's first token, tokens (<= 128), position of the first); a step's tiles cover once every token that the launch is to serve, the other rows of out are left
-    alone.  q, out and tiles begin on 16 bytes."""
+    alone.  scratch (float32): at least `flash_prefill_8bit_scratch` of them, which nobody else on the stream needs; without them the call takes its own.
+    q, out, tiles and scratch begin on 16 bytes."""
     _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, "flash_prefill_8bit")
     _need(tiles, torch.int32, "tiles", 2)
     if tiles.shape[1] != 4:
         raise KernelError(f"flash_prefill_8bit: tiles {tuple(tiles.shape)} must be [n, 4]")
+    floats = flash_prefill_8bit_scratch(head_dim, q.device)
+    if scratch is None:
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+    _need(scratch, torch.float32, "scratch", 1)
+    if scratch.shape[0] < floats:
+        raise KernelError(f"flash_prefill_8bit: {floats} floats of scratch are wanted, got {scratch.shape[0]}")
     _check(_fn("flash_tc5_8bit", "vl_flash_prefill_8bit", {"FA_HD": head_dim})(
         q, q.shape[1], out, k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], tiles, tiles.shape[0], num_heads, num_kv_heads, head_dim,
-        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), err, _stream()), "vl_flash_prefill_8bit")
+        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), scratch, floats, err, _stream()), "vl_flash_prefill_8bit")
     return out
 
 
