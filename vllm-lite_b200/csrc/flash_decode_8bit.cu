@@ -676,11 +676,12 @@ extern "C" int vl_flash_decode_8bit(const void* q, int q_stride, const void* kca
     if (T <= 0) return VL_OK;
     if (hd != HD) return VL_ERR_UNSUPPORTED;
     if (nq <= 0 || nkv <= 0 || nq % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || q_stride < nq * hd || q_stride % 4) return VL_ERR_ARGUMENT;
-    if (bound <= 0 || !out || !arrivals || !scratch || floats < 3ll * T * nq * (hd + 2)) return VL_ERR_ARGUMENT;
+    if (bound <= 0 || !out || !arrivals || !scratch) return VL_ERR_ARGUMENT;
     if (((uintptr_t)q & 7) || (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)scratch) & 15)) return VL_ERR_ARGUMENT;
     const int grp = nq / nkv, wide_heads = grp > 8 && HD <= 128 ? 16 : 8, htiles = (grp + wide_heads - 1) / wide_heads;
     const long long most = (long long)T * nkv * htiles * ((bound + BN - 1) / BN);
     if ((long long)num_pages * nkv * page_size >= (1ll << 31) || most >= (1ll << 30)) return VL_ERR_UNSUPPORTED;
+    if (floats < 3ll * T * nq * (hd + 2)) return VL_ERR_ARGUMENT;
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
