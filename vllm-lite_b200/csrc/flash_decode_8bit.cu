@@ -4,10 +4,15 @@
 //     s_j = (q . k_j) * sk_j * scale;   p = softmax_j(s);   o = sum_j p_j (v_j * sv_j),
 // k_j, v_j e4m3 values, sk_j, sv_j the powers of two of their pages.
 //
-// Bound by one read of the keys and values, and next by what it takes to bring them from 8 bits to the tensor cores.  No shared memory and no
-// copies on the way: a warp loads 16 keys' rows and 16 values' rows straight into the registers that mma.sync m16n8k16 wants them in, the next 16
-// while these are worked on, and a lane's share of a row is 16 bytes in a row (features may be dealt out to the lanes in any order as long as
-// queries and keys, or outputs and values, agree).  e4m3 values are halves exactly (cvt.rn.f16x2.e4m3x2), so the products are of halves:
+// Bound by one read of the keys and values, and next by what it takes to bring them from 8 bits to the tensor cores.  Products of 8-bit operands would
+// save that, but mma.sync of them is not the tensor cores' own here (18 to 24 instructions each), and tcgen05's smallest tile has 64 rows or more where a token has
+// 4 to 16 heads.  So e4m3 values become halves (exactly: cvt.rn.f16x2.e4m3x2, two cycles a warp) and mma.sync m16n8k16 multiplies them.
+//
+// A warp has a ring of two stages of its own in shared memory, into which it copies rows as they are (cp.async, 16 bytes a lane), a stage ahead: SUB
+// tiles of 16 keys' and 16 values' rows, in strides with which no two of a quad's or an eighth's loads meet in a bank.  From there a lane takes 16 bytes
+// in a row of each row it needs (features may be dealt out to the lanes in any order as long as queries and keys, or outputs and values, agree).  Two tiles
+// side by side give the scheduler two independent chains: with one, rings were no faster than loads straight into registers (decode of 64 requests 74 us), with
+// two 67.  Four blocks an SM would spill registers; two of four warps each do not.
 //     S^T [16 keys, 8 heads] += K [16, 16] Q^T,      O^T [16 features, 8 heads] += V^T [16, 16 keys] P^T:
 // keys and features are the tile's 16 rows, heads its 8 columns: groups of up to 8 query heads cost one such tile, up to 16 two (template NT).  V's rows
 // come key by key; bytes of four keys are put side by side by byte permutations (4 for 16 values) before they become halves.  P leaves the
@@ -17,10 +22,15 @@
 // lets p reach 2^8 before the row is rescaled, so numbers lie below 2^14 and are normal down to 2^-20 of the base's weight.
 // The maximum of a warp's keys is looked for only where some score has passed the base by 8 (one vote a tile instead of shuffles).
 //
-// The keys of all (token, KV head, tile of heads) items, one item behind the other, are cut into runs of equal length in steps of 64 keys, one run a block; an
+// The keys of all (token, KV head, tile of heads) items, one item behind the other, are cut into runs of equal length in steps of BN keys, one run a block, as many
+// runs as blocks are resident at once (two or three rounds of shorter runs: 68 to 74 us where equal runs take 67).  An
 // item that lies in one run is finished there, the others leave partial results (numerator, maximum, sum) that the block which
-// arrives last at the item's counter adds up in the order of the pieces.  Where the cuts lie, and with them the last bits of a result, follows from the
-// lengths of all requests and the room for pieces.
+// arrives last at the item's counter adds up in the order of the pieces; where an item's pieces are more than 64 KB a second launch adds them up.
+// Where the cuts lie, and with them the last bits of a result, follows from the lengths of all requests and the room for pieces.
+//
+// Measured in a graph (heads of 128): 64 requests of 400 to 4,096 tokens, 8 KV heads: 67 us, 4.4 TB/s; 8 of 3,500 to 4,096: 21 us; two of 50,000 to 65,536
+// with 16 heads a KV head: 37 us; one of 2,800: 10.4 us.  A kernel that reads as many bytes and does nothing else takes 46, 11.5, 20 and 1.9 us.  The rest: some 5 us from the
+// launch to the first product (position, table, data: three latencies behind one another), 4 for each further item that a block begins, 3 for the joining.
 // Keys outside lo..p, or on pages that the table does not hold (flagged), weigh nothing whatever their bytes and scales are; a page whose scale is not a
 // number makes the result NaN where one of its keys is read.
 #include "cache_8bit.cuh"

@@ -7,17 +7,26 @@
 // A block owns consecutive tokens of one request and ALL query heads of one KV head (up to 128): rows of its one or two query tiles of 128 are
 // (token, head) pairs, so a short portion fills a tile as a long one does and a tile's mask is as sharp as its few tokens.  It walks that request's
 // keys in tiles of 64, which both query tiles read.  Roles:
-//   warps 0..3 (and 4..7), a thread per row   read the scores of a key tile from TMEM, keep the running maximum and sum of their row, write
-//        P as halves into TMEM, where the scores were, and, when a row's maximum has grown by more than 2^8, rescale the row's output there.
-//        While one query tile's rows are exponentiated the tensor cores work on the other's products;
-//   four warps each      bring keys and values: 16 bytes a load into registers, one tile ahead, e4m3 to halves (exact), times a power of two, into two
-//        stages of 128-byte swizzled rows each for keys and values.  The pages' scales are folded in here: page by page 2^(e - E + 7), E the largest
+//   warps 0..3 (and 4..7), a thread per row   read the scores of a key tile from TMEM, write P as halves where the scores were, keep the sum of their row and,
+//        beside that, its largest score: a row's base is an older maximum, and only when it has been passed by 2^8 it is moved, the row's output
+//        in TMEM scaled and the scores weighed again.  While one query tile's rows are exponentiated the tensor cores work on the other's products;
+//   one warp             looks up where the keys' rows are and their pages' scales, up to 8 tiles ahead;
+//   four warps for keys, four for values   bring them: 16 bytes a load into registers, two tiles ahead, e4m3 to halves (exact), times a power of two, into two or
+//        three stages of 128-byte swizzled rows.  The pages' scales are folded in here: page by page 2^(e - E + 7), E the largest
 //        exponent of all pages that the block reads (found first; 448 * 2^7 is below the largest half), so that scores and outputs of all tiles are in one
 //        unit, which a row's own factor and the end undo.  Exact down to pages 2^15 below the largest, to within 2^-41 of the largest number else.
 //        Rows that no query of the block reads, or that the table does not hold (flagged), are zeros.  A page whose scale is not a number gives
 //        keys of NaN and values of zero: who may read it gets NaN, rows that may not replace the score;
-//   one warp             looks up where the keys' rows are and their pages' scales, up to 8 tiles ahead;
 //   one warp a query tile   issues S = Q K^T (both K-major) into one of two score buffers and O += P V (P from TMEM, V as stored: N contiguous).
+// Where a launch has so few tokens that half of the SMs would be without a block, each item's keys are shared out among several, which leave base, sum and
+// output as they are for a second launch to join.
+//
+// Measured in a graph (32 heads of 128, 8 KV heads): a prompt of 2,048 tokens 54 us, 0.64 PFLOP/s; three portions of 512 at position 2,500 112 us, 0.57; 8 tokens
+// behind 8,000 keys 26 us.  A step of 64 keys takes a block 1.0 us where exponentials alone (16 a cycle and SM) take 0.54 and the products 0.55: two warps of
+// softmax to a scheduler do not hide their own latencies, and 96 registers a thread allow no more of them.  What a block takes besides, some 8 us: queries and
+// scales (3 us), the first keys (2), the last product and the output (2).  Steps on the way: P through shared memory and keys and values by the same four warps 75 and 165 us.
+// Taken back: turns between the two query tiles' exponentials, scores in parts of 16 or 32 columns, two loading warps with more registers, one
+// block walking several items (its state costs registers and a quarter of the speed).
 // Roundings: queries times a power of two of their row (largest number in [2^14, 2^15)) and the probabilities, 2^7 p with p up to 2^8, are halves.
 // Every wait on an mbarrier is bounded; when one expires the block records VL_DEV_WAIT_EXPIRED, stops, and still frees its TMEM.
 #include "cache_8bit.cuh"
@@ -490,7 +499,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             }
         }
         if (!ok && lead) atomicExch(&failed, 1);
-    } else if (role < SOFT && warp / 4 < groups) {                                      // ---- softmax: a thread per row ----
+    } else if (role < SOFT && warp / 4 < groups) {                       // ---- softmax: a thread per row ----
         const int gr = warp / 4, row = (warp & 3) * 32 + lane, tk = gr * tokens + row / heads;
         const int qpos = pos0 + min(tk, count - 1);
         const int first_key = (window > 0 && qpos - window + 1 > 0) ? qpos - window + 1 : 0;

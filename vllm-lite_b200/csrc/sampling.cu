@@ -20,13 +20,22 @@
 // these integers too, floor(min_p 2^40).
 //
 // vl_apply_penalties works on ragged per-row lists.
-// vl_sample: a cluster of 1 to 8 blocks holds a row in shared memory, so that it is read from memory once, whatever the options.  A threshold (top-k's by
-// counts, top-p's by masses) is found in three steps.  All values are sorted into SMP_BINS bins of their distance from the maximum, a partition that keeps
-// their order (subtraction and the cut are monotone); the blocks add up a share of the bins each and a scan finds the bin with which the sum is reached.
-// The few values of that bin are brought together in every block, and there the threshold's key is found 8 bits at a time, until what is left
+// vl_sample: a cluster of 1 to 8 blocks holds a row in shared memory, so that it is read from memory once, whatever the options.
+//
+// The first look: half-unit bins of the distance from the maximum (each lane counts in a column of its own, so no two meet) say how many tokens are near enough
+// to be kept at all: those with which top-k's count is reached, or top-p's mass with room for what lies behind.  Few of them (SMP_FEW) go to one
+// block with their places in the row, which sorts them (up to SMP_RANKED: each is compared with each) and finishes the row alone; the other blocks are done.
+//
+// Else a threshold (top-k's by counts, top-p's by masses) is found in three steps.  All values are sorted into SMP_BINS bins of their distance from the maximum, a
+// partition that keeps their order (subtraction and the cut are monotone); the blocks add up a share of the bins each and a scan finds the bin with which the sum
+// is reached.  The few values of that bin are brought together in every block, and there the threshold's key is found 8 bits at a time, until what is left
 // is kept whole.  (Should they be more than SMP_LIST, as in a row of one value, the 8 bits at a time go over the cluster's whole row.)  Behind top-k, top-p's sum runs over
 // what top-k left.  Values 32 and more below the maximum have mass 0 and are in no bin: no threshold need be found among them.  Any vocabulary
 // size; what of a slice shared memory does not hold (rows of more than some 390,000) is read again in each pass.
+//
+// Bound by latencies: reading another block's shared memory takes 0.5 us, a barrier of the cluster 0.4, and there are some ten steps behind one another.  One row
+// of 151,936 logits with top-k 20, top-p 0.95 and min-p 0.02: 15.5 us in a graph, 64 rows of mixed options 51 us (0.76 TB/s); through thresholds alone, a
+// conversion a mass and 64-bit atomics a bin, 56 and 168.
 #include "common.cuh"
 #include <cooperative_groups.h>
 
