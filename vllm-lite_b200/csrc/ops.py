@@ -928,14 +928,14 @@ def attention_8bit_supported(dtype, head_dim) -> bool:
 
 
 def _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim):
-    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        _need(t, E4M3, n, 4)
-    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        _need(t, torch.float32, n, 2)
-    shape = k_cache.shape
-    if shape != v_cache.shape or shape[1] != num_kv_heads or shape[3] != head_dim or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
+    """Its pages and their size."""
+    _need(k_cache, E4M3, "k_cache", 4); _need(v_cache, E4M3, "v_cache", 4)
+    _need(k_scale, torch.float32, "k_scale", 2); _need(v_scale, torch.float32, "v_scale", 2)
+    shape = pages, heads, page_size, features = k_cache.shape
+    if heads != num_kv_heads or features != head_dim or v_cache.shape != shape or k_scale.shape != (pages, heads) or v_scale.shape != (pages, heads):
         raise KernelError(f"a cache in 8 bits [pages, {num_kv_heads}, page size, {head_dim}] has scales [pages, {num_kv_heads}]: got {tuple(shape)}, "
                           f"{tuple(v_cache.shape)} and {tuple(k_scale.shape)}, {tuple(v_scale.shape)}")
+    return pages, page_size
 
 
 def _need_heads(num_heads, num_kv_heads, head_dim, name):
@@ -955,38 +955,39 @@ def qk_norm_rope_write_8bit(qkv, positions, slots, cu_seqlens, q_weight, k_weigh
     multiple of 4.  Angles are those of the exact products position * inv_freq."""
     _need(qkv, torch.bfloat16, "qkv", 2); _need(positions, torch.int32, "positions", 1)
     _need_heads(num_heads, num_kv_heads, head_dim, "qk_norm_rope_write_8bit")
-    T = qkv.shape[0]
-    if qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim or positions.shape[0] != T:
+    T, width = qkv.shape
+    if width != (num_heads + 2 * num_kv_heads) * head_dim or positions.numel() != T:
         raise KernelError(f"qkv {tuple(qkv.shape)} does not match heads {num_heads}+2*{num_kv_heads} x {head_dim}")
     B = pages = page_size = 0
     if slots is not None:
-        if any(t is None for t in (cu_seqlens, k_cache, v_cache, k_scale, v_scale)):
+        if cu_seqlens is None or k_cache is None or v_cache is None or k_scale is None or v_scale is None:
             raise KernelError("qk_norm_rope_write_8bit: slots go with cu_seqlens, a cache and its scales")
         _need(slots, torch.int32, "slots", 1); _need(cu_seqlens, torch.int32, "cu_seqlens", 1)
-        _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim)
-        if slots.shape[0] != T or cu_seqlens.shape[0] < 1:
-            raise KernelError(f"qk_norm_rope_write_8bit: {slots.shape[0]} slots for {T} tokens, {cu_seqlens.shape[0]} bounds of requests")
-        B, pages, page_size = cu_seqlens.shape[0] - 1, k_cache.shape[0], k_cache.shape[2]
+        pages, page_size = _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim)
+        B = cu_seqlens.numel() - 1
+        if slots.numel() != T or B < 0:
+            raise KernelError(f"qk_norm_rope_write_8bit: {slots.numel()} slots for {T} tokens, {B + 1} bounds of requests")
     else:
         cu_seqlens = k_cache = v_cache = k_scale = v_scale = None
     for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is not None:
             _need(w, torch.float32, n, 1)
-            if w.shape[0] != head_dim:
+            if w.numel() != head_dim:
                 raise KernelError(f"{n} must have head_dim={head_dim} entries")
     if inv_freq is not None:
         _need(inv_freq, torch.float32, "inv_freq", 1)
-        if inv_freq.shape[0] * 2 != rotary_dim or rotary_dim % 4 or rotary_dim > head_dim:
+        if inv_freq.numel() * 2 != rotary_dim or rotary_dim % 4 or rotary_dim > head_dim:
             raise KernelError(f"qk_norm_rope_write_8bit: inv_freq has rotary_dim / 2 entries, rotary_dim is a multiple of 4 and at most head_dim; got "
                               f"{inv_freq.shape[0]}, {rotary_dim}")
     if q_out is None:
-        q_out = qkv
+        q_out, q_width = qkv, width
     else:
         _need(q_out, torch.bfloat16, "q_out", 2)
-        if q_out.shape != (T, num_heads * head_dim):
-            raise KernelError(f"q_out {tuple(q_out.shape)} must be [{T}, {num_heads * head_dim}]")
+        q_width = num_heads * head_dim
+        if q_out.shape != (T, q_width):
+            raise KernelError(f"q_out {tuple(q_out.shape)} must be [{T}, {q_width}]")
     _check(_fn("cache_8bit", "vl_qk_norm_rope_write_8bit")(
-        qkv, qkv.shape[1], q_out, q_out.shape[1], positions, slots, cu_seqlens, B, q_weight, k_weight, float(eps), inv_freq,
+        qkv, width, q_out, q_width, positions, slots, cu_seqlens, B, q_weight, k_weight, float(eps), inv_freq,
         int(rotary_dim if inv_freq is not None else 0), k_cache, v_cache, k_scale, v_scale, T, num_heads, num_kv_heads, head_dim, page_size, pages,
         err, _stream()), "vl_qk_norm_rope_write_8bit")
     return q_out
@@ -1002,11 +1003,13 @@ def flash_decode_8bit_scratch(num_tokens, num_heads, num_kv_heads, head_dim):
 def _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, name):
     _need(q, torch.bfloat16, "q", 2); _need(out, torch.bfloat16, "out", 2); _need(block_table, torch.int32, "block_table", 2)
     _need_heads(num_heads, num_kv_heads, head_dim, name)
-    _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim)
-    if q.shape[1] < num_heads * head_dim or out.shape != (q.shape[0], num_heads * head_dim):
+    pages, page_size = _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim)
+    T, width = q.shape
+    if width < num_heads * head_dim or out.shape != (T, num_heads * head_dim):
         raise KernelError(f"{name}: q {tuple(q.shape)}, out {tuple(out.shape)} for {num_heads} heads of {head_dim}")
     if not scale > 0 or (window or 0) < 0:
         raise KernelError(f"{name}: scale {scale} and window {window} must be positive (window None or 0: every earlier key)")
+    return T, width, pages, page_size
 
 
 def flash_decode_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, req_index, positions, num_heads, num_kv_heads, head_dim, scale, window,
@@ -1017,16 +1020,16 @@ def flash_decode_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, r
     out are left alone.  scratch (float32) and arrivals (int32, zero before and after each call): at least `flash_decode_8bit_scratch` of them, which nobody
     else on the stream needs; without them the call takes its own.  Pages may have any number of positions; q begins on 8 bytes, scratch on 16.
     `settled`: as in `flash_decode`."""
-    _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, "flash_decode_8bit")
+    T, width, pages, page_size = _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window,
+                                                      "flash_decode_8bit")
     _need(req_index, torch.int32, "req_index", 1); _need(positions, torch.int32, "positions", 1)
-    T = q.shape[0]
-    if req_index.shape[0] != T or positions.shape[0] != T:
-        raise KernelError(f"flash_decode_8bit: {T} tokens, {req_index.shape[0]} request numbers, {positions.shape[0]} positions")
+    if req_index.numel() != T or positions.numel() != T:
+        raise KernelError(f"flash_decode_8bit: {T} tokens, {req_index.numel()} request numbers, {positions.numel()} positions")
     if int(max_context) < 1:
         raise KernelError(f"flash_decode_8bit: max_context {max_context}")
     if token_index is not None:
         _need(token_index, torch.int32, "token_index", 1)
-        T = token_index.shape[0]
+        T = token_index.numel()
     if T == 0:
         return out
     floats, counters = flash_decode_8bit_scratch(T, num_heads, num_kv_heads, head_dim)
@@ -1035,18 +1038,30 @@ def flash_decode_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, r
     if arrivals is None:
         arrivals = torch.zeros(counters, dtype=torch.int32, device=q.device)
     _need(scratch, torch.float32, "scratch", 1); _need(arrivals, torch.int32, "arrivals", 1)
-    if scratch.shape[0] < floats or arrivals.shape[0] < counters:
-        raise KernelError(f"flash_decode_8bit: {floats} floats of scratch and {counters} counters are wanted, got {scratch.shape[0]} and {arrivals.shape[0]}")
+    if scratch.numel() < floats or arrivals.numel() < counters:
+        raise KernelError(f"flash_decode_8bit: {floats} floats of scratch and {counters} counters are wanted, got {scratch.numel()} and {arrivals.numel()}")
     _check(_fn("flash_decode_8bit", "vl_flash_decode_8bit", {"FA_HD": head_dim})(
-        q, q.shape[1], k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], req_index, positions, T, num_heads, num_kv_heads, head_dim,
-        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), int(max_context), scratch, floats, err, token_index, out,
+        q, width, k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], req_index, positions, T, num_heads, num_kv_heads, head_dim,
+        page_size, pages, float(scale), int(window or 0), int(max_context), scratch, floats, err, token_index, out,
         arrivals, int(settled), _stream()), "vl_flash_decode_8bit")
     return out
 
 
+_sm_counts = {}
+
+
+def _sm_count(device):
+    count = _sm_counts.get(device)
+    if count is None:
+        count = torch.cuda.get_device_properties(device).multi_processor_count
+        if device is not None:                                           # (None: the current one, which may be another next time)
+            _sm_counts[device] = count
+    return count
+
+
 def flash_prefill_8bit_scratch(head_dim, device=None):
     """Floats of scratch memory that `flash_prefill_8bit` wants on a device: a partial output for every SM."""
-    return torch.cuda.get_device_properties(device).multi_processor_count * (256 if head_dim <= 128 else 128) * (head_dim + 2)
+    return _sm_count(device) * (256 if head_dim <= 128 else 128) * (head_dim + 2)
 
 
 def flash_prefill_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, tiles, num_heads, num_kv_heads, head_dim, scale, window, err, scratch=None):
@@ -1054,19 +1069,24 @@ def flash_prefill_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, 
     tile's first token, tokens (<= 128), position of the first); a step's tiles cover once every token that the launch is to serve, the other rows of out are left
     alone.  scratch (float32): at least `flash_prefill_8bit_scratch` of them, which nobody else on the stream needs; without them the call takes its own.
     q, out, tiles and scratch begin on 16 bytes."""
-    _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, "flash_prefill_8bit")
+    _, width, pages, page_size = _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window,
+                                                      "flash_prefill_8bit")
     _need(tiles, torch.int32, "tiles", 2)
-    if tiles.shape[1] != 4:
+    count, four = tiles.shape
+    if four != 4:
         raise KernelError(f"flash_prefill_8bit: tiles {tuple(tiles.shape)} must be [n, 4]")
-    floats = flash_prefill_8bit_scratch(head_dim, q.device)
-    if scratch is None:
-        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
-    _need(scratch, torch.float32, "scratch", 1)
-    if scratch.shape[0] < floats:
-        raise KernelError(f"flash_prefill_8bit: {floats} floats of scratch are wanted, got {scratch.shape[0]}")
+    device, floats = q.device, 0
+    if scratch is not None:
+        floats = flash_prefill_8bit_scratch(head_dim, device)
+        _need(scratch, torch.float32, "scratch", 1)
+        if scratch.numel() < floats:
+            raise KernelError(f"flash_prefill_8bit: {floats} floats of scratch are wanted, got {scratch.numel()}")
+    elif 2 * count * num_kv_heads <= _sm_count(device):                  # (keys of more tiles are not shared out)
+        floats = flash_prefill_8bit_scratch(head_dim, device)
+        scratch = torch.empty(floats, dtype=torch.float32, device=device)
     _check(_fn("flash_tc5_8bit", "vl_flash_prefill_8bit", {"FA_HD": head_dim})(
-        q, q.shape[1], out, k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], tiles, tiles.shape[0], num_heads, num_kv_heads, head_dim,
-        k_cache.shape[2], k_cache.shape[0], float(scale), int(window or 0), scratch, floats, err, _stream()), "vl_flash_prefill_8bit")
+        q, width, out, k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], tiles, count, num_heads, num_kv_heads, head_dim,
+        page_size, pages, float(scale), int(window or 0), scratch, floats, err, _stream()), "vl_flash_prefill_8bit")
     return out
 
 
