@@ -169,6 +169,14 @@ def test_write(nq, nkv, hd, ps, rot, before, new, normed):
 
 
 @gpu
+@pytest.mark.parametrize("nkv,hd,ps", [(5, 128, 16), (6, 64, 32), (3, 32, 64), (7, 256, 16), (5, 128, 17), (9, 128, 64)])
+def test_write_of_several_heads_at_a_time(nkv, hd, ps):
+    """Pages that a few warps hold, and more pages than a launch needs to share angles: heads beside one another, their number no multiple of a block's."""
+    test_write(nkv * 2, nkv, hd, ps, hd, [0, 5, ps - 1, 3 * ps, 7], [40, 1, 30, 2 * ps + 3, 60], True)
+    test_write(nkv, nkv, hd, ps, 0, [11, 0], [700, 350], False)
+
+
+@gpu
 def test_far_positions():
     """Angles of positions that float32 holds, whose products with a frequency it does not: off by the rounding of the sine's own arithmetic only."""
     nq, nkv, hd, ps = 2, 1, 128, 64

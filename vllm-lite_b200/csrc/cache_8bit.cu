@@ -15,7 +15,7 @@
 //   narrow:  any other head, a warp a row, 4-byte accesses.
 //
 // Measured in a graph: 64 single tokens of 32 + 2 x 8 heads of 128 4.9 us (a block a page took 16.4, most of it in blocks of one row); a portion of 4,096 tokens
-// at position 700 29.9 us, 92 MB at 3.1 TB/s (4-byte accesses 108); five portions of 77 with heads of 80 and pages of 16 7.0 us.  Bound by latencies: single tokens by loads behind
+// at position 700 27.9 us, 92 MB at 3.3 TB/s (4-byte accesses 108); five portions of 77 with heads of 80 and pages of 16 7.0 us.  Bound by latencies: single tokens by loads behind
 // one another (position and slot, the scale, the row, the page's rows where a scale grows), a portion by the loads of a page's rows and the barrier before its scale is known.
 //
 // Angles are pos * inv_freq as a number of turns in double precision, of which the fraction alone is left (in float32 the product is off by up to 2^-24 of
@@ -404,13 +404,13 @@ struct WideRow {
     }
 };
 
-template <int HD>
+// AT: warps on a head, whose rows of a page they hold in one pass where that is possible; other heads of the block are beside them.
+template <int HD, int AT>
 __global__ void __launch_bounds__(NT, HD <= 128 ? 4 : 2)           // (a portion of 2,048 tokens: 64 registers 17.6 us, 80 20.6, 121 20.9)
 write_8bit_wide_kernel(const __grid_constant__ Step st) {
     using R = WideRow<HD>;
     constexpr int TURNS = HD <= 128 ? 2 : 4;                 // groups of rows a warp holds
-    constexpr int GROUP = WARPS * R::AT_ONCE, PASS = TURNS * GROUP;
-    extern __shared__ __align__(16) float2 s_table[];        // keys: [PASS][HD / 2]; queries: [WARPS][HD / 2]
+    extern __shared__ __align__(16) float2 s_table[];        // keys: [the pass's rows][HD / 2]; queries: [WARPS][HD / 2]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / R::LANES, i0 = 8 * (lane % R::LANES);
     pdl_launch_dependents();
     if (!st.early) pdl_wait();
@@ -452,7 +452,9 @@ write_8bit_wide_kernel(const __grid_constant__ Step st) {
         }
         return;
     }
-    // ---- a page of keys or values of heads_a_block KV heads ----
+    // ---- a page of keys or values of heads_a_block KV heads, of which as many at a time as there are warps for ----
+    constexpr int GROUP = AT * R::AT_ONCE, PASS = TURNS * GROUP;
+    const int my_warp = warp % AT;
     __shared__ unsigned s_top[2][WARPS];
     const bool values = blockIdx.x & 1;
     const int parts = (st.nkv + st.heads_a_block - 1) / st.heads_a_block, part = (int)(blockIdx.x >> 1) % parts;
@@ -473,7 +475,10 @@ write_8bit_wide_kernel(const __grid_constant__ Step st) {
     if (strange && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT);
     strange = __syncthreads_or(strange);                     // (a row whose slot is another place's is left out)
     pdl_wait();                                              // qkv comes from the kernel before
-    for (int kvh = part * st.heads_a_block, turn = 0; kvh < min(st.nkv, (part + 1) * st.heads_a_block); ++kvh, turn ^= 1) {
+    const int end = min(st.nkv, (part + 1) * st.heads_a_block);
+    for (int first = part * st.heads_a_block, turn = 0; first < end; first += WARPS / AT, turn ^= 1) {
+        const bool none = first + warp / AT >= end;       // (no head is left for this warp: it goes along)
+        const int kvh = none ? first : first + warp / AT;
         const size_t head = (size_t)v.page * st.nkv + kvh;
         unsigned char* cache = (values ? st.vcache : st.kcache) + head * st.page_size * HD;
         float* scale = (values ? st.vscale : st.kscale) + head;
@@ -490,15 +495,15 @@ write_8bit_wide_kernel(const __grid_constant__ Step st) {
             }
 #pragma unroll
             for (int u = 0; u < TURNS; ++u) {
-                const int i = base + u * GROUP + warp * R::AT_ONCE + sub;
-                mine[u] = i < v.n && !(strange && st.slots[v.tok0 + i] != v.slot0 + i);
+                const int i = base + u * GROUP + my_warp * R::AT_ONCE + sub;
+                mine[u] = !none && i < v.n && !(strange && st.slots[v.tok0 + i] != v.slot0 + i);
                 if (mine[u]) r[u].load(src + (size_t)(v.tok0 + i) * st.row_stride, i0);
                 else r[u].clear();
             }
 #pragma unroll
             for (int u = 0; u < TURNS; ++u) {
                 if (w) r[u].norm(wa, wb, st.eps);
-                if (turned && mine[u]) r[u].turn(s_table + (u * GROUP + warp * R::AT_ONCE + sub) * R::HALF + i0);
+                if (turned && mine[u]) r[u].turn(s_table + (u * GROUP + my_warp * R::AT_ONCE + sub) * R::HALF + i0);
             }
         };
         for (int base = 0; base <= last; base += PASS) {
@@ -510,16 +515,17 @@ write_8bit_wide_kernel(const __grid_constant__ Step st) {
         top = __reduce_max_sync(0xffffffffu, top);
         if (lane == 0) s_top[turn][warp] = top;
         __syncthreads();
-        for (int i = 0; i < WARPS; ++i) top = max(top, s_top[turn][i]);
+        for (int i = 0; i < AT; ++i) top = max(top, s_top[turn][warp - my_warp + i]);
         const float now = new_scale(top, v.row0, old), inv = inverse_of(now);
         for (int base = last; base >= 0; base -= PASS) {     // (the last pass is still held)
             if (base != last) take(base);
 #pragma unroll
             for (int u = 0; u < TURNS; ++u)
-                if (mine[u]) r[u].store(cache + (size_t)(v.row0 + base + u * GROUP + warp * R::AT_ONCE + sub) * HD, i0, inv);
+                if (mine[u]) r[u].store(cache + (size_t)(v.row0 + base + u * GROUP + my_warp * R::AT_ONCE + sub) * HD, i0, inv);
         }
-        if (v.row0 && now > old) move_rows(cache, v.row0 * HD, old * inv, threadIdx.x, NT);
-        if (threadIdx.x == 0) *scale = now;                  // (everybody has read it: a barrier ago)
+        if (none) continue;
+        if (v.row0 && now > old) move_rows(cache, v.row0 * HD, old * inv, my_warp * 32 + lane, AT * 32);
+        if (my_warp == 0 && lane == 0) *scale = now;         // (everybody has read it: a barrier ago)
     }
 }
 
@@ -553,19 +559,24 @@ extern "C" int vl_qk_norm_rope_write_8bit(const void* qkv, int row_stride, void*
     // 300 portions of 8: 4 heads 21, 1 12).
     st.heads_a_warp = wide ? (T >= 256 ? 16 : 8) : (T >= 256 ? 8 : (T >= 32 ? 4 : 2));
     st.heads_a_block = !wide || T < 32 * pages || pages * nkv < 256 ? 1 : (pages * nkv < 512 ? 2 : 4);
+    // Two warps a head where they hold the rows that a page can get: small pages and short portions leave none idle (2,048 tokens on pages of 16: 18 us, 30 with
+    // eight; 300 portions of 8 tokens 17 and 37).
+    const int rows = page_size < (T + B - 1) / (B > 0 ? B : 1) ? page_size : (T + B - 1) / (B > 0 ? B : 1), a_warp = (hd <= 128 ? 2 : 4) * (512 / hd);
+    const bool few = wide && rows <= 2 * a_warp;
+    if (few && st.heads_a_block < WARPS / 2) st.heads_a_block = WARPS / 2 < nkv ? WARPS / 2 : nkv;
     st.page_blocks = (int)(pages * ((nkv + st.heads_a_block - 1) / st.heads_a_block) * 2);
     const long long units = (long long)T * ((nq + st.heads_a_warp - 1) / st.heads_a_warp), blocks = st.page_blocks + (units + WARPS - 1) / WARPS;
     if (blocks >= (1ll << 31) || pages * nkv * 2 >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
     if (!wide)
         return vl_launch_waiting(hd <= 128 ? write_8bit_narrow_kernel<128> : write_8bit_narrow_kernel<256>, dim3((unsigned)blocks), dim3(NT), 0, s, st);
-    const int rows = (hd <= 128 ? 2 : 4) * WARPS * (512 / hd), smem = (inv_freq ? (rows > WARPS ? rows : WARPS) * hd / 2 * 8 : 0);
+    const int angles = a_warp * (few ? 2 : WARPS) > WARPS ? a_warp * (few ? 2 : WARPS) : WARPS, smem = inv_freq ? angles * hd / 2 * 8 : 0;
     auto launch = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return (int)e;
         return vl_launch_waiting(kernel, dim3((unsigned)blocks), dim3(NT), (size_t)smem, s, st);
     };
-    if (hd == 32) return launch(write_8bit_wide_kernel<32>);
-    if (hd == 64) return launch(write_8bit_wide_kernel<64>);
-    if (hd == 128) return launch(write_8bit_wide_kernel<128>);
-    return launch(write_8bit_wide_kernel<256>);
+    if (hd == 32) return few ? launch(write_8bit_wide_kernel<32, 2>) : launch(write_8bit_wide_kernel<32, WARPS>);
+    if (hd == 64) return few ? launch(write_8bit_wide_kernel<64, 2>) : launch(write_8bit_wide_kernel<64, WARPS>);
+    if (hd == 128) return few ? launch(write_8bit_wide_kernel<128, 2>) : launch(write_8bit_wide_kernel<128, WARPS>);
+    return few ? launch(write_8bit_wide_kernel<256, 2>) : launch(write_8bit_wide_kernel<256, WARPS>);
 }
