@@ -23,13 +23,13 @@
 // The maximum of a warp's keys is looked for only where some score has passed the base by 8 (one vote a tile instead of shuffles).
 //
 // The keys of all (token, KV head, tile of heads) items, one item behind the other, are cut into runs of equal length in steps of BN keys, one run a block, as many
-// runs as blocks are resident at once (two or three rounds of shorter runs: 68 to 74 us where equal runs take 67).  An
+// runs as blocks are resident at once (two or three rounds of shorter runs: 68 to 74 us where equal runs take 67).  Where items are few, none shares a run with another.  An
 // item that lies in one run is finished there, the others leave partial results (numerator, maximum, sum) that the block which
 // arrives last at the item's counter adds up in the order of the pieces; where an item's pieces are more than 64 KB a second launch adds them up.
 // Where the cuts lie, and with them the last bits of a result, follows from the lengths of all requests and the room for pieces.
 //
-// Measured in a graph (heads of 128): 64 requests of 400 to 4,096 tokens, 8 KV heads: 67 us, 4.4 TB/s; 8 of 3,500 to 4,096: 21 us; two of 50,000 to 65,536
-// with 16 heads a KV head: 37 us; one of 2,800: 10.4 us.  A kernel that reads as many bytes and does nothing else takes 46, 11.5, 20 and 1.9 us.  The rest: some 5 us from the
+// Measured in a graph (heads of 128): 64 requests of 400 to 4,096 tokens, 8 KV heads: 67 us, 4.4 TB/s; 8 of 3,500 to 4,096: 19 us (runs that reach into a second item 21); two of 50,000 to
+// 65,536 with 16 heads a KV head: 33 us (37); one of 2,800: 10.5 us.  A kernel that reads as many bytes and does nothing else takes 46, 11.5, 20 and 1.9 us.  The rest: some 5 us from the
 // launch to the first product (position, table, data: three latencies behind one another), 4 for each further item that a block begins, 3 for the joining.
 // Keys outside lo..p, or on pages that the table does not hold (flagged), weigh nothing whatever their bytes and scales are; a page whose scale is not a
 // number makes the result NaN where one of its keys is read.
@@ -206,24 +206,55 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         __syncthreads();
         return total - all + x;
     };
-    int n0 = 0, u0 = 0;                                      // the first round is kept
-    for (int z0 = 0; z0 < T; z0 += NTHREADS) {
-        int n;
-        const int u = round(z0, n);
-        if (z0 == 0) { n0 = n; u0 = u; }
-    }
-    const int grid = gridDim.x, all_steps = total, run = blockIdx.x;
-    const int per = max((all_steps + grid - 1) / grid, MIN_RUN);
-    const int first = (int)min((long long)run * per, (long long)all_steps), last = min(first + per, all_steps);
-    const int held = min(HEADS, grp);                        // rows that a piece leaves
+    const int grid = gridDim.x, run = blockIdx.x, held = min(HEADS, grp);                  // held: rows that a piece leaves
     const Scratch left(scratch, grid, held);
-    total = 0;
-    for (int z0 = 0; z0 < T; z0 += NTHREADS) {
-        int n = n0, u = u0;
-        if (z0 > 0 || T > NTHREADS) u = round(z0, n);
-        if (u > first && u - n <= first) { s_z = z0 + tid; s_before = u - n; }
+    // Few items: no run reaches into a second one (beginning that costs as much as four steps).  An item takes whole runs, the last one of which may be
+    // shorter, and a run is as short as there are blocks for: a token a lane, each warp by itself.
+    const bool apart = T <= 32 && 2 * T * ny <= grid;
+    int per, first, last, z = T, before = 0;                 // the run, the token that it begins in, the steps ahead of that
+    auto span_of = [&](int steps) { return apart ? (steps + per - 1) / per * per : steps; };
+    if (apart) {
+        int lo = 0;
+        const int keys = lane < T ? keys_of(lane, nullptr, &lo) : 0, steps = steps_of(lo, keys);
+        const int all = __reduce_add_sync(0xffffffffu, ny * steps);
+        per = max((all + grid - 1) / grid, MIN_RUN);
+        auto runs_of = [&](int length) { return __reduce_add_sync(0xffffffffu, ny * ((steps + length - 1) / length)); };
+        if (runs_of(per) > grid)
+            for (int enough = all / (grid - T * ny) + 1; per < enough;) {              // (as long, the runs' rounding up is made good)
+                const int mid = (per + enough) / 2;
+                if (runs_of(mid) <= grid) enough = mid;
+                else per = mid + 1;
+            }
+        const int n = ny * span_of(steps);
+        int u = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, u, o); if (lane >= o) u += y; }
+        const int end = __shfl_sync(0xffffffffu, u, 31);
+        first = min(run * per, end);
+        last = min(first + per, end);
+        const unsigned here = __ballot_sync(0xffffffffu, u > first && u - n <= first);
+        if (here) { z = __ffs(here) - 1; before = __shfl_sync(0xffffffffu, u - n, z); }
+    } else {
+        int n0 = 0, u0 = 0;                                  // the first round is kept
+        for (int z0 = 0; z0 < T; z0 += NTHREADS) {
+            int n;
+            const int u = round(z0, n);
+            if (z0 == 0) { n0 = n; u0 = u; }
+        }
+        const int all_steps = total;
+        per = max((all_steps + grid - 1) / grid, MIN_RUN);
+        first = (int)min((long long)run * per, (long long)all_steps);
+        last = min(first + per, all_steps);
+        total = 0;
+        for (int z0 = 0; z0 < T; z0 += NTHREADS) {
+            int n = n0, u = u0;
+            if (z0 > 0 || T > NTHREADS) u = round(z0, n);
+            if (u > first && u - n <= first) { s_z = z0 + tid; s_before = u - n; }
+        }
+        __syncthreads();
+        z = s_z;
+        before = s_before;
     }
-    __syncthreads();
     pdl_wait();                                              // q and the cache are written by the kernel before
     // the places without keys: rows of zeros, and the ones beyond the bound are flagged
     for (int z = blockIdx.x; z < T; z += grid) {
@@ -235,7 +266,6 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
             for (int y = tid; y < ny; y += NTHREADS) __stcg(left.info + z * ny + y, make_int4(0, 0, 0, 0));
     }
 
-    int z = s_z, before = s_before;
     auto piece_at = [&](int at) -> Piece {                   // the piece that begins with step `at`: its item's share of this run
         Piece p;
         int lo = 0, keys = 0, tz = 0;
@@ -244,12 +274,12 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         while (at < last && z < T) {
             keys = keys_of(z, &p.tok, &lo);
             tz = steps_of(lo, keys);
-            if (at < before + ny * tz) break;
-            before += ny * tz;
+            if (at < before + ny * span_of(tz)) break;
+            before += ny * span_of(tz);
             ++z;
         }
         if (at >= last || z >= T) return p;
-        const int y = (at - before) / tz, start = before + y * tz, htile = y % htiles;       // the item's first step
+        const int span = span_of(tz), y = (at - before) / span, start = before + y * span, htile = y % htiles;     // the item's first step
         p.req = z < NTHREADS ? s_req[z] : req_index[p.tok];
         p.kvh = y / htiles;
         p.stop = min(last, start + tz);
@@ -272,7 +302,7 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
     for (int number = 0;; ++number) {
         const Piece pc = piece_at(at);
         if (pc.heads == 0) break;
-        at = pc.stop;
+        at = apart ? last : pc.stop;
         const int* table = block_table + (size_t)pc.req * max_blocks;
 
         float o[NT][OT][4], less[NT][2], l[NT][2];           // less: SHIFT less the base, a maximum of the scores so far
