@@ -177,6 +177,14 @@ def test_write_of_several_heads_at_a_time(nkv, hd, ps):
 
 
 @gpu
+@pytest.mark.parametrize("hd,rot,ps", [(128, 128, 16), (80, 80, 8), (256, 0, 64)])
+@pytest.mark.parametrize("new", [[0, 2], [2, 0], [0, 0, 3], [3, 0, 1, 0], [1, 0, 0, 30, 1, 0] + [0] * 26, [7, 0, 0, 0, 0, 0, 0]])
+def test_write_of_as_many_tokens_as_requests_but_not_one_each(hd, rot, ps, new):
+    assert sum(new) == len(new)
+    test_write(4, 2, hd, ps, rot, [(5 * i) % (ps + 3) for i in range(len(new))], new, True)
+
+
+@gpu
 def test_far_positions():
     """Angles of positions that float32 holds, whose products with a frequency it does not: off by the rounding of the sine's own arithmetic only."""
     nq, nkv, hd, ps = 2, 1, 128, 64

@@ -9,7 +9,7 @@
 // that were there the new scale; then the rows are written, and where the scale has grown the page's earlier rows are read, multiplied by the quotient of the scales
 // (a power of two) and written back.  Which page of which request a block takes follows from a sum over the requests that every block makes itself.  Other blocks
 // take the queries.  Three kernels:
-//   singles: every request brings one token (a decode step), a warp a token and head, no sums over requests;
+//   singles: as many tokens as requests (a decode step), a warp a token and head, no sums over requests;
 //   wide:    heads of 32, 64, 128 or 256 features that are rotated as a whole or not at all: 16-byte accesses, hd / 16 lanes a row, angles of a
 //            page's rows once for several heads;
 //   narrow:  any other head, a warp a row, 4-byte accesses.
@@ -236,7 +236,7 @@ __device__ __forceinline__ void query_heads(const Step& st, int tok, int h0, int
 }
 }  // namespace
 
-// Every request brings one token: a warp a token and key or value head, or a token and heads_a_warp query heads.
+// As many tokens as requests, one each as a rule: a warp a token and key or value head, or a token and heads_a_warp query heads.
 template <int MAXHD>
 __global__ void __launch_bounds__(NT)
 write_8bit_singles_kernel(const __grid_constant__ Step st) {
@@ -251,10 +251,18 @@ write_8bit_singles_kernel(const __grid_constant__ Step st) {
         query_heads<MAXHD>(st, tok, (u - pages) * st.heads_a_warp, min(st.nq, (u - pages + 1) * st.heads_a_warp));
         return;
     }
-    // (a token that no request's bounds hold is padding)
     const int pos = st.positions[tok], slot = st.slots[tok];
-    if (st.cu[tok] != tok || st.cu[tok + 1] != tok + 1 || pos < 0 || slot < 0) return;
+    if (pos < 0 || slot < 0) return;
     const int row0 = pos % st.page_size, page = slot / st.page_size;
+    int n = 1;                                               // as many tokens as requests, but not one each: the first token of a page takes the page's others
+    if (st.cu[tok] != tok || st.cu[tok + 1] != tok + 1) {
+        int b = 0;
+        for (int step = 1 << 30; step; step >>= 1)           // the last request that begins at this token or before
+            if (b + step < st.B && st.cu[b + step] <= tok) b += step;
+        const int lo = st.cu[b], hi = st.cu[b + 1];
+        if (lo < 0 || lo > tok || hi <= tok || hi > st.T || (lo != tok && row0)) return;           // (padding, or not the first)
+        n = min(st.page_size - row0, hi - tok);
+    }
     if (page >= st.num_pages || slot - page * st.page_size != row0) {
         if (lane == 0 && u == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT);
         return;
@@ -269,12 +277,29 @@ write_8bit_singles_kernel(const __grid_constant__ Step st) {
     pdl_wait();
     const float old = row0 ? *scale : 0.f;
     Row<MAXHD> r;
-    r.load(st.qkv + (size_t)tok * st.row_stride + (size_t)(st.nq + (values ? st.nkv : 0) + kvh) * hd, lane, hd, turned);
-    if (!values && st.kw) r.norm(st.kw, st.eps, lane, hd, turned);
-    if (turned) r.turn(cs);
-    const float now = new_scale(__reduce_max_sync(0xffffffffu, r.top()), row0, old), inv = inverse_of(now);
-    unsigned char* dst = cache + (size_t)row0 * hd;
-    r.each(lane, hd, turned, [&](int i, float2 v) { *reinterpret_cast<unsigned short*>(dst + i) = to_e4m3x2(v.x * inv, v.y * inv); });
+    auto take = [&](int i) {
+        if (turned && i > 0) Row<MAXHD>::angles(cs, st.positions[tok + i], st.inv_freq, lane, turned);
+        r.load(st.qkv + (size_t)(tok + i) * st.row_stride + (size_t)(st.nq + (values ? st.nkv : 0) + kvh) * hd, lane, hd, turned);
+        if (!values && st.kw) r.norm(st.kw, st.eps, lane, hd, turned);
+        if (turned) r.turn(cs);
+    };
+    take(0);
+    unsigned top = r.top();
+    for (int i = 1; i < n; ++i) {
+        if (st.slots[tok + i] != slot + i) { if (lane == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT); continue; }
+        take(i);
+        top = max(top, r.top());
+    }
+    const float now = new_scale(__reduce_max_sync(0xffffffffu, top), row0, old), inv = inverse_of(now);
+    for (int i = n - 1; i >= 0; --i) {                       // (the last row, of one token the only one, is still held)
+        if (i > 0 && st.slots[tok + i] != slot + i) continue;
+        if (i < n - 1) {
+            if (turned && i == 0) Row<MAXHD>::angles(cs, pos, st.inv_freq, lane, turned);
+            take(i);
+        }
+        unsigned char* dst = cache + (size_t)(row0 + i) * hd;
+        r.each(lane, hd, turned, [&](int c, float2 v) { *reinterpret_cast<unsigned short*>(dst + c) = to_e4m3x2(v.x * inv, v.y * inv); });
+    }
     if (row0 && now > old) move_rows(cache, row0 * hd, old * inv, lane, 32);       // (false for NaN: rows under a scale that is none need no other)
     if (lane == 0) *scale = now;
 }
