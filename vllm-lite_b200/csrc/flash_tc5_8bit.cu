@@ -192,6 +192,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     int2* s_found = reinterpret_cast<int2*>(s_row_scale + GROUPS * BM);                          // keys, values: [FOUND][BN] cache row (-1: zeros) and factor
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (smem_u32(smem) & 1023u) {                                        // (uniform) never expected; the tiles would be misread
+        pdl_wait();
         if (tid == 0 && err) atomicOr(err, VL_DEV_WAIT_EXPIRED | VL_DEV_IN_FLASH_8BIT);
         return;
     }
@@ -201,9 +202,8 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     int head = (int)blockIdx.x, number = num_tiles * cuts - 1 - (int)blockIdx.y, part = 0, parts = 1;
     if (split) {
         const Split plan(list, split / (nkv * htiles));
-        if (plan.blocks == 0) return;
-        head = (int)blockIdx.x / plan.blocks;
-        if (head >= nkv * htiles) return;
+        head = plan.blocks ? (int)blockIdx.x / plan.blocks : nkv * htiles;
+        if (head >= nkv * htiles) { pdl_wait(); return; }                // (a launch that does not wait would end before the ones ahead of it)
         const int x = (int)blockIdx.x - head * plan.blocks;
         number = -1;
 #pragma unroll
@@ -218,7 +218,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         }
     }
     const Item item(list, number);
-    if (item.n == 0) return;                                             // (the whole block)
+    if (item.n == 0) { pdl_wait(); return; }                             // (the whole block)
     const int from = (int)((long long)item.n * part / parts), n_tiles = (int)((long long)item.n * (part + 1) / parts) - from;
     const int req = item.req, tok0 = item.tok0, pos0 = item.pos0, count = item.count, jt0 = item.jt0 + from;
     const int kvh = head / htiles, grp = nq / nkv, hbase = (head - kvh * htiles) * heads;
@@ -657,7 +657,7 @@ flash_tc5_8bit_join_kernel(const int4* __restrict__ tiles, int num_tiles, int cu
     const List list = {tiles, num_tiles, cuts, tokens, window};
     const int in_list = num_tiles * cuts, head = (int)blockIdx.x / in_list, number = (int)blockIdx.x - head * in_list;
     const Item item(list, number);
-    if (item.n <= MIN_PART) return;
+    if (item.n <= MIN_PART) { pdl_wait(); return; }                      // (every block waits: the launch behind this one waits for no other)
     const Split plan(list, split / (nkv * htiles));
     int first = 0, parts = 0;
 #pragma unroll
@@ -666,11 +666,11 @@ flash_tc5_8bit_join_kernel(const int4* __restrict__ tiles, int num_tiles, int cu
             first = head * plan.blocks + __shfl_sync(0xffffffffu, plan.before[u], number % 32);
             parts = __shfl_sync(0xffffffffu, plan.parts[u], number % 32);
         }
+    pdl_wait();
     if (parts <= 1) return;                                              // (one block had them all)
     const int grp = nq / nkv, kvh = head / htiles, hbase = (head - kvh * htiles) * heads, nheads = min(heads, grp - hbase);
     const int row = threadIdx.x, rr = row & (BM - 1), t = rr / heads, tk = row / BM * tokens + t, h = rr - t * heads;
     if (t >= tokens || tk >= item.count || h >= nheads) return;
-    pdl_wait();
     const float2* ml = partial.ml + (size_t)first * ROWS + row;
     float top = -INFINITY;
     for (int k = 0; k < parts; ++k) top = fmaxf(top, ml[(size_t)k * ROWS].x);
