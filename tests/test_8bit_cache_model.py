@@ -204,6 +204,17 @@ def test_refusals():
         plan_with_8_bit_cache(dataclasses.replace(plan, layers=(dataclasses.replace(block, mixer=None),) + tuple(plan.layers[1:])), "bfloat16")
 
 
+@pytest.mark.parametrize("head_dim", [8, 24, 100, 272, 512])
+def test_heads_that_have_no_form(head_dim):
+    from vllm_lite_b200.engine import load_model_dir
+    from vllm_lite_b200.parts.eight_bit import cache_in_8_bits
+    _, plan, _ = load_model_dir(H.model_dir("A"), "bfloat16", "cpu")
+    layers = list(plan.layers)
+    layers[-1] = dataclasses.replace(layers[-1], mixer=dataclasses.replace(layers[-1].mixer, head_dim=head_dim))
+    with pytest.raises(ValueError, match=f"layer {len(layers) - 1}: .*{head_dim}"):
+        cache_in_8_bits(dataclasses.replace(plan, layers=tuple(layers)))
+
+
 def test_one_cache_has_one_type():
     from vllm_lite_b200.cache import PagedKV
     from vllm_lite_b200.cache.spec import widened

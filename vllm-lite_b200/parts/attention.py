@@ -45,6 +45,8 @@ def has_options(spec: AttentionSpec) -> bool:
 def check_eight_bit_cache(spec: AttentionSpec):
     """Raises ValueError for an attention whose cache has no form in 8 bits."""
     rot = spec.position.dim if hasattr(spec.position, "dim") else 0
+    if not ops.attention_8bit_supported(torch.bfloat16, spec.head_dim):
+        raise ValueError(f"a cache in 8 bits wants heads of 16 to 256 features in steps of 16, got {spec.head_dim}")
     if has_options(spec) or rot % 4:
         raise ValueError("a cache in 8 bits goes with plain grouped-query attention: no gate, sink, cap or bias on its scores, no kept keys, no row work, a "
                          f"rotated part of a multiple of 4 features (got {rot})")
