@@ -682,6 +682,20 @@ def test_tensors_on_the_cpu_are_refused():
 
 
 @gpu
+def test_another_device_than_the_current_one(monkeypatch):
+    cache = Cache(1, 64, 2, 16, 64).fill([64])
+    pos, req, cu, slots = batch(cache, [0], [4])
+    qkv = queries(4, 4, 64, 1, extra=2 * 2 * 64)
+    out = torch.empty(4, 256, dtype=torch.bfloat16, device=DEV)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    for call in (lambda: ops.qk_norm_rope_write_8bit(qkv, pos, slots, cu, None, None, EPS, None, 0, *cache.tensors, 4, 2, 64, cache.err),
+                 lambda: ops.flash_decode_8bit(qkv, out, *cache.tensors, cache.table, req, pos, 4, 2, 64, 0.1, None, 64, cache.err),
+                 lambda: ops.flash_prefill_8bit(qkv, out, *cache.tensors, cache.table, tiles_of([0], [4]), 4, 2, 64, 0.1, None, cache.err)):
+        with pytest.raises(ops.KernelError, match="current device"):
+            call()
+
+
+@gpu
 def test_refusals():
     nq, nkv, hd, ps = 4, 2, 64, 16
     cache = Cache(1, 64, nkv, ps, hd).fill([64])

@@ -927,10 +927,17 @@ def attention_8bit_supported(dtype, head_dim) -> bool:
     return dtype == torch.bfloat16 and head_dim % 16 == 0 and 16 <= head_dim <= 256
 
 
+def _need_here(t, name):
+    """A launch runs on the current device, whose kernels see no other one's memory."""
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise KernelError(f"{name} lies on {t.device}, which is not the current device")
+
+
 def _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim):
     """Its pages and their size."""
     _need(k_cache, E4M3, "k_cache", 4); _need(v_cache, E4M3, "v_cache", 4)
     _need(k_scale, torch.float32, "k_scale", 2); _need(v_scale, torch.float32, "v_scale", 2)
+    _need_here(k_cache, "k_cache")
     shape = pages, heads, page_size, features = k_cache.shape
     if heads != num_kv_heads or features != head_dim or v_cache.shape != shape or k_scale.shape != (pages, heads) or v_scale.shape != (pages, heads):
         raise KernelError(f"a cache in 8 bits [pages, {num_kv_heads}, page size, {head_dim}] has scales [pages, {num_kv_heads}]: got {tuple(shape)}, "
@@ -954,6 +961,7 @@ def qk_norm_rope_write_8bit(qkv, positions, slots, cu_seqlens, q_weight, k_weigh
     one being the request's own.  One launch writes a page for one request only.  q goes to q_out [T, nq hd], or stays in qkv.  rotary_dim is a
     multiple of 4.  Angles are those of the exact products position * inv_freq."""
     _need(qkv, torch.bfloat16, "qkv", 2); _need(positions, torch.int32, "positions", 1)
+    _need_here(qkv, "qkv")
     _need_heads(num_heads, num_kv_heads, head_dim, "qk_norm_rope_write_8bit")
     T, width = qkv.shape
     if width != (num_heads + 2 * num_kv_heads) * head_dim or positions.numel() != T:
@@ -1002,6 +1010,7 @@ def flash_decode_8bit_scratch(num_tokens, num_heads, num_kv_heads, head_dim):
 
 def _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window, name):
     _need(q, torch.bfloat16, "q", 2); _need(out, torch.bfloat16, "out", 2); _need(block_table, torch.int32, "block_table", 2)
+    _need_here(q, "q")
     _need_heads(num_heads, num_kv_heads, head_dim, name)
     pages, page_size = _need_8bit_cache(k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim)
     T, width = q.shape
