@@ -396,6 +396,25 @@ def test_few_tokens_with_many_keys(nq, nkv, hd, ps, window, own):
 
 
 @gpu
+@pytest.mark.parametrize("nq,nkv,hd,ps,window,tokens", [(32, 8, 128, 64, None, 1260), (64, 8, 64, 16, None, 640), (128, 16, 32, 64, 1200, 700), (40, 8, 256, 64, None, 600)])
+def test_last_round_of_few_blocks(nq, nkv, hd, ps, window, tokens):
+    """More blocks than SMs and few of them in the last round, whose keys are shared out; prompts of several lengths, so that some have too few keys for it."""
+    before, new = [700, 0, 900], [tokens - 300, 200, 100]
+    cache = Cache(len(new), max(b + n for b, n in zip(before, new)), nkv, ps, hd, seed=4).fill([b + n for b, n in zip(before, new)], seed=hd + 1)
+    pos, req, _, _ = batch(cache, before, new)
+    q = queries(tokens, nq, hd, 9)
+    out = torch.full((tokens, nq * hd), 3.0, dtype=torch.bfloat16, device=DEV)
+    whole = torch.full_like(out, 3.0)
+    tiles = tiles_of(before, new)
+    for o, scratch in ((out, None), (whole, torch.empty(ops.flash_prefill_8bit_scratch(hd, DEV), device=DEV))):
+        ops.flash_prefill_8bit(q, o, *cache.tensors, cache.table, tiles, nq, nkv, hd, hd ** -0.5, window, cache.err, scratch=scratch)
+    assert int(cache.err) == 0 and torch.equal(out, whole)
+    g = torch.Generator().manual_seed(1)
+    check_attention(cache, q, out, pos, req, nq, window, hd ** -0.5, sorted({0, 1, 63, 64, tokens - 301, tokens - 300, tokens - 101, tokens - 100, tokens - 1}
+                                                                            | set(torch.randint(0, tokens, (12,), generator=g).tolist())))
+
+
+@gpu
 @pytest.mark.parametrize("which", ["k_scale", "v_scale"])
 def test_a_lost_page_among_shared_keys(which):
     """One share of the keys is none: so is the result of those who read it, whatever share it is, and nobody else's."""

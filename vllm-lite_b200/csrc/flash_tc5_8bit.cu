@@ -19,9 +19,10 @@
 //        keys of NaN and values of zero: who may read it gets NaN, rows that may not replace the score;
 //   one warp a query tile   issues S = Q K^T (both K-major) into one of two score buffers and O += P V (P from TMEM, V as stored: N contiguous).
 // Where a launch has so few tokens that half of the SMs would be without a block, each item's keys are shared out among several, which leave base, sum and
-// output as they are for a second launch to join.
+// output as they are for a second launch to join.  So are the keys of the items that would be the few blocks of a last round.
 //
-// Measured in a graph (32 heads of 128, 8 KV heads): a prompt of 2,048 tokens 54 us, 0.64 PFLOP/s; three portions of 512 at position 2,500 112 us, 0.57; 8 tokens
+// Measured in a graph (32 heads of 128, 8 KV heads): a prompt of 2,048 tokens 54 us, 0.64 PFLOP/s; three portions of 512 at position 2,500 92 us, 0.70
+// (every block whole: 112); 8 tokens
 // behind 8,000 keys 26 us.  A step of 64 keys takes a block 1.0 us where exponentials alone (16 a cycle and SM) take 0.54 and the products 0.55: two warps of
 // softmax to a scheduler do not hide their own latencies, and 96 registers a thread allow no more of them.  What a block takes besides, some 8 us: queries and
 // scales (3 us), the first keys (2), the last product and the output (2).  Steps on the way: P through shared memory and keys and values by the same four warps 75 and 165 us.
@@ -52,7 +53,7 @@ constexpr unsigned KV_STAGE = BN * CB * ROW_BYTES;     // CB blocks of [64 rows]
 constexpr int STAGES = HD <= 128 ? 3 : 2;              // of keys, and of values
 constexpr unsigned TILE_BYTES = GROUPS * Q_BYTES + 2 * STAGES * KV_STAGE;
 constexpr int ROWS = GROUPS * BM;
-constexpr int MIN_PART = 4, MOST_ITEMS = 160;          // splitting of keys: key tiles of a block at least, items a head at most
+constexpr int MIN_PART = 4, MOST_ITEMS = 160, MOST_ROUNDS = 8;        // splitting of keys: key tiles of a block at least, items a head and rounds at most
 constexpr int FOUND = 8;                               // key tiles whose rows are looked up ahead
 constexpr unsigned SMEM_BYTES = TILE_BYTES + 512 + GROUPS * BM * 4 + 2 * FOUND * BN * 8;
 constexpr unsigned TMEM_COLS = 512;                    // scores 2 x 64 a query tile, behind them the outputs
@@ -168,7 +169,12 @@ struct Split {
         }
     }
 };
-struct Partial { float4* out; float2* ml; };                             // out [blocks][HD / 4][ROWS], ml (base, sum) [blocks][ROWS]
+// Where a launch has more blocks than SMs and its last round is short of blocks: that round's items, with the shortest rows of keys, in parts each.
+struct Tail {
+    int whole, parts;                                                    // items ahead of them; parts each, 0: none
+    __device__ __forceinline__ int parts_of(const Item& item) const { return min(parts, (item.n + MIN_PART - 1) / MIN_PART); }
+};
+struct Partial { float4* out; float2* ml; };                             // out [blocks with parts][HD / 4][ROWS], ml (base, sum) [blocks with parts][ROWS]
 }  // namespace
 
 // tiles[i] = {row of the block table, index of the tile's first token in the step, tokens (<= 128), position of the first}
@@ -176,7 +182,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict__ out, const unsigned char* __restrict__ kcache,
                       const unsigned char* __restrict__ vcache, const float* __restrict__ kscale, const float* __restrict__ vscale,
                       const int* __restrict__ block_table, int max_blocks, const int4* __restrict__ tiles, int num_tiles, int nq, int nkv, int page_size,
-                      int num_pages, float scale_log2, int window, unsigned* err, int heads, int htiles, int tokens, int cuts, int split, Partial partial) {
+                      int num_pages, float scale_log2, int window, unsigned* err, int heads, int htiles, int tokens, int cuts, int split, Tail tail, Partial partial) {
     extern __shared__ __align__(1024) unsigned char smem[];              // (the block's only shared memory, so it begins the window)
     unsigned char* Qs = smem;                                            // GROUPS
     unsigned char* Ks = Qs + GROUPS * Q_BYTES;                           // STAGES
@@ -199,9 +205,16 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     pdl_launch_dependents();
     // This block's item and its key tiles from .. to; the items with the longest rows of keys first, or a share of an item's keys.
     const List list = {tiles, num_tiles, cuts, tokens, window};
-    int head = (int)blockIdx.x, number = num_tiles * cuts - 1 - (int)blockIdx.y, part = 0, parts = 1;
+    int head = (int)blockIdx.x, number = num_tiles * cuts - 1 - (int)blockIdx.y, part = 0, parts = 1, place = -1;
+    if (tail.parts) {
+        place = (int)blockIdx.x - tail.whole;
+        const int id = place < 0 ? (int)blockIdx.x : tail.whole + place / tail.parts;
+        head = id % (nkv * htiles);
+        number = num_tiles * cuts - 1 - id / (nkv * htiles);
+    }
     if (split) {
         const Split plan(list, split / (nkv * htiles));
+        place = (int)blockIdx.x;
         head = plan.blocks ? (int)blockIdx.x / plan.blocks : nkv * htiles;
         if (head >= nkv * htiles) { pdl_wait(); return; }                // (a launch that does not wait would end before the ones ahead of it)
         const int x = (int)blockIdx.x - head * plan.blocks;
@@ -218,7 +231,8 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         }
     }
     const Item item(list, number);
-    if (item.n == 0) { pdl_wait(); return; }                             // (the whole block)
+    if (tail.parts && place >= 0) { part = place % tail.parts; parts = tail.parts_of(item); }
+    if (item.n == 0 || part >= parts) { pdl_wait(); return; }            // (the whole block)
     const int from = (int)((long long)item.n * part / parts), n_tiles = (int)((long long)item.n * (part + 1) / parts) - from;
     const int req = item.req, tok0 = item.tok0, pos0 = item.pos0, count = item.count, jt0 = item.jt0 + from;
     const int kvh = head / htiles, grp = nq / nkv, hbase = (head - kvh * htiles) * heads;
@@ -596,7 +610,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             tc5_fence_after();
             const float unit = power_of_two(top_v - FOLD);
             const bool live = row < tokens * heads && tk < count;
-            float4* dst = partial.out + (size_t)blockIdx.x * (HD / 4) * ROWS + gr * BM + row;
+            float4* dst = partial.out + (size_t)place * (HD / 4) * ROWS + gr * BM + row;
 #pragma unroll
             for (int c0 = 0; c0 < HD; c0 += 32) {
                 unsigned ov[32];
@@ -607,7 +621,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                         dst[(size_t)(c0 / 4 + i) * ROWS] = make_float4(__uint_as_float(ov[4 * i]) * unit, __uint_as_float(ov[4 * i + 1]) * unit,
                                                                        __uint_as_float(ov[4 * i + 2]) * unit, __uint_as_float(ov[4 * i + 3]) * unit);
             }
-            if (live) partial.ml[(size_t)blockIdx.x * ROWS + gr * BM + row] = make_float2(m, l);
+            if (live) partial.ml[(size_t)place * ROWS + gr * BM + row] = make_float2(m, l);
         } else {
             tc5_fence_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l, unit = power_of_two(top_v - FOLD);
@@ -652,20 +666,22 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
 // item and 16 columns, a thread a row.
 __global__ void __launch_bounds__(ROWS)
 flash_tc5_8bit_join_kernel(const int4* __restrict__ tiles, int num_tiles, int cuts, int tokens, int window, int nq, int nkv, int heads, int htiles, int split,
-                           Partial partial, bf16* __restrict__ out) {
+                           Tail tail, Partial partial, bf16* __restrict__ out) {
     pdl_launch_dependents();
     const List list = {tiles, num_tiles, cuts, tokens, window};
-    const int in_list = num_tiles * cuts, head = (int)blockIdx.x / in_list, number = (int)blockIdx.x - head * in_list;
+    const int in_list = num_tiles * cuts, id = tail.whole + (int)blockIdx.x, head = id % (nkv * htiles), number = in_list - 1 - id / (nkv * htiles);
     const Item item(list, number);
     if (item.n <= MIN_PART) { pdl_wait(); return; }                      // (every block waits: the launch behind this one waits for no other)
-    const Split plan(list, split / (nkv * htiles));
-    int first = 0, parts = 0;
+    int first = (int)blockIdx.x * tail.parts, parts = tail.parts_of(item);
+    if (split) {
+        const Split plan(list, split / (nkv * htiles));
 #pragma unroll
-    for (int u = 0; u < Split::U; ++u)
-        if (number / 32 == u) {
-            first = head * plan.blocks + __shfl_sync(0xffffffffu, plan.before[u], number % 32);
-            parts = __shfl_sync(0xffffffffu, plan.parts[u], number % 32);
-        }
+        for (int u = 0; u < Split::U; ++u)
+            if (number / 32 == u) {
+                first = head * plan.blocks + __shfl_sync(0xffffffffu, plan.before[u], number % 32);
+                parts = __shfl_sync(0xffffffffu, plan.parts[u], number % 32);
+            }
+    }
     pdl_wait();
     if (parts <= 1) return;                                              // (one block had them all)
     const int grp = nq / nkv, kvh = head / htiles, hbase = (head - kvh * htiles) * heads, nheads = min(heads, grp - hbase);
@@ -714,25 +730,29 @@ extern "C" int vl_flash_prefill_8bit(const void* q, int q_stride, void* out, con
     if ((long long)num_pages * nkv * page_size >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
     const int grp = nq / nkv, heads = grp < BM ? grp : BM, htiles = (grp + heads - 1) / heads, tokens = BM / heads;
     const int cuts = (128 + GROUPS * tokens - 1) / (GROUPS * tokens);
-    if ((long long)num_tiles * cuts > 65535) return VL_ERR_UNSUPPORTED;
+    if ((long long)num_tiles * cuts > 65535 || (long long)num_tiles * cuts * nkv * htiles >= (1ll << 31)) return VL_ERR_UNSUPPORTED;
     int device, sms;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(flash_tc5_8bit_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
     if (e != cudaSuccess) return (int)e;
-    // Keys are split where the rows of keys may be long and at least every second SM would be without a block.
+    // Keys are shared out where their rows may be long, if at least every second SM would be without a block, or without one in the last of few rounds (three
+    // portions of 512 at position 2,500, 184 blocks on 148 SMs: 112 us with every block whole).
     const int in_list = num_tiles * cuts;
     const long long blocks = (long long)in_list * nkv * htiles, reach = (long long)max_blocks * page_size;
     const long long keys = window > 0 && window + GROUPS * tokens < reach ? window + GROUPS * tokens : reach;
-    const int split = scratch && in_list <= MOST_ITEMS && 2 * blocks <= sms && keys >= 2 * MIN_PART * BN ? sms : 0;
-    if (split && floats < (long long)sms * ROWS * (HD + 2)) return VL_ERR_ARGUMENT;
-    const Partial partial = {(float4*)scratch, split ? (float2*)(scratch + (long long)sms * ROWS * HD) : nullptr};
+    const bool shared = scratch && keys >= 2 * MIN_PART * BN;
+    const int split = shared && in_list <= MOST_ITEMS && 2 * blocks <= sms ? sms : 0, over = (int)(blocks % sms);
+    const bool last = shared && blocks > sms && blocks <= MOST_ROUNDS * sms && over && 2 * over <= sms;
+    const Tail tail = {(int)(last ? blocks - over : split ? 0 : blocks), last ? sms / over : 0};
+    if ((split || last) && floats < (long long)sms * ROWS * (HD + 2)) return VL_ERR_ARGUMENT;
+    const Partial partial = {(float4*)scratch, split || last ? (float2*)(scratch + (long long)sms * ROWS * HD) : nullptr};
     cudaStream_t s = (cudaStream_t)stream;
-    const int rc = vl_launch_waiting(flash_tc5_8bit_kernel, split ? dim3(sms) : dim3(nkv * htiles, in_list), dim3(NTHREADS), SMEM_BYTES, s, (const bf16*)q, q_stride,
+    const int rc = vl_launch_waiting(flash_tc5_8bit_kernel, split ? dim3(sms) : last ? dim3(tail.whole + over * tail.parts) : dim3(nkv * htiles, in_list), dim3(NTHREADS), SMEM_BYTES, s, (const bf16*)q, q_stride,
                                      (bf16*)out, (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks,
                                      (const int4*)tiles, num_tiles, nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, err, heads, htiles, tokens,
-                                     cuts, split, partial);
-    if (rc != VL_OK || !split) return rc;
-    return vl_launch_waiting(flash_tc5_8bit_join_kernel, dim3((unsigned)blocks, HD / 16), dim3(ROWS), 0, s, (const int4*)tiles, num_tiles, cuts, tokens, window, nq,
-                             nkv, heads, htiles, split, partial, (bf16*)out);
+                                     cuts, split, tail, partial);
+    if (rc != VL_OK || !(split || last)) return rc;
+    return vl_launch_waiting(flash_tc5_8bit_join_kernel, dim3((unsigned)(split ? blocks : over), HD / 16), dim3(ROWS), 0, s, (const int4*)tiles, num_tiles, cuts, tokens, window, nq,
+                             nkv, heads, htiles, split, tail, partial, (bf16*)out);
 }

@@ -1090,7 +1090,7 @@ def flash_prefill_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, 
         _need(scratch, torch.float32, "scratch", 1)
         if scratch.numel() < floats:
             raise KernelError(f"flash_prefill_8bit: {floats} floats of scratch are wanted, got {scratch.numel()}")
-    elif 2 * count * num_kv_heads <= _sm_count(device):                  # (keys of more tiles are not shared out)
+    elif count * num_kv_heads <= 8 * _sm_count(device):                  # (keys of more tiles are not shared out)
         floats = flash_prefill_8bit_scratch(head_dim, device)
         scratch = torch.empty(floats, dtype=torch.float32, device=device)
     _check(_fn("flash_tc5_8bit", "vl_flash_prefill_8bit", {"FA_HD": head_dim})(
