@@ -21,13 +21,13 @@
 // Where a launch has so few tokens that half of the SMs would be without a block, each item's keys are shared out among several, which leave base, sum and
 // output as they are for a second launch to join.  So are the keys of the items that would be the few blocks of a last round.
 //
-// Measured in a graph (32 heads of 128, 8 KV heads): a prompt of 2,048 tokens 54 us, 0.64 PFLOP/s; three portions of 512 at position 2,500 92 us, 0.70
-// (every block whole: 112); 8 tokens
-// behind 8,000 keys 26 us.  A step of 64 keys takes a block 1.0 us where exponentials alone (16 a cycle and SM) take 0.54 and the products 0.55: two warps of
-// softmax to a scheduler do not hide their own latencies, and 96 registers a thread allow no more of them.  What a block takes besides, some 8 us: queries and
-// scales (3 us), the first keys (2), the last product and the output (2).  Steps on the way: P through shared memory and keys and values by the same four warps 75 and 165 us.
-// Taken back: turns between the two query tiles' exponentials, scores in parts of 16 or 32 columns, two loading warps with more registers, one
-// block walking several items (its state costs registers and a quarter of the speed).
+// Measured in a graph (32 heads of 128, 8 KV heads): a prompt of 2,048 tokens 54 us, 0.64 PFLOP/s; three portions of 512 at position 2,500 91 us, 0.70 (every
+// block whole: 112); 8 tokens behind 8,000 keys 27 us.  A step of 64 keys takes a block 1.0 us where exponentials alone (16 a cycle and SM) take 0.54, the products 0.55
+// and shared memory's traffic 0.65.  No unit is full (issue slots and the exponential unit about half, ALUs and tensor cores a third): a step is a chain of waits, loads
+// from TMEM, weights and votes.  What a block takes besides, some 8 us: queries and scales (3 us), the first keys (2), the last product and the output (2).
+// Steps on the way: P through shared memory and keys and values by the same four warps 75 and 165 us.
+// Taken back: two threads a row (three portions of 512 94 for 92), turns between the two query tiles' exponentials (103 and 119 for 117), scores in parts of
+// 16 or 32 columns (119 and 116 for 114), two loading warps with more registers (115), one block walking several items (its state costs registers and a quarter of the speed).
 // Roundings: queries times a power of two of their row (largest number in [2^14, 2^15)) and the probabilities, 2^7 p with p up to 2^8, are halves.
 // Every wait on an mbarrier is bounded; when one expires the block records VL_DEV_WAIT_EXPIRED, stops, and still frees its TMEM.
 #include "cache_8bit.cuh"
@@ -367,7 +367,9 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         const unsigned char* my_cache = cache + c0 * 16;
         const int2* my_found = found + r0;
         auto place = [&](int r, int c, int half) { return (unsigned)(c >> 2) * (BN * ROW_BYTES) + swizzled(r, 2 * (c & 3) + half); };
-        unsigned char *my_a = stages + place(r0, c0, 0), *my_b = stages + place(r0, c0, 1);
+        // (eight lanes store 16 bytes at a time, and pieces 4 on lie in another block of rows but in the banks of pieces 0 to 3: they store their second half first)
+        const bool flip = PIECES >= 8 && (c0 & 4);
+        unsigned char *my_a = stages + place(r0, c0, flip), *my_b = stages + place(r0, c0, !flip);
         auto load = [&](uint4 (&x)[EACH], int it) {
             const int2* f = my_found + (it % FOUND) * BN;
 #pragma unroll
@@ -391,7 +393,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                 const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
                 if (!EVEN && idx >= BN * PIECES) continue;
                 const unsigned f = (unsigned)fold[EVEN ? i * APART : r - r0].y;
-                const unsigned* w = &x[i].x;
+                const unsigned w[4] = {EVEN && flip ? x[i].z : x[i].x, EVEN && flip ? x[i].w : x[i].y, EVEN && flip ? x[i].x : x[i].z, EVEN && flip ? x[i].y : x[i].w};
                 uint4 a, b;
                 a.x = times(half2_low(w[0]), f); a.y = times(half2_high(w[0]), f); a.z = times(half2_low(w[1]), f); a.w = times(half2_high(w[1]), f);
                 b.x = times(half2_low(w[2]), f); b.y = times(half2_high(w[2]), f); b.z = times(half2_low(w[3]), f); b.w = times(half2_high(w[3]), f);
