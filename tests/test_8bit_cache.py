@@ -177,6 +177,13 @@ def test_write_of_several_heads_at_a_time(nkv, hd, ps):
 
 
 @gpu
+@pytest.mark.parametrize("nkv,hd,ps", [(3, 128, 64), (5, 64, 100), (2, 256, 48), (4, 32, 256), (2, 112, 100)])
+def test_write_of_one_long_portion_among_short_ones(nkv, hd, ps):
+    """Far more rows for some pages than portions have on average."""
+    test_write(nkv * 3, nkv, hd, ps, hd, [7] + [(11 * i) % ps for i in range(9)], [2 * ps + 30] + [1] * 4 + [2] * 5, True)
+
+
+@gpu
 @pytest.mark.parametrize("hd,rot,ps", [(128, 128, 16), (80, 80, 8), (256, 0, 64)])
 @pytest.mark.parametrize("new", [[0, 2], [2, 0], [0, 0, 3], [3, 0, 1, 0], [1, 0, 0, 30, 1, 0] + [0] * 26, [7, 0, 0, 0, 0, 0, 0]])
 def test_write_of_as_many_tokens_as_requests_but_not_one_each(hd, rot, ps, new):
