@@ -251,54 +251,55 @@ write_8bit_singles_kernel(const __grid_constant__ Step st) {
         query_heads<MAXHD>(st, tok, (u - pages) * st.heads_a_warp, min(st.nq, (u - pages + 1) * st.heads_a_warp));
         return;
     }
-    const int pos = st.positions[tok], slot = st.slots[tok];
+    const int pos = st.positions[tok], slot = st.slots[tok], c0 = st.cu[tok], c1 = st.cu[tok + 1];
     if (pos < 0 || slot < 0) return;
     const int row0 = pos % st.page_size, page = slot / st.page_size;
-    int n = 1;                                               // as many tokens as requests, but not one each: the first token of a page takes the page's others
-    if (st.cu[tok] != tok || st.cu[tok + 1] != tok + 1) {
-        int b = 0;
-        for (int step = 1 << 30; step; step >>= 1)           // the last request that begins at this token or before
-            if (b + step < st.B && st.cu[b + step] <= tok) b += step;
-        const int lo = st.cu[b], hi = st.cu[b + 1];
-        if (lo < 0 || lo > tok || hi <= tok || hi > st.T || (lo != tok && row0)) return;           // (padding, or not the first)
-        n = min(st.page_size - row0, hi - tok);
-    }
     if (page >= st.num_pages || slot - page * st.page_size != row0) {
         if (lane == 0 && u == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT);
         return;
     }
     const bool values = u & 1;
     const int kvh = u >> 1, turned = values || !st.inv_freq ? 0 : st.rot;
+    int n = 1;                                               // as many tokens as requests, but not one each: the first token of a page takes the page's others
+    if (c0 != tok || c1 != tok + 1) {
+        int b = 0;
+#pragma unroll 1
+        for (int step = 1 << 30; step; step >>= 1)           // the last request that begins at this token or before
+            if (b + step < st.B && st.cu[b + step] <= tok) b += step;
+        const int lo = st.cu[b], hi = st.cu[b + 1];
+        if (lo < 0 || lo > tok || hi <= tok || hi > st.T || (lo != tok && row0)) return;           // (padding, or not the first)
+        n = min(st.page_size - row0, hi - tok);
+    }
     const size_t head = (size_t)page * st.nkv + kvh;
     unsigned char* cache = (values ? st.vcache : st.kcache) + head * st.page_size * hd;
     float* scale = (values ? st.vscale : st.kscale) + head;
-    float4 cs[Row<MAXHD>::UR];
-    if (turned) Row<MAXHD>::angles(cs, pos, st.inv_freq, lane, turned);
-    pdl_wait();
-    const float old = row0 ? *scale : 0.f;
+    // Two passes over the rows, one behind the other in the same code; a single row stays in registers in between.  (With the rare case in code of its own, unrolled
+    // or called, each layer of a step took 4 us more: decode at batch 1 303 tokens/s, 318 so.)
     Row<MAXHD> r;
-    auto take = [&](int i) {
-        if (turned && i > 0) Row<MAXHD>::angles(cs, st.positions[tok + i], st.inv_freq, lane, turned);
-        r.load(st.qkv + (size_t)(tok + i) * st.row_stride + (size_t)(st.nq + (values ? st.nkv : 0) + kvh) * hd, lane, hd, turned);
-        if (!values && st.kw) r.norm(st.kw, st.eps, lane, hd, turned);
-        if (turned) r.turn(cs);
-    };
-    take(0);
-    unsigned top = r.top();
-    for (int i = 1; i < n; ++i) {
-        if (st.slots[tok + i] != slot + i) { if (lane == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT); continue; }
-        take(i);
-        top = max(top, r.top());
-    }
-    const float now = new_scale(__reduce_max_sync(0xffffffffu, top), row0, old), inv = inverse_of(now);
-    for (int i = n - 1; i >= 0; --i) {                       // (the last row, of one token the only one, is still held)
-        if (i > 0 && st.slots[tok + i] != slot + i) continue;
-        if (i < n - 1) {
-            if (turned && i == 0) Row<MAXHD>::angles(cs, pos, st.inv_freq, lane, turned);
-            take(i);
+    unsigned top = 0;
+    float old = 0.f, now = 0.f, inv = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < 2 * n; ++k) {
+        const int i = k < n ? k : k - n;
+        if (i && st.slots[tok + i] != slot + i) { if (lane == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT); continue; }
+        if (k == n) {
+            now = new_scale(__reduce_max_sync(0xffffffffu, top), row0, old);
+            inv = inverse_of(now);
         }
-        unsigned char* dst = cache + (size_t)(row0 + i) * hd;
-        r.each(lane, hd, turned, [&](int c, float2 v) { *reinterpret_cast<unsigned short*>(dst + c) = to_e4m3x2(v.x * inv, v.y * inv); });
+        if (k == 0 || n > 1) {
+            float4 cs[Row<MAXHD>::UR];
+            if (turned) Row<MAXHD>::angles(cs, pos + i, st.inv_freq, lane, turned);
+            pdl_wait();
+            if (k == 0 && row0) old = *scale;
+            r.load(st.qkv + (size_t)(tok + i) * st.row_stride + (size_t)(st.nq + (values ? st.nkv : 0) + kvh) * hd, lane, hd, turned);
+            if (!values && st.kw) r.norm(st.kw, st.eps, lane, hd, turned);
+            if (turned) r.turn(cs);
+        }
+        if (k < n) top = max(top, r.top());
+        else {
+            unsigned char* dst = cache + (size_t)(row0 + i) * hd;
+            r.each(lane, hd, turned, [&](int c, float2 v) { *reinterpret_cast<unsigned short*>(dst + c) = to_e4m3x2(v.x * inv, v.y * inv); });
+        }
     }
     if (row0 && now > old) move_rows(cache, row0 * hd, old * inv, lane, 32);       // (false for NaN: rows under a scale that is none need no other)
     if (lane == 0) *scale = now;
