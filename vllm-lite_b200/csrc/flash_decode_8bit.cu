@@ -34,7 +34,6 @@
 // Keys outside lo..p, or on pages that the table does not hold (flagged), weigh nothing whatever their bytes and scales are; a page whose scale is not a
 // number makes the result NaN where one of its keys is read.
 #include "cache_8bit.cuh"
-#include <type_traits>
 
 #ifndef FA_HD
 #define FA_HD 128
@@ -413,10 +412,9 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
         auto note = [&](const Where& w, int u, int stage) {
             if (lane < (WIDE ? 1 : 16)) s_scale[warp][stage][u][lane] = w.vs != w.vs ? make_float2(w.vs, 0.f) : make_float2(w.ks, w.vs);
         };
-        // PART: a step with keys that are not read.  The step's tiles side by side, so that one's chain of products, exponentials and conversions
-        // runs beside another's.
-        auto work = [&](auto partly, int st, int stage) {
-            constexpr bool PART = decltype(partly)::value;
+        // The step's tiles side by side, so that one's chain of products, exponentials and conversions runs beside another's.  (One code for steps with and without
+        // keys that are not read: with one for each, layers of a step took 0.3 us more, for what the comparisons save.)
+        auto work = [&](int st, int stage) {
             const unsigned char* const keys = ring + stage * STAGE + g * KS + t * KL * 4;
             const unsigned char* const values = ring + stage * STAGE + 16 * KS + 2 * t * VS + g * VL * 4;
             float2 scale0[SUB], scale1[SUB];
@@ -452,14 +450,14 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
             for (int u = 0; u < SUB; ++u) {
                 const int k0 = st * BN + (warp * SUB + u) * 16;
                 // keys that are not read weigh nothing: those outside the piece, and those without a page, whose scale is left 0
-                none0[u] = PART && (scale0[u].x == 0.f || k0 + g < pc.c0 || k0 + g >= pc.c1);
-                none1[u] = PART && (scale1[u].x == 0.f || k0 + g + 8 < pc.c0 || k0 + g + 8 >= pc.c1);
+                none0[u] = scale0[u].x == 0.f || k0 + g < pc.c0 || k0 + g >= pc.c1;
+                none1[u] = scale1[u].x == 0.f || k0 + g + 8 < pc.c0 || k0 + g + 8 >= pc.c1;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         x[u][n][c] = fmaf(s[u][n][c], (c < 2 ? scale0[u].x : scale1[u].x) * qs[n][c & 1], less[n][c & 1]);
-                        if (PART && (c < 2 ? none0[u] : none1[u])) x[u][n][c] = -INFINITY;
+                        if (c < 2 ? none0[u] : none1[u]) x[u][n][c] = -INFINITY;
                         top = fmaxf(top, x[u][n][c]);        // (no base yet: +inf)
                     }
             }
@@ -577,12 +575,7 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
                 advance();
                 copies_wait<1>();
                 __syncwarp();                                // every lane's copies have landed
-                const int k0 = st * BN + warp * SUB * 16;
-                bool whole = k0 >= pc.c0 && k0 + 16 * SUB <= pc.c1;
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) whole = whole && s_scale[warp][stage][u][0].x != 0.f;
-                if (whole) work(std::false_type(), st, stage);
-                else work(std::true_type(), st, stage);
+                work(st, stage);
                 __syncwarp();                                // the stage has been read
             }
         } else {
@@ -603,7 +596,7 @@ flash_decode_8bit_kernel(const bf16* __restrict__ q, int q_stride, const unsigne
                 for (int u = 0; u < SUB; ++u) w[u] = find((st + 2) * SUB + u);             // (used a step later)
                 copies_wait<1>();
                 __syncwarp();
-                work(std::true_type(), st, stage);
+                work(st, stage);
                 __syncwarp();
             }
         }
