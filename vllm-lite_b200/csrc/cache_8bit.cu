@@ -14,7 +14,7 @@
 //            page's rows once for several heads;
 //   narrow:  any other head, a warp a row, 4-byte accesses.
 //
-// Measured in a graph: 64 single tokens of 32 + 2 x 8 heads of 128 4.9 us (a block a page took 16.4, most of it in blocks of one row); a portion of 4,096 tokens
+// Measured in a graph: 64 single tokens of 32 + 2 x 8 heads of 128 4.5 us (a block a page took 16.4, most of it in blocks of one row); a portion of 4,096 tokens
 // at position 700 27.9 us, 92 MB at 3.3 TB/s (4-byte accesses 108); five portions of 77 with heads of 80 and pages of 16 7.0 us.  Bound by latencies: single tokens by loads behind
 // one another (position and slot, the scale, the row, the page's rows where a scale grows), a portion by the loads of a page's rows and the barrier before its scale is known.
 //
@@ -581,8 +581,8 @@ extern "C" int vl_qk_norm_rope_write_8bit(const void* qkv, int row_stride, void*
     const long long pages = slots ? (T < (long long)T / page_size + 2ll * B ? T : (long long)T / page_size + 2ll * B) : 0;
     const bool wide = (hd == 32 || hd == 64 || hd == 128 || hd == 256) && (!inv_freq || rot == hd) && row_stride % 8 == 0 && q_stride % 8 == 0 &&
                       (((uintptr_t)qkv | (uintptr_t)q_out) & 15) == 0;
-    // Several heads share a page's angles where blocks are enough without and a page has rows for its threads (4,096 tokens: 4 heads 27.8 us, 2 29.7, 1 34.5;
-    // 300 portions of 8: 4 heads 21, 1 12).
+    // Several heads share a page's angles where blocks are enough without and a page has rows for its threads (4,096 tokens, 8 KV heads: 4 heads 27.8 us, 2 29.7,
+    // 1 34.5; 8 portions of 300, 4 KV heads: 4 heads 21, 1 12).
     st.heads_a_warp = wide ? (T >= 256 ? 16 : 8) : (T >= 256 ? 8 : (T >= 32 ? 4 : 2));
     st.heads_a_block = !wide || T < 32 * pages || pages * nkv < 256 ? 1 : (pages * nkv < 512 ? 2 : 4);
     // Two warps a head where they hold the rows that a page can get: small pages and short portions leave none idle (2,048 tokens on pages of 16: 18 us, 30 with

@@ -720,7 +720,8 @@ flash_tc5_8bit_join_kernel(const int4* __restrict__ tiles, int num_tiles, int cu
 
 extern "C" int vl_flash_prefill_8bit_head_dim() { return HD; }
 
-// scratch (may be null: no keys are split): SMs * ROWS * (hd + 2) floats from a 16-byte boundary.  q rows and `out` rows begin on 16 bytes; caches [pages, nkv, page_size, hd] e4m3, scales [pages, nkv]; pages of any number of positions.
+// scratch (may be null: no keys are shared out): SMs * ROWS * (hd + 2) floats from a 16-byte boundary.  q rows and `out` rows begin on 16 bytes; caches
+// [pages, nkv, page_size, hd] e4m3, scales [pages, nkv]; pages of any number of positions.
 extern "C" int vl_flash_prefill_8bit(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const float* kscale,
                                      const float* vscale, const int* block_table, int max_blocks, const int* tiles, int num_tiles, int nq, int nkv,
                                      int hd, int page_size, int num_pages, float scale, int window, float* scratch, long long floats, unsigned* err, void* stream) {
@@ -750,11 +751,12 @@ extern "C" int vl_flash_prefill_8bit(const void* q, int q_stride, void* out, con
     if ((split || last) && floats < (long long)sms * ROWS * (HD + 2)) return VL_ERR_ARGUMENT;
     const Partial partial = {(float4*)scratch, split || last ? (float2*)(scratch + (long long)sms * ROWS * HD) : nullptr};
     cudaStream_t s = (cudaStream_t)stream;
-    const int rc = vl_launch_waiting(flash_tc5_8bit_kernel, split ? dim3(sms) : last ? dim3(tail.whole + over * tail.parts) : dim3(nkv * htiles, in_list), dim3(NTHREADS), SMEM_BYTES, s, (const bf16*)q, q_stride,
+    const int rc = vl_launch_waiting(flash_tc5_8bit_kernel, split ? dim3(sms) : last ? dim3(tail.whole + over * tail.parts) : dim3(nkv * htiles, in_list),
+                                     dim3(NTHREADS), SMEM_BYTES, s, (const bf16*)q, q_stride,
                                      (bf16*)out, (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks,
                                      (const int4*)tiles, num_tiles, nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, err, heads, htiles, tokens,
                                      cuts, split, tail, partial);
     if (rc != VL_OK || !(split || last)) return rc;
-    return vl_launch_waiting(flash_tc5_8bit_join_kernel, dim3((unsigned)(split ? blocks : over), HD / 16), dim3(ROWS), 0, s, (const int4*)tiles, num_tiles, cuts, tokens, window, nq,
-                             nkv, heads, htiles, split, tail, partial, (bf16*)out);
+    return vl_launch_waiting(flash_tc5_8bit_join_kernel, dim3((unsigned)(split ? blocks : over), HD / 16), dim3(ROWS), 0, s, (const int4*)tiles, num_tiles, cuts,
+                             tokens, window, nq, nkv, heads, htiles, split, tail, partial, (bf16*)out);
 }
