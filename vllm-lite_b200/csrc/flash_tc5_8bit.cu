@@ -11,8 +11,8 @@
 //        beside that, its largest score: a row's base is an older maximum, and only when it has been passed by 2^8 it is moved, the row's output
 //        in TMEM scaled and the scores weighed again.  While one query tile's rows are exponentiated the tensor cores work on the other's products;
 //   one warp             looks up where the keys' rows are and their pages' scales, up to 8 tiles ahead;
-//   four warps for keys, four for values   bring them: 16 bytes a load into registers, two tiles ahead, e4m3 to halves (exact), times a power of two, into two or
-//        three stages of 128-byte swizzled rows.  The pages' scales are folded in here: page by page 2^(e - E + 7), E the largest
+//   four warps for keys, four for values   bring them: 16 bytes a load into registers, two tiles ahead, e4m3 to halves (exact), times a power of two, into two
+//        stages of 128-byte swizzled rows.  The pages' scales are folded in here: page by page 2^(e - E + 7), E the largest
 //        exponent of all pages that the block reads (found first; 448 * 2^7 is below the largest half), so that scores and outputs of all tiles are in one
 //        unit, which a row's own factor and the end undo.  Exact down to pages 2^15 below the largest, to within 2^-41 of the largest number else.
 //        Rows that no query of the block reads, or that the table does not hold (flagged), are zeros.  A page whose scale is not a number gives
@@ -21,7 +21,7 @@
 // Where a launch has so few tokens that half of the SMs would be without a block, each item's keys are shared out among several, which leave base, sum and
 // output as they are for a second launch to join.  So are the keys of the items that would be the few blocks of a last round.
 //
-// Measured in a graph (32 heads of 128, 8 KV heads): a prompt of 2,048 tokens 54 us, 0.64 PFLOP/s; three portions of 512 at position 2,500 91 us, 0.70 (every
+// Measured in a graph (32 heads of 128, 8 KV heads): a prompt of 2,048 tokens 53 us, 0.65 PFLOP/s; three portions of 512 at position 2,500 90 us, 0.71 (every
 // block whole: 112); 8 tokens behind 8,000 keys 27 us.  A step of 64 keys takes a block 1.0 us where exponentials alone (16 a cycle and SM) take 0.54, the products 0.55
 // and shared memory's traffic 0.65.  No unit is full (issue slots and the exponential unit about half, ALUs and tensor cores a third): a step is a chain of waits, loads
 // from TMEM, weights and votes.  What a block takes besides, some 8 us: queries and scales (3 us), the first keys (2), the last product and the output (2).
@@ -50,7 +50,7 @@ constexpr int NTHREADS = 32 * (LOAD0 + 2 * LOADERS), LOAD_THREADS = 32 * LOADERS
 constexpr unsigned ROW_BYTES = 128;
 constexpr unsigned Q_BYTES = BM * CB * ROW_BYTES;      // CB blocks of [128 rows][128 bytes]
 constexpr unsigned KV_STAGE = BN * CB * ROW_BYTES;     // CB blocks of [64 rows][128 bytes]
-constexpr int STAGES = HD <= 128 ? 3 : 2;              // of keys, and of values
+constexpr int STAGES = 2;                              // of keys, and of values (a prompt of 2,048: 2 52.9 us, 3 54.2, 4 56.3)
 constexpr unsigned TILE_BYTES = GROUPS * Q_BYTES + 2 * STAGES * KV_STAGE;
 constexpr int ROWS = GROUPS * BM;
 constexpr int MIN_PART = 4, MOST_ITEMS = 160, MOST_ROUNDS = 8;        // splitting of keys: key tiles of a block at least, items a head and rounds at most
@@ -114,6 +114,12 @@ __device__ __forceinline__ void mma_tmem(unsigned tmem_c, unsigned tmem_a, unsig
 }
 // byte offset of the 16-byte chunk `chunk` (0..7) of row `row` in a tile of 128-byte swizzled rows
 __device__ __forceinline__ unsigned swizzled(int row, int chunk) { return (unsigned)row * ROW_BYTES + (unsigned)((chunk ^ (row & 7)) << 4); }
+// (no tile of the cache is read twice by a block)
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+    uint4 r;
+    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
 __device__ __forceinline__ unsigned times(unsigned h2, unsigned f2) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h2), *reinterpret_cast<const __half2*>(&f2));
     return *reinterpret_cast<const unsigned*>(&r);
@@ -188,11 +194,11 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     unsigned char* Ks = Qs + GROUPS * Q_BYTES;                           // STAGES
     unsigned char* Vs = Ks + STAGES * KV_STAGE;                          // STAGES
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(smem + TILE_BYTES);
-    unsigned long long *k_full = bars, *k_empty = bars + 3, *v_full = bars + 6, *v_empty = bars + 9;
-    unsigned long long *s_full = bars + 12, *p_full = bars + 16, *pv_done = bars + 20;           // [GROUPS][2 buffers]
-    unsigned long long *found_full = bars + 24, *found_empty = bars + 24 + FOUND;
-    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(bars + 24 + 2 * FOUND);
-    int* words = reinterpret_cast<int*>(bars + 25 + 2 * FOUND);
+    unsigned long long *k_full = bars, *k_empty = bars + STAGES, *v_full = bars + 2 * STAGES, *v_empty = bars + 3 * STAGES;
+    unsigned long long *s_full = bars + 4 * STAGES, *p_full = s_full + 4, *pv_done = p_full + 4;           // [GROUPS][2 buffers]
+    unsigned long long *found_full = pv_done + 4, *found_empty = found_full + FOUND;
+    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(found_empty + FOUND);
+    int* words = reinterpret_cast<int*>(found_empty + FOUND + 1);
     int &failed = words[0], &top_k = words[1], &top_v = words[2];
     float* s_row_scale = reinterpret_cast<float*>(smem + TILE_BYTES + 512);                      // [GROUPS * BM]
     int2* s_found = reinterpret_cast<int2*>(s_row_scale + GROUPS * BM);                          // keys, values: [FOUND][BN] cache row (-1: zeros) and factor
@@ -244,9 +250,9 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     const int per_head = 65536 / heads + 1;                              // (r * per_head) >> 16 is r / heads for rows of a tile
 
     // (barrier i by thread i; the numbers of arrivals in the order of `bars`)
-    if (tid < 24 + 2 * FOUND) {
+    if (tid < 4 * STAGES + 12 + 2 * FOUND) {
         const int i = tid;
-        const int count = i < 12 ? (i / 3 % 2 ? groups : LOAD_THREADS) : i < 16 ? 1 : i < 20 ? BM : i < 24 + FOUND ? 1 : 2 * LOADERS;
+        const int count = i < 4 * STAGES ? (i / STAGES % 2 ? groups : LOAD_THREADS) : i < 4 * STAGES + 4 ? 1 : i < 4 * STAGES + 8 ? BM : i < 4 * STAGES + 12 + FOUND ? 1 : 2 * LOADERS;
         mbar_init(&bars[i], count);
         mbar_fence_init();
     } else if (tid == NTHREADS - 1) {
@@ -377,11 +383,11 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
                 x[i] = make_uint4(0u, 0u, 0u, 0u);
                 if constexpr (EVEN) {
                     const int row = f[i * APART].x;
-                    if (row >= 0) x[i] = __ldg(reinterpret_cast<const uint4*>(my_cache + (size_t)row * HD));
+                    if (row >= 0) x[i] = load_once(reinterpret_cast<const uint4*>(my_cache + (size_t)row * HD));
                 } else {
                     const int idx = i * LOAD_THREADS + ct, r = idx / PIECES, c = idx - r * PIECES;
                     const int row = idx < BN * PIECES ? f[r - r0].x : -1;
-                    if (row >= 0) x[i] = __ldg(reinterpret_cast<const uint4*>(cache + (size_t)row * HD + c * 16));
+                    if (row >= 0) x[i] = load_once(reinterpret_cast<const uint4*>(cache + (size_t)row * HD + c * 16));
                 }
             }
         };
