@@ -81,6 +81,33 @@ def test_draws(V, kind):
 
 
 @gpu
+@pytest.mark.parametrize("V", [342880, 342881, 343001, 420001, 1000003])
+def test_rows_that_shared_memory_does_not_hold(V):
+    """Slices longer than what a block holds, all logits far below zero, behind a launch that leaves large numbers in every block's shared memory: a number that is
+    none of the row's would stand above its maximum."""
+    R = 3
+    g = torch.Generator(device=DEV).manual_seed(V)
+    logits = torch.randn(R, V, generator=g, device=DEV) * 3 - 60
+    big = torch.full((4096, 4096), 1e4, dtype=torch.bfloat16, device=DEV)
+    seen = 0
+    for k, tp, mp in itertools.product((0, 1, 40, 5000), (1.0, 0.9), (0.0, 0.05, 1.0)):
+        u = torch.rand(R, generator=g, device=DEV)
+        big @ big
+        got, lp = draw(logits, 0.9, k, tp, mp, u, logprob=True)
+        assert (lp <= 0).all() and (got >= 0).all() and (got < V).all()
+        for r in range(R):
+            want = reference(logits[r], 0.9, k, tp, mp, float(u[r]))
+            seen += want is not None
+            assert want is None or int(got[r]) == want, (k, tp, mp, r)
+    assert seen > 24
+    big @ big
+    got, lp = draw(logits, 0.0, 0, 1.0, 0.0, 0.5, logprob=True)
+    # masses are whole multiples of 2^-40 of the largest, rounded down, of exponentials that are off by 2^-22 of themselves
+    want = torch.log_softmax(logits.to(D), dim=1).amax(dim=1)
+    assert torch.equal(got.long(), logits.argmax(dim=1)) and ((lp.to(D) - want).abs() <= 2.0 ** -22 + V * 2.0 ** -40 + 2.0 ** -23 * want.abs()).all()
+
+
+@gpu
 def test_min_p_keeps_the_probable_ones():
     """Tokens at known probabilities relative to the first: kept up to the bound and at it, in every order with the other options; each can be drawn."""
     rel = torch.tensor([1.0, 0.5, 0.25, 0.125, 0.0625, 0.03125])

@@ -31,7 +31,7 @@
 // is reached.  The few values of that bin are brought together in every block, and there the threshold's key is found 8 bits at a time, until what is left
 // is kept whole.  (Should they be more than SMP_LIST, as in a row of one value, the 8 bits at a time go over the cluster's whole row.)  Behind top-k, top-p's sum runs over
 // what top-k left.  Values 32 and more below the maximum have mass 0 and are in no bin: no threshold need be found among them.  Any vocabulary
-// size; what of a slice shared memory does not hold (rows of more than some 390,000) is read again in each pass.
+// size; what of a slice shared memory does not hold (in rows of more than 342,880) is read again in each pass.
 //
 // Bound by latencies: reading another block's shared memory takes 0.5 us, a barrier of the cluster 0.4, and there are some ten steps behind one another.  One row
 // of 151,936 logits with top-k 20, top-p 0.95 and min-p 0.02: 15.5 us in a graph, 64 rows of mixed options 51 us (0.76 TB/s); through thresholds alone, a
@@ -636,8 +636,9 @@ extern "C" int vl_apply_penalties(float* logits, long long row_stride, int R, in
     return vl_launch_status();
 }
 
-// Values of a slice that a block's shared memory holds beside its tables.
-#define SMP_HELD_MAX ((200 * 1024 - (int)sizeof(SampleShared)) / 4)
+// Values of a slice that a block's shared memory holds beside its tables, a multiple of the four that it is read by.
+constexpr int SMP_HELD_MAX = (200 * 1024 - (int)sizeof(SampleShared)) / 16 * 4;
+static_assert(SMP_HELD_MAX % 4 == 0, "shared memory is read in pieces of four values");
 
 extern "C" int vl_sample(const float* logits, long long row_stride, int R, int V,
                          const float* temperature, const int* top_k, const float* top_p, const float* min_p,
