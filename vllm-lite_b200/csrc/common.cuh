@@ -149,8 +149,8 @@ static inline bool vl_pdl_enabled() { return g_vl_pdl == 1; }
 extern "C" void vl_set_pdl(int on) { g_vl_pdl = (on && !vl_pdl_forbidden()) ? 1 : 0; }
 extern "C" int vl_get_pdl() { return g_vl_pdl; }
 
-// A kernel that touches no global memory at all before its pdl_wait(), and that works in no clusters, may carry the attribute whatever the
-// switch says: it then only saves the gap between two launches (`vl_launch_waiting`; a call outside a recorded step starts 1 to 4 us
+// A kernel that touches no global memory at all before its pdl_wait(), or none but what its caller says that copies brought (`settled`), and that works
+// in no clusters, may carry the attribute whatever the switch says: it then only saves the gap between two launches (`vl_launch_waiting`; a call outside a recorded step starts 1 to 4 us
 // sooner: launched the plain way, kernels behind one another begin on ticks of 2.05 us).
 template <typename... KArgs, typename... Args>
 static inline int vl_launch_as(bool dependent, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,

@@ -188,7 +188,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict__ out, const unsigned char* __restrict__ kcache,
                       const unsigned char* __restrict__ vcache, const float* __restrict__ kscale, const float* __restrict__ vscale,
                       const int* __restrict__ block_table, int max_blocks, const int4* __restrict__ tiles, int num_tiles, int nq, int nkv, int page_size,
-                      int num_pages, float scale_log2, int window, unsigned* err, int heads, int htiles, int tokens, int cuts, int split, Tail tail, Partial partial) {
+                      int num_pages, float scale_log2, int window, unsigned* err, int heads, int htiles, int tokens, int cuts, int split, Tail tail, Partial partial,
+                      int settled) {
     extern __shared__ __align__(1024) unsigned char smem[];              // (the block's only shared memory, so it begins the window)
     unsigned char* Qs = smem;                                            // GROUPS
     unsigned char* Ks = Qs + GROUPS * Q_BYTES;                           // STAGES
@@ -209,6 +210,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         return;
     }
     pdl_launch_dependents();
+    if (!settled) pdl_wait();                                            // a kernel before this one may be writing the list or the table
     // This block's item and its key tiles from .. to; the items with the longest rows of keys first, or a share of an item's keys.
     const List list = {tiles, num_tiles, cuts, tokens, window};
     int head = (int)blockIdx.x, number = num_tiles * cuts - 1 - (int)blockIdx.y, part = 0, parts = 1, place = -1;
@@ -260,7 +262,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         top_k = top_v = EXP_MIN;
     }
     const int worker = warp < SOFT ? tid : tid - 32 * (LOAD0 - SOFT), first_page = lo / page_size, last_page = hi / page_size;
-    auto page_at = [&](int blk) -> int {                                 // (the table is the step's description: no kernel writes it)
+    auto page_at = [&](int blk) -> int {
         const int page = blk <= last_page && blk < max_blocks ? table[blk] : -1;
         return page < num_pages ? page : -1;
     };
@@ -674,8 +676,9 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
 // item and 16 columns, a thread a row.
 __global__ void __launch_bounds__(ROWS)
 flash_tc5_8bit_join_kernel(const int4* __restrict__ tiles, int num_tiles, int cuts, int tokens, int window, int nq, int nkv, int heads, int htiles, int split,
-                           Tail tail, Partial partial, bf16* __restrict__ out) {
+                           Tail tail, Partial partial, bf16* __restrict__ out, int settled) {
     pdl_launch_dependents();
+    if (!settled) pdl_wait();
     const List list = {tiles, num_tiles, cuts, tokens, window};
     const int in_list = num_tiles * cuts, id = tail.whole + (int)blockIdx.x, head = id % (nkv * htiles), number = in_list - 1 - id / (nkv * htiles);
     const Item item(list, number);
@@ -726,11 +729,12 @@ flash_tc5_8bit_join_kernel(const int4* __restrict__ tiles, int num_tiles, int cu
 
 extern "C" int vl_flash_prefill_8bit_head_dim() { return HD; }
 
+namespace {
 // scratch (may be null: no keys are shared out): SMs * ROWS * (hd + 2) floats from a 16-byte boundary.  q rows and `out` rows begin on 16 bytes; caches
 // [pages, nkv, page_size, hd] e4m3, scales [pages, nkv]; pages of any number of positions.
-extern "C" int vl_flash_prefill_8bit(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const float* kscale,
-                                     const float* vscale, const int* block_table, int max_blocks, const int* tiles, int num_tiles, int nq, int nkv,
-                                     int hd, int page_size, int num_pages, float scale, int window, float* scratch, long long floats, unsigned* err, void* stream) {
+int flash_prefill_8bit(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const float* kscale,
+                       const float* vscale, const int* block_table, int max_blocks, const int* tiles, int num_tiles, int nq, int nkv,
+                       int hd, int page_size, int num_pages, float scale, int window, float* scratch, long long floats, unsigned* err, void* stream, int settled) {
     if (num_tiles <= 0) return VL_OK;
     if (hd != HD) return VL_ERR_UNSUPPORTED;
     if (nq <= 0 || nkv <= 0 || nq % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || window < 0 || q_stride < nq * hd) return VL_ERR_ARGUMENT;
@@ -761,8 +765,23 @@ extern "C" int vl_flash_prefill_8bit(const void* q, int q_stride, void* out, con
                                      dim3(NTHREADS), SMEM_BYTES, s, (const bf16*)q, q_stride,
                                      (bf16*)out, (const unsigned char*)kcache, (const unsigned char*)vcache, kscale, vscale, block_table, max_blocks,
                                      (const int4*)tiles, num_tiles, nq, nkv, page_size, num_pages, scale * 1.4426950408889634f, window, err, heads, htiles, tokens,
-                                     cuts, split, tail, partial);
+                                     cuts, split, tail, partial, settled);
     if (rc != VL_OK || !(split || last)) return rc;
     return vl_launch_waiting(flash_tc5_8bit_join_kernel, dim3((unsigned)(split ? blocks : over), HD / 16), dim3(ROWS), 0, s, (const int4*)tiles, num_tiles, cuts,
-                             tokens, window, nq, nkv, heads, htiles, split, tail, partial, (bf16*)out);
+                             tokens, window, nq, nkv, heads, htiles, split, tail, partial, (bf16*)out, settled);
+}
+}  // namespace
+
+extern "C" int vl_flash_prefill_8bit(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const float* kscale,
+                                     const float* vscale, const int* block_table, int max_blocks, const int* tiles, int num_tiles, int nq, int nkv,
+                                     int hd, int page_size, int num_pages, float scale, int window, float* scratch, long long floats, unsigned* err, void* stream) {
+    return flash_prefill_8bit(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, tiles, num_tiles, nq, nkv, hd, page_size, num_pages, scale,
+                              window, scratch, floats, err, stream, 0);
+}
+// ... whose tiles and block_table copies brought, not kernels: they are read before the kernels ahead in the stream have ended.
+extern "C" int vl_flash_prefill_8bit_settled(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const float* kscale,
+                                             const float* vscale, const int* block_table, int max_blocks, const int* tiles, int num_tiles, int nq, int nkv,
+                                             int hd, int page_size, int num_pages, float scale, int window, float* scratch, long long floats, unsigned* err, void* stream) {
+    return flash_prefill_8bit(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, tiles, num_tiles, nq, nkv, hd, page_size, num_pages, scale,
+                              window, scratch, floats, err, stream, 1);
 }

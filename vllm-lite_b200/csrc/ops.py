@@ -160,6 +160,8 @@ _SIGNATURES = {
                                                     c_void_p, c_void_p, c_int, c_void_p],
     ("flash_tc5_8bit", "vl_flash_prefill_8bit"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                                   c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_longlong, c_void_p, c_void_p],
+    ("flash_tc5_8bit", "vl_flash_prefill_8bit_settled"): [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                                          c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_longlong, c_void_p, c_void_p],
     ("sampling", "vl_apply_penalties"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_void_p],
     ("sampling", "vl_sample"): [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -1073,11 +1075,13 @@ def flash_prefill_8bit_scratch(head_dim, device=None):
     return _sm_count(device) * (256 if head_dim <= 128 else 128) * (head_dim + 2)
 
 
-def flash_prefill_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, tiles, num_heads, num_kv_heads, head_dim, scale, window, err, scratch=None):
+def flash_prefill_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, tiles, num_heads, num_kv_heads, head_dim, scale, window, err, scratch=None,
+                       settled=False):
     """Attention of prompt portions over a cache in 8 bits, q and out as in `flash_decode_8bit`.  tiles int32 [n, 4]: (row of the block table, index of the
     tile's first token, tokens (<= 128), position of the first); a step's tiles cover once every token that the launch is to serve, the other rows of out are left
     alone.  scratch (float32): at least `flash_prefill_8bit_scratch` of them, which nobody else on the stream needs; without them the call takes its own.
-    q, out, tiles and scratch begin on 16 bytes."""
+    q, out, tiles and scratch begin on 16 bytes.  `settled`: copies, not kernels, brought block_table and tiles, so that the kernel may read them before the ones ahead of
+    it have ended."""
     _, width, pages, page_size = _attention_8bit_args(q, out, k_cache, v_cache, k_scale, v_scale, block_table, num_heads, num_kv_heads, head_dim, scale, window,
                                                       "flash_prefill_8bit")
     _need(tiles, torch.int32, "tiles", 2)
@@ -1093,9 +1097,10 @@ def flash_prefill_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, 
     elif count * num_kv_heads <= 8 * _sm_count(device):                  # (keys of more tiles are not shared out)
         floats = flash_prefill_8bit_scratch(head_dim, device)
         scratch = torch.empty(floats, dtype=torch.float32, device=device)
-    _check(_fn("flash_tc5_8bit", "vl_flash_prefill_8bit", {"FA_HD": head_dim})(
+    name = "vl_flash_prefill_8bit_settled" if settled else "vl_flash_prefill_8bit"
+    _check(_fn("flash_tc5_8bit", name, {"FA_HD": head_dim})(
         q, width, out, k_cache, v_cache, k_scale, v_scale, block_table, block_table.shape[1], tiles, count, num_heads, num_kv_heads, head_dim,
-        page_size, pages, float(scale), int(window or 0), scratch, floats, err, _stream()), "vl_flash_prefill_8bit")
+        page_size, pages, float(scale), int(window or 0), scratch, floats, err, _stream()), name)
     return out
 
 

@@ -162,7 +162,8 @@ def run_8bit(qkv, out, cache, group, step, spec, scale):
         single(qkv.shape[0], group.max_context)
         return out
     floats = ops.flash_prefill_8bit_scratch(spec.head_dim, qkv.device)
-    ops.flash_prefill_8bit(*common, step.query_tiles, *sizes, step.err, scratch=step.workspace.get(step.tag + "attn8.parts", (floats,), torch.float32))
+    ops.flash_prefill_8bit(*common, step.query_tiles, *sizes, step.err, scratch=step.workspace.get(step.tag + "attn8.parts", (floats,), torch.float32),
+                           settled=getattr(step, "settled", False))
     if step.single_tokens is not None:
         single(step.single_tokens.shape[0], step.single_context, step.single_tokens)
     return out
