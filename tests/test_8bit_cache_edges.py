@@ -5,7 +5,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from test_8bit_cache import Cache, D, DEV, batch, check_attention, queries, tiles_of
+from test_8bit_cache import Cache, D, DEV, batch, check_attention, copies, least_scale, queries, tiles_of, turned_heads
 from vllm_lite_b200.csrc import ops
 
 gpu = pytest.mark.gpu
@@ -69,3 +69,92 @@ def test_a_step_says_who_brought_its_description(monkeypatch, settled):
     cache = SimpleNamespace(k=None, v=None, k_scale=None, v_scale=None)
     attention_dispatch.run_8bit(torch.zeros(9, 512), None, cache, SimpleNamespace(block_table=None, max_context=9), step, spec, 0.1)
     assert said == [bool(settled)] * 2 and "settled" in StepBatch.__dataclass_fields__
+
+
+# ---------------------------------------------------------------------------------------------- tokens that are not written, among others that are
+def check_rows(cache, was, x, slots, req, pos, which):
+    """Keys or values x [T, nkv, hd], in 64 bits and off by `slack` of a head's largest, against what the cache holds: a row that is written, under the least power
+    of two for the rows written and, unless row 0 is among them, the one the page had; other rows of a page up to its request's last token
+    as they were, unless the page begins anew."""
+    ps, slots = cache.ps, slots.tolist()
+    now, before, scale, scale_before = (cache.k, was[0], cache.k_scale, was[2]) if which == "k" else (cache.v, was[1], cache.v_scale, was[3])
+    pages = {}
+    for t, s in enumerate(slots):                                                  # (a page that no token of its request goes to is not touched)
+        if s >= 0:
+            pages.setdefault(s // ps, {})[s % ps] = t
+    reach = {}
+    for t in range(len(slots)):
+        page = int(cache.table[int(req[t]), int(pos[t]) // ps])
+        reach[page] = max(reach.get(page, 0), int(pos[t]) % ps + 1)
+    for page in range(now.shape[0]):
+        rows = pages.get(page, {})
+        same = lambda a, b: torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        if not rows:
+            assert same(now[page], before[page]) and torch.equal(scale.view(torch.int32)[page], scale_before.view(torch.int32)[page])
+            continue
+        for h in range(cache.nkv):
+            new = torch.stack([x[t, h] for t in rows.values()])
+            old = 0.0 if 0 in rows else float(scale_before[page, h])
+            s, top = float(scale[page, h]), float(new.abs().max())
+            assert max(old, least_scale(top * (1 - 2.0 ** -18))) <= s <= max(old, least_scale(top * (1 + 2.0 ** -18)))
+            for r in range(ps):
+                got = now[page, h, r].to(D) * s
+                if r in rows:
+                    want = x[rows[r], h]
+                    assert ((got - want).abs() <= torch.maximum(2.0 ** -4 * want.abs(), torch.tensor(2.0 ** -10 * s, dtype=D, device=DEV)) * (1 + 2.0 ** -10)
+                            + 2.0 ** -18 * top).all(), (page, h, r)
+                elif 0 in rows or r >= reach[page]:
+                    assert same(now[page, h, r], before[page, h, r]), (page, h, r)
+                else:
+                    assert ((got - before[page, h, r].to(D) * old).abs() <= (2.0 ** -10 * s if s > old else 0.0)).all(), (page, h, r)
+
+
+@gpu
+@pytest.mark.parametrize("hd,ps,rot,before,new", [
+    (128, 64, 128, [30, 0, 64, 10], [200, 70, 10, 1]), (128, 16, 0, [5, 0, 16], [40, 33, 3]), (256, 100, 256, [20], [300]), (32, 256, 32, [100, 0], [300, 20]),
+    (80, 16, 80, [3, 0], [40, 20]), (128, 64, 64, [10, 64], [150, 30]), (144, 200, 0, [30], [100]),
+    (64, 16, 64, [9, 0, 20], [3, 0, 0]), (80, 8, 80, [3, 0, 5, 16, 0, 0], [1, 1, 4, 0, 0, 0]), (256, 16, 0, [7] + [0] * 39, [40] + [0] * 39), (128, 64, 128, [5, 64, 0, 9], [1] * 4)])
+@pytest.mark.parametrize("pattern", ["first", "last alone", "every third", "half", "all but one page"])
+def test_some_tokens_are_not_written(hd, ps, rot, before, new, pattern):
+    nq, nkv = 4, 2
+    longest = max(b + n for b, n in zip(before, new))
+    cache = Cache(len(new), longest, nkv, ps, hd, seed=2)
+    whole = cache.table.clone()
+    cache.fill([longest] * len(new), seed=hd, spread=6).table = whole              # pages that hold rows of older tokens all over
+    pos, req, cu, slots = batch(cache, before, new)
+    T = sum(new)
+    g = torch.Generator(device=DEV).manual_seed(hd + ps)
+    at = torch.arange(T, device=DEV) - cu[req.long()]
+    count = (cu[1:] - cu[:-1])[req.long()]
+    drop = {"first": at == 0, "last alone": at < count - 1, "every third": (at + req) % 3 == 0, "half": torch.rand(T, generator=g, device=DEV) < 0.5,
+            "all but one page": pos // ps != before[0] // ps}[pattern]
+    slots = torch.where(drop, torch.full_like(slots, -1), slots)
+    qkv = (torch.randn(T, (nq + 2 * nkv) * hd, generator=g, device=DEV) * torch.exp2(4 * torch.randn(T, 1, generator=g, device=DEV))).to(torch.bfloat16)
+    inv_freq = (1e6 ** (-torch.arange(0, rot, 2, dtype=D, device=DEV) / max(rot, 1))).float() if rot else None
+    was, rows = copies(cache), qkv.view(T, nq + 2 * nkv, hd)
+    q = torch.full((T, nq * hd), 3.0, dtype=torch.bfloat16, device=DEV)
+    ops.qk_norm_rope_write_8bit(qkv, pos, slots, cu, None, None, 1e-6, inv_freq, rot, *cache.tensors, nq, nkv, hd, cache.err, q_out=q)
+    assert int(cache.err) == 0
+    turned = turned_heads(rows[:, :nq + nkv], None, pos, inv_freq, rot)
+    want = turned[:, :nq]
+    assert ((q.to(D).view(T, nq, hd) - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * want.abs().amax(dim=2, keepdim=True)).all()
+    check_rows(cache, was, turned[:, nq:], slots, req, pos, "k")
+    check_rows(cache, was, rows[:, nq + nkv:].to(D), slots, req, pos, "v")
+
+
+@gpu
+@pytest.mark.parametrize("hd,ps", [(128, 64), (80, 16)])
+@pytest.mark.parametrize("new", [[20], [5, 0, 0, 0, 0]])
+def test_slots_of_another_row_behind_tokens_that_are_not_written(hd, ps, new):
+    """The first slot of a page that is one says where the page is: flagged where it is another row's, below the pool's first or beyond its last."""
+    nkv = 2
+    cache = Cache(len(new), 32, nkv, ps, hd).fill([32] * len(new))
+    pos, req, cu, slots = batch(cache, [3] * len(new), new)
+    was = copies(cache)
+    qkv = torch.ones(sum(new), 3 * nkv * hd, dtype=torch.bfloat16, device=DEV)
+    for third in (1, 2, int(slots[2]) + 1, cache.k.shape[0] * ps + 5, (1 << 31) - 1):
+        cache.err.zero_()
+        bad = slots.clone()
+        bad[:2], bad[2], bad[3:] = -1, third, -5
+        ops.qk_norm_rope_write_8bit(qkv, pos, bad, cu, None, None, 1e-6, None, 0, *cache.tensors, nkv, nkv, hd, cache.err)
+        assert int(cache.err) == 2 and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache.tensors, was)), third

@@ -6,8 +6,8 @@
 //
 // A page's rows belong to one request and a request's tokens follow one another, so one block sees all that a page gets of one KV head's keys or
 // values, and nothing is exchanged between blocks: it takes the step's new rows of that page, their largest |x|, and with it and the scale of the rows
-// that were there the new scale; then the rows are written, and where the scale has grown the page's earlier rows are read, multiplied by the quotient of the scales
-// (a power of two) and written back.  Which page of which request a block takes follows from a sum over the requests that every block makes itself.  Other blocks
+// that were there the new scale; then the rows are written, and where the scale has grown the page's earlier rows (and those between that are not written) are read, multiplied by
+// the quotient of the scales (a power of two) and written back.  Which page of which request a block takes follows from a sum over the requests that every block makes itself.  Other blocks
 // take the queries.  Three kernels:
 //   singles: as many tokens as requests (a decode step), a warp a token and head, no sums over requests;
 //   wide:    heads of 32, 64, 128 or 256 features that are rotated as a whole or not at all: 16-byte accesses, hd / 16 lanes a row, angles of a
@@ -148,14 +148,15 @@ struct Step {                                          // what every kernel is g
     int page_blocks, heads_a_warp, heads_a_block, early;
 };
 
-// The step's new rows of one page: tokens tok0 .. tok0 + n - 1 into rows row0 .., slots from slot0 on; n 0: none that the block may write.
-struct Visit { int tok0, row0, n, slot0, page; };
+// The step's new rows of one page: tokens tok0 .. tok0 + n - 1 into rows row0 .., slots from slot0 on; n 0: none that the block may write.  Tokens of a negative
+// slot are left out; `held`: the rows ahead of the first one that is written (0: the page begins anew).
+struct Visit { int tok0, row0, n, slot0, page, held; };
 
 // What the launch's page number `visit` is; all threads of the block call it.  Which request it falls into: a sum over the requests, a request a thread.
 __device__ __forceinline__ Visit find_visit(const Step& st, int visit) {
     __shared__ int s_sum[WARPS], s_req, s_visit;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Visit v = {0, 0, 0, 0, 0};
+    Visit v = {0, 0, 0, 0, 0, 0};
     if (threadIdx.x == 0) s_req = -1;
     __syncthreads();
     for (int b0 = 0, before = 0; b0 < st.B; b0 += NT) {
@@ -187,24 +188,30 @@ __device__ __forceinline__ Visit find_visit(const Step& st, int visit) {
     const int lo = st.cu[req], off = st.positions[lo] % st.page_size, skip = s_visit ? s_visit * st.page_size - off : 0;
     v.row0 = s_visit ? 0 : off;
     v.tok0 = lo + skip;
+    const int n = min(st.page_size - v.row0, st.cu[req + 1] - v.tok0);
+    int ahead = 0;
     v.slot0 = st.slots[v.tok0];
-    if (v.slot0 < 0) return v;                               // (a call that reads another call's cache, a padded token)
+#pragma unroll 1
+    while (v.slot0 < 0 && ++ahead < n) v.slot0 = st.slots[v.tok0 + ahead];
+    if (v.slot0 < 0) return v;                               // (none of the page's tokens is written)
+    v.slot0 -= ahead;
+    v.held = v.row0 + ahead;
     v.page = v.slot0 / st.page_size;
     if (v.page >= st.num_pages || v.slot0 - v.page * st.page_size != v.row0) {
         if (threadIdx.x == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT);
         return v;
     }
-    v.n = min(st.page_size - v.row0, st.cu[req + 1] - v.tok0);
+    v.n = n;
     return v;
 }
 
-// the scale of a page whose new rows' largest |x| has the bits `top`, and that held rows before (row0 > 0) under `old`
-__device__ __forceinline__ float new_scale(unsigned top, int row0, float old) {
+// the scale of a page whose new rows' largest |x| has the bits `top`, and that held rows before (held > 0) under `old`
+__device__ __forceinline__ float new_scale(unsigned top, int held, float old) {
     const float now = scale_of(top);
-    if (!row0) return now;
+    if (!held) return now;
     return old == old && now == now ? fmaxf(old, now) : __uint_as_float(0x7fc00000u);
 }
-// a page's first `bytes` bytes moved to a scale that has grown (f: old / new), by `count` threads
+// `bytes` bytes of a page moved to a scale that has grown (f: old / new), by `count` threads
 __device__ __forceinline__ void move_rows(unsigned char* cache, int bytes, float f, int thread, int count) {
     uint4* rows = reinterpret_cast<uint4*>(cache);
     for (int i = thread; i < bytes / 16; i += count) rows[i] = times(rows[i], f);
@@ -251,17 +258,12 @@ write_8bit_singles_kernel(const __grid_constant__ Step st) {
         query_heads<MAXHD>(st, tok, (u - pages) * st.heads_a_warp, min(st.nq, (u - pages + 1) * st.heads_a_warp));
         return;
     }
-    const int pos = st.positions[tok], slot = st.slots[tok], c0 = st.cu[tok], c1 = st.cu[tok + 1];
-    if (pos < 0 || slot < 0) return;
-    const int row0 = pos % st.page_size, page = slot / st.page_size;
-    if (page >= st.num_pages || slot - page * st.page_size != row0) {
-        if (lane == 0 && u == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT);
-        return;
-    }
-    const bool values = u & 1;
-    const int kvh = u >> 1, turned = values || !st.inv_freq ? 0 : st.rot;
-    int n = 1;                                               // as many tokens as requests, but not one each: the first token of a page takes the page's others
-    if (c0 != tok || c1 != tok + 1) {
+    const int pos = st.positions[tok], c0 = st.cu[tok], c1 = st.cu[tok + 1];
+    int slot = st.slots[tok], n = 1, ahead = 0;
+    if (pos < 0) return;
+    const int row0 = pos % st.page_size;
+    // as many tokens as requests, but not one each: the first token of a page takes the page's others, and looks for the first that is written
+    if (__builtin_expect(c0 != tok || c1 != tok + 1, 0)) {
         int b = 0;
 #pragma unroll 1
         for (int step = 1 << 30; step; step >>= 1)           // the last request that begins at this token or before
@@ -269,7 +271,18 @@ write_8bit_singles_kernel(const __grid_constant__ Step st) {
         const int lo = st.cu[b], hi = st.cu[b + 1];
         if (lo < 0 || lo > tok || hi <= tok || hi > st.T || (lo != tok && row0)) return;           // (padding, or not the first)
         n = min(st.page_size - row0, hi - tok);
+#pragma unroll 1
+        while (slot < 0 && ++ahead < n) slot = st.slots[tok + ahead];
     }
+    if (slot < 0) return;
+    slot -= ahead;
+    const int page = slot / st.page_size;
+    if (page >= st.num_pages || slot - page * st.page_size != row0) {
+        if (lane == 0 && u == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT);
+        return;
+    }
+    const bool values = u & 1;
+    const int kvh = u >> 1, turned = values || !st.inv_freq ? 0 : st.rot, held = row0 + ahead;
     const size_t head = (size_t)page * st.nkv + kvh;
     unsigned char* cache = (values ? st.vcache : st.kcache) + head * st.page_size * hd;
     float* scale = (values ? st.vscale : st.kscale) + head;
@@ -281,16 +294,19 @@ write_8bit_singles_kernel(const __grid_constant__ Step st) {
 #pragma unroll 1
     for (int k = 0; k < 2 * n; ++k) {
         const int i = k < n ? k : k - n;
-        if (i && st.slots[tok + i] != slot + i) { if (lane == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT); continue; }
         if (k == n) {
-            now = new_scale(__reduce_max_sync(0xffffffffu, top), row0, old);
+            now = new_scale(__reduce_max_sync(0xffffffffu, top), held, old);
             inv = inverse_of(now);
+        }
+        if (__builtin_expect(n > 1, 0)) {
+            const int mine = st.slots[tok + i];
+            if (mine != slot + i) { if (lane == 0 && mine >= 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT); continue; }
         }
         if (k == 0 || n > 1) {
             float4 cs[Row<MAXHD>::UR];
             if (turned) Row<MAXHD>::angles(cs, pos + i, st.inv_freq, lane, turned);
             pdl_wait();
-            if (k == 0 && row0) old = *scale;
+            if (k == ahead && held) old = *scale;
             r.load(st.qkv + (size_t)(tok + i) * st.row_stride + (size_t)(st.nq + (values ? st.nkv : 0) + kvh) * hd, lane, hd, turned);
             if (!values && st.kw) r.norm(st.kw, st.eps, lane, hd, turned);
             if (turned) r.turn(cs);
@@ -301,7 +317,16 @@ write_8bit_singles_kernel(const __grid_constant__ Step st) {
             r.each(lane, hd, turned, [&](int c, float2 v) { *reinterpret_cast<unsigned short*>(dst + c) = to_e4m3x2(v.x * inv, v.y * inv); });
         }
     }
-    if (row0 && now > old) move_rows(cache, row0 * hd, old * inv, lane, 32);       // (false for NaN: rows under a scale that is none need no other)
+    if (held && now > old) {                                 // (false for NaN: rows under a scale that is none need no other)
+        move_rows(cache, row0 * hd, old * inv, lane, 32);
+        if (__builtin_expect(n > 1, 0))                      // rows between that are not written
+#pragma unroll 1
+            for (int i = 0; i < n; ++i)
+                if (st.slots[tok + i] != slot + i && lane < hd / 16) {
+                    uint4* row = reinterpret_cast<uint4*>(cache + (size_t)(row0 + i) * hd) + lane;
+                    *row = times(*row, old * inv);
+                }
+    }
     if (lane == 0) *scale = now;
 }
 
@@ -332,16 +357,17 @@ write_8bit_narrow_kernel(const __grid_constant__ Step st) {
     const float* w = values ? nullptr : st.kw;
     const bf16* src = st.qkv + (size_t)(st.nq + (values ? st.nkv : 0) + kvh) * hd;
     pdl_wait();                                              // qkv comes from the kernel before
-    const float old = v.row0 ? *scale : 0.f;
+    const float old = v.held ? *scale : 0.f;
     Row<MAXHD> r[ROWS];
     bool mine[ROWS];
-    unsigned top = 0, strange = 0;
+    unsigned top = 0, left_out = 0, strange = 0;
     auto take = [&](int base) {                              // this warp's rows of the pass that begins with row `base`
 #pragma unroll
         for (int u = 0; u < ROWS; ++u) {
             const int i = base + u * WARPS + warp;
             mine[u] = i < v.n;
-            if (mine[u] && st.slots[v.tok0 + i] != v.slot0 + i) { mine[u] = false; strange = 1; }
+            const int slot = mine[u] ? st.slots[v.tok0 + i] : 0;
+            if (mine[u] && slot != v.slot0 + i) { mine[u] = false; left_out = 1; strange |= slot >= 0; }
             if (mine[u]) r[u].load(src + (size_t)(v.tok0 + i) * st.row_stride, lane, hd, turned);
         }
 #pragma unroll
@@ -366,9 +392,9 @@ write_8bit_narrow_kernel(const __grid_constant__ Step st) {
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) s_top[warp] = top;
     if (strange && lane == 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT);
-    __syncthreads();
+    left_out = __syncthreads_or(left_out);
     for (int i = 0; i < WARPS; ++i) top = max(top, s_top[i]);
-    const float now = new_scale(top, v.row0, old), inv = inverse_of(now);
+    const float now = new_scale(top, v.held, old), inv = inverse_of(now);
     // Whole passes that registers no longer hold are made again, the last one first (pages of more than 64 rows, heads beyond 128).
     for (int base = last; base >= 0; base -= PASS) {
         if (base != last) take(base);
@@ -379,7 +405,12 @@ write_8bit_narrow_kernel(const __grid_constant__ Step st) {
             r[u].each(lane, hd, turned, [&](int i, float2 x) { *reinterpret_cast<unsigned short*>(dst + i) = to_e4m3x2(x.x * inv, x.y * inv); });
         }
     }
-    if (v.row0 && now > old) move_rows(cache, v.row0 * hd, old * inv, threadIdx.x, NT);
+    if (v.held && now > old) {
+        move_rows(cache, v.row0 * hd, old * inv, threadIdx.x, NT);
+        if (left_out)
+            for (int i = warp; i < v.n; i += WARPS)
+                if (st.slots[v.tok0 + i] != v.slot0 + i) move_rows(cache + (size_t)(v.row0 + i) * hd, hd, old * inv, lane, 32);
+    }
     if (threadIdx.x == 0) *scale = now;
 }
 
@@ -495,11 +526,14 @@ write_8bit_wide_kernel(const __grid_constant__ Step st) {
     };
     const int last = (v.n - 1) / PASS * PASS;
     if (turned && last == 0) angles(0);
-    unsigned strange = 0;
-    for (int i = threadIdx.x; i < v.n; i += NT)
-        if (st.slots[v.tok0 + i] != v.slot0 + i) strange = 1;
-    if (strange && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT);
-    strange = __syncthreads_or(strange);                     // (a row whose slot is another place's is left out)
+    unsigned left_out = 0;
+    for (int i = threadIdx.x; i < v.n; i += NT) {
+        const int slot = st.slots[v.tok0 + i];
+        if (slot == v.slot0 + i) continue;
+        left_out = 1;
+        if (slot >= 0 && st.err) atomicOr(st.err, VL_DEV_BAD_SLOT);
+    }
+    left_out = __syncthreads_or(left_out);
     pdl_wait();                                              // qkv comes from the kernel before
     const int end = min(st.nkv, (part + 1) * st.heads_a_block);
     for (int first = part * st.heads_a_block, turn = 0; first < end; first += WARPS / AT, turn ^= 1) {
@@ -509,7 +543,7 @@ write_8bit_wide_kernel(const __grid_constant__ Step st) {
         unsigned char* cache = (values ? st.vcache : st.kcache) + head * st.page_size * HD;
         float* scale = (values ? st.vscale : st.kscale) + head;
         const bf16* src = st.qkv + (size_t)(st.nq + (values ? st.nkv : 0) + kvh) * HD;
-        const float old = v.row0 ? *scale : 0.f;
+        const float old = v.held ? *scale : 0.f;
         R r[TURNS];
         bool mine[TURNS];
         unsigned top = 0;
@@ -522,7 +556,7 @@ write_8bit_wide_kernel(const __grid_constant__ Step st) {
 #pragma unroll
             for (int u = 0; u < TURNS; ++u) {
                 const int i = base + u * GROUP + my_warp * R::AT_ONCE + sub;
-                mine[u] = !none && i < v.n && !(strange && st.slots[v.tok0 + i] != v.slot0 + i);
+                mine[u] = !none && i < v.n && !(left_out && st.slots[v.tok0 + i] != v.slot0 + i);
                 if (mine[u]) r[u].load(src + (size_t)(v.tok0 + i) * st.row_stride, i0);
                 else r[u].clear();
             }
@@ -542,7 +576,7 @@ write_8bit_wide_kernel(const __grid_constant__ Step st) {
         if (lane == 0) s_top[turn][warp] = top;
         __syncthreads();
         for (int i = 0; i < AT; ++i) top = max(top, s_top[turn][warp - my_warp + i]);
-        const float now = new_scale(top, v.row0, old), inv = inverse_of(now);
+        const float now = new_scale(top, v.held, old), inv = inverse_of(now);
         for (int base = last; base >= 0; base -= PASS) {     // (the last pass is still held)
             if (base != last) take(base);
 #pragma unroll
@@ -550,13 +584,19 @@ write_8bit_wide_kernel(const __grid_constant__ Step st) {
                 if (mine[u]) r[u].store(cache + (size_t)(v.row0 + base + u * GROUP + my_warp * R::AT_ONCE + sub) * HD, i0, inv);
         }
         if (none) continue;
-        if (v.row0 && now > old) move_rows(cache, v.row0 * HD, old * inv, my_warp * 32 + lane, AT * 32);
+        if (v.held && now > old) {
+            move_rows(cache, v.row0 * HD, old * inv, my_warp * 32 + lane, AT * 32);
+            if (left_out)
+                for (int i = my_warp; i < v.n; i += AT)
+                    if (st.slots[v.tok0 + i] != v.slot0 + i) move_rows(cache + (size_t)(v.row0 + i) * HD, HD, old * inv, lane, 32);
+        }
         if (my_warp == 0 && lane == 0) *scale = now;         // (everybody has read it: a barrier ago)
     }
 }
 
 // qkv [T, row_stride] bfloat16 = q | k | v heads of hd features; q_out [T, q_stride] (may be qkv).  Tokens cu[b] .. cu[b + 1] are those of
-// request b at consecutive positions; slots [T] = page * page_size + position % page_size, negative: not written; null: no cache at all.
+// request b at consecutive positions; slots [T] = page * page_size + position % page_size, negative: not written (the row keeps what it stands for, unless the
+// page begins anew with its first row); null: no cache at all.
 // Caches [pages, nkv, page_size, hd] e4m3, scales [pages, nkv].
 extern "C" int vl_qk_norm_rope_write_8bit(const void* qkv, int row_stride, void* q_out, int q_stride, const int* positions, const int* slots,
                                           const int* cu, int B, const float* qw, const float* kw, float eps, const float* inv_freq, int rot,

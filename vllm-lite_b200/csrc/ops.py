@@ -960,7 +960,7 @@ def qk_norm_rope_write_8bit(qkv, positions, slots, cu_seqlens, q_weight, k_weigh
     the page's first row and grows as rows join, and the page's earlier rows are moved to a scale that has grown.  A NaN or an infinity makes the scale
     of its page NaN.  Tokens cu_seqlens[b] to cu_seqlens[b + 1] (int32 [B + 1]) are request b's, at consecutive positions; token t goes to slots[t] =
     page * page_size + positions[t] % page_size (negative: it is not written; slots None: none is), rows of a page before its request's first new
-    one being the request's own.  One launch writes a page for one request only.  q goes to q_out [T, nq hd], or stays in qkv.  rotary_dim is a
+    one being the request's own.  A row that is not written keeps what it stands for, unless its page starts anew in the same call.  One launch writes a page for one request only.  q goes to q_out [T, nq hd], or stays in qkv.  rotary_dim is a
     multiple of 4.  Angles are those of the exact products position * inv_freq."""
     _need(qkv, torch.bfloat16, "qkv", 2); _need(positions, torch.int32, "positions", 1)
     _need_here(qkv, "qkv")
