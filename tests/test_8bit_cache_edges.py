@@ -158,3 +158,102 @@ def test_slots_of_another_row_behind_tokens_that_are_not_written(hd, ps, new):
         bad[:2], bad[2], bad[3:] = -1, third, -5
         ops.qk_norm_rope_write_8bit(qkv, pos, bad, cu, None, None, 1e-6, None, 0, *cache.tensors, nkv, nkv, hd, cache.err)
         assert int(cache.err) == 2 and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache.tensors, was)), third
+
+
+# ---------------------------------------------------------------------------------------------- pages whose sizes lie far apart
+def far_apart(cache, lengths, small, bits, which):
+    """Makes the pages `small` (numbers within a request) of every request 2^bits smaller."""
+    for name in which:
+        scale = getattr(cache, name)
+        for r, n in enumerate(lengths):
+            for b in range(-(-n // cache.ps)):
+                if b in small:
+                    scale[int(cache.table[r, b])] *= 2.0 ** -bits
+
+
+@gpu
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 2, 128), (4, 4, 16), (6, 1, 48), (5, 1, 256), (2, 1, 80), (130, 1, 32)])
+@pytest.mark.parametrize("bits", [22, 23, 33, 45, 80])
+@pytest.mark.parametrize("which", [("k_scale",), ("v_scale",), ("k_scale", "v_scale")])
+def test_rows_that_read_small_pages_alone(nq, nkv, hd, bits, which):
+    """A prompt whose first two pages are far smaller than its later ones: the tokens of the first two read no other, and get what single tokens get.  (Their
+    queries are as much larger as their keys are smaller, so that their scores are ordinary ones.)"""
+    ps, n = 32, 128
+    cache = Cache(2, n, nkv, ps, hd, seed=1).fill([n, n], seed=hd, spread=1)
+    far_apart(cache, [n, n], (0, 1), bits, which)
+    pos, req, _, _ = batch(cache, [0, 0], [n, n])
+    q = queries(2 * n, nq, hd, 8)
+    if "k_scale" in which:
+        q = torch.where((pos < 2 * ps)[:, None], q * 2.0 ** bits, q)
+    out = torch.full((2 * n, nq * hd), 3.0, dtype=torch.bfloat16, device=DEV)
+    sizes = (nq, nkv, hd, hd ** -0.5, None)
+    early = [0, 1, 2, 30, 31, 32, 33, 63, 128, 150, 191]
+    ops.flash_prefill_8bit(q, out, *cache.tensors, cache.table, tiles_of([0, 0], [n, n]), *sizes, cache.err)
+    assert int(cache.err) == 0
+    check_attention(cache, q, out, pos, req, nq, None, hd ** -0.5, early)
+    if "k_scale" not in which:                                                     # (else the larger keys' scores leave a later row nothing to be off by)
+        check_attention(cache, q, out, pos, req, nq, None, hd ** -0.5, [64, 65, 127, 192, 255])
+    assert torch.isfinite(out).all()
+    alone = torch.full_like(out, 3.0)
+    ops.flash_decode_8bit(q, alone, *cache.tensors, cache.table, req, pos, *sizes, n, cache.err)
+    check_attention(cache, q, alone, pos, req, nq, None, hd ** -0.5, early)
+
+
+@gpu
+@pytest.mark.parametrize("nq,nkv,hd,ps", [(4, 2, 64, 64), (3, 1, 144, 16), (4, 1, 128, 40), (2, 2, 32, 7)])
+@pytest.mark.parametrize("before,new", [([1500, 300], [90, 20]), ([0, 900], [700, 256])])
+@pytest.mark.parametrize("bits", [25, 50])
+def test_windows_that_leave_large_pages_behind(nq, nkv, hd, ps, before, new, bits):
+    """Every fourth stretch of 256 tokens is large, and a window of 150 reads it from some tokens alone; keys shared out among blocks and whole."""
+    lengths, window = [b + n for b, n in zip(before, new)], 150
+    cache = Cache(2, max(lengths), nkv, ps, hd, seed=1).fill(lengths, seed=hd, spread=1)
+    small = [b for b in range(-(-max(lengths) // ps)) if b * ps // 256 % 4 != 1]
+    far_apart(cache, lengths, small, bits, ("v_scale",))
+    pos, req, _, _ = batch(cache, before, new)
+    q, out = queries(sum(new), nq, hd, 8), torch.full((sum(new), nq * hd), 3.0, dtype=torch.bfloat16, device=DEV)
+    ops.flash_prefill_8bit(q, out, *cache.tensors, cache.table, tiles_of(before, new), nq, nkv, hd, hd ** -0.5, window, cache.err)
+    assert int(cache.err) == 0
+    check_attention(cache, q, out, pos, req, nq, window, hd ** -0.5, sorted(set(range(0, sum(new), 13)) | {new[0] - 1, new[0], sum(new) - 1}))
+
+
+@gpu
+def test_few_tokens_behind_pages_far_apart():
+    """Shares of one item's keys, some of which hold pages far apart and some not."""
+    nq, nkv, hd, ps, before, new = 8, 2, 128, 64, [1900, 700], [5, 3]
+    lengths = [b + n for b, n in zip(before, new)]
+    cache = Cache(2, max(lengths), nkv, ps, hd, seed=1).fill(lengths, seed=3, spread=1)
+    far_apart(cache, lengths, (3, 9, 10, 29), 40, ("v_scale",))
+    far_apart(cache, lengths, (5, 10, 28), 40, ("k_scale",))
+    pos, req, _, _ = batch(cache, before, new)
+    q, out = queries(8, nq, hd, 8), torch.full((8, nq * hd), 3.0, dtype=torch.bfloat16, device=DEV)
+    ops.flash_prefill_8bit(q, out, *cache.tensors, cache.table, tiles_of(before, new), nq, nkv, hd, hd ** -0.5, None, cache.err)
+    assert int(cache.err) == 0
+    check_attention(cache, q, out, pos, req, nq, None, hd ** -0.5)
+
+
+@gpu
+def test_lost_and_missing_pages_among_pages_far_apart():
+    """What a page's scale that is none, and a page that the table does not hold, do elsewhere, they do here."""
+    nq, nkv, hd, ps, n = 4, 2, 64, 32, 256
+    cache = Cache(1, n, nkv, ps, hd).fill([n], spread=1)
+    far_apart(cache, [n], (0, 1), 40, ("v_scale",))
+    pos, req = torch.arange(n, dtype=torch.int32, device=DEV), torch.zeros(n, dtype=torch.int32, device=DEV)
+    q = queries(n, nq, hd, 3)
+    for which in ("k_scale", "v_scale"):
+        scale = getattr(cache, which)
+        kept = scale.clone()
+        scale[int(cache.table[0, 1]), 1] = float("nan")
+        for window in (None, 40):
+            out = ops.flash_prefill_8bit(q, torch.full_like(q, 3.0), *cache.tensors, cache.table, tiles_of([0], [n]), nq, nkv, hd, hd ** -0.5, window, cache.err)
+            nan = torch.isnan(out.view(n, nkv, -1))
+            reads = (pos >= ps) & ((pos - window + 1 < 2 * ps) if window else torch.ones_like(pos, dtype=torch.bool))
+            assert not nan[:, 0].any() and torch.equal(nan[:, 1].all(dim=1), reads) and torch.equal(nan[:, 1].any(dim=1), reads)
+        scale.copy_(kept)
+    assert int(cache.err) == 0
+    for bad in (-1, cache.k.shape[0]):
+        table = cache.table.clone()
+        table[0, 2] = bad
+        cache.err.zero_()
+        out = ops.flash_prefill_8bit(q, torch.full_like(q, 3.0), *cache.tensors, table, tiles_of([0], [n]), nq, nkv, hd, hd ** -0.5, None, cache.err)
+        assert int(cache.err) == 4 and torch.isfinite(out).all()
+        check_attention(cache, q, out, pos, req, nq, None, hd ** -0.5, [0, 31, 63])

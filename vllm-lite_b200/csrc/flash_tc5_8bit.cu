@@ -14,7 +14,8 @@
 //   four warps for keys, four for values   bring them: 16 bytes a load into registers, two tiles ahead, e4m3 to halves (exact), times a power of two, into two
 //        stages of 128-byte swizzled rows.  The pages' scales are folded in here: page by page 2^(e - E + 7), E the largest
 //        exponent of all pages that the block reads (found first; 448 * 2^7 is below the largest half), so that scores and outputs of all tiles are in one
-//        unit, which a row's own factor and the end undo.  Exact down to pages 2^15 below the largest, to within 2^-41 of the largest number else.
+//        unit, which a row's own factor and the end undo.  Exact down to pages 2^22 below the largest.  A block that reads pages further apart takes its rows
+//        one by one, a warp a row, in float32 (some of its rows may read the small pages alone; pages of the least scale, 2^-100, are counted as zeros beside larger ones);
 //        Rows that no query of the block reads, or that the table does not hold (flagged), are zeros.  A page whose scale is not a number gives
 //        keys of NaN and values of zero: who may read it gets NaN, rows that may not replace the score;
 //   one warp a query tile   issues S = Q K^T (both K-major) into one of two score buffers and O += P V (P from TMEM, V as stored: N contiguous).
@@ -62,6 +63,7 @@ constexpr int PIECES = HD / 16, EACH = (BN * PIECES + LOAD_THREADS - 1) / LOAD_T
 constexpr int QL = HD <= 16 ? 2 : HD <= 32 ? 4 : HD <= 64 ? 8 : HD <= 128 ? 16 : 32;      // lanes a row of queries or of the output, 8 features each
 constexpr float RESCALE_ABOVE = 8.0f, P_SHIFT = 7.0f;
 constexpr int FOLD = 7;
+constexpr int FAR = 24 - 9 + FOLD;                     // pages' exponents that e4m3 values, multiples of 2^-9, and halves, of 2^-24, leave room for
 
 __host__ __device__ constexpr unsigned idesc_f16(int m, int n) {       // float32 sums of halves: bits 4-5 = 1, operand types 0
     return (1u << 4) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
@@ -181,6 +183,106 @@ struct Tail {
     __device__ __forceinline__ int parts_of(const Item& item) const { return min(parts, (item.n + MIN_PART - 1) / MIN_PART); }
 };
 struct Partial { float4* out; float2* ml; };                             // out [blocks with parts][HD / 4][ROWS], ml (base, sum) [blocks with parts][ROWS]
+// What a block reads and writes, for `rows_alone`.
+struct Block {
+    const bf16* q; int q_stride; bf16* out; const unsigned char *kcache, *vcache; const float *kscale, *vscale; const int* table; int max_blocks;
+    int nq, nkv, page_size, num_pages; float scale_log2; int window; unsigned* err; int heads, tokens, kvh, h0, nheads, tok0, pos0, count, groups, lo, hi;
+    int parts, place; Partial partial;
+};
+// The block's rows one by one, a warp a row, in float32: for pages too far apart for one unit, which are not met in earnest (a prompt of 2,048 tokens 7 ms).  It is
+// called: within the kernel it cost the tensor cores' way 1 to 2 us of 53 and 92.
+__device__ __noinline__ void rows_alone(const Block& b) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per_head = 65536 / b.heads + 1;
+    constexpr int W = (HD / 2 + 31) / 32, AT_ONCE = 4;               // pairs of features a lane, keys on their way together
+#pragma unroll 1
+    for (int r = warp; r < b.groups * BM; r += NTHREADS / 32) {
+        const int rr = r & (BM - 1), t = (rr * per_head) >> 16, tk = (r / BM) * b.tokens + t, h = rr - t * b.heads;
+        if (t >= b.tokens || tk >= b.count || h >= b.nheads) continue;
+        const int qpos = b.pos0 + tk, last = min(b.hi, qpos);
+        const bf16* row = b.q + (size_t)(b.tok0 + tk) * b.q_stride + (size_t)(b.h0 + h) * HD;
+        float2 x[W], o[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const int i = lane + 32 * w;
+            x[w] = i < HD / 2 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(row + 2 * i)) : make_float2(0.f, 0.f);
+            o[w] = make_float2(0.f, 0.f);
+        }
+        float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+        for (int key = b.window > 0 ? max(b.lo, qpos - b.window + 1) : b.lo; key <= last;) {
+            const int blk = key / b.page_size, end = min(last, blk * b.page_size + (b.page_size - 1)), page = blk < b.max_blocks ? b.table[blk] : -1;
+            if (page < 0 || page >= b.num_pages) {
+                if (lane == 0 && b.err) atomicOr(b.err, VL_DEV_BAD_PAGE);
+                key = end + 1;
+                continue;
+            }
+            const size_t head = (size_t)page * b.nkv + b.kvh, at = (head * b.page_size + (key - blk * b.page_size)) * HD;
+            const unsigned char *kp = b.kcache + at, *vp = b.vcache + at;
+            const float ks = b.kscale[head] * b.scale_log2, vs = b.vscale[head];
+#pragma unroll 1
+            for (; key <= end; key += AT_ONCE, kp += AT_ONCE * HD, vp += AT_ONCE * HD) {
+                unsigned short k[AT_ONCE][W], v[AT_ONCE][W];
+#pragma unroll
+                for (int j = 0; j < AT_ONCE; ++j)
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        const int i = lane + 32 * w;
+                        const bool there = key + j <= end && i < HD / 2;
+                        k[j][w] = there ? *reinterpret_cast<const unsigned short*>(kp + j * HD + 2 * i) : 0;
+                        v[j][w] = there ? *reinterpret_cast<const unsigned short*>(vp + j * HD + 2 * i) : 0;
+                    }
+                auto two = [](unsigned short e) {
+                    const unsigned half2 = to_half2(e);
+                    return __half22float2(*reinterpret_cast<const __half2*>(&half2));
+                };
+#pragma unroll
+                for (int j = 0; j < AT_ONCE; ++j) {
+                    if (key + j > end) continue;
+                    float s = 0.f;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        const float2 y = two(k[j][w]);
+                        s += x[w].x * y.x + x[w].y * y.y;
+                    }
+                    s = warp_sum(s) * ks;
+                    if (s > m) {
+                        const float corr = exp2f(m - s);
+                        l *= corr;
+#pragma unroll
+                        for (int w = 0; w < W; ++w) { o[w].x *= corr; o[w].y *= corr; }
+                        m = s;
+                    }
+                    const float p = exp2f(s - m), pv = p * vs;
+                    l += p;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        const float2 y = two(v[j][w]);
+                        o[w].x += pv * y.x; o[w].y += pv * y.y;
+                    }
+                }
+            }
+            key = end + 1;
+        }
+        if (b.parts > 1) {                                             // (in the units of the other shares)
+            const float unit = power_of_two((int)P_SHIFT);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const int i = lane + 32 * w;
+                if (i < HD / 2)
+                    reinterpret_cast<float2*>(b.partial.out + ((size_t)b.place * (HD / 4) + i / 2) * ROWS + r)[i & 1] = make_float2(o[w].x * unit, o[w].y * unit);
+            }
+            if (lane == 0) b.partial.ml[(size_t)b.place * ROWS + r] = make_float2(m, l * unit);
+        } else {
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            bf16* dst = b.out + ((size_t)(b.tok0 + tk) * b.nq + b.h0 + h) * HD;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const int i = lane + 32 * w;
+                if (i < HD / 2) *reinterpret_cast<__nv_bfloat162*>(dst + 2 * i) = __floats2bfloat162_rn(o[w].x * inv, o[w].y * inv);
+            }
+        }
+    }
+}
 }  // namespace
 
 // tiles[i] = {row of the block table, index of the tile's first token in the step, tokens (<= 128), position of the first}
@@ -200,7 +302,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     unsigned long long *found_full = pv_done + 4, *found_empty = found_full + FOUND;
     unsigned& tmem_slot = *reinterpret_cast<unsigned*>(found_empty + FOUND);
     int* words = reinterpret_cast<int*>(found_empty + FOUND + 1);
-    int &failed = words[0], &top_k = words[1], &top_v = words[2];
+    int &failed = words[0], &top_k = words[1], &top_v = words[2], &low_k = words[3], &low_v = words[4];
     float* s_row_scale = reinterpret_cast<float*>(smem + TILE_BYTES + 512);                      // [GROUPS * BM]
     int2* s_found = reinterpret_cast<int2*>(s_row_scale + GROUPS * BM);                          // keys, values: [FOUND][BN] cache row (-1: zeros) and factor
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -260,6 +362,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     } else if (tid == NTHREADS - 1) {
         failed = 0;
         top_k = top_v = EXP_MIN;
+        low_k = low_v = 128;
     }
     const int worker = warp < SOFT ? tid : tid - 32 * (LOAD0 - SOFT), first_page = lo / page_size, last_page = hi / page_size;
     auto page_at = [&](int blk) -> int {
@@ -295,7 +398,7 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     // The largest exponents of the pages that the block reads, and the queries as halves; the first loads of both are on their way at once.
     // QL lanes a query row, 8 features each; rows of no token are zeros.
     if (warp < SOFT || warp >= LOAD0) {
-        int ek = EXP_MIN, ev = EXP_MIN;
+        int ek = EXP_MIN, ev = EXP_MIN, lk = 128, lv = 128;
         pdl_wait();
         constexpr int AT_ONCE = WORKERS / QL;
         constexpr int AHEAD = (GROUPS * BM + AT_ONCE - 1) / AT_ONCE;
@@ -309,8 +412,11 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             if (live) raw[u] = *reinterpret_cast<const uint4*>(q + (size_t)(tok0 + tk) * q_stride + (size_t)(h0 + h) * HD + c * 8);
         }
         auto exponents = [&](float ks, float vs) {
-            if (ks == ks) ek = max(ek, (int)(__float_as_uint(ks) >> 23) - 127);
-            if (vs == vs) ev = max(ev, (int)(__float_as_uint(vs) >> 23) - 127);
+            const int k = (int)(__float_as_uint(ks) >> 23) - 127, v = (int)(__float_as_uint(vs) >> 23) - 127;
+            if (ks == ks) ek = max(ek, k);
+            if (vs == vs) ev = max(ev, v);
+            if (k > EXP_MIN) lk = min(lk, k);                            // (NaN's is 128)
+            if (v > EXP_MIN) lv = min(lv, v);
         };
         const float ks = page >= 0 ? kscale[(size_t)page * nkv + kvh] : 0.f, vs = page >= 0 ? vscale[(size_t)page * nkv + kvh] : 0.f;
         for (int blk = first_page + worker + WORKERS; blk <= last_page; blk += WORKERS) {
@@ -339,7 +445,9 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
         exponents(ks, vs);
         ek = __reduce_max_sync(0xffffffffu, ek);
         ev = __reduce_max_sync(0xffffffffu, ev);
-        if (lane == 0) { atomicMax(&top_k, ek); atomicMax(&top_v, ev); }
+        lk = __reduce_min_sync(0xffffffffu, lk);
+        lv = __reduce_min_sync(0xffffffffu, lv);
+        if (lane == 0) { atomicMax(&top_k, ek); atomicMax(&top_v, ev); atomicMin(&low_k, lk); atomicMin(&low_v, lv); }
     } else {
         if (warp == FIND_WARP) {
 #pragma unroll
@@ -360,7 +468,10 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
     const unsigned tmem_base = tmem_slot;
 
     const int role = warp_number();
-    if (role >= LOAD0) {                                                 // ---- keys and values ----
+    if (top_k - low_k > FAR || top_v - low_v > FAR) {                    // ---- pages too far apart for one unit ----
+        rows_alone({q, q_stride, out, kcache, vcache, kscale, vscale, table, max_blocks, nq, nkv, page_size, num_pages, scale_log2, window, err, heads, tokens, kvh, h0,
+                    nheads, tok0, pos0, count, groups, lo, hi, parts, place, partial});
+    } else if (role >= LOAD0) {                                                 // ---- keys and values ----
         const bool values = role >= LOAD0 + LOADERS;
         const int ct = (tid - LOAD0 * 32) % LOAD_THREADS;
         const unsigned char* cache = values ? vcache : kcache;
