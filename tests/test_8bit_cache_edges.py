@@ -257,3 +257,44 @@ def test_lost_and_missing_pages_among_pages_far_apart():
         out = ops.flash_prefill_8bit(q, torch.full_like(q, 3.0), *cache.tensors, table, tiles_of([0], [n]), nq, nkv, hd, hd ** -0.5, None, cache.err)
         assert int(cache.err) == 4 and torch.isfinite(out).all()
         check_attention(cache, q, out, pos, req, nq, None, hd ** -0.5, [0, 31, 63])
+
+
+# ---------------------------------------------------------------------------------------------- the largest sizes
+@pytest.mark.parametrize("T,bound,code", [(1, (1 << 31) - 1, -2), (1, (1 << 31) - 128, -2), (1, (1 << 30) + 1, -2), (64, (1 << 31) - 1, -2), (200, 1 << 30, -2)])
+def test_bounds_beyond_the_largest_are_refused_before_any_launch(T, bound, code):
+    host = torch.zeros(64)                                   # never read or written
+    at = -host.data_ptr() % 16 + host.data_ptr()
+    got = ops._fn("flash_decode_8bit", "vl_flash_decode_8bit", {"FA_HD": 128})(
+        at, 256, at, at, at, at, at, 2, at, at, T, 2, 1, 128, 64, 4, 0.1, 0, bound, at, 3 * T * 2 * 130, None, None, at, at, 0, 0)
+    assert got == code
+
+
+@gpu
+def test_windows_wider_than_any_context():
+    """The widest window that is a number, and no window, are one thing: the same results, to the bit, however keys are shared out."""
+    nq, nkv, hd, ps, n = 8, 2, 128, 64, 3000
+    cache = Cache(2, n, nkv, ps, hd, seed=1).fill([n, 1000], seed=3)
+    q = queries(5, nq, hd, 8)
+    pos, req, _, _ = batch(cache, [n - 4, 999], [4, 1])
+    results = {}
+    for window in (None, (1 << 31) - 1, (1 << 31) - 100, 1 << 30):
+        prompt, single = torch.full_like(q, 3.0), torch.full_like(q, 3.0)
+        ops.flash_prefill_8bit(q, prompt, *cache.tensors, cache.table, tiles_of([n - 4, 999], [4, 1]), nq, nkv, hd, hd ** -0.5, window, cache.err)
+        ops.flash_decode_8bit(q, single, *cache.tensors, cache.table, req, pos, nq, nkv, hd, hd ** -0.5, window, n, cache.err)
+        results[window] = (prompt, single)
+    assert int(cache.err) == 0
+    check_attention(cache, q, results[None][0], pos, req, nq, None, hd ** -0.5)
+    assert all(torch.equal(a, b) for r in results.values() for a, b in zip(r, results[None]))
+
+
+@gpu
+def test_a_bound_as_large_as_it_may_be():
+    nq, nkv, hd, ps = 8, 2, 128, 64
+    cache = Cache(2, 500, nkv, ps, hd, seed=1).fill([500, 40], seed=3)
+    q, out = queries(2, nq, hd, 8), torch.full((2, nq * hd), 3.0, dtype=torch.bfloat16, device=DEV)
+    pos, req, _, _ = batch(cache, [499, 39], [1, 1])
+    ops.flash_decode_8bit(q, out, *cache.tensors, cache.table, req, pos, nq, nkv, hd, hd ** -0.5, None, 1 << 30, cache.err)
+    check_attention(cache, q, out, pos, req, nq, None, hd ** -0.5)
+    with pytest.raises(ops.KernelError):
+        ops.flash_decode_8bit(q, out, *cache.tensors, cache.table, req, pos, nq, nkv, hd, hd ** -0.5, None, (1 << 30) + 1, cache.err)
+    assert int(cache.err) == 0

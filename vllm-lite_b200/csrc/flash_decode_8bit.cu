@@ -700,7 +700,7 @@ flash_decode_8bit_merge_kernel(float* scratch, int runs, int held, int grp, int 
 extern "C" int vl_flash_decode_8bit_head_dim() { return HD; }
 
 // q [T, q_stride] bfloat16, out [.., nq * hd]; caches [pages, nkv, page_size, hd] e4m3, scales [pages, nkv]; positions from `bound` on are
-// flagged and get rows of zeros.  scratch: `floats` of them, the more the shorter the runs may be, 3 * T * nq * (hd + 2) at least; arrivals: T * nq counters, zero
+// flagged and get rows of zeros; it is 2^30 at most.  scratch: `floats` of them, the more the shorter the runs may be, 3 * T * nq * (hd + 2) at least; arrivals: T * nq counters, zero
 // before and after.
 extern "C" int vl_flash_decode_8bit(const void* q, int q_stride, const void* kcache, const void* vcache, const float* kscale, const float* vscale,
                                     const int* block_table, int max_blocks, const int* req_index, const int* positions, int T, int nq, int nkv, int hd,
@@ -712,7 +712,8 @@ extern "C" int vl_flash_decode_8bit(const void* q, int q_stride, const void* kca
     if (bound <= 0 || !out || !arrivals || !scratch) return VL_ERR_ARGUMENT;
     if (((uintptr_t)q & 7) || (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)scratch) & 15)) return VL_ERR_ARGUMENT;
     const int grp = nq / nkv, wide_heads = grp > 8 && HD <= 128 ? 16 : 8, htiles = (grp + wide_heads - 1) / wide_heads;
-    const long long most = (long long)T * nkv * htiles * ((bound + BN - 1) / BN);
+    const long long most = (long long)T * nkv * htiles * ((bound - 1) / BN + 1);
+    if (bound > (1 << 30)) return VL_ERR_UNSUPPORTED;        // (positions, rounded up to steps, are whole numbers of 32 bits)
     if ((long long)num_pages * nkv * page_size >= (1ll << 31) || most >= (1ll << 30)) return VL_ERR_UNSUPPORTED;
     if (floats < 3ll * T * nq * (hd + 2)) return VL_ERR_ARGUMENT;
     int dev = 0, sms = 0;

@@ -864,7 +864,7 @@ int flash_prefill_8bit(const void* q, int q_stride, void* out, const void* kcach
     // portions of 512 at position 2,500, 184 blocks on 148 SMs: 112 us with every block whole).
     const int in_list = num_tiles * cuts;
     const long long blocks = (long long)in_list * nkv * htiles, reach = (long long)max_blocks * page_size;
-    const long long keys = window > 0 && window + GROUPS * tokens < reach ? window + GROUPS * tokens : reach;
+    const long long near = (long long)window + GROUPS * tokens, keys = window > 0 && near < reach ? near : reach;
     const bool shared = scratch && keys >= 2 * MIN_PART * BN;
     const int split = shared && in_list <= MOST_ITEMS && 2 * blocks <= sms ? sms : 0, over = (int)(blocks % sms);
     const bool last = shared && blocks > sms && blocks <= MOST_ROUNDS * sms && over && 2 * over <= sms;

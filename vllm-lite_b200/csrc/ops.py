@@ -1027,7 +1027,8 @@ def flash_decode_8bit(q, out, k_cache, v_cache, k_scale, v_scale, block_table, r
                       max_context, err, token_index=None, scratch=None, arrivals=None, settled=False):
     """Attention of single tokens over a cache in 8 bits (`qk_norm_rope_write_8bit`): q bfloat16 [T, >= nq hd] (its first columns are read), out bfloat16
     [T, nq hd]; token t, at positions[t] of the request whose pages row req_index[t] of block_table names, reads every key up to its own or the last `window`.
-    Tokens at negative positions and (flagged) at max_context or beyond get rows of zeros.  token_index (int32): only these tokens, the others' rows of
+    Tokens at negative positions and (flagged) at max_context or beyond get rows of zeros; max_context is 2^30 at most, and 2^30
+    steps (of 64 or 128 keys, for a KV head and up to 8 or 16 of its query heads) or more over all tokens are refused.  token_index (int32): only these tokens, the others' rows of
     out are left alone.  scratch (float32) and arrivals (int32, zero before and after each call): at least `flash_decode_8bit_scratch` of them, which nobody
     else on the stream needs; without them the call takes its own.  Pages may have any number of positions; q begins on 8 bytes, scratch on 16.
     `settled`: as in `flash_decode`."""
