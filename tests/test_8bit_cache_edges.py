@@ -298,3 +298,32 @@ def test_a_bound_as_large_as_it_may_be():
     with pytest.raises(ops.KernelError):
         ops.flash_decode_8bit(q, out, *cache.tensors, cache.table, req, pos, nq, nkv, hd, hd ** -0.5, None, (1 << 30) + 1, cache.err)
     assert int(cache.err) == 0
+
+
+# ---------------------------------------------------------------------------------------------- queries that are no numbers
+@gpu
+@pytest.mark.parametrize("nq,nkv,hd", [(4, 2, 64), (8, 1, 128), (3, 3, 48), (2, 1, 256)])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("before,window,far", [(0, None, False), (0, 20, False), (1500, None, False), (0, None, True)])
+def test_a_query_that_holds_an_infinity(nq, nkv, hd, bad, before, window, far):
+    """All scores of such a head are infinite or none, and a softmax of them is none, also where every one of them is minus infinity (keys of positive numbers alone);
+    nobody else's result changes."""
+    ps, n = 32, 70
+    cache = Cache(1, before + n, nkv, ps, hd).fill([before + n], spread=1)
+    cache.k.view(torch.uint8).bitwise_and_(0x7f)
+    if far:
+        far_apart(cache, [before + n], (0,), 40, ("v_scale",))
+    pos, req, _, _ = batch(cache, [before], [n])
+    q = queries(n, nq, hd, 3)
+    q.view(n, nq, hd)[33, nq - 1, 7] = bad
+    q.view(n, nq, hd)[0, 0, 9] = bad
+    want = torch.zeros(n, nq, dtype=torch.bool, device=DEV)
+    want[33, nq - 1] = want[0, 0] = True
+    prompt, single = torch.full_like(q, 3.0), torch.full_like(q, 3.0)
+    ops.flash_prefill_8bit(q, prompt, *cache.tensors, cache.table, tiles_of([before], [n]), nq, nkv, hd, hd ** -0.5, window, cache.err)
+    ops.flash_decode_8bit(q, single, *cache.tensors, cache.table, req, pos, nq, nkv, hd, hd ** -0.5, window, before + n, cache.err)
+    assert int(cache.err) == 0
+    for out in (prompt, single):
+        nan = torch.isnan(out.view(n, nq, hd))
+        assert torch.equal(nan.all(dim=2), want) and torch.equal(nan.any(dim=2), want)
+    check_attention(cache, q, prompt, pos, req, nq, window, hd ** -0.5, [1, 2, 31, 32, 34, 69])

@@ -437,6 +437,8 @@ flash_tc5_8bit_kernel(const bf16* __restrict__ q, int q_stride, bf16* __restrict
             const float f = power_of_two(-e);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = pack_half(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+            // a query with a NaN or an infinity is NaN all along: its scores might all be -inf as those of a row without keys are
+            if (__builtin_expect(top >= 0x7f80u, 0)) raw[u] = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u);
             if (r < groups * BM && c < HD / 8) {
                 *reinterpret_cast<uint4*>(Qs + (r / BM) * Q_BYTES + (unsigned)(c >> 3) * (BM * ROW_BYTES) + swizzled(rr, c & 7)) = raw[u];
                 if (c == 0) s_row_scale[r] = scale_log2 * power_of_two(e);
