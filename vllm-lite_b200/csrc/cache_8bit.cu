@@ -14,8 +14,9 @@
 //            page's rows once for several heads;
 //   narrow:  any other head, a warp a row, 4-byte accesses.
 //
-// Measured in a graph: 64 single tokens of 32 + 2 x 8 heads of 128 4.5 us (a block a page took 16.4, most of it in blocks of one row); a portion of 4,096 tokens
-// at position 700 27.9 us, 92 MB at 3.3 TB/s (4-byte accesses 108); five portions of 77 with heads of 80 and pages of 16 7.0 us.  Bound by latencies: single tokens by loads behind
+// Measured in a graph: 64 single tokens of 32 + 2 x 8 heads of 128 4.4 us, 4.9 with q in place (a block a page took 16.4, most of it in blocks of one row); a portion of
+// 4,096 tokens at position 700 27.8 us, 92 MB at 3.3 TB/s (through the narrow kernel, heads of 96 108 us, heads of 128 of which 64 features turn 112); five portions of 77 with
+// heads of 80 and pages of 16 6.9 us.  Bound by latencies: single tokens by loads behind
 // one another (position and slot, the scale, the row, the page's rows where a scale grows), a portion by the loads of a page's rows and the barrier before its scale is known.
 //
 // Angles are pos * inv_freq as a number of turns in double precision, of which the fraction alone is left (in float32 the product is off by up to 2^-24 of
@@ -625,8 +626,8 @@ extern "C" int vl_qk_norm_rope_write_8bit(const void* qkv, int row_stride, void*
     // 1 34.5; 8 portions of 300, 4 KV heads: 4 heads 21, 1 12).
     st.heads_a_warp = wide ? (T >= 256 ? 16 : 8) : (T >= 256 ? 8 : (T >= 32 ? 4 : 2));
     st.heads_a_block = !wide || T < 32 * pages || pages * nkv < 256 ? 1 : (pages * nkv < 512 ? 2 : 4);
-    // Two warps a head where they hold the rows that a page can get: small pages and short portions leave none idle (2,048 tokens on pages of 16: 18 us, 30 with
-    // eight; 300 portions of 8 tokens 17 and 37).
+    // Two warps a head where they hold the rows that a page can get: small pages and short portions leave none idle (32 + 2 x 8 heads of 128: 2,048 tokens on pages
+    // of 16 17.6 us, 29 with eight; 300 portions of 8 tokens 28 and 71).
     const int rows = page_size < (T + B - 1) / (B > 0 ? B : 1) ? page_size : (T + B - 1) / (B > 0 ? B : 1), a_warp = (hd <= 128 ? 2 : 4) * (512 / hd);
     const bool few = wide && rows <= 2 * a_warp;
     if (few && st.heads_a_block < WARPS / 2) st.heads_a_block = WARPS / 2 < nkv ? WARPS / 2 : nkv;

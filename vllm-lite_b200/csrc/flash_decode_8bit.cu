@@ -19,7 +19,8 @@
 // first product with keys along the lanes and enters the second with heads along them: one movmatrix for 8 keys.
 // Roundings to fewer bits: q times a power of two (its largest number lies in [2^14, 2^15), so bfloat16's bits stay down to 2^-28 of
 // it) and p sv, as halves.  Sums, maxima and outputs are float32.  p sv is held in units of the largest sv so far, E, times 2^6: a running base
-// lets p reach 2^8 before the row is rescaled, so numbers lie below 2^14 and are normal down to 2^-20 of the base's weight.
+// lets p reach 2^8 before the row is rescaled, so numbers lie below 2^14 and are normal down to 2^-20 of the base's weight (and what lies 2^-31 below the
+// largest value that the token reads may vanish).
 // The maximum of a warp's keys is looked for only where some score has passed the base by 8 (one vote a tile instead of shuffles).
 //
 // The keys of all (token, KV head, tile of heads) items, one item behind the other, are cut into runs of equal length in steps of BN keys, one run a block, as many
@@ -149,7 +150,6 @@ struct Scratch {
     int4* info;                                        // of an item in pieces: slot of the first, of the second, how many (0: none), token
     __host__ __device__ Scratch(float* p, long long runs, int heads)
         : part(p), ml(reinterpret_cast<float2*>(p + 2 * runs * heads * HD)), info(reinterpret_cast<int4*>(p + (2 * runs * heads * (HD + 2) + 3) / 4 * 4)) {}
-    static __host__ __device__ long long floats(long long runs, int heads, long long items) { return (2 * runs * heads * (HD + 2) + 3) / 4 * 4 + 4 * items; }
 };
 
 // WIDE: pages of a multiple of 16 positions, so that 16 keys lie on one page.

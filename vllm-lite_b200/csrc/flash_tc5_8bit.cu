@@ -22,8 +22,8 @@
 // Where a launch has so few tokens that half of the SMs would be without a block, each item's keys are shared out among several, which leave base, sum and
 // output as they are for a second launch to join.  So are the keys of the items that would be the few blocks of a last round.
 //
-// Measured in a graph (32 heads of 128, 8 KV heads): a prompt of 2,048 tokens 53 us, 0.65 PFLOP/s; three portions of 512 at position 2,500 90 us, 0.71 (every
-// block whole: 112); 8 tokens behind 8,000 keys 27 us.  A step of 64 keys takes a block 1.0 us where exponentials alone (16 a cycle and SM) take 0.54, the products 0.55
+// Measured in a graph (32 heads of 128, 8 KV heads), tiles and table settled: a prompt of 2,048 tokens 53 us, 0.65 PFLOP/s; three portions of 512 at position 2,500 90 us,
+// 0.71 (every block whole: 112); 8 tokens behind 8,000 keys 27 us.  Where they are not, what follows from them begins behind the wait for the kernel ahead: 54, 92 and 32.  A step of 64 keys takes a block 1.0 us where exponentials alone (16 a cycle and SM) take 0.54, the products 0.55
 // and shared memory's traffic 0.65.  No unit is full (issue slots and the exponential unit about half, ALUs and tensor cores a third): a step is a chain of waits, loads
 // from TMEM, weights and votes.  What a block takes besides, some 8 us: queries and scales (3 us), the first keys (2), the last product and the output (2).
 // Steps on the way: P through shared memory and keys and values by the same four warps 75 and 165 us.
